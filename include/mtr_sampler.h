@@ -55,6 +55,9 @@ extern "C" {
 #define MTR_MAX_EOS_IDS 16
 #define MTR_MAX_EOS_RANGES 2
 #define MTR_MAX_LB_EOS 8
+#define MTR_MAX_I8_D_MODEL 131072 /* 127 * 128 * 131072 < 2^31: the int32 sums cannot wrap */
+#define MTR_MAX_I8_ROWS (1 << 22)
+#define MTR_MAX_TOP_N 32
 
 /* Return codes of every entry point. */
 typedef enum MtrStatus {
@@ -300,6 +303,137 @@ int mtr_lmhead_launch(const MtrLmHeadArgs* args, void* stream);
  * wait for its results).  sampler->logits must be lm->logits (bf16, same row
  * stride and vocabulary) and the sampler's rows must lie inside lm->rows. */
 int mtr_lmhead_sample_launch(const MtrLmHeadArgs* lm, const MtrSamplerArgs* sampler, void* stream);
+
+/*
+ * 8-bit output projection.  Rows of hidden states and of the weight are held
+ * as int8 with one fp32 scale per row:
+ *   scale[r] = RN32(max_k |x[r, k]| / 127),  q[r, k] = RNE(RN32(x[r, k] / scale[r]))
+ * (q = 0 for a row of zeros, or one so small that its scale rounds to 0; a row
+ * with a NaN or an infinity gets scale NaN and q = 0).
+ */
+typedef struct MtrQuantizeArgs {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrQuantizeArgs) */
+  const void* x;                /* [rows, cols], x_dtype */
+  int64_t x_row_stride;         /* elements */
+  int32_t x_dtype;              /* MtrDType */
+  int32_t rows;
+  int32_t cols;                 /* >= 1 */
+  int32_t reserved0;
+  int8_t* q;                    /* [rows, cols] */
+  int64_t q_row_stride;         /* bytes; bytes past cols are left as they are */
+  float* scale;                 /* [rows] */
+} MtrQuantizeArgs;
+
+int mtr_quantize_rows_validate(const MtrQuantizeArgs* args);
+int mtr_quantize_rows_launch(const MtrQuantizeArgs* args, void* stream);
+
+/*
+ * logits[r, v] = RN(RN32(RN32(float(sum_k q[r, k] * weight[v, k])) * scale[r]) * weight_scale[v])
+ * with q, scale the quantised hidden states (quantised by this call, into the
+ * workspace) and the sum exact in int32: mtr_lmhead_launch with a quarter to a
+ * half of its weight traffic and twice its tensor rate.
+ */
+typedef struct MtrLmHeadI8Args {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrLmHeadI8Args) */
+  const void* hidden;           /* [rows, d_model], hidden_dtype */
+  int64_t hidden_row_stride;    /* elements */
+  const int8_t* weight;         /* [vocab, d_model], 16-byte aligned */
+  int64_t weight_row_stride;    /* bytes, multiple of 16 */
+  const float* weight_scale;    /* [vocab] */
+  void* logits;                 /* [rows, vocab], logits_dtype; must not overlap the inputs */
+  int64_t logits_row_stride;    /* elements */
+  int32_t hidden_dtype;         /* MtrDType */
+  int32_t logits_dtype;         /* MtrDType */
+  int32_t rows;                 /* 0 .. MTR_MAX_I8_ROWS */
+  int32_t d_model;              /* 1 .. MTR_MAX_I8_D_MODEL */
+  int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
+  int32_t reserved0;
+  void* workspace;              /* 256-byte aligned; one call's at a time */
+  int64_t workspace_bytes;      /* >= mtr_lmhead_i8_workspace(rows, d_model) */
+  uint32_t* error_word;         /* device word or NULL: bits set when a bounded wait gave up */
+} MtrLmHeadI8Args;
+
+/* Workspace bytes of a call (0 for rows <= 0 or d_model <= 0). */
+int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model);
+int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* args);
+int mtr_lmhead_i8_launch(const MtrLmHeadI8Args* args, void* stream);
+
+/* As mtr_lmhead_sample_launch, with the 8-bit projection (the sampler's
+ * logits_dtype must be the projection's). */
+int mtr_lmhead_i8_sample_launch(const MtrLmHeadI8Args* lm, const MtrSamplerArgs* sampler, void* stream);
+
+/*
+ * Log probabilities of given tokens, entropy, log-sum-exp and top alternatives
+ * of each row, under softmax(logits / temperature):
+ *   lse = log sum_v e^(x_v), x = logits / temperature;  log p_v = x_v - lse;
+ *   entropy = -sum_v p_v log p_v (nats; masked ids, p = 0, add nothing).
+ * The alternatives are the top_n largest logits, equal ones in id order; an id
+ * whose logit is -inf is none, and missing ones read id -1, log p -inf.
+ * A token below 0 is no token (a padded position): its log p is 0.  One >=
+ * vocab counts as none too and sets MTR_ROW_BAD_ID.
+ * A row of -inf alone (MTR_ROW_ALL_MASKED): log p and lse -inf, entropy 0.
+ * A row with NaN or +inf (MTR_ROW_NONFINITE): NaN, and ids -1.
+ */
+typedef struct MtrLogprobArgs {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrLogprobArgs) */
+  const void* logits;           /* [rows, vocab] */
+  int64_t logits_row_stride;    /* elements */
+  const void* tokens;           /* [rows] ids, or NULL: no tokens */
+  int32_t logits_dtype;         /* MtrDType */
+  int32_t tokens_dtype;         /* MtrIdType */
+  int32_t rows;
+  int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
+  int32_t top_n;                /* 0 .. MTR_MAX_TOP_N */
+  float temperature;            /* > 0, finite, with a finite reciprocal */
+  float* out_logprobs;          /* [rows] or NULL */
+  float* out_entropy;           /* [rows] or NULL */
+  float* out_lse;               /* [rows] or NULL */
+  int64_t* out_top_ids;         /* [rows, top_n]; required when top_n > 0 */
+  float* out_top_logprobs;      /* [rows, top_n]; required when top_n > 0 */
+  float* out_stats;             /* [rows, 4] or NULL, 16-byte aligned: largest logit, log of
+                                   sum_v e^((logit_v - largest) / temperature), entropy, 0 --
+                                   what mtr_logprob_grad_launch reads */
+  uint32_t* out_status;         /* [rows] MTR_ROW_* bits or NULL */
+} MtrLogprobArgs;
+
+int mtr_logprob_validate(const MtrLogprobArgs* args);
+int mtr_logprob_launch(const MtrLogprobArgs* args, void* stream);
+
+/*
+ * Gradient of mtr_logprob_launch's outputs with respect to the logits:
+ *   grad_v = [ p_v (g_lse - g_logprob - sum_j g_top_j - g_entropy (log p_v + entropy))
+ *              + [v = token] g_logprob + sum_j [v = top_id_j] g_top_j ] / temperature
+ * rounded once to the logits' type.  Rows whose forward reads NaN give NaN,
+ * rows of -inf alone give 0; a token that is none and an alternative of id -1
+ * take no part.
+ */
+typedef struct MtrLogprobGradArgs {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrLogprobGradArgs) */
+  const void* logits;           /* [rows, vocab], as in the forward call */
+  int64_t logits_row_stride;    /* elements */
+  const void* tokens;           /* as in the forward call */
+  int32_t logits_dtype;         /* MtrDType */
+  int32_t tokens_dtype;         /* MtrIdType */
+  int32_t rows;
+  int32_t vocab;
+  int32_t top_n;                /* alternatives that g_top is given for (0: none) */
+  float temperature;            /* as in the forward call */
+  const float* stats;           /* [rows, 4], the forward call's out_stats */
+  const int64_t* top_ids;       /* [rows, top_n], the forward call's; required when top_n > 0 */
+  const float* g_logprobs;      /* [rows] or NULL (zeros) */
+  const float* g_entropy;       /* [rows] or NULL */
+  const float* g_lse;           /* [rows] or NULL */
+  const float* g_top;           /* [rows, top_n]; required when top_n > 0 */
+  void* grad_logits;            /* [rows, vocab], logits_dtype; must not overlap the logits */
+  int64_t grad_row_stride;      /* elements */
+} MtrLogprobGradArgs;
+
+int mtr_logprob_grad_validate(const MtrLogprobGradArgs* args);
+int mtr_logprob_grad_launch(const MtrLogprobGradArgs* args, void* stream);
 
 /* ABI identity: MTR_ABI_VERSION and sizeof(MtrSamplerArgs) of the library. */
 int mtr_abi_version(void);

@@ -26,6 +26,9 @@ MAX_GRAMMAR_CLASSES = 32
 MAX_EOS_IDS = 16
 MAX_EOS_RANGES = 2
 MAX_LB_EOS = 8
+MAX_I8_D_MODEL = 131072
+MAX_I8_ROWS = 1 << 22
+MAX_TOP_N = 32
 
 # MtrStatus
 OK = 0
@@ -182,6 +185,100 @@ class MtrLmHeadArgs(ctypes.Structure):
     ]
 
 
+class MtrQuantizeArgs(ctypes.Structure):
+    """include/mtr_sampler.h MtrQuantizeArgs: rows to int8 with a scale each."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("x", c_void_p),
+        ("x_row_stride", c_int64),
+        ("x_dtype", c_int32),
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("reserved0", c_int32),
+        ("q", c_void_p),
+        ("q_row_stride", c_int64),
+        ("scale", c_void_p),
+    ]
+
+
+class MtrLmHeadI8Args(ctypes.Structure):
+    """include/mtr_sampler.h MtrLmHeadI8Args: the 8-bit output projection."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("hidden", c_void_p),
+        ("hidden_row_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_row_stride", c_int64),
+        ("weight_scale", c_void_p),
+        ("logits", c_void_p),
+        ("logits_row_stride", c_int64),
+        ("hidden_dtype", c_int32),
+        ("logits_dtype", c_int32),
+        ("rows", c_int32),
+        ("d_model", c_int32),
+        ("vocab", c_int32),
+        ("reserved0", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("error_word", c_void_p),
+    ]
+
+
+class MtrLogprobArgs(ctypes.Structure):
+    """include/mtr_sampler.h MtrLogprobArgs: log probabilities of given tokens."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("logits", c_void_p),
+        ("logits_row_stride", c_int64),
+        ("tokens", c_void_p),
+        ("logits_dtype", c_int32),
+        ("tokens_dtype", c_int32),
+        ("rows", c_int32),
+        ("vocab", c_int32),
+        ("top_n", c_int32),
+        ("temperature", c_float),
+        ("out_logprobs", c_void_p),
+        ("out_entropy", c_void_p),
+        ("out_lse", c_void_p),
+        ("out_top_ids", c_void_p),
+        ("out_top_logprobs", c_void_p),
+        ("out_stats", c_void_p),
+        ("out_status", c_void_p),
+    ]
+
+
+class MtrLogprobGradArgs(ctypes.Structure):
+    """include/mtr_sampler.h MtrLogprobGradArgs: gradient of MtrLogprobArgs' outputs."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("logits", c_void_p),
+        ("logits_row_stride", c_int64),
+        ("tokens", c_void_p),
+        ("logits_dtype", c_int32),
+        ("tokens_dtype", c_int32),
+        ("rows", c_int32),
+        ("vocab", c_int32),
+        ("top_n", c_int32),
+        ("temperature", c_float),
+        ("stats", c_void_p),
+        ("top_ids", c_void_p),
+        ("g_logprobs", c_void_p),
+        ("g_entropy", c_void_p),
+        ("g_lse", c_void_p),
+        ("g_top", c_void_p),
+        ("grad_logits", c_void_p),
+        ("grad_row_stride", c_int64),
+    ]
+
+
 # Every symbol include/mtr_sampler.h declares: (name, restype, argtypes).
 EXPORTS = {
     "mtr_abi_version": (ctypes.c_int, []),
@@ -197,6 +294,17 @@ EXPORTS = {
     "mtr_lmhead_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadArgs), c_void_p]),
     "mtr_lmhead_sample_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadArgs), ctypes.POINTER(MtrSamplerArgs),
                                                 c_void_p]),
+    "mtr_quantize_rows_validate": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeArgs)]),
+    "mtr_quantize_rows_launch": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeArgs), c_void_p]),
+    "mtr_lmhead_i8_workspace": (c_int64, [c_int32, c_int32]),
+    "mtr_lmhead_i8_validate": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args)]),
+    "mtr_lmhead_i8_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args), c_void_p]),
+    "mtr_lmhead_i8_sample_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args), ctypes.POINTER(MtrSamplerArgs),
+                                                   c_void_p]),
+    "mtr_logprob_validate": (ctypes.c_int, [ctypes.POINTER(MtrLogprobArgs)]),
+    "mtr_logprob_launch": (ctypes.c_int, [ctypes.POINTER(MtrLogprobArgs), c_void_p]),
+    "mtr_logprob_grad_validate": (ctypes.c_int, [ctypes.POINTER(MtrLogprobGradArgs)]),
+    "mtr_logprob_grad_launch": (ctypes.c_int, [ctypes.POINTER(MtrLogprobGradArgs), c_void_p]),
 }
 
 
@@ -319,3 +427,33 @@ def lmhead_launch(args: MtrLmHeadArgs, stream: int | None) -> None:
 def lmhead_sample_launch(lm: MtrLmHeadArgs, args: MtrSamplerArgs, stream: int | None) -> None:
     check(load().mtr_lmhead_sample_launch(ctypes.byref(lm), ctypes.byref(args), c_void_p(stream or 0)),
           "mtr_lmhead_sample_launch")
+
+
+def sized(cls, **fields):
+    """An argument struct with its identity filled in (``abi_version``, ``struct_size``)."""
+    return cls(abi_version=ABI_VERSION, struct_size=ctypes.sizeof(cls), **fields)
+
+
+def quantize_rows_launch(args: MtrQuantizeArgs, stream: int | None) -> None:
+    check(load().mtr_quantize_rows_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_quantize_rows_launch")
+
+
+def lmhead_i8_workspace(rows: int, d_model: int) -> int:
+    return load().mtr_lmhead_i8_workspace(rows, d_model)
+
+
+def lmhead_i8_launch(args: MtrLmHeadI8Args, stream: int | None) -> None:
+    check(load().mtr_lmhead_i8_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_lmhead_i8_launch")
+
+
+def lmhead_i8_sample_launch(lm: MtrLmHeadI8Args, args: MtrSamplerArgs, stream: int | None) -> None:
+    check(load().mtr_lmhead_i8_sample_launch(ctypes.byref(lm), ctypes.byref(args), c_void_p(stream or 0)),
+          "mtr_lmhead_i8_sample_launch")
+
+
+def logprob_launch(args: MtrLogprobArgs, stream: int | None) -> None:
+    check(load().mtr_logprob_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_logprob_launch")
+
+
+def logprob_grad_launch(args: MtrLogprobGradArgs, stream: int | None) -> None:
+    check(load().mtr_logprob_grad_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_logprob_grad_launch")

@@ -20,8 +20,9 @@ CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmtr_sampler.so"
 SOURCES = [CSRC / "mtr_sampler.cu", CSRC / "mtr_stream.cu", CSRC / "mtr_stream_bf16.cu", CSRC / "mtr_stream_f16.cu",
-           CSRC / "mtr_stream_f32.cu", CSRC / "mtr_lmhead.cu"]
-HEADERS = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh", CSRC / "mtr_stream.cuh"]
+           CSRC / "mtr_stream_f32.cu", CSRC / "mtr_lmhead.cu", CSRC / "mtr_lmhead_i8.cu", CSRC / "mtr_logprob.cu"]
+HEADERS = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh", CSRC / "mtr_stream.cuh",
+           CSRC / "mtr_tc.cuh"]
 BUILD_DIR = PKG_DIR / "_build"
 
 COMPILE_FLAGS = [
@@ -48,10 +49,13 @@ def _nvcc() -> str:
 
 
 def _deps(src: Path) -> list:
-    """Headers a translation unit includes (the stream kernel's also include mtr_stream.cuh)."""
+    """Headers a translation unit includes (the stream kernel's also include mtr_stream.cuh, the
+    projections' mtr_tc.cuh)."""
     deps = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh"]
     if src.name.startswith("mtr_stream"):
         deps.append(CSRC / "mtr_stream.cuh")
+    if src.name.startswith("mtr_lmhead"):
+        deps.append(CSRC / "mtr_tc.cuh")
     return deps
 
 

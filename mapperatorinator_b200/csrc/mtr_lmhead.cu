@@ -34,10 +34,7 @@
 // CTAs exit (no early launch_dependents): admitted during the epilogue, the
 // sampler's CTAs crowded onto the few SMs without a 150 KB projection CTA and
 // the pair took 1.9 us longer.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include "mtr_common.cuh"
+#include "mtr_tc.cuh"
 
 namespace mtr {
 namespace lm {
@@ -45,7 +42,6 @@ namespace lm {
 constexpr int BM = 128;
 constexpr int BK = 64;  // bf16 elements per 128-byte swizzled row
 constexpr int UK = 16;  // K of one tcgen05.mma kind::f16
-constexpr uint64_t WAIT_NS = 200000000ull;  // 200 ms: far beyond any healthy wait
 
 struct Params {
   __nv_bfloat16* out;
@@ -56,57 +52,8 @@ struct Params {
   uint32_t* err;
 };
 
-// ---------------------------------------------------------------- PTX wrappers
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+using namespace tc;
 
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-// Waits for the phase with parity `ph` to complete; false after `budget_ns`
-// nanoseconds (0: a single poll).  The clock is read only every 4096 polls:
-// a healthy hand-off completes long before the first read.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t ph, uint64_t budget_ns) {
-  const uint32_t a = smem_u32(b);
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(ph)
-        : "memory");
-    if (done) return true;
-    if (budget_ns == 0) return false;
-    if ((i & 4095u) == 0u) {
-      const uint64_t t = global_ns();
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > budget_ns) return false;
-    }
-  }
-}
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -114,14 +61,6 @@ __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t adesc, uint64_t
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
       : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major tile with the 128-byte swizzle:
-// rows of 128 bytes, 8-row atoms 1024 bytes apart (stride byte offset), leading
-// byte offset 16 (unused by this layout), descriptor version 1, layout type 2.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) |
-         ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
 
 // Instruction descriptor of kind::f16: fp32 accumulator (bits 4-5 = 1), bf16 A
@@ -288,19 +227,6 @@ __global__ void __launch_bounds__(128, 1)
 }
 
 // ---------------------------------------------------------------- host side
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, []() {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = (PFN_cuTensorMapEncodeTiled_v12000)f;
-  });
-  return fn;
-}
-
 // 2-D bf16 tensor map over a row-major [rows, cols] matrix (cols contiguous),
 // box of BK columns x box_rows rows, 128-byte swizzle, out-of-range rows read 0.
 static bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows) {

@@ -16,6 +16,7 @@ step can be captured in a CUDA graph next to the decoder replay.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Sequence
@@ -23,6 +24,8 @@ from typing import Sequence
 import torch
 
 from . import _native as N
+from .int8_head import Int8Weight, lmhead_i8_args, on_device
+from .scoring import TokenLogprobs, token_logprobs as score_tokens
 
 _TORCH_DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
 
@@ -233,6 +236,12 @@ class FusedSampler:
     lookback bias -> top-k -> top-p -> draw.  Device state per row: last
     time-shift value (monotonic mask), previous token (grammar), unfinished
     flag, previous EOS probability (lookback bias).
+
+    With ``token_logprobs=n`` every step also scores the tokens it emits under the
+    distribution they come from (the processed scores), with that distribution's
+    entropy and n most probable ids: ``self.token_logprobs`` is then the last
+    step's :class:`~mapperatorinator_b200.scoring.TokenLogprobs`, in which rows
+    that had finished before the step (``track_finished``) have log probability 0.
     """
 
     def __init__(self, *, vocab_size: int, num_rows: int, device, cfg_scale: float = 1.0,
@@ -245,7 +254,8 @@ class FusedSampler:
                  top_k: int = 0, top_p: float = 1.0, top_p_mode: str = "hf", do_sample: bool = True,
                  eos_token_ids: Sequence[int] = (), eos_ranges: Sequence[tuple[int, int]] = (),
                  pad_token_id: int = 0, track_finished: bool = False,
-                 return_scores: bool = False, return_logprobs: bool = False, lookback: dict | None = None):
+                 return_scores: bool = False, return_logprobs: bool = False, lookback: dict | None = None,
+                 token_logprobs: int | None = None):
         self.device = torch.device(device)
         self.vocab_size = int(vocab_size)
         self.num_rows = int(num_rows)
@@ -306,7 +316,11 @@ class FusedSampler:
         a.out_ids = self.out_ids.data_ptr()
         a.out_status = self.status.data_ptr()
         self.scores = self.logprobs = None
-        if return_scores:
+        if token_logprobs is not None and not 0 <= int(token_logprobs) <= N.MAX_TOP_N:
+            raise ValueError(f"token_logprobs must be 0 .. {N.MAX_TOP_N} alternatives")
+        self._score_top = None if token_logprobs is None else int(token_logprobs)
+        self.token_logprobs: TokenLogprobs | None = None
+        if return_scores or token_logprobs is not None:
             self.scores = torch.empty((B, V), dtype=torch.float32, device=self.device)
             a.out_scores = self.scores.data_ptr()
             a.out_scores_row_stride = V
@@ -423,36 +437,61 @@ class FusedSampler:
         if self._base.select_mode == N.SELECT_SAMPLE:
             uniforms = _uniforms(self.num_rows, logits.device, uniforms, generator)
         a = self._args(logits, input_ids, uniforms, id_buffer, cur_len)
+        finished = self._finished_before()
         N.launch(a, torch.cuda.current_stream(logits.device).cuda_stream)
+        self._score(finished)
         if input_ids is not None:
             self._scan_next = False
             self._prev_from_ids_next = False
         self._last_uniforms = uniforms  # keep alive until the kernel has consumed them
         return self.out_ids
 
-    def step_hidden(self, hidden: torch.Tensor, weight: torch.Tensor, input_ids: torch.Tensor | None = None,
+    def _finished_before(self) -> torch.Tensor | None:
+        """The rows whose token this step will pad, kept for :meth:`_score`."""
+        if self._score_top is None or not self._base.unfinished:
+            return None
+        return self.unfinished == 0
+
+    def _score(self, finished: torch.Tensor | None) -> None:
+        if self._score_top is None:
+            return
+        ids = self.out_ids if finished is None else self.out_ids.masked_fill(finished, -1)
+        self.token_logprobs = score_tokens(self.scores, ids, top_n=self._score_top)
+
+    def step_hidden(self, hidden: torch.Tensor, weight: torch.Tensor | Int8Weight, input_ids: torch.Tensor | None = None,
                     uniforms: torch.Tensor | None = None, generator: torch.Generator | None = None, *,
                     id_buffer: torch.Tensor | None = None, cur_len=None, tile_n: int = 0) -> torch.Tensor:
         """The decoder's last hidden states to the next tokens: the tensor-core
         output projection (``lm_head_logits``) writes bf16 logits that this
         step's fused kernel reads, launched as its programmatic dependent.
         ``hidden`` has the logits' rows ([2B, d] with CFG).  The logits stay
-        readable in ``self.lm_logits`` until the next call."""
+        readable in ``self.lm_logits`` until the next call.  An
+        :class:`~mapperatorinator_b200.int8_head.Int8Weight` takes the 8-bit
+        projection (``lm_head_logits_int8``) instead."""
         _require_cuda(hidden, "hidden")
+        i8 = isinstance(weight, Int8Weight)
         rows = hidden.shape[0]
         if rows != (2 * self.num_rows if self._base.cfg_enabled else self.num_rows):
             raise ValueError(f"hidden has {rows} rows")
-        if weight.shape[0] != self.vocab_size:
-            raise ValueError(f"weight vocabulary {weight.shape[0]} != {self.vocab_size}")
+        vocab = (weight.q if i8 else weight).shape[0]
+        if vocab != self.vocab_size:
+            raise ValueError(f"weight vocabulary {vocab} != {self.vocab_size}")
         buf = getattr(self, "lm_logits", None)
         if buf is None or buf.shape != (rows, self.vocab_size) or buf.device != hidden.device:
             buf = torch.empty((rows, self.vocab_size), dtype=torch.bfloat16, device=hidden.device)
             self.lm_logits = buf
-        lm = _lmhead_args(hidden, weight, buf, tile_n)
+        if i8:
+            lm, work = lmhead_i8_args(hidden, weight.q, weight.scale, buf)
+        else:
+            lm = _lmhead_args(hidden, weight, buf, tile_n)
         if self._base.select_mode == N.SELECT_SAMPLE:
             uniforms = _uniforms(self.num_rows, hidden.device, uniforms, generator)
         a = self._args(buf, input_ids, uniforms, id_buffer, cur_len)
-        N.lmhead_sample_launch(lm, a, torch.cuda.current_stream(hidden.device).cuda_stream)
+        finished = self._finished_before()
+        with on_device(hidden.device) if i8 else contextlib.nullcontext():
+            (N.lmhead_i8_sample_launch if i8 else N.lmhead_sample_launch)(
+                lm, a, torch.cuda.current_stream(hidden.device).cuda_stream)
+        self._score(finished)
         if input_ids is not None:
             self._scan_next = False
             self._prev_from_ids_next = False
