@@ -307,7 +307,7 @@ int mtr_lmhead_sample_launch(const MtrLmHeadArgs* lm, const MtrSamplerArgs* samp
 /*
  * 8-bit output projection.  Rows of hidden states and of the weight are held
  * as int8 with one fp32 scale per row:
- *   scale[r] = RN32(max_k |x[r, k]| / 127),  q[r, k] = RNE(RN32(x[r, k] / scale[r]))
+ *   scale[r] = RN32(max_k |x[r, k]| * RN32(1 / 127)),  q[r, k] = RNE(RN32(x[r, k] / scale[r]))
  * (q = 0 for a row of zeros, or one so small that its scale rounds to 0; a row
  * with a NaN or an infinity gets scale NaN and q = 0).
  */

@@ -331,6 +331,8 @@ def library_path() -> Path:
 def load(path: str | Path | None = None) -> ctypes.CDLL:
     """Load (once) and check the native library."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -2,7 +2,7 @@
 // sm_100a tensor cores, feeding the fused sampler.
 //
 // Rows of the hidden states and of the weight are held as int8 with one fp32
-// scale each: scale = max|x| / 127, q = round(x / scale), so
+// scale each: scale = max|x| RN(1/127), q = round(x / scale), so
 //   logits[r, v] = (sum_k q_h[r, k] q_w[v, k]) scale_h[r] scale_w[v].
 // The sum is exact: |sum| <= 127 * 128 * d < 2^31 for d <= 131072, and
 // tcgen05.mma kind::i8 accumulates in int32 tensor memory.  Rounding happens
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantPara
   top = tops[0];
   for (int w = 1; w < QUANT_THREADS / 32; ++w) top = max_nan(top, tops[w]);
   const bool finite = top < pos_inf();
-  const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fc00000);
+  const float s = finite ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
   if (tid == 0) p.scale[row] = s;
   for (int k = tid; k < p.cols; k += QUANT_THREADS)
     q[k] = s > 0.0f ? (int8_t)__float2int_rn(__fdiv_rn(to_f(x[k]), s)) : (int8_t)0;

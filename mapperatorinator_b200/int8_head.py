@@ -12,7 +12,6 @@ sums and scales the sums by both: the counterpart of
 
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple
 
 import torch
@@ -22,11 +21,13 @@ from . import _native as N
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
 
 
-def on_device(device: torch.device):
-    """Makes ``device`` the current one for a launch (a no-op when it is already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def launch_on(device: torch.device, launch, *args) -> None:
+    """``launch(*args, stream)`` on ``device``'s current stream, with the device made current for it."""
+    if device.index == torch._C._cuda_getDevice():
+        launch(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            launch(*args, torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def matrix(t: torch.Tensor, what: str, dtypes=_DTYPES) -> int:
@@ -63,8 +64,9 @@ class Int8Weight(NamedTuple):
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """int8 rows and their fp32 scales: ``scale = max|x| / 127`` of each row and
-    ``q = round(x / scale)`` (half to even).  A row of zeros gives zeros and scale
+    """int8 rows and their fp32 scales: ``scale = max|x| * (1 / 127)`` of each
+    row (the reciprocal and the product rounded to fp32) and ``q = round(x /
+    scale)`` (half to even).  A row of zeros gives zeros and scale
     0; a row with a NaN or an infinity gives zeros and scale NaN.  The int8 rows
     start on 16-byte boundaries (``q`` may be a view of wider rows)."""
     stride = matrix(x, "x")
@@ -76,8 +78,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     a = N.sized(N.MtrQuantizeArgs, x=x.data_ptr(), x_row_stride=stride, x_dtype=_DTYPES[x.dtype], rows=rows, cols=cols,
                 q=q.data_ptr(), q_row_stride=wide, scale=scale.data_ptr())
-    with on_device(x.device):
-        N.quantize_rows_launch(a, torch.cuda.current_stream(x.device).cuda_stream)
+    launch_on(x.device, N.quantize_rows_launch, a)
     return q[:, :cols], scale
 
 
@@ -119,6 +120,5 @@ def lm_head_logits_int8(hidden: torch.Tensor, weight_q: torch.Tensor, weight_sca
             raise TypeError(f"out_dtype {out_dtype} is not supported (float32, bfloat16, float16)")
         out = torch.empty((hidden.shape[0], weight_q.shape[0]), dtype=out_dtype, device=hidden.device)
     a, work = lmhead_i8_args(hidden, weight_q, weight_scale, out)
-    with on_device(hidden.device):
-        N.lmhead_i8_launch(a, torch.cuda.current_stream(hidden.device).cuda_stream)
+    launch_on(hidden.device, N.lmhead_i8_launch, a)
     return out

@@ -16,7 +16,6 @@ step can be captured in a CUDA graph next to the decoder replay.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Sequence
@@ -24,7 +23,7 @@ from typing import Sequence
 import torch
 
 from . import _native as N
-from .int8_head import Int8Weight, lmhead_i8_args, on_device
+from .int8_head import Int8Weight, launch_on, lmhead_i8_args
 from .scoring import TokenLogprobs, token_logprobs as score_tokens
 
 _TORCH_DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
@@ -488,9 +487,10 @@ class FusedSampler:
             uniforms = _uniforms(self.num_rows, hidden.device, uniforms, generator)
         a = self._args(buf, input_ids, uniforms, id_buffer, cur_len)
         finished = self._finished_before()
-        with on_device(hidden.device) if i8 else contextlib.nullcontext():
-            (N.lmhead_i8_sample_launch if i8 else N.lmhead_sample_launch)(
-                lm, a, torch.cuda.current_stream(hidden.device).cuda_stream)
+        if i8:
+            launch_on(hidden.device, N.lmhead_i8_sample_launch, lm, a)
+        else:
+            N.lmhead_sample_launch(lm, a, torch.cuda.current_stream(hidden.device).cuda_stream)
         self._score(finished)
         if input_ids is not None:
             self._scan_next = False

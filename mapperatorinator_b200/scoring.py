@@ -17,7 +17,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
-from .int8_head import _DTYPES, _same_device, matrix, on_device
+from .int8_head import _DTYPES, _same_device, launch_on, matrix
 
 
 class TokenLogprobs(NamedTuple):
@@ -56,10 +56,10 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
     if not 0 <= n <= N.MAX_TOP_N:
         raise ValueError(f"top_n must be 0 .. {N.MAX_TOP_N}")
     f32 = torch.float32
-    logprobs = torch.empty(rows, dtype=f32, device=device) if tokens is not None else None
-    entropy = torch.empty(rows, dtype=f32, device=device)
-    lse = torch.empty(rows, dtype=f32, device=device)
     stats = torch.empty((rows, 4), dtype=f32, device=device)
+    entropy, lse, logprobs = torch.empty((3, rows), dtype=f32, device=device).unbind(0)
+    if tokens is None:
+        logprobs = None
     top_ids = torch.empty((rows, n), dtype=torch.int64, device=device)
     top_logprobs = torch.empty((rows, n), dtype=f32, device=device)
     a = N.sized(N.MtrLogprobArgs, logits=logits.data_ptr(), logits_row_stride=stride, logits_dtype=_DTYPES[logits.dtype],
@@ -72,8 +72,7 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
         a.out_top_ids, a.out_top_logprobs = top_ids.data_ptr(), top_logprobs.data_ptr()
     if status is not None:
         a.out_status = status.data_ptr()
-    with on_device(device):
-        N.logprob_launch(a, torch.cuda.current_stream(device).cuda_stream)
+    launch_on(device, N.logprob_launch, a)
     return TokenLogprobs(logprobs, entropy, lse, top_ids, top_logprobs, stats)
 
 
@@ -135,31 +134,32 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
         a.g_lse = gz.data_ptr()
     if n:
         a.top_ids, a.g_top = top_ids.data_ptr(), gt.data_ptr()
-    with on_device(device):
-        N.logprob_grad_launch(a, torch.cuda.current_stream(device).cuda_stream)
+    launch_on(device, N.logprob_grad_launch, a)
     return out
 
 
 class _TokenLogprobs(torch.autograd.Function):
+    """The differentiable outputs; the whole result is left in ``hold``."""
+
     @staticmethod
-    def forward(ctx, logits, tokens, top_n, temperature, status):
+    def forward(ctx, logits, tokens, top_n, temperature, status, hold):
         r = _forward(logits, tokens, top_n, temperature, status)
         ctx.save_for_backward(logits, tokens, r.stats, r.top_ids)
         ctx.temperature = temperature
-        ctx.mark_non_differentiable(r.top_ids, r.stats)
         ctx.set_materialize_grads(False)
-        return tuple(r)
+        hold.append(r)
+        return r.logprobs, r.entropy, r.lse, r.top_logprobs
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprobs, g_entropy, g_lse, _ids, g_top, _stats):
+    def backward(ctx, g_logprobs, g_entropy, g_lse, g_top):
         logits, tokens, stats, top_ids = ctx.saved_tensors
         if g_logprobs is None and g_entropy is None and g_lse is None and g_top is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         saved = TokenLogprobs(None, None, None, top_ids, None, stats)
         grad = token_logprobs_backward(logits, tokens, saved, grad_logprobs=g_logprobs, grad_entropy=g_entropy,
                                        grad_lse=g_lse, grad_top_logprobs=g_top, temperature=ctx.temperature)
-        return grad, None, None, None, None
+        return grad, None, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top_n: int = 0, temperature: float = 1.0,
@@ -184,5 +184,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     flow from ``logprobs``, ``entropy``, ``lse`` and ``top_logprobs`` to the
     logits (once; not through ``top_ids``)."""
     if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_n, temperature, status))
+        hold: list = []
+        logprobs, entropy, lse, top_logprobs = _TokenLogprobs.apply(logits, tokens, top_n, temperature, status, hold)
+        return TokenLogprobs(logprobs, entropy, lse, hold[0].top_ids, top_logprobs, hold[0].stats)
     return _forward(logits, tokens, top_n, temperature, status)

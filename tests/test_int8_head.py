@@ -21,7 +21,7 @@ def plain_quantize(x):
     x = x.float().cpu()
     top = x.abs().amax(1)
     bad = ~torch.isfinite(x).all(1)
-    scale = torch.where(bad, math.nan, top / 127.0)
+    scale = torch.where(bad, math.nan, top * torch.tensor(1 / 127, dtype=torch.float32))
     q = torch.where((scale > 0)[:, None], x / scale[:, None], 0.0)
     return torch.round(q.nan_to_num(0.0)).to(torch.int8), scale
 
