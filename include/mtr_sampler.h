@@ -57,6 +57,7 @@ extern "C" {
 #define MTR_MAX_LB_EOS 8
 #define MTR_MAX_I8_D_MODEL 131072 /* 127 * 128 * 131072 < 2^31: the int32 sums cannot wrap */
 #define MTR_MAX_I8_ROWS (1 << 22)
+#define MTR_MAX_SCORE_ROWS (1 << 27)
 #define MTR_MAX_TOP_N 32
 
 /* Return codes of every entry point. */
@@ -384,7 +385,7 @@ typedef struct MtrLogprobArgs {
   const void* tokens;           /* [rows] ids, or NULL: no tokens */
   int32_t logits_dtype;         /* MtrDType */
   int32_t tokens_dtype;         /* MtrIdType */
-  int32_t rows;
+  int32_t rows;                 /* 0 .. MTR_MAX_SCORE_ROWS */
   int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
   int32_t top_n;                /* 0 .. MTR_MAX_TOP_N */
   float temperature;            /* > 0, finite, with a finite reciprocal */

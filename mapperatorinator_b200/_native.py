@@ -28,6 +28,7 @@ MAX_EOS_RANGES = 2
 MAX_LB_EOS = 8
 MAX_I8_D_MODEL = 131072
 MAX_I8_ROWS = 1 << 22
+MAX_SCORE_ROWS = 1 << 27
 MAX_TOP_N = 32
 
 # MtrStatus

@@ -57,9 +57,9 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
         raise ValueError(f"top_n must be 0 .. {N.MAX_TOP_N}")
     f32 = torch.float32
     stats = torch.empty((rows, 4), dtype=f32, device=device)
-    entropy, lse, logprobs = torch.empty((3, rows), dtype=f32, device=device).unbind(0)
-    if tokens is None:
-        logprobs = None
+    entropy = torch.empty(rows, dtype=f32, device=device)
+    lse = torch.empty(rows, dtype=f32, device=device)
+    logprobs = torch.empty(rows, dtype=f32, device=device) if tokens is not None else None
     top_ids = torch.empty((rows, n), dtype=torch.int64, device=device)
     top_logprobs = torch.empty((rows, n), dtype=f32, device=device)
     a = N.sized(N.MtrLogprobArgs, logits=logits.data_ptr(), logits_row_stride=stride, logits_dtype=_DTYPES[logits.dtype],

@@ -327,10 +327,13 @@ def test_small_entropies_keep_their_digits(cuda_device):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab,stride,offset", [(100, 101, 1), (4096, 4099, 3), (4095, 4095, 5), (20000, 20003, 7)])
+@pytest.mark.parametrize("vocab,stride,offset", [(100, 101, 1), (4096, 4099, 3), (4095, 4095, 5), (20000, 20003, 7), (8193, 8193, 1),
+                                                 (2049, 2049, 0), (4097, 4097, 2)])
 def test_strided_rows_off_any_boundary(cuda_device, dtype, vocab, stride, offset):
     rows = 11
     x, t = inputs(cuda_device, rows, vocab, dtype, seed=5)
+    t[::2] = vocab - 1
+    t[1] = 0
     wide = torch.full((rows * stride + offset,), math.nan, dtype=dtype, device=cuda_device)  # what is not the row's is not read
     view = wide[offset:].as_strided((rows, vocab), (stride, 1))
     view.copy_(x)
