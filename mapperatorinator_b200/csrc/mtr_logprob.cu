@@ -15,15 +15,14 @@
 // HBM as long as a score costs few instructions: 6.5 TB/s feed an SM 12 bf16
 // scores a clock, and its four schedulers issue 128 lanes, so 10 a score are
 // all there are.  Per score: unpack (1), the two packed steps of
-// t = (x - m) (-log2(e) / T) (2 x 1/2), one unsigned minimum, 2^-t (1), and the
-// packed sums of 2^-t and of 2^-t t (2 x 1/2); the maximum is packed too (1/2).
-// The minimum does three things at once: t >= 0 compares as an unsigned word,
-// so masked scores (t = +inf) and far ones become t = 1000, whose 2^-t is 0
-// and whose product with t is 0 as well (inf would give NaN), and a score equal
-// to the maximum, whose t is -0 = 0x80000000, becomes 1000 too and so leaves
-// the sums: it is counted in n.  NaN is found by the maximum, which keeps it.
-#include <stdio.h>
-#include <stdlib.h>
+// d = (x - m) (log2(e) / T) (2 x 1/2), one signed minimum, 2^d (1), and the
+// packed sums of 2^d and of 2^d d (2 x 1/2); the maximum is packed too (1/2).
+// The minimum does three things at once: d <= 0 compares as a signed word from
+// -0 = 0x80000000 up to -inf, so masked scores (d = -inf) and far ones become
+// d = -1000, whose 2^d is 0 and whose product with d is 0 as well (-inf would
+// give NaN), and a score equal to the maximum, whose d is +0 = 0, becomes -1000
+// too and so leaves the sums: it is counted in n.  NaN is found by the maximum,
+// which keeps it.
 #include "mtr_common.cuh"
 
 namespace mtr {
@@ -120,17 +119,17 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int32_t ids32, int64
 struct Part {
   float m;   // -inf: nothing but masked scores so far
   float n;   // logits equal to m (0 while m = -inf)
-  float s;   // sum of 2^-t over the others
-  float u;   // sum of 2^-t t
+  float s;   // sum of 2^d over the others
+  float u;   // sum of 2^d d
 };
 
 __device__ __forceinline__ Part empty_part() { return Part{neg_inf(), 0.0f, 0.0f, 0.0f}; }
 
-// `p` about a larger maximum M: its terms shrink by 2^-g, g = (M - m) scale, and
-// each t grows by g; what equalled m is one of the others now.
+// `p` about a larger maximum M: its terms shrink by 2^g, g = (m - M) scale, and
+// each d falls by |g|; what equalled m is one of the others now.
 __device__ __forceinline__ void move_to(Part& p, float M, float scale) {
   if (p.m > neg_inf()) {
-    const float g = fminf((M - p.m) * scale, 1000.0f), f = ex2(-g), t = p.s + p.n;
+    const float g = fmaxf((p.m - M) * scale, -1000.0f), f = ex2(g), t = p.s + p.n;
     p.s = t * f;
     p.u = fmaf(t, g, p.u) * f;
     p.n = 0.0f;
@@ -172,7 +171,7 @@ __device__ __forceinline__ Row row_of(const Part& p, float inv_t) {
   } else {
     const float rest = p.s + (p.n - 1.0f);
     r.log_s = log1pf(rest);
-    r.entropy = r.log_s + LN2 * p.u / (1.0f + rest);
+    r.entropy = r.log_s - LN2 * p.u / (1.0f + rest);
     r.lse = fmaf(p.m, inv_t, r.log_s);
   }
   return r;
@@ -281,26 +280,67 @@ __device__ __forceinline__ float warp_sort_desc(float v, int lane) {
 
 constexpr int MAX_WARPS = 8;
 constexpr int MAX_CLUSTER = 8;
-constexpr int LIST = 512;  // candidates of a row's alternatives
 
+template <int W>
 struct Shared {
-  Part part[MAX_WARPS];
-  float nth[MAX_WARPS], rth[MAX_WARPS];
+  static constexpr int LIST = 64 * (W + 1);  // candidates of a row's alternatives
+  u64 list[LIST];
+  u64 best[MTR_MAX_TOP_N];  // a cluster CTA's own n largest
+  u64 bound[2];
+  // by the row's parity: a warp may be a row ahead of another
+  Part part[2][W];
+  float nth[2][W], rth[2][W];
+  int count[2];     // candidates found (where they pass LIST, the list is not complete)
   Part cta;         // read by the cluster's other CTAs
   float cta_nth, cta_rth;
-  int count;        // candidates listed (may pass LIST: then the list is not complete)
-  uint8_t winner[MAX_WARPS][32];
-  u64 key[MAX_WARPS];
-  u64 list[LIST];
+  uint16_t found[W][128];
+  uint8_t winner[W][32];
 };
 
-// One row per CTA, or per cluster of CTAs, of up to 8 warps.
+// A row as one CTA sees it: single logits before the first 16-byte boundary
+// and behind the last, and the CTA's run [v0, v1) of the vectors between.
+template <typename T>
+struct Span {
+  const T* x;
+  int head, vecs, v0, v1;
+  __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head); }
+};
+template <typename T>
+__device__ __forceinline__ Span<T> span_of(const FwdParams& p, int64_t row, int rank) {
+  constexpr int E = Vec<T>::E;
+  Span<T> r;
+  r.x = (const T*)p.logits + row * p.stride;
+  const int off = (int)(((uintptr_t)r.x & 15u) / sizeof(T));
+  r.head = min(off ? E - off : 0, p.vocab);
+  r.vecs = (p.vocab - r.head) / E;
+  const int run = p.cluster > 1 ? (r.vecs + p.cluster - 1) / p.cluster : r.vecs;
+  r.v0 = min(rank * run, r.vecs);
+  r.v1 = min(r.v0 + run, r.vecs);
+  return r;
+}
+
+constexpr int TILE = 8;  // vectors of a thread's tile
+
+// tile starting at vector t0 of the CTA's run; masked scores behind its end
+template <typename T, int THREADS>
+__device__ __forceinline__ void load_tile(uint4 (&w)[TILE], const Span<T>& r, int t0, int tid) {
+  const uint4* b = r.body() + t0 + tid;
+  if (t0 + THREADS * TILE <= r.v1) {
+#pragma unroll
+    for (int j = 0; j < TILE; ++j) w[j] = b[j * THREADS];
+  } else {
+    constexpr uint32_t F = Vec<T>::FILL;
+#pragma unroll
+    for (int j = 0; j < TILE; ++j) w[j] = t0 + tid + j * THREADS < r.v1 ? b[j * THREADS] : make_uint4(F, F, F, F);
+  }
+}
+
+// A CTA of W warps takes one row after another (a cluster of CTAs takes one).
 //
-// The row is its 16-byte vectors, dealt to the CTAs in runs and to the threads
-// in turn, and up to 2 (E - 1) logits before the first boundary and behind the
-// last, which are lanes' single scores of the first warp.  A thread has TV
-// vectors in flight; a warp keeps one maximum (one redux for each tile of TV
-// vectors), so that its lanes' sums move to a new maximum together and rarely.
+// A thread's tile is TILE vectors; the next tile, of this row or of the CTA's
+// next one, is under way while one is summed.  A warp keeps one maximum (one
+// redux a tile), so that its lanes' sums move to a new maximum together and
+// rarely.
 //
 // Alternatives: with lm the lanes' maxima, any T with at least n logits >= T
 // bounds the n largest from below.  Two such T are at hand: the n-th largest lm
@@ -308,259 +348,292 @@ struct Shared {
 // largest lm, r n-th part of the warps (n <= r warps).  The larger of the two
 // leaves about n to 3 n lanes with lm >= T, whose vectors are read again (from
 // L2) for the list of candidates, which are ranked by comparing all pairs.  A
-// list that overflows (many equal logits) falls back to one pass for each
-// alternative.
-template <typename T, int TV>
-__global__ void __launch_bounds__(MAX_WARPS * 32, 2) logprob_kernel(const FwdParams p) {
+// list that overflows (many equal logits) still holds more than n candidates:
+// the n-th of them is a better T, and the candidates are looked for again.
+template <typename T, int W>
+__global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams p) {
   typedef Vec<T> X;
-  constexpr int E = X::E;
-  __shared__ Shared sh;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = blockDim.x, warps = threads >> 5;
+  constexpr int E = X::E, THREADS = W * 32;
+  __shared__ Shared<W> sh;
+  constexpr int LIST = Shared<W>::LIST;
+  const int tid = threadIdx.x, warp = W > 1 ? tid >> 5 : 0, lane = tid & 31;
   const int cs = p.cluster, rank = cs > 1 ? (int)(blockIdx.x % cs) : 0;
-  const int64_t row = cs > 1 ? blockIdx.x / cs : blockIdx.x;
-  const int V = p.vocab;
+  const int64_t step = cs > 1 ? gridDim.x / cs : gridDim.x;
+  int64_t row = cs > 1 ? blockIdx.x / cs : blockIdx.x;
+  const int V = p.vocab, n = p.top_n;
   const float scale = p.scale;
-  if (tid == 0) sh.count = 0;
+  auto cta_sync = [&]() {
+    if (W > 1) __syncthreads();
+    else __syncwarp();
+  };
+  if (tid < 2) sh.count[tid] = 0;
   wait_prior_grid();
-  const T* x = (const T*)p.logits + row * p.stride;
-  // the token and its logit, needed last, are asked for first
-  int64_t token = -1;
-  float token_x = 0.0f;
-  if (tid == 0 && rank == 0 && p.tokens) {
-    token = load_id(p.tokens, p.ids32, row);
-    if (token >= 0 && token < V) token_x = to_f(x[token]);
-  }
-  const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
-  const int head = min(off ? E - off : 0, V), vecs = (V - head) / E, tail = V - head - vecs * E;
-  const uint4* body = reinterpret_cast<const uint4*>(x + head);
-  const int run = (vecs + cs - 1) / cs, v0 = min(rank * run, vecs), v1 = min(v0 + run, vecs);
+  Span<T> sp = span_of<T>(p, row, rank);
+  uint4 next[TILE];
+  load_tile<T, THREADS>(next, sp, sp.v0, tid);
 
-  Part a = empty_part();
-  float lm = neg_inf();  // the lane's largest logit
-  // the single scores: lanes 0 .. head - 1 and 16 .. 16 + tail - 1
-  float single = neg_inf();
-  int single_id = -1;
-  if (warp == 0 && rank == 0) {
-    if (lane < head) single_id = lane;
-    else if (lane >= 16 && lane < 16 + tail) single_id = V - tail + lane - 16;
-    if (single_id >= 0) single = to_f(x[single_id]);
-  }
-  bool bad = false;
-  if (warp == 0 && rank == 0 && head + tail > 0) {
-    const float top = warp_max_nan(single);
-    bad = !(top < pos_inf());
-    if (!bad && top > neg_inf()) {
-      a.m = top;
-      if (single == top) a.n = 1.0f;
-      else if (single > neg_inf()) {
-        const float t = fminf((top - single) * scale, 1000.0f);
-        a.s = ex2(-t);
-        a.u = a.s * t;
+  for (int parity = 0; row < p.rows; row += step, parity ^= 1) {
+    // the token and its logit, needed last, are asked for first
+    int64_t token = -1;
+    float token_x = 0.0f;
+    if (tid == 0 && rank == 0 && p.tokens) {
+      token = load_id(p.tokens, p.ids32, row);
+      if (token >= 0 && token < V) token_x = to_f(sp.x[token]);
+    }
+    const int tail = V - sp.head - sp.vecs * E;
+    Part a = empty_part();
+    float lm = neg_inf();  // the lane's largest logit
+    bool bad = false;
+    // the single scores: lanes 0 .. head - 1 and 16 .. 16 + tail - 1 of the first warp
+    float single = neg_inf();
+    int single_id = -1;
+    if (warp == 0 && rank == 0 && sp.head + tail > 0) {
+      if (lane < sp.head) single_id = lane;
+      else if (lane >= 16 && lane < 16 + tail) single_id = V - tail + lane - 16;
+      if (single_id >= 0) single = to_f(sp.x[single_id]);
+      const float top = warp_max_nan(single);
+      bad = !(top < pos_inf());
+      if (!bad && top > neg_inf()) {
+        a.m = top;
+        if (single == top) a.n = 1.0f;
+        else if (single > neg_inf()) {
+          const float d = fmaxf((single - top) * scale, -1000.0f);
+          a.s = ex2(d);
+          a.u = a.s * d;
+        }
+        lm = single;
       }
-      lm = single;
     }
-  }
-  u64 s2 = 0, u2 = 0;  // pairs of partial sums, added to a.s, a.u when the maximum moves
-  for (int t0 = v0; t0 < v1; t0 += threads * TV) {
-    uint4 w[TV];
-    typename X::Top top[TV];
+    Span<T> after = sp;
+    u64 s2 = 0, u2 = 0;  // pairs of partial sums, added to a.s, a.u when the maximum moves
+    auto sum_tile = [&](const uint4 (&w)[TILE]) {
+      typename X::Top top[TILE];
 #pragma unroll
-    for (int j = 0; j < TV; ++j) {
-      const int i = t0 + j * threads + tid;
-      w[j] = i < v1 ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+      for (int j = 0; j < TILE; ++j) top[j] = X::top(w[j]);
+      typename X::Top all = top[0];
+#pragma unroll
+      for (int j = 1; j < TILE; ++j) all = X::larger(all, top[j]);
+      const float mine = X::value(all), most = warp_max_nan(mine);
+      if (!(most < pos_inf())) bad = true;
+      lm = fmaxf(lm, mine);
+      if (most > a.m) {
+        float lo, hi;
+        up2(s2, lo, hi);
+        a.s += lo + hi;
+        up2(u2, lo, hi);
+        a.u += lo + hi;
+        s2 = u2 = 0;
+        move_to(a, most, scale);
+      }
+      if (bad || !(a.m > neg_inf())) return;
+      if (mine == a.m) {
+        const typename X::Top m = X::pattern(a.m);
+#pragma unroll
+        for (int j = 0; j < TILE; ++j)
+          if (X::has(top[j], m)) {
+            float f[E];
+            X::unpack(w[j], f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) a.n += f[e] == a.m ? 1.0f : 0.0f;
+          }
+      }
+      const float nm = 0.0f - a.m;  // +0 for both zeros, so that equal scores differ by +0
+      const u64 nm2 = pk2(nm, nm), sc2 = pk2(scale, scale);
+#pragma unroll
+      for (int j = 0; j < TILE; ++j) {
+        float f[E];
+        X::unpack(w[j], f);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          float d0, d1;
+          up2(mul2(add2(pk2(f[e], f[e + 1]), nm2), sc2), d0, d1);
+          d0 = __int_as_float(min(__float_as_int(d0), (int)0xc47a0000));  // -1000
+          d1 = __int_as_float(min(__float_as_int(d1), (int)0xc47a0000));
+          const u64 e2 = pk2(ex2(d0), ex2(d1));
+          s2 = add2(s2, e2);
+          u2 = fma2(e2, pk2(d0, d1), u2);
+        }
+      }
+    };
+    // the tile behind the one at t0 - THREADS TILE: this row's, or the next row's first
+    auto ask = [&](uint4 (&w)[TILE], int t0) {
+      if (t0 < sp.v1) {
+        load_tile<T, THREADS>(w, sp, t0, tid);
+      } else if (row + step < p.rows) {
+        after = span_of<T>(p, row + step, rank);
+        load_tile<T, THREADS>(w, after, after.v0, tid);
+      }
+    };
+    for (int t0 = sp.v0 + THREADS * TILE;; t0 += THREADS * TILE) {
+      uint4 w[TILE];
+#pragma unroll
+      for (int j = 0; j < TILE; ++j) w[j] = next[j];
+      ask(next, t0);
+      sum_tile(w);
+      if (t0 >= sp.v1) break;
     }
-#pragma unroll
-    for (int j = 0; j < TV; ++j) top[j] = X::top(w[j]);
-    typename X::Top all = top[0];
-#pragma unroll
-    for (int j = 1; j < TV; ++j) all = X::larger(all, top[j]);
-    const float mine = X::value(all), most = warp_max_nan(mine);
-    if (!(most < pos_inf())) bad = true;
-    lm = fmaxf(lm, mine);
-    if (most > a.m) {
+    {
       float lo, hi;
       up2(s2, lo, hi);
       a.s += lo + hi;
       up2(u2, lo, hi);
       a.u += lo + hi;
-      s2 = u2 = 0;
-      move_to(a, most, scale);
     }
-    if (bad || !(a.m > neg_inf())) continue;
-    if (mine == a.m) {
-      const typename X::Top m = X::pattern(a.m);
+    a.n = warp_sum(a.n);
+    a.s = warp_sum(a.s);
+    a.u = warp_sum(a.u);
+    if (bad) a = Part{neg_inf(), 0.0f, qnan(), 0.0f};
+
+    // join the warps, then the CTAs
+    float nth = neg_inf(), rth = neg_inf();
+    if (n > 0) {
+      const float sorted = warp_sort_desc(lm, lane);
+      nth = __shfl_sync(FULL, sorted, n - 1);
+      rth = __shfl_sync(FULL, sorted, (n + W * cs - 1) / (W * cs) - 1);
+    }
+    if (W > 1) {
+      if (lane == 0) {
+        sh.part[parity][warp] = a;
+        sh.nth[parity][warp] = nth;
+        sh.rth[parity][warp] = rth;
+      }
+      __syncthreads();
+      // every group of W lanes joins the W parts
+      a = lanes_join(sh.part[parity][lane % W], W, scale);
+      nth = sh.nth[parity][lane % W];
+      rth = sh.rth[parity][lane % W];
 #pragma unroll
-      for (int j = 0; j < TV; ++j)
-        if (X::has(top[j], m)) {
-          float f[E];
-          X::unpack(w[j], f);
+      for (int o = 1; o < W; o <<= 1) {
+        nth = fmaxf(nth, __shfl_xor_sync(FULL, nth, o));
+        rth = fminf(rth, __shfl_xor_sync(FULL, rth, o));
+      }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (cs > 1) {
+      if (tid == 0) {
+        sh.cta = a;
+        sh.cta_nth = nth;
+        sh.cta_rth = rth;
+      }
+      cluster.sync();
+      const Shared<W>* other = cluster.map_shared_rank(&sh, lane % cs);
+      a = lanes_join(other->cta, cs, scale);
+      nth = other->cta_nth;
+      rth = other->cta_rth;
+      for (int o = 1; o < cs; o <<= 1) {
+        nth = fmaxf(nth, __shfl_xor_sync(FULL, nth, o));
+        rth = fminf(rth, __shfl_xor_sync(FULL, rth, o));
+      }
+    }
+    const Row r = row_of(a, p.inv_t);
+    if (tid == 0 && rank == 0) {
+      uint32_t st = r.bad ? MTR_ROW_NONFINITE : r.none ? MTR_ROW_ALL_MASKED : 0u;
+      if (p.tokens) {
+        if (token >= V) st |= MTR_ROW_BAD_ID;
+        if (p.logprobs) p.logprobs[row] = (token < 0 || token >= V) ? 0.0f : log_prob(token_x, r, p.inv_t);
+      }
+      if (p.entropy) p.entropy[row] = r.entropy;
+      if (p.lse) p.lse[row] = r.lse;
+      if (p.stats) p.stats[row] = make_float4(r.m, r.log_s, r.entropy, 0.0f);
+      if (p.status) p.status[row] = st;
+    }
+    if (n == 0) {
+      if (cs > 1) cluster.sync();  // this CTA's parts have been read
+      sp = after;
+      continue;
+    }
+
+    // candidates: keys of the scores that reach the bound
+    u64 bound = order_key(fmaxf(nth, rth), 0xffffffffu);
+    int c = 0;
+    if (tid == 0) sh.count[parity ^ 1] = 0;
+    auto list = [&](float f, int id) {
+      const u64 k = order_key(f, (uint32_t)id);
+      const bool hit = k >= bound && f > neg_inf();
+      const unsigned hits = __ballot_sync(FULL, hit);
+      if (hits == 0) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sh.count[parity], __popc(hits));
+      at = __shfl_sync(FULL, at, 0) + __popc(hits & ((1u << lane) - 1u));
+      if (hit && at < LIST) sh.list[at] = k;
+    };
+    while (!r.bad && !r.none) {
+      const float least = key_value(bound);
+      if (warp == 0 && rank == 0 && sp.head + tail > 0) list(single, single_id);
+      const bool won = lm >= least && lm > neg_inf();
+      const unsigned winners = __ballot_sync(FULL, won);
+      if (won) sh.winner[warp][__popc(winners & ((1u << lane) - 1u))] = (uint8_t)lane;
+      __syncwarp();
+      // a half warp reads one winner's vectors, 16 at a time, for four winners in turn
+      const uint4* body = sp.body();
+      const int most_of = (sp.v1 - sp.v0 - warp * 32 + THREADS - 1) / THREADS;  // vectors of the warp's first lane
+      const int count = __popc(winners);
+      for (int first = 0; first < count; first += 8)
+        for (int i0 = 0; i0 < most_of; i0 += 16) {
+          uint4 w[4];
+          int at[4];
 #pragma unroll
-          for (int e = 0; e < E; ++e) a.n += f[e] == a.m ? 1.0f : 0.0f;
+          for (int j = 0; j < 4; ++j) {
+            const int who = first + 2 * j + (lane >> 4), i = i0 + (lane & 15);
+            at[j] = who < count ? sp.v0 + warp * 32 + sh.winner[warp][who] + i * THREADS : sp.v1;
+            w[j] = at[j] < sp.v1 ? body[at[j]] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+          }
+          int found = 0;  // vectors that hold a candidate
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float most = X::value(X::top(w[j]));
+            const bool hit = most >= least && most > neg_inf();
+            const unsigned hits = __ballot_sync(FULL, hit);
+            if (hit) sh.found[warp][found + __popc(hits & ((1u << lane) - 1u))] = (uint16_t)at[j];
+            found += __popc(hits);
+          }
+          __syncwarp();
+          for (int k = 0; k < found * E; k += 32) {  // their scores, one a lane
+            const int slot = (k + lane) / E, id = slot < found ? sp.head + sh.found[warp][slot] * E + lane % E : -1;
+            list(id >= 0 ? to_f(sp.x[id]) : neg_inf(), id);
+          }
+          __syncwarp();
         }
-    }
-    const float nm = 0.0f - a.m;  // +0 for both zeros, so that equal scores differ by +0
-    const u64 nm2 = pk2(nm, nm), ns2 = pk2(-scale, -scale);
-#pragma unroll
-    for (int j = 0; j < TV; ++j) {
-      float f[E];
-      X::unpack(w[j], f);
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        float t0f, t1f;
-        up2(mul2(add2(pk2(f[e], f[e + 1]), nm2), ns2), t0f, t1f);
-        t0f = __uint_as_float(min(__float_as_uint(t0f), 0x447a0000u));  // 1000
-        t1f = __uint_as_float(min(__float_as_uint(t1f), 0x447a0000u));
-        const u64 e2 = pk2(ex2(-t0f), ex2(-t1f));
-        s2 = add2(s2, e2);
-        u2 = fma2(e2, pk2(t0f, t1f), u2);
+      cta_sync();
+      c = sh.count[parity];
+      if (c <= LIST) break;
+      // overflow: the list's n-th key is the new bound (LIST > n, so the count falls)
+      for (int i = tid; i < LIST; i += THREADS) {
+        const u64 k = sh.list[i];
+        int place = 0;
+        for (int j = 0; j < LIST; ++j) place += sh.list[j] > k;
+        if (place == n - 1) sh.bound[parity] = k;
       }
+      cta_sync();
+      bound = sh.bound[parity];
+      if (tid == 0) sh.count[parity] = 0;
+      cta_sync();
     }
-  }
-  {
-    float lo, hi;
-    up2(s2, lo, hi);
-    a.s += lo + hi;
-    up2(u2, lo, hi);
-    a.u += lo + hi;
-  }
-  a.n = warp_sum(a.n);
-  a.s = warp_sum(a.s);
-  a.u = warp_sum(a.u);
-  if (bad) a = Part{neg_inf(), 0.0f, qnan(), 0.0f};
-
-  // join the warps, then the CTAs
-  const int n = p.top_n;
-  float nth = neg_inf(), rth = neg_inf();
-  if (n > 0) {
-    const float sorted = warp_sort_desc(lm, lane);
-    nth = __shfl_sync(FULL, sorted, n - 1);
-    rth = __shfl_sync(FULL, sorted, (n + warps * cs - 1) / (warps * cs) - 1);
-  }
-  if (warps > 1) {
-    if (lane == 0) {
-      sh.part[warp] = a;
-      sh.nth[warp] = nth;
-      sh.rth[warp] = rth;
-    }
-    __syncthreads();
-    const int width = MAX_WARPS;
-    a = lane < warps ? sh.part[lane] : empty_part();
-    a = lanes_join(a, width, scale);
-    nth = lane < warps ? sh.nth[lane] : neg_inf();
-    rth = lane < warps ? sh.rth[lane] : pos_inf();
-#pragma unroll
-    for (int o = 1; o < MAX_WARPS; o <<= 1) {
-      nth = fmaxf(nth, __shfl_xor_sync(FULL, nth, o));
-      rth = fminf(rth, __shfl_xor_sync(FULL, rth, o));
-    }
-    // lanes 8 .. 31 joined empty parts: lane 0 has the CTA's
-    a = Part{__shfl_sync(FULL, a.m, 0), __shfl_sync(FULL, a.n, 0), __shfl_sync(FULL, a.s, 0), __shfl_sync(FULL, a.u, 0)};
-    nth = __shfl_sync(FULL, nth, 0);
-    rth = __shfl_sync(FULL, rth, 0);
-  } else {
-    __syncwarp();  // sh.count = 0 before the first candidate
-  }
-  cg::cluster_group cluster = cg::this_cluster();
-  if (cs > 1) {
-    if (tid == 0) {
-      sh.cta = a;
-      sh.cta_nth = nth;
-      sh.cta_rth = rth;
-    }
-    cluster.sync();
-    Part q = empty_part();
-    float qn = neg_inf(), qr = pos_inf();
-    if (lane < cs) {
-      const Shared* other = cluster.map_shared_rank(&sh, lane);
-      q = other->cta;
-      qn = other->cta_nth;
-      qr = other->cta_rth;
-    }
-    a = lanes_join(q, MAX_CLUSTER, scale);
-#pragma unroll
-    for (int o = 1; o < MAX_CLUSTER; o <<= 1) {
-      qn = fmaxf(qn, __shfl_xor_sync(FULL, qn, o));
-      qr = fminf(qr, __shfl_xor_sync(FULL, qr, o));
-    }
-    a = Part{__shfl_sync(FULL, a.m, 0), __shfl_sync(FULL, a.n, 0), __shfl_sync(FULL, a.s, 0), __shfl_sync(FULL, a.u, 0)};
-    nth = __shfl_sync(FULL, qn, 0);
-    rth = __shfl_sync(FULL, qr, 0);
-  }
-  const Row r = row_of(a, p.inv_t);
-  if (tid == 0 && rank == 0) {
-    uint32_t st = r.bad ? MTR_ROW_NONFINITE : r.none ? MTR_ROW_ALL_MASKED : 0u;
-    if (p.tokens) {
-      if (token >= V) st |= MTR_ROW_BAD_ID;
-      if (p.logprobs) p.logprobs[row] = (token < 0 || token >= V) ? 0.0f : log_prob(token_x, r, p.inv_t);
-    }
-    if (p.entropy) p.entropy[row] = r.entropy;
-    if (p.lse) p.lse[row] = r.lse;
-    if (p.stats) p.stats[row] = make_float4(r.m, r.log_s, r.entropy, 0.0f);
-    if (p.status) p.status[row] = st;
-  }
-  if (n == 0) {
-    if (cs > 1) cluster.sync();  // this CTA's parts have been read
-    return;
-  }
-
-  // candidates
-  const float bound = fmaxf(nth, rth);
-  auto push = [&](float f, int id) {
-    const int at = atomicAdd(&sh.count, 1);
-    if (at < LIST) sh.list[at] = order_key(f, (uint32_t)id);
-  };
-  if (!r.bad && !r.none) {
-    if (single >= bound && single > neg_inf()) push(single, single_id);
-    // the winners' vectors, dealt to the lanes in turn, four loads in flight each
-    const bool won = lm >= bound && lm > neg_inf();
-    const unsigned winners = __ballot_sync(FULL, won);
-    if (won) sh.winner[warp][__popc(winners & ((1u << lane) - 1u))] = (uint8_t)lane;
-    __syncwarp();
-    const int each = (v1 - v0 - warp * 32 + threads - 1) / threads;  // vectors of the warp's first lane
-    const int all = each > 0 ? __popc(winners) * each : 0;
-    for (int base = 0; base < all; base += 128) {
-      uint4 w[4];
-      int at[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = base + j * 32 + lane, who = k / each;
-        at[j] = k < all ? v0 + warp * 32 + sh.winner[warp][who] + (k - who * each) * threads : v1;
-        w[j] = at[j] < v1 ? body[at[j]] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+    if (cs > 1) {
+      // the CTAs' own n largest, ranked by the first CTA
+      for (int i = tid; i < c; i += THREADS) {
+        const u64 k = sh.list[i];
+        int place = 0;
+        for (int j = 0; j < c; ++j) place += sh.list[j] > k;
+        if (place < n) sh.best[place] = k;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float most = X::value(X::top(w[j]));
-        if (most >= bound && most > neg_inf()) {
-          float f[E];
-          X::unpack(w[j], f);
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (f[e] >= bound && f[e] > neg_inf()) push(f[e], head + at[j] * E + e);
+      if (tid == 0) sh.count[parity] = min(c, n);
+      cluster.sync();
+      if (rank == 0) {
+        c = 0;
+        for (int k = 0; k < cs; ++k) {
+          const Shared<W>* other = cluster.map_shared_rank(&sh, k);
+          const int more = other->count[parity];
+          for (int i = tid; i < more; i += THREADS) sh.list[c + i] = other->best[i];
+          c += more;
         }
       }
+      cluster.sync();  // the others' keys have been read
+      if (rank != 0) return;
     }
-  }
-  __syncthreads();
-  int c = sh.count;
-  if (cs > 1) {
-    cluster.sync();
-    if (rank == 0 && c <= LIST) {
-      for (int k = 1; k < cs && c <= LIST; ++k) {
-        const Shared* other = cluster.map_shared_rank(&sh, k);
-        const int more = other->count;
-        if (c + more <= LIST)
-          for (int i = tid; i < more; i += threads) sh.list[c + i] = other->list[i];
-        c += more;
-      }
-    }
-    __syncthreads();
-    cluster.sync();  // the others' lists have been read
-    if (rank != 0) return;
-  }
-  int64_t* ids = p.top_ids + row * n;
-  float* lps = p.top_logprobs + row * n;
-  if (c <= LIST) {
-    for (int i = tid; i < c; i += threads) {
+    int64_t* ids = p.top_ids + row * n;
+    float* lps = p.top_logprobs + row * n;
+    for (int i = tid; i < c; i += THREADS) {
       const u64 k = sh.list[i];
       int place = 0;
       for (int j = 0; j < c; ++j) place += sh.list[j] > k;
@@ -569,36 +642,12 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) logprob_kernel(const FwdPar
         lps[place] = log_prob(key_value(k), r, p.inv_t);
       }
     }
-    for (int j = c + tid; j < n; j += threads) {
+    for (int j = c + tid; j < n; j += THREADS) {
       ids[j] = -1;
       lps[j] = r.bad ? qnan() : neg_inf();
     }
-    return;
-  }
-  // the list overflowed: the largest key below the last one, n times
-  u64 last = ~0ull;
-  for (int j = 0; j < n; ++j) {
-    u64 best = 0;
-    if (last)
-      for (int v = tid; v < V; v += threads) {
-        const float f = to_f(x[v]);
-        const u64 k = f > neg_inf() ? order_key(f, (uint32_t)v) : 0;
-        if (k < last && k > best) best = k;
-      }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const u64 q = __shfl_xor_sync(FULL, best, o);
-      best = q > best ? q : best;
-    }
-    if (lane == 0) sh.key[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < warps; ++w) best = sh.key[w] > best ? sh.key[w] : best;
-    __syncthreads();
-    if (tid == 0) {
-      ids[j] = best ? key_id(best) : -1;
-      lps[j] = best ? log_prob(key_value(best), r, p.inv_t) : neg_inf();
-    }
-    last = best;
+    if (W == 1) __syncwarp();  // the list has been read before the next row's candidates
+    sp = after;
   }
 }
 
@@ -759,21 +808,48 @@ static cudaError_t launch(K kern, const P& p, dim3 grid, int threads, int cluste
 
 static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
 
-constexpr int TILE = 16;
-
-// Warps and CTAs of a row.
+// Warps and CTAs of a row, by how many rows there are to fill the device's 16
+// warps an SM and how long they are.  Measured (us, 148 SMs):
+//   8192 x 4096 bf16      1 warp 18.0, 2 23.0, 4 44.6     enough rows: a warp each
+//   2000 x 65533 bf16     1 warp 50.4, 2 52.6, 4 48.1, 8 57.3   long rows: 4
+//   1024 x 131072 fp32    1 warp 99.1, 2 81.7, 4 80.8, 8 83.6
+//   256 x 65536 fp16      1 warp 24.6, 4 11.4, 8 10.6, 4 CTAs of 8 25.8
+//   64 x 4096 fp32, n = 5 1 warp 5.4, 4 4.2, 8 4.5        256 vectors a warp at least
+//   1 x 131072 fp32       8 warps 14.7, 4 CTAs of 8 9.8, 8 CTAs 9.7
+// More warps than the rows need cost their joins; clusters pay only where they
+// give idle SMs work.
 struct Shape {
-  int threads, cluster;
+  int warps, cluster;
 };
 static Shape shape_for(int64_t rows, int vocab, int es) {
   const int64_t vecs = ((int64_t)vocab * es + 15) / 16, sms = device_sms();
-  const char* ov = getenv("LPSHAPE");
-  if (ov) { int w, c; sscanf(ov, "%d,%d", &w, &c); return {32 * w, c}; }
-  int warps = 1;
-  while (warps < MAX_WARPS && (vecs > 32ll * TILE * warps || (rows * warps < 16 * sms && vecs > 128 * warps))) warps *= 2;
-  int cluster = 1;
-  while (cluster < MAX_CLUSTER && vecs > 4096ll * cluster) cluster *= 2;
-  return {32 * warps, cluster};
+  int warps = vecs >= 4096 ? 4 : 1;
+  while (warps < MAX_WARPS && rows * warps < 16 * sms && vecs > 256 * warps) warps *= 2;
+  int cluster = 1;  // only of 8 warps: MAX_CLUSTER * MTR_MAX_TOP_N keys must fit the list
+  while (warps == MAX_WARPS && cluster < MAX_CLUSTER && vecs > 2048ll * cluster && rows * cluster < sms) cluster *= 2;
+  return {warps, cluster};
+}
+
+template <typename T, int W>
+static cudaError_t launch_fwd(FwdParams p, int cluster, cudaStream_t s) {
+  auto kern = logprob_kernel<T, W>;
+  p.cluster = cluster;
+  if (cluster > 1) return launch(kern, p, dim3((unsigned)(p.rows * cluster), 1, 1), 32 * W, cluster, s);
+  int occ = 0;
+  const cudaError_t e = cached_occupancy((const void*)kern, 32 * W, 0, &occ);
+  if (e != cudaSuccess) return e;
+  const int64_t room = (int64_t)(occ > 0 ? occ : 1) * device_sms();
+  return launch(kern, p, dim3((unsigned)(p.rows < room ? p.rows : room), 1, 1), 32 * W, 1, s);
+}
+template <typename T>
+static cudaError_t launch_fwd(const FwdParams& p, cudaStream_t s) {
+  const Shape g = shape_for(p.rows, p.vocab, sizeof(T));
+  switch (g.warps) {
+    case 1: return launch_fwd<T, 1>(p, g.cluster, s);
+    case 2: return launch_fwd<T, 2>(p, g.cluster, s);
+    case 4: return launch_fwd<T, 4>(p, g.cluster, s);
+    default: return launch_fwd<T, 8>(p, g.cluster, s);
+  }
 }
 
 template <typename T>
@@ -852,16 +928,13 @@ int mtr_logprob_launch(const MtrLogprobArgs* a, void* stream) {
   p.top_logprobs = a->out_top_logprobs;
   p.stats = (float4*)a->out_stats;
   p.status = a->out_status;
-  const Shape g = shape_for(p.rows, p.vocab, esize(a->logits_dtype));
-  p.cluster = g.cluster;
+  p.cluster = 1;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
-  const dim3 grid((unsigned)(p.rows * g.cluster), 1, 1);
   switch (a->logits_dtype) {
-    case MTR_DTYPE_F32: e = launch(logprob_kernel<float, TILE>, p, grid, g.threads, g.cluster, s); break;
-    case MTR_DTYPE_BF16: { const char* tv = getenv("LPTV"); int t = tv ? atoi(tv) : TILE;
-      e = t == 4 ? launch(logprob_kernel<__nv_bfloat16, 4>, p, grid, g.threads, g.cluster, s) : t == 8 ? launch(logprob_kernel<__nv_bfloat16, 8>, p, grid, g.threads, g.cluster, s) : launch(logprob_kernel<__nv_bfloat16, TILE>, p, grid, g.threads, g.cluster, s); break; }
-    default: e = launch(logprob_kernel<__half, TILE>, p, grid, g.threads, g.cluster, s); break;
+    case MTR_DTYPE_F32: e = launch_fwd<float>(p, s); break;
+    case MTR_DTYPE_BF16: e = launch_fwd<__nv_bfloat16>(p, s); break;
+    default: e = launch_fwd<__half>(p, s); break;
   }
   mtr::set_last_cuda_error((int)e);
   return e == cudaSuccess ? MTR_OK : MTR_ERR_CUDA;
