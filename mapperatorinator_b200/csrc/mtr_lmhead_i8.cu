@@ -9,26 +9,29 @@
 // three times, each to fp32 or wider than the result: float(sum) (24 of at most
 // 31 bits), the product with scale_h and the one with scale_w; then once more
 // to the logits' type.
+#include <stdlib.h>
+
+#include <type_traits>
+
 #include "mtr_tc.cuh"
+#include "mtr_vec.cuh"
 
 namespace mtr {
 namespace i8 {
 
 using namespace tc;
 
-constexpr int BM = 128;
-constexpr int BN = 128;
+constexpr int BM = 128;  // rows of a CTA's tile
 constexpr int BK = 128;  // int8 elements of one 128-byte swizzled row
 constexpr int UK = 32;   // K of one tcgen05.mma kind::i8
-constexpr int STAGES = 4;
-constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr uint32_t RING_BYTES = STAGES * STAGE_BYTES + 1024;  // + alignment slack
 constexpr int QUANT_THREADS = 256;
 
 struct QuantParams {
   const void* x;
   int64_t x_stride;
+  int32_t rows;
   int32_t cols;
+  int32_t threads_per_row;
   int8_t* q;
   int64_t q_stride;
   float* scale;
@@ -42,50 +45,136 @@ struct ProjParams {
   int32_t rows;
   int32_t vocab;
   int32_t kblocks;
+  int32_t m_tiles, n_tiles;
+  int32_t a_bytes;   // bytes of a hidden tile's copy
+  int32_t store_tma; // logits rows are 16-byte aligned: tiles leave by TMA
   uint32_t* err;
 };
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float magnitude(const uint4& w, float) {
+  return max_nan(max_nan(fabsf(__uint_as_float(w.x)), fabsf(__uint_as_float(w.y))),
+                 max_nan(fabsf(__uint_as_float(w.z)), fabsf(__uint_as_float(w.w))));
+}
 template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-
-// max that gives NaN when an operand is NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
+__device__ __forceinline__ float magnitude(uint4 w, T) {
+  w.x &= 0x7fff7fffu;
+  w.y &= 0x7fff7fffu;
+  w.z &= 0x7fff7fffu;
+  w.w &= 0x7fff7fffu;
+  return Vec<T>::value(Vec<T>::top(w));
 }
 
-// One CTA per row: the largest magnitude, then the quotients.
-template <typename T>
-__global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantParams p) {
-  __shared__ float tops[QUANT_THREADS / 32];
-  const int tid = threadIdx.x;
-  wait_prior_grid();
-  const int64_t row = blockIdx.x;
-  const T* x = (const T*)p.x + row * p.x_stride;
-  int8_t* q = p.q + row * p.q_stride;
-  float top = 0.0f;
-  for (int k = tid; k < p.cols; k += QUANT_THREADS) top = max_nan(top, fabsf(to_f(x[k])));
+// The divisor of a row: q(x) = the byte of RNE(RN(x / s)).  The product with
+// RN(1 / s) is within 127 (2^-23 + 2^-24) < 2^-15 of the quotient that is asked
+// for, so it rounds to the same whole number unless it lies that near to a
+// half; those few are divided.  A scale below 2^-100 divides throughout (its
+// reciprocal may overflow).
+struct Divisor {
+  float s, inv;
+  bool zero, divide;
+};
+__device__ __forceinline__ Divisor divisor_of(float top) {
+  Divisor d;
+  d.s = top < pos_inf() ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
+  d.zero = !(d.s > 0.0f);
+  d.divide = d.s < 0x1p-100f;
+  d.inv = d.zero || d.divide ? 0.0f : __fdiv_rn(1.0f, d.s);
+  return d;
+}
+constexpr float WHOLE = 12582912.0f;  // 1.5 2^23: y + WHOLE holds RNE(y) in its low bits, |y| < 2^22
+__device__ __forceinline__ uint32_t quotient(float x, const Divisor& d) {
+  return __float_as_uint(__fadd_rn(__fdiv_rn(x, d.s), WHOLE));
+}
+template <int N>
+__device__ __forceinline__ void quotients(const float (&x)[N], const Divisor& d, uint32_t (&w)[N / 4]) {
+  uint32_t b[N];
+  float near = 0.0f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(FULL, top, o));
-  if ((tid & 31) == 0) tops[tid >> 5] = top;
-  __syncthreads();
-  top = tops[0];
-  for (int w = 1; w < QUANT_THREADS / 32; ++w) top = max_nan(top, tops[w]);
-  const bool finite = top < pos_inf();
-  const float s = finite ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
-  if (tid == 0) p.scale[row] = s;
-  for (int k = tid; k < p.cols; k += QUANT_THREADS)
-    q[k] = s > 0.0f ? (int8_t)__float2int_rn(__fdiv_rn(to_f(x[k]), s)) : (int8_t)0;
+  for (int e = 0; e < N; ++e) {
+    const float y = __fmul_rn(x[e], d.inv), r = __fadd_rn(y, WHOLE);
+    b[e] = __float_as_uint(r);
+    near = fmaxf(near, fabsf(__fsub_rn(y, __fsub_rn(r, WHOLE))));
+  }
+  if (near > 0.5f - 0x1p-15f || d.divide) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) b[e] = quotient(x[e], d);
+  }
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    const uint32_t lo = __byte_perm(b[4 * i], b[4 * i + 1], 0x0040), hi = __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040);
+    w[i] = d.zero ? 0u : __byte_perm(lo, hi, 0x5410);
+  }
+}
+
+// Rows to int8: threads_per_row threads (a power of two, 32 .. 256) hold a row's
+// first QUANT_VECS vectors each between the two passes over it (the largest
+// magnitude, the quotients); longer rows are read again from L2.  HBM bounds it:
+// 3 bytes a bf16 value.  VEC: rows of x and q allow 16-byte loads and stores of
+// as many quotients; else every value is its own access.
+constexpr int QUANT_VECS = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantParams p) {
+  constexpr int E = VEC ? Vec<T>::E : 1;
+  __shared__ float tops[QUANT_THREADS / 32];
+  const int per = p.threads_per_row, sub = threadIdx.x / per, tid = threadIdx.x % per;
+  wait_prior_grid();
+  const int64_t row = (int64_t)blockIdx.x * (QUANT_THREADS / per) + sub;
+  const bool live = row < p.rows;
+  const T* x = (const T*)p.x + (live ? row : 0) * p.x_stride;
+  int8_t* q = p.q + (live ? row : 0) * p.q_stride;
+  const int vecs = live ? p.cols / E : 0, behind = vecs * E, rest = live ? p.cols - behind : 0;
+  float top = 0.0f;
+  uint4 w[QUANT_VECS];
+  T one[QUANT_VECS];
+  if (VEC) {
+#pragma unroll
+    for (int j = 0; j < QUANT_VECS; ++j) {
+      w[j] = make_uint4(0u, 0u, 0u, 0u);
+      const int i = tid + j * per;
+      if (i < vecs) w[j] = reinterpret_cast<const uint4*>(x)[i];
+    }
+#pragma unroll
+    for (int j = 0; j < QUANT_VECS; ++j) top = max_nan(top, magnitude(w[j], T()));
+    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) top = max_nan(top, magnitude(reinterpret_cast<const uint4*>(x)[i], T()));
+    if (tid < rest) top = max_nan(top, fabsf(to_f(x[behind + tid])));
+  } else {
+#pragma unroll
+    for (int j = 0; j < QUANT_VECS; ++j) {
+      const int i = tid + j * per;
+      one[j] = i < vecs ? x[i] : from_f<T>(0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < QUANT_VECS; ++j) top = max_nan(top, fabsf(to_f(one[j])));
+    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) top = max_nan(top, fabsf(to_f(x[i])));
+  }
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
+  if (per > 32) {
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int k = 0; k < per / 32; ++k) top = max_nan(top, tops[sub * (per / 32) + k]);
+  }
+  const Divisor d = divisor_of(top);
+  if (live && tid == 0) p.scale[row] = d.s;
+  if constexpr (VEC) {
+    auto put = [&](int i, const uint4& v) {
+      float f[E];
+      uint32_t b[E / 4];
+      Vec<T>::unpack(v, f);
+      quotients(f, d, b);
+      if constexpr (E == 8) reinterpret_cast<uint2*>(q)[i] = make_uint2(b[0], b[1]);
+      else reinterpret_cast<uint32_t*>(q)[i] = b[0];
+    };
+#pragma unroll
+    for (int j = 0; j < QUANT_VECS; ++j)
+      if (tid + j * per < vecs) put(tid + j * per, w[j]);
+    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) put(i, reinterpret_cast<const uint4*>(x)[i]);
+    if (tid < rest) q[behind + tid] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[behind + tid]), d);
+  } else {
+#pragma unroll
+    for (int j = 0; j < QUANT_VECS; ++j)
+      if (tid + j * per < vecs) q[tid + j * per] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(one[j]), d);
+    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) q[i] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[i]), d);
+  }
 }
 
 __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
@@ -116,165 +205,384 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// One CTA per 128 x 128 tile of logits: one thread loads (TMA, 4-stage ring), one
-// issues the products, then all four warps scale and store the accumulator.
-template <typename Tout>
-__global__ void __launch_bounds__(128, 1)
+// Tiles of 128 rows x BN vocabulary ids for one CTA (CG = 1), or of 256 rows x BN
+// for a pair of CTAs (CG = 2) whose products run on both tensor cores at once:
+// each CTA loads its own 128 rows and half of the ids, and each half is read
+// by both, which halves the shared-memory traffic of the ids.  At BN = 256 a
+// 128-byte step of K costs an SM 512 clocks of products; one CTA alone would
+// write 48 KB and read 48 KB of shared memory meanwhile (192 B a clock, of 128
+// there are), one of a pair 32 KB each (128).
+//
+// Persistent: a CTA (pair) takes tile after tile, with two accumulators in tensor
+// memory, so that one tile is scaled and stored while the next is multiplied.
+//   warp 0, one lane   producer: TMA loads into a ring of STAGES stages
+//   warp 1, one lane   issues the products (of a pair: the first CTA's only);
+//                      the whole warp allocates and frees the tensor memory
+//   warps 2-9          epilogue: warp w owns tensor memory lanes 32 (w % 4) ..,
+//                      tile rows, and half of the columns (two warps a
+//                      scheduler: one alone waits on its own tensor-memory loads
+//                      and conversions); scales them, rounds, stages 32 rows x 128 bytes
+//                      in shared memory (16-byte pieces XOR-swizzled by row) and
+//                      sends them by TMA, or row by row where rows of logits are
+//                      not 16-byte aligned
+// Every wait is bounded; one that gives up sets the error word and ends the
+// CTA's loops, which then gives its copies time to land and returns.
+constexpr int EPI = 8;  // epilogue warps
+constexpr int PROJ_THREADS = 64 + 32 * EPI;
+
+template <int CG, int BN>
+struct Geo {
+  static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN / CG * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr uint32_t BOX_BYTES = 32 * 128;                    // one epilogue warp's staging buffer
+  static constexpr uint32_t OUT_BYTES = EPI * 2 * BOX_BYTES;         // two for each warp
+  static constexpr int STAGES = (int)((220 * 1024 - OUT_BYTES) / STAGE_BYTES) < 8 ? (int)((220 * 1024 - OUT_BYTES) / STAGE_BYTES) : 8;
+  static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + 1024;  // + alignment slack
+  static constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;        // tensor-memory columns
+};
+
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// an arrival on a barrier of the cluster, at a shared::cluster address
+__device__ __forceinline__ void arrive_at(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// arrives on the barrier at this offset in both CTAs of the pair
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   smem_u32(bar)),
+               "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(smem_u32(src))
+               : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float scaled(uint32_t acc, float rs, float cs) {
+  return __fmul_rn(__fmul_rn(__int2float_rn((int)acc), rs), cs);
+}
+
+template <int CG, int BN, typename Tout>
+__global__ void __launch_bounds__(PROJ_THREADS, 1)
     lmhead_i8_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
-                     const ProjParams p) {
+                     const __grid_constant__ CUtensorMap map_out, const ProjParams p) {
+  typedef Geo<CG, BN> G;
+  constexpr int S = G::STAGES;
+  constexpr int CB = BN * (int)sizeof(Tout) < 128 ? BN : 128 / (int)sizeof(Tout);  // columns of a staging buffer
+  constexpr int PIECES = CB * (int)sizeof(Tout) / 16;                              // 16-byte pieces of its rows
   extern __shared__ uint8_t dsm_raw[];
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], done;
+  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile uint32_t abort_flag;
-  __shared__ float col_scale[BN];
+  __shared__ volatile uint32_t abort_flag, epilogue_stop;
+  __shared__ __align__(16) float col_scale[2][BN];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * BM;
+  const int cta = CG > 1 ? (int)(blockIdx.x % CG) : 0;  // within the pair
   const uint32_t raw = smem_u32(dsm_raw);
   uint8_t* ring = dsm_raw + (((raw + 1023u) & ~1023u) - raw);
-  auto a_tile = [&](int s) { return ring + (size_t)s * STAGE_BYTES; };
-  auto b_tile = [&](int s) { return ring + (size_t)s * STAGE_BYTES + A_BYTES; };
+  auto a_tile = [&](int s) { return ring + (size_t)s * G::STAGE_BYTES; };
+  auto b_tile = [&](int s) { return ring + (size_t)s * G::STAGE_BYTES + G::A_BYTES; };
 
-  const int KB = p.kblocks;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_h) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_w) : "memory");
+    if (p.store_tma) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_out) : "memory");
+    for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&done, 1);
-    abort_flag = 0u;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], EPI * CG);
+    }
+    abort_flag = epilogue_stop = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                 "r"((uint32_t)BN)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if (warp == 1) {
+    if (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(G::COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(G::COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
-  wait_prior_grid();
-  if (n0 + (int)threadIdx.x < p.vocab) col_scale[threadIdx.x] = p.col_scale[n0 + threadIdx.x];
   tc_fence_before();
   __syncthreads();
+  if (CG > 1) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  wait_prior_grid();
+
+  const int tiles = p.m_tiles * p.n_tiles, first = (int)(blockIdx.x / CG), step = (int)(gridDim.x / CG);
+  const int KB = p.kblocks;
+  // eight row tiles by all columns, rows first: the tiles in flight share rows and ids in L2
+  auto place = [&](int t, int& m0, int& n0) {
+    constexpr int GROUP = 8;
+    const int per = GROUP * p.n_tiles, g = t / per, in = t - g * per;
+    const int high = min(GROUP, p.m_tiles - g * GROUP);
+    n0 = in / high * BN;
+    m0 = ((g * GROUP + in % high) * CG + cta) * BM;
+  };
 
   if (warp == 0 && lane == 0) {
-    int issued = 0;
-    for (int kb = 0; kb < KB; ++kb) {
-      const int s = kb % STAGES;
-      if (kb >= STAGES && !mbar_wait(&empty[s], ((kb / STAGES) & 1) ^ 1, WAIT_NS)) {
-        abort_flag = 1u;
-        if (p.err) atomicOr(p.err, 1u);
-        break;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      int m0, n0;
+      place(t, m0, n0);
+      for (int kb = 0; kb < KB; ++kb, ++it) {
+        const int s = it % S;
+        if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, WAIT_NS)) {
+          abort_flag = 1u;
+          if (p.err) atomicOr(p.err, 1u);
+        }
+        if (abort_flag) {
+          ok = false;
+          break;
+        }
+        if (CG == 1) {
+          mbar_expect_tx(&full[s], (uint32_t)p.a_bytes + G::B_BYTES);
+          tma_load_2d(a_tile(s), &map_h, kb * BK, m0, &full[s]);
+          tma_load_2d(b_tile(s), &map_w, kb * BK, n0, &full[s]);
+        } else {
+          // the first CTA's barrier counts both CTAs' bytes
+          if (cta == 0) mbar_expect_tx(&full[s], 2 * ((uint32_t)p.a_bytes + G::B_BYTES));
+          const uint32_t bar = map_to(smem_u32(&full[s]), 0);
+          load_pair(a_tile(s), &map_h, kb * BK, m0, bar);
+          load_pair(b_tile(s), &map_w, kb * BK, n0 + cta * (BN / CG), bar);
+        }
       }
-      if (abort_flag) break;
-      mbar_expect_tx(&full[s], STAGE_BYTES);
-      tma_load_2d(a_tile(s), &map_h, kb * BK, m0, &full[s]);
-      tma_load_2d(b_tile(s), &map_w, kb * BK, n0, &full[s]);
-      issued = kb + 1;
     }
-    // copies still in flight land before the CTA may leave (bounded)
-    for (int kb = (issued > STAGES ? issued - STAGES : 0); kb < issued; ++kb)
-      mbar_wait(&full[kb % STAGES], (kb / STAGES) & 1, abort_flag ? WAIT_NS : 0ull);
-  } else if (warp == 1 && lane == 0) {
-    constexpr uint32_t idesc = idesc_i8(BM, BN);
-    for (int kb = 0; kb < KB; ++kb) {
-      const int s = kb % STAGES;
-      if (!mbar_wait(&full[s], (kb / STAGES) & 1, WAIT_NS) || abort_flag) {
+    // the last stages are free: every copy has landed and every arrival on these barriers is in
+    for (uint32_t j = it > (uint32_t)S ? it - S : 0; ok && j < it; ++j) ok = mbar_wait(&empty[j % S], (j / S) & 1, WAIT_NS);
+    if (!ok) {  // copies under way get time to land before the CTA may leave
+      const uint64_t t0 = global_ns();
+      while (global_ns() - t0 < 2000000ull) {
+      }
+    }
+  } else if (warp == 1 && lane == 0 && cta == 0) {
+    constexpr uint32_t idesc = idesc_i8(BM * CG, BN);
+    uint32_t it = 0, n = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step, ++n) {
+      const int acc = n & 1;
+      if (n >= 2 && !mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1, WAIT_NS)) {
         abort_flag = 1u;
         if (p.err) atomicOr(p.err, 2u);
-        break;
       }
+      if (abort_flag) break;
       tc_fence_after();
-      const uint32_t a0 = smem_u32(a_tile(s)), b0 = smem_u32(b_tile(s));
+      for (int kb = 0; kb < KB; ++kb, ++it) {
+        const int s = it % S;
+        if (!mbar_wait(&full[s], (it / S) & 1, WAIT_NS) || abort_flag) {
+          abort_flag = 1u;
+          if (p.err) atomicOr(p.err, 2u);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(a_tile(s)), b0 = smem_u32(b_tile(s));
 #pragma unroll
-      for (int k = 0; k < BK / UK; ++k)
-        mma_i8(tmem, sw128_desc(a0 + k * UK), sw128_desc(b0 + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
-      tc_commit(&empty[s]);
+        for (int k = 0; k < BK / UK; ++k) {
+          if (CG == 1)
+            mma_i8(tmem + acc * BN, sw128_desc(a0 + k * UK), sw128_desc(b0 + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
+          else
+            mma_i8_pair(tmem + acc * BN, sw128_desc(a0 + k * UK), sw128_desc(b0 + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
+        }
+        if (CG == 1) tc_commit(&empty[s]);
+        else commit_pair(&empty[s]);
+      }
+      if (!ok) break;
+      if (CG == 1) tc_commit(&acc_full[acc]);
+      else commit_pair(&acc_full[acc]);
     }
-    tc_commit(&done);
+  } else if (warp >= 2) {
+    constexpr int HALF = BN / (EPI / 4) < CB ? CB : BN / (EPI / 4);  // columns of a warp
+    const int quad = warp & 3, c0 = (warp - 2) / 4 * HALF, et = threadIdx.x - 64;
+    uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 2) * 2 * G::BOX_BYTES;
+    uint32_t n = 0, sent = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step, ++n) {
+      const int acc = n & 1;
+      int m0, n0;
+      place(t, m0, n0);
+      // the tile's scales, while it is multiplied
+      for (int i = et; i < BN; i += 32 * EPI) col_scale[acc][i] = n0 + i < p.vocab ? p.col_scale[n0 + i] : 0.0f;
+      const int row = m0 + quad * 32 + lane;
+      const float rs = row < p.rows ? p.row_scale[row] : 0.0f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
+      bool waited = true;
+      if (lane == 0) waited = mbar_wait(&acc_full[acc], (n >> 1) & 1, WAIT_NS);
+      waited = __shfl_sync(FULL, waited, 0) != 0;
+      if (!waited && lane == 0) {
+        abort_flag = 1u;
+        epilogue_stop = 1u;
+        if (p.err) atomicOr(p.err, 4u);
+      }
+      // the epilogue warps stop together: only they write this flag, and only before this barrier
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
+      ok = epilogue_stop == 0u;
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
+#pragma unroll 1
+      for (int c = c0; c < c0 + HALF && c < BN; c += CB, ++sent) {
+        uint8_t* out = box + (sent & 1) * G::BOX_BYTES;
+        if (p.store_tma) {  // this buffer's previous tile has been read
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < CB; h += 32) {
+          uint32_t v[32];
+          tmem_ld32(base + (uint32_t)(c + h), v);
+          tmem_wait_ld();
+          constexpr int EP = 16 / (int)sizeof(Tout);
+#pragma unroll
+          for (int q = 0; q < 32 / EP; ++q) {
+            float f[EP];
+#pragma unroll
+            for (int e = 0; e < EP; e += 4) {
+              const float4 cs = *reinterpret_cast<const float4*>(&col_scale[acc][c + h + q * EP + e]);
+              f[e] = scaled(v[q * EP + e], rs, cs.x);
+              f[e + 1] = scaled(v[q * EP + e + 1], rs, cs.y);
+              f[e + 2] = scaled(v[q * EP + e + 2], rs, cs.z);
+              f[e + 3] = scaled(v[q * EP + e + 3], rs, cs.w);
+            }
+            const uint4 w = pack<Tout>(f);
+            const int piece = (h / EP + q) ^ (lane & (PIECES - 1));
+            *reinterpret_cast<uint4*>(out + lane * (PIECES * 16) + piece * 16) = w;
+          }
+        }
+        if (p.store_tma) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (m0 + quad * 32 < p.rows && n0 + c < p.vocab) store_2d(&map_out, out, n0 + c, m0 + quad * 32);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c));
+          Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c;
+          for (int r = 0; r < high; ++r, dst += p.out_stride)
+#pragma unroll
+            for (int x = 0; x < CB; x += 32) {
+              const int i = x + lane, piece = (i * (int)sizeof(Tout) / 16) ^ (r & (PIECES - 1));
+              if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(out + r * (PIECES * 16) + piece * 16 + i * (int)sizeof(Tout) % 16);
+            }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();  // the warp's part of the accumulator has been read
+      __syncwarp();
+      if (lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));
+    }
+    if (p.store_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
-
-  bool waited = true;
-  if (lane == 0) waited = mbar_wait(&done, 0, WAIT_NS);
-  waited = __shfl_sync(FULL, waited, 0) != 0;
-  tc_fence_after();
-  const bool go = __all_sync(FULL, waited && !abort_flag);
-  if (!waited && lane == 0 && p.err) atomicOr(p.err, 4u);
-  if (go) {
-    const int row = m0 + warp * 32 + lane;
-    const float rs = row < p.rows ? p.row_scale[row] : 0.0f;
-    Tout* dst = (Tout*)p.out + (int64_t)row * p.out_stride + n0;
-#pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
-      uint32_t v[32];
-      tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, v);
-      tmem_wait_ld();
-      if (row < p.rows) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (n0 + c + j < p.vocab)
-            dst[c + j] = from_f<Tout>(__fmul_rn(__fmul_rn(__int2float_rn((int)v[j]), rs), col_scale[c + j]));
-      }
-    }
-  }
   tc_fence_before();
   __syncthreads();
-  if (warp == 2) {
+  if (CG > 1) cluster_sync();  // the pair's products and arrivals are over
+  if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
+    if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::COLS) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::COLS) : "memory");
   }
 }
 
 // ---------------------------------------------------------------- host side
-// 2-D byte tensor map over a row-major [rows, cols] matrix, box of BK columns x
-// box_rows rows, 128-byte swizzle, 0 outside the matrix.
-static bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows) {
+// 2-D tensor map over a row-major [rows, cols] matrix, box of box_cols x
+// box_rows, 128-byte swizzle; reads 0 and writes nothing outside the matrix.
+static bool make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes,
+                     int box_cols, int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)row_stride};
-  const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static cudaLaunchConfig_t config(dim3 grid, int threads, size_t dyn, cudaStream_t s, cudaLaunchAttribute* attr) {
+static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
+
+static cudaLaunchConfig_t config(dim3 grid, int threads, size_t dyn, int cluster, cudaStream_t s, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = dyn;
   cfg.stream = s;
-  cfg.numAttrs = launch_attrs(attr, 1, true);
+  cfg.numAttrs = launch_attrs(attr, cluster, true);
   cfg.attrs = attr;
   return cfg;
 }
 
 static cudaError_t launch_quantize(const void* x, int64_t x_stride, int dtype, int rows, int cols, int8_t* q,
                                    int64_t q_stride, float* scale, cudaStream_t s) {
-  const QuantParams p{x, x_stride, cols, q, q_stride, scale};
+  const int es = esize(dtype), e = 16 / es;
+  const bool vec = (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0 && (uintptr_t)q % e == 0 && q_stride % e == 0;
+  const int64_t units = vec ? cols / e : cols;
+  int per = 32;
+  while (per < QUANT_THREADS && units > (int64_t)per * QUANT_VECS) per *= 2;
+  const QuantParams p{x, x_stride, rows, cols, per, q, q_stride, scale};
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config(dim3((unsigned)rows, 1, 1), QUANT_THREADS, 0, s, attr);
+  const int high = QUANT_THREADS / per;
+  const cudaLaunchConfig_t cfg = config(dim3((unsigned)((rows + high - 1) / high), 1, 1), QUANT_THREADS, 0, 1, s, attr);
   switch (dtype) {
-    case MTR_DTYPE_F32: return cudaLaunchKernelEx(&cfg, quantize_kernel<float>, p);
-    case MTR_DTYPE_BF16: return cudaLaunchKernelEx(&cfg, quantize_kernel<__nv_bfloat16>, p);
-    default: return cudaLaunchKernelEx(&cfg, quantize_kernel<__half>, p);
+    case MTR_DTYPE_F32: return cudaLaunchKernelEx(&cfg, vec ? quantize_kernel<float, true> : quantize_kernel<float, false>, p);
+    case MTR_DTYPE_BF16:
+      return cudaLaunchKernelEx(&cfg, vec ? quantize_kernel<__nv_bfloat16, true> : quantize_kernel<__nv_bfloat16, false>, p);
+    default: return cudaLaunchKernelEx(&cfg, vec ? quantize_kernel<__half, true> : quantize_kernel<__half, false>, p);
   }
 }
 
-template <typename Tout>
-static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale,
-                               cudaStream_t s) {
-  CUtensorMap mh, mw;
-  if (!make_map(&mh, q, a.rows, a.d_model, q_stride, BM) ||
-      !make_map(&mw, a.weight, a.vocab, a.d_model, a.weight_row_stride, BN))
+template <int CG, int BN, typename Tout>
+static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
+  typedef Geo<CG, BN> G;
+  CUtensorMap mh, mw, mo;
+  // a tile of fewer rows than 128 copies only those that there are, in eights
+  const int high = CG == 1 && a.rows < BM ? (a.rows + 7) / 8 * 8 : BM;
+  if (!make_map(&mh, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, a.rows, a.d_model, q_stride, BK, high) ||
+      !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.weight, a.vocab, a.d_model, a.weight_row_stride, BK, BN / CG))
     return cudaErrorInvalidValue;
-  auto kern = lmhead_i8_kernel<Tout>;
+  const int es = sizeof(Tout);
+  const bool tma = BN * es >= 128 && (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
+  const CUtensorMapDataType type = std::is_same<Tout, float>::value           ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<Tout, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (tma) {
+    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, 128 / es, 32)) return cudaErrorInvalidValue;
+  } else {
+    mo = mh;
+  }
+  auto kern = lmhead_i8_kernel<CG, BN, Tout>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
@@ -282,17 +590,50 @@ static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&]() {
-    attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING_BYTES);
+    attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::DYN);
   });
   if (attr_err[dev] != cudaSuccess) return attr_err[dev];
-  const ProjParams p{row_scale, a.weight_scale, a.logits, a.logits_row_stride, a.rows, a.vocab, (a.d_model + BK - 1) / BK, a.error_word};
+  ProjParams p;
+  p.row_scale = row_scale;
+  p.col_scale = a.weight_scale;
+  p.out = a.logits;
+  p.out_stride = a.logits_row_stride;
+  p.rows = a.rows;
+  p.vocab = a.vocab;
+  p.kblocks = (a.d_model + BK - 1) / BK;
+  p.m_tiles = (a.rows + BM * CG - 1) / (BM * CG);
+  p.n_tiles = (a.vocab + BN - 1) / BN;
+  p.a_bytes = high * BK;
+  p.store_tma = tma;
+  p.err = a.error_word;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, room = device_sms() / CG;
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
-      config(dim3((unsigned)((a.vocab + BN - 1) / BN), (unsigned)((a.rows + BM - 1) / BM), 1), 128, RING_BYTES, s, attr);
-  return cudaLaunchKernelEx(&cfg, kern, mh, mw, p);
+      config(dim3((unsigned)((tiles < room ? tiles : room) * CG), 1, 1), PROJ_THREADS, G::DYN, CG, s, attr);
+  return cudaLaunchKernelEx(&cfg, kern, mh, mw, mo, p);
 }
 
-static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
+template <typename Tout>
+static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
+  const char* ov = getenv("I8TILE");
+  int v = ov ? atoi(ov) : 0;
+  if (!v) {
+    const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
+    v = a.rows > BM && (a.rows + 255) / 256 * ((a.vocab + 255) / 256) >= sms / 2 ? 2256
+        : m * ((a.vocab + 127) / 128) >= sms                                      ? 1128
+        : m * ((a.vocab + 63) / 64) >= sms                                        ? 1064
+                                                                                   : 1032;
+  }
+  switch (v) {
+    case 1032: return launch_tiles<1, 32, Tout>(a, q, q_stride, row_scale, s);
+    case 1064: return launch_tiles<1, 64, Tout>(a, q, q_stride, row_scale, s);
+    case 1128: return launch_tiles<1, 128, Tout>(a, q, q_stride, row_scale, s);
+    case 1256: return launch_tiles<1, 256, Tout>(a, q, q_stride, row_scale, s);
+    case 2128: return launch_tiles<2, 128, Tout>(a, q, q_stride, row_scale, s);
+    default: return launch_tiles<2, 256, Tout>(a, q, q_stride, row_scale, s);
+  }
+}
+
 static bool dtype_ok(int32_t dtype) { return dtype >= MTR_DTYPE_F32 && dtype <= MTR_DTYPE_F16; }
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
