@@ -64,11 +64,11 @@ __device__ __forceinline__ float magnitude(uint4 w, T) {
   return Vec<T>::value(Vec<T>::top(w));
 }
 
-// The divisor of a row: q(x) = the byte of RNE(RN(x / s)).  The product with
-// RN(1 / s) is within 127 (2^-23 + 2^-24) < 2^-15 of the quotient that is asked
-// for, so it rounds to the same whole number unless it lies that near to a
-// half; those few are divided.  A scale below 2^-100 divides throughout (its
-// reciprocal may overflow).
+// The divisor of a row: q(x) = the byte of RNE(RN(x / s)).  With y = RN(1 / s),
+// q0 = RN(x y), r = RN(x - q0 s) (exact) and q1 = RN(q0 + r y), q1 is the
+// correctly rounded quotient (Markstein) unless s has an all-ones significand;
+// three steps, packed two values at a time.  Those scales, and the ones so
+// small that 1 / s or r could leave the normal range, divide instead.
 struct Divisor {
   float s, inv;
   bool zero, divide;
@@ -77,7 +77,7 @@ __device__ __forceinline__ Divisor divisor_of(float top) {
   Divisor d;
   d.s = top < pos_inf() ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
   d.zero = !(d.s > 0.0f);
-  d.divide = d.s < 0x1p-100f;
+  d.divide = d.s < 0x1p-90f || (__float_as_uint(d.s) & 0x7fffffu) == 0x7fffffu;
   d.inv = d.zero || d.divide ? 0.0f : __fdiv_rn(1.0f, d.s);
   return d;
 }
@@ -88,16 +88,19 @@ __device__ __forceinline__ uint32_t quotient(float x, const Divisor& d) {
 template <int N>
 __device__ __forceinline__ void quotients(const float (&x)[N], const Divisor& d, uint32_t (&w)[N / 4]) {
   uint32_t b[N];
-  float near = 0.0f;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float y = __fmul_rn(x[e], d.inv), r = __fadd_rn(y, WHOLE);
-    b[e] = __float_as_uint(r);
-    near = fmaxf(near, fabsf(__fsub_rn(y, __fsub_rn(r, WHOLE))));
-  }
-  if (near > 0.5f - 0x1p-15f || d.divide) {
+  if (d.divide) {
 #pragma unroll
     for (int e = 0; e < N; ++e) b[e] = quotient(x[e], d);
+  } else {
+    const u64 y2 = pk2(d.inv, d.inv), ns2 = pk2(-d.s, -d.s), whole2 = pk2(WHOLE, WHOLE);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const u64 x2 = pk2(x[e], x[e + 1]), q0 = mul2(x2, y2), q1 = fma2(fma2(q0, ns2, x2), y2, q0);
+      float lo, hi;
+      up2(add2(q1, whole2), lo, hi);
+      b[e] = __float_as_uint(lo);
+      b[e + 1] = __float_as_uint(hi);
+    }
   }
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
@@ -154,6 +157,7 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantPara
     for (int k = 0; k < per / 32; ++k) top = max_nan(top, tops[sub * (per / 32) + k]);
   }
   const Divisor d = divisor_of(top);
+  allow_dependents();
   if (live && tid == 0) p.scale[row] = d.s;
   if constexpr (VEC) {
     auto put = [&](int i, const uint4& v) {
@@ -220,8 +224,8 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 //                      the whole warp allocates and frees the tensor memory
 //   warps 2-9          epilogue: warp w owns tensor memory lanes 32 (w % 4) ..,
 //                      tile rows, and half of the columns (two warps a
-//                      scheduler: one alone waits on its own tensor-memory loads
-//                      and conversions); scales them, rounds, stages 32 rows x 128 bytes
+//                      scheduler, so that one works while the other waits for
+//                      tensor memory); scales them, rounds, stages 32 rows x 128 bytes
 //                      in shared memory (16-byte pieces XOR-swizzled by row) and
 //                      sends them by TMA, or row by row where rows of logits are
 //                      not 16-byte aligned
@@ -234,9 +238,11 @@ template <int CG, int BN>
 struct Geo {
   static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN / CG * BK, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr uint32_t BOX_BYTES = 32 * 128;                    // one epilogue warp's staging buffer
-  static constexpr uint32_t OUT_BYTES = EPI * 2 * BOX_BYTES;         // two for each warp
-  static constexpr int STAGES = (int)((220 * 1024 - OUT_BYTES) / STAGE_BYTES) < 8 ? (int)((220 * 1024 - OUT_BYTES) / STAGE_BYTES) : 8;
-  static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + 1024;  // + alignment slack
+  static constexpr uint32_t OUT_BYTES = EPI * BOX_BYTES;
+  static constexpr uint32_t FIXED = 2560;                            // barriers, flags, column scales
+  static constexpr int FIT = (int)((227 * 1024 - OUT_BYTES - FIXED) / STAGE_BYTES);
+  static constexpr int STAGES = FIT < 8 ? FIT : 8;
+  static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + FIXED;
   static constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;        // tensor-memory columns
 };
 
@@ -245,9 +251,12 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-// an arrival on a barrier of the cluster, at a shared::cluster address
+// an arrival on a barrier of the cluster, at a shared::cluster address; the
+// default scope orders what the barrier is for, the reads of tensor memory
+// before it (a cluster-wide release waits for the warp's shared-memory and
+// global stores as well: 31.7 us where this takes 27.5, 8192 x 768 -> 4096)
 __device__ __forceinline__ void arrive_at(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -280,8 +289,29 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ float scaled(uint32_t acc, float rs, float cs) {
-  return __fmul_rn(__fmul_rn(__int2float_rn((int)acc), rs), cs);
+// 32 accumulators to fp32, rounded to nearest even.  Below 2^22 in magnitude
+// (all but a few: the bound is 127^2 d) the sum m = acc + bits(1.5 2^23) is the
+// word of the float 1.5 2^23 + acc, so an integer and half a packed float
+// addition convert it; the conversion instruction runs at a quarter of that
+// rate and would bound the epilogue (2048 clocks a 128 x 256 tile).
+__device__ __forceinline__ void to_floats(uint32_t (&v)[32]) {
+  constexpr uint32_t BIAS = 0x4b400000u;  // 1.5 2^23
+  uint32_t far = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) far |= (v[i] + BIAS) ^ 0x4b000000u;
+  if (__any_sync(FULL, far >= 0x800000u)) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__int2float_rn((int)v[i]));
+  } else {
+    const u64 back = pk2(-12582912.0f, -12582912.0f);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float lo, hi;
+      up2(add2(pk2(__uint_as_float(v[i] + BIAS), __uint_as_float(v[i + 1] + BIAS)), back), lo, hi);
+      v[i] = __float_as_uint(lo);
+      v[i + 1] = __float_as_uint(hi);
+    }
+  }
 }
 
 template <int CG, int BN, typename Tout>
@@ -292,16 +322,21 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   constexpr int S = G::STAGES;
   constexpr int CB = BN * (int)sizeof(Tout) < 128 ? BN : 128 / (int)sizeof(Tout);  // columns of a staging buffer
   constexpr int PIECES = CB * (int)sizeof(Tout) / 16;                              // 16-byte pieces of its rows
-  extern __shared__ uint8_t dsm_raw[];
-  __shared__ __align__(8) uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
-  __shared__ uint32_t tmem_slot;
-  __shared__ volatile uint32_t abort_flag, epilogue_stop;
-  __shared__ __align__(16) float col_scale[2][BN];
+  struct Fixed {
+    uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+    uint32_t tmem_slot;
+    volatile uint32_t abort_flag;
+    __align__(16) float col_scale[EPI][64];
+  };
+  static_assert(sizeof(Fixed) <= G::FIXED, "fixed part of the shared memory");
+  // the swizzle patterns of ring and staging repeat every 1024 bytes
+  extern __shared__ __align__(1024) uint8_t ring[];
+  Fixed& fx = *reinterpret_cast<Fixed*>(ring + (size_t)S * G::STAGE_BYTES + G::OUT_BYTES);
+  uint64_t *const full = fx.full, *const empty = fx.empty, *const acc_full = fx.acc_full, *const acc_empty = fx.acc_empty;
+  volatile uint32_t& abort_flag = fx.abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = CG > 1 ? (int)(blockIdx.x % CG) : 0;  // within the pair
-  const uint32_t raw = smem_u32(dsm_raw);
-  uint8_t* ring = dsm_raw + (((raw + 1023u) & ~1023u) - raw);
   auto a_tile = [&](int s) { return ring + (size_t)s * G::STAGE_BYTES; };
   auto b_tile = [&](int s) { return ring + (size_t)s * G::STAGE_BYTES + G::A_BYTES; };
 
@@ -317,16 +352,16 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], EPI * CG);
     }
-    abort_flag = epilogue_stop = 0u;
+    abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
     if (CG == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(G::COLS) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&fx.tmem_slot)), "r"(G::COLS) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(G::COLS) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&fx.tmem_slot)), "r"(G::COLS) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
   }
@@ -334,8 +369,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   __syncthreads();
   if (CG > 1) cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  wait_prior_grid();
+  const uint32_t tmem = fx.tmem_slot;
 
   const int tiles = p.m_tiles * p.n_tiles, first = (int)(blockIdx.x / CG), step = (int)(gridDim.x / CG);
   const int KB = p.kblocks;
@@ -347,6 +381,27 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     n0 = in / high * BN;
     m0 = ((g * GROUP + in % high) * CG + cta) * BM;
   };
+
+  // The weight tiles of the first stages are asked for before the quantisation of
+  // the hidden states is waited for: that kernel lets this one in only after its
+  // own wait, when whatever wrote the weight has completed.
+  uint32_t early = 0;
+  if (warp == 0 && lane == 0) {
+    for (int t = first; t < tiles && early < (uint32_t)S; t += step) {
+      int m0, n0;
+      place(t, m0, n0);
+      for (int kb = 0; kb < KB && early < (uint32_t)S; ++kb, ++early) {
+        if (CG == 1) {
+          mbar_expect_tx(&full[early], (uint32_t)p.a_bytes + G::B_BYTES);
+          tma_load_2d(b_tile(early), &map_w, kb * BK, n0, &full[early]);
+        } else {
+          if (cta == 0) mbar_expect_tx(&full[early], 2 * ((uint32_t)p.a_bytes + G::B_BYTES));
+          load_pair(b_tile(early), &map_w, kb * BK, n0 + cta * (BN / CG), map_to(smem_u32(&full[early]), 0));
+        }
+      }
+    }
+  }
+  wait_prior_grid();
 
   if (warp == 0 && lane == 0) {
     uint32_t it = 0;
@@ -365,15 +420,19 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
           break;
         }
         if (CG == 1) {
-          mbar_expect_tx(&full[s], (uint32_t)p.a_bytes + G::B_BYTES);
+          if (it >= early) {
+            mbar_expect_tx(&full[s], (uint32_t)p.a_bytes + G::B_BYTES);
+            tma_load_2d(b_tile(s), &map_w, kb * BK, n0, &full[s]);
+          }
           tma_load_2d(a_tile(s), &map_h, kb * BK, m0, &full[s]);
-          tma_load_2d(b_tile(s), &map_w, kb * BK, n0, &full[s]);
         } else {
           // the first CTA's barrier counts both CTAs' bytes
-          if (cta == 0) mbar_expect_tx(&full[s], 2 * ((uint32_t)p.a_bytes + G::B_BYTES));
           const uint32_t bar = map_to(smem_u32(&full[s]), 0);
+          if (it >= early) {
+            if (cta == 0) mbar_expect_tx(&full[s], 2 * ((uint32_t)p.a_bytes + G::B_BYTES));
+            load_pair(b_tile(s), &map_w, kb * BK, n0 + cta * (BN / CG), bar);
+          }
           load_pair(a_tile(s), &map_h, kb * BK, m0, bar);
-          load_pair(b_tile(s), &map_w, kb * BK, n0 + cta * (BN / CG), bar);
         }
       }
     }
@@ -421,79 +480,101 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       else commit_pair(&acc_full[acc]);
     }
   } else if (warp >= 2) {
-    constexpr int HALF = BN / (EPI / 4) < CB ? CB : BN / (EPI / 4);  // columns of a warp
-    const int quad = warp & 3, c0 = (warp - 2) / 4 * HALF, et = threadIdx.x - 64;
-    uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 2) * 2 * G::BOX_BYTES;
-    uint32_t n = 0, sent = 0;
-    bool ok = true;
-    for (int t = first; t < tiles && ok; t += step, ++n) {
+    // a warp's columns, a staging buffer's at a time
+    constexpr int PART = BN / (EPI / 4) < CB ? CB : BN / (EPI / 4);
+    const int quad = warp & 3, c0 = (warp - 2) / 4 * PART;
+    uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 2) * G::BOX_BYTES;
+    float* cs = fx.col_scale[warp - 2];
+    // the scales of a tile, asked for a tile ahead: columns lane, lane + 32, ... and the lane's row
+    float cs_next[PART / 32], rs_next = 0.0f;
+    auto ask = [&](int t) {
+      int m0, n0;
+      place(t, m0, n0);
+#pragma unroll
+      for (int i = 0; i < PART / 32; ++i) {
+        const int col = n0 + c0 + i * 32 + lane;
+        cs_next[i] = c0 < BN && col < p.vocab ? p.col_scale[col] : 0.0f;
+      }
+      const int row = m0 + quad * 32 + lane;
+      rs_next = row < p.rows ? p.row_scale[row] : 0.0f;
+    };
+    if (first < tiles) ask(first);
+    uint32_t n = 0;
+    for (int t = first; t < tiles; t += step, ++n) {
       const int acc = n & 1;
       int m0, n0;
       place(t, m0, n0);
-      // the tile's scales, while it is multiplied
-      for (int i = et; i < BN; i += 32 * EPI) col_scale[acc][i] = n0 + i < p.vocab ? p.col_scale[n0 + i] : 0.0f;
-      const int row = m0 + quad * 32 + lane;
-      const float rs = row < p.rows ? p.row_scale[row] : 0.0f;
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
+      float cs_now[PART / 32];
+#pragma unroll
+      for (int i = 0; i < PART / 32; ++i) cs_now[i] = cs_next[i];
+      const float rs = rs_next;
+      if (t + step < tiles) ask(t + step);
       bool waited = true;
       if (lane == 0) waited = mbar_wait(&acc_full[acc], (n >> 1) & 1, WAIT_NS);
       waited = __shfl_sync(FULL, waited, 0) != 0;
-      if (!waited && lane == 0) {
-        abort_flag = 1u;
-        epilogue_stop = 1u;
-        if (p.err) atomicOr(p.err, 4u);
-      }
-      // the epilogue warps stop together: only they write this flag, and only before this barrier
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
-      ok = epilogue_stop == 0u;
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
-#pragma unroll 1
-      for (int c = c0; c < c0 + HALF && c < BN; c += CB, ++sent) {
-        uint8_t* out = box + (sent & 1) * G::BOX_BYTES;
-        if (p.store_tma) {  // this buffer's previous tile has been read
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          __syncwarp();
+      if (!waited) {
+        if (lane == 0) {
+          abort_flag = 1u;
+          if (p.err) atomicOr(p.err, 4u);
         }
+        break;
+      }
+      tc_fence_after();
+      const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + c0);
+      const bool live = c0 < BN && m0 + quad * 32 < p.rows && n0 + c0 < p.vocab;
 #pragma unroll
-        for (int h = 0; h < CB; h += 32) {
-          uint32_t v[32];
-          tmem_ld32(base + (uint32_t)(c + h), v);
-          tmem_wait_ld();
-          constexpr int EP = 16 / (int)sizeof(Tout);
+      for (int g = 0; g < PART; g += CB) {
+        if (!live) break;
+        uint32_t v[CB / 32][32];
+#pragma unroll
+        for (int h = 0; h < CB / 32; ++h) tmem_ld32(base + (uint32_t)(g + h * 32), v[h]);
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < CB / 32; ++h) cs[h * 32 + lane] = cs_now[g / 32 + h];
+        __syncwarp();
+        tmem_wait_ld();
+        const u64 rs2 = pk2(rs, rs);
+        constexpr int EP = 16 / (int)sizeof(Tout);
+        uint4 w[PIECES];
+#pragma unroll
+        for (int h = 0; h < CB / 32; ++h) {
+          to_floats(v[h]);
 #pragma unroll
           for (int q = 0; q < 32 / EP; ++q) {
             float f[EP];
 #pragma unroll
             for (int e = 0; e < EP; e += 4) {
-              const float4 cs = *reinterpret_cast<const float4*>(&col_scale[acc][c + h + q * EP + e]);
-              f[e] = scaled(v[q * EP + e], rs, cs.x);
-              f[e + 1] = scaled(v[q * EP + e + 1], rs, cs.y);
-              f[e + 2] = scaled(v[q * EP + e + 2], rs, cs.z);
-              f[e + 3] = scaled(v[q * EP + e + 3], rs, cs.w);
+              const float4 c4 = *reinterpret_cast<const float4*>(&cs[h * 32 + q * EP + e]);
+              const uint32_t* a4 = &v[h][q * EP + e];
+              up2(mul2(mul2(pk2(__uint_as_float(a4[0]), __uint_as_float(a4[1])), rs2), pk2(c4.x, c4.y)), f[e], f[e + 1]);
+              up2(mul2(mul2(pk2(__uint_as_float(a4[2]), __uint_as_float(a4[3])), rs2), pk2(c4.z, c4.w)), f[e + 2], f[e + 3]);
             }
-            const uint4 w = pack<Tout>(f);
-            const int piece = (h / EP + q) ^ (lane & (PIECES - 1));
-            *reinterpret_cast<uint4*>(out + lane * (PIECES * 16) + piece * 16) = w;
+            w[h * 32 / EP + q] = pack<Tout>(f);
           }
         }
+        if (p.store_tma) {  // the buffer's previous contents have been read
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q)
+          *reinterpret_cast<uint4*>(box + lane * (PIECES * 16) + (q ^ (lane & (PIECES - 1))) * 16) = w[q];
         if (p.store_tma) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            if (m0 + quad * 32 < p.rows && n0 + c < p.vocab) store_2d(&map_out, out, n0 + c, m0 + quad * 32);
+            if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
           __syncwarp();
-          const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c));
-          Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c;
+          const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c0 + g));
+          Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c0 + g;
           for (int r = 0; r < high; ++r, dst += p.out_stride)
 #pragma unroll
             for (int x = 0; x < CB; x += 32) {
-              const int i = x + lane, piece = (i * (int)sizeof(Tout) / 16) ^ (r & (PIECES - 1));
-              if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(out + r * (PIECES * 16) + piece * 16 + i * (int)sizeof(Tout) % 16);
+              const int i = x + lane, in = i * (int)sizeof(Tout), piece = in / 16 ^ (r & (PIECES - 1));
+              if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(box + r * (PIECES * 16) + piece * 16 + in % 16);
             }
           __syncwarp();
         }
@@ -619,10 +700,11 @@ static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_
   int v = ov ? atoi(ov) : 0;
   if (!v) {
     const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
-    v = a.rows > BM && (a.rows + 255) / 256 * ((a.vocab + 255) / 256) >= sms / 2 ? 2256
-        : m * ((a.vocab + 127) / 128) >= sms                                      ? 1128
-        : m * ((a.vocab + 63) / 64) >= sms                                        ? 1064
-                                                                                   : 1032;
+    v = m * ((a.vocab + 31) / 32) <= sms      ? 1032
+        : m * ((a.vocab + 63) / 64) <= sms    ? 1064
+        : m * ((a.vocab + 127) / 128) <= sms  ? 1128
+        : a.rows > BM                         ? 2256
+                                              : 1256;
   }
   switch (v) {
     case 1032: return launch_tiles<1, 32, Tout>(a, q, q_stride, row_scale, s);

@@ -164,11 +164,6 @@ __device__ __forceinline__ float log_prob(float x, const Row& r, float inv_t) {
   return (x - r.m) * inv_t - r.log_s;
 }
 
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-  u64 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ float warp_max_nan(float v) {
   float r;
   asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));

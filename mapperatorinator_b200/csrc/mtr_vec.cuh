@@ -25,6 +25,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // 16 bytes of a row: E values, their packed maximum, their fp32 values.
 template <typename T>
 struct Vec;
