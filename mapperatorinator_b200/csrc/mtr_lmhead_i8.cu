@@ -373,9 +373,9 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
 
   const int tiles = p.m_tiles * p.n_tiles, first = (int)(blockIdx.x / CG), step = (int)(gridDim.x / CG);
   const int KB = p.kblocks;
-  // eight row tiles by all columns, rows first: the tiles in flight share rows and ids in L2
+  // sixteen row tiles by all columns, rows first: the tiles in flight share rows and ids in L2
   auto place = [&](int t, int& m0, int& n0) {
-    constexpr int GROUP = 8;
+    constexpr int GROUP = 16;
     const int per = GROUP * p.n_tiles, g = t / per, in = t - g * per;
     const int high = min(GROUP, p.m_tiles - g * GROUP);
     n0 = in / high * BN;

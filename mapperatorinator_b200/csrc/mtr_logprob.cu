@@ -153,7 +153,7 @@ __device__ __forceinline__ Row row_of(const Part& p, float inv_t) {
   } else {
     const float rest = p.s + (p.n - 1.0f);
     r.log_s = log1pf(rest);
-    r.entropy = r.log_s - LN2 * p.u / (1.0f + rest);
+    r.entropy = r.log_s - __fdividef(LN2 * p.u, 1.0f + rest);
     r.lse = fmaf(p.m, inv_t, r.log_s);
   }
   return r;
@@ -168,11 +168,6 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   float r;
   asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-  return v;
 }
 // the lanes' values in descending order (none is NaN)
 __device__ __forceinline__ float warp_sort_desc(float v, int lane) {
@@ -244,6 +239,13 @@ __device__ __forceinline__ void load_tile(uint4 (&w)[TILE], const Span<T>& r, in
   }
 }
 
+// how many of list[0 .. c) are larger than k
+__device__ __forceinline__ int place_of(const u64* list, int c, u64 k) {
+  int place = 0;
+  for (int j = 0; j < c; ++j) place += list[j] > k;
+  return place;
+}
+
 // A CTA of W warps takes one row after another (a cluster of CTAs takes one).
 //
 // A thread's tile is TILE vectors; the next tile, of this row or of the CTA's
@@ -254,8 +256,9 @@ __device__ __forceinline__ void load_tile(uint4 (&w)[TILE], const Span<T>& r, in
 // Alternatives: with lm the lanes' maxima, any T with at least n logits >= T
 // bounds the n largest from below.  Two such T are at hand: the n-th largest lm
 // of a warp, the best warp's taken, and the smallest over all warps of the r-th
-// largest lm, r n-th part of the warps (n <= r warps).  The larger of the two
-// leaves about n to 3 n lanes with lm >= T, whose vectors are read again (from
+// largest lm, r n-th part of the warps (n <= r warps).  (The n-th of 32 maxima
+// is a poor bound when n is near 32; then a lane keeps two maxima.)  The larger
+// of the two leaves about n to 3 n lanes with lm >= T, whose vectors are read again (from
 // L2) for the list of candidates, which are ranked by comparing all pairs.  A
 // list that overflows (many equal logits) still holds more than n candidates:
 // the n-th of them is a better T, and the candidates are looked for again.
@@ -270,6 +273,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
   const int64_t step = cs > 1 ? gridDim.x / cs : gridDim.x;
   int64_t row = cs > 1 ? blockIdx.x / cs : blockIdx.x;
   const int V = p.vocab, n = p.top_n;
+  const bool split = n > 24;  // bounds from 64 maxima a warp instead of 32
   const float scale = p.scale;
   auto cta_sync = [&]() {
     if (W > 1) __syncthreads();
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
     }
     const int tail = V - sp.head - sp.vecs * E;
     Part a = empty_part();
-    float lm = neg_inf();  // the lane's largest logit
+    float lm[2] = {neg_inf(), neg_inf()};  // the lane's largest logits, of its tiles' even and odd vectors
     bool bad = false;
     // the single scores: lanes 0 .. head - 1 and 16 .. 16 + tail - 1 of the first warp
     float single = neg_inf();
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
           a.s = ex2(d);
           a.u = a.s * d;
         }
-        lm = single;
+        lm[0] = single;
       }
     }
     Span<T> after = sp;
@@ -319,12 +323,20 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
       typename X::Top top[TILE];
 #pragma unroll
       for (int j = 0; j < TILE; ++j) top[j] = X::top(w[j]);
-      typename X::Top all = top[0];
+      typename X::Top even = top[0], odd = top[1];
 #pragma unroll
-      for (int j = 1; j < TILE; ++j) all = X::larger(all, top[j]);
-      const float mine = X::value(all), most = warp_max_nan(mine);
+      for (int j = 2; j < TILE; j += 2) {
+        even = X::larger(even, top[j]);
+        odd = X::larger(odd, top[j + 1]);
+      }
+      const float mine = X::value(X::larger(even, odd)), most = warp_max_nan(mine);
       if (!(most < pos_inf())) bad = true;
-      lm = fmaxf(lm, mine);
+      if (split) {
+        lm[0] = fmaxf(lm[0], X::value(even));
+        lm[1] = fmaxf(lm[1], X::value(odd));
+      } else {
+        lm[0] = fmaxf(lm[0], mine);
+      }
       if (most > a.m) {
         float lo, hi;
         up2(s2, lo, hi);
@@ -388,15 +400,22 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
       up2(u2, lo, hi);
       a.u += lo + hi;
     }
-    a.n = warp_sum(a.n);
-    a.s = warp_sum(a.s);
-    a.u = warp_sum(a.u);
+    a.n = (float)__reduce_add_sync(FULL, (unsigned)a.n);
+    u64 su = pk2(a.s, a.u);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) su = add2(su, __shfl_xor_sync(FULL, su, o));
+    up2(su, a.s, a.u);
     if (bad) a = Part{neg_inf(), 0.0f, qnan(), 0.0f};
 
     // join the warps, then the CTAs
     float nth = neg_inf(), rth = neg_inf();
     if (n > 0) {
-      const float sorted = warp_sort_desc(lm, lane);
+      float sorted = warp_sort_desc(lm[0], lane);
+      if (split) {
+        // the 32 largest of both halves: the larger of each pair of a descending and an ascending sequence
+        sorted = fmaxf(sorted, __shfl_sync(FULL, warp_sort_desc(lm[1], lane), 31 - lane));
+        sorted = warp_sort_desc(sorted, lane);
+      }
       nth = __shfl_sync(FULL, sorted, n - 1);
       rth = __shfl_sync(FULL, sorted, (n + W * cs - 1) / (W * cs) - 1);
     }
@@ -456,20 +475,22 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
     u64 bound = order_key(fmaxf(nth, rth), 0xffffffffu);
     int c = 0;
     if (tid == 0) sh.count[parity ^ 1] = 0;
+    bool again = false;
     auto list = [&](float f, int id) {
-      const u64 k = order_key(f, (uint32_t)id);
-      const bool hit = k >= bound && f > neg_inf();
+      bool hit = f >= key_value(bound) && f > neg_inf();
+      if (again) hit = hit && order_key(f, (uint32_t)id) >= bound;
       const unsigned hits = __ballot_sync(FULL, hit);
       if (hits == 0) return;
       int at = 0;
       if (lane == 0) at = atomicAdd(&sh.count[parity], __popc(hits));
       at = __shfl_sync(FULL, at, 0) + __popc(hits & ((1u << lane) - 1u));
-      if (hit && at < LIST) sh.list[at] = k;
+      if (hit && at < LIST) sh.list[at] = order_key(f, (uint32_t)id);
     };
     while (!r.bad && !r.none) {
       const float least = key_value(bound);
       if (warp == 0 && rank == 0 && sp.head + tail > 0) list(single, single_id);
-      const bool won = lm >= least && lm > neg_inf();
+      const float top = fmaxf(lm[0], lm[1]);
+      const bool won = top >= least && top > neg_inf();
       const unsigned winners = __ballot_sync(FULL, won);
       if (won) sh.winner[warp][__popc(winners & ((1u << lane) - 1u))] = (uint8_t)lane;
       __syncwarp();
@@ -509,12 +530,12 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
       // overflow: the list's n-th key is the new bound (LIST > n, so the count falls)
       for (int i = tid; i < LIST; i += THREADS) {
         const u64 k = sh.list[i];
-        int place = 0;
-        for (int j = 0; j < LIST; ++j) place += sh.list[j] > k;
+        const int place = place_of(sh.list, LIST, k);
         if (place == n - 1) sh.bound[parity] = k;
       }
       cta_sync();
       bound = sh.bound[parity];
+      again = true;
       if (tid == 0) sh.count[parity] = 0;
       cta_sync();
     }
@@ -522,8 +543,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
       // the CTAs' own n largest, ranked by the first CTA
       for (int i = tid; i < c; i += THREADS) {
         const u64 k = sh.list[i];
-        int place = 0;
-        for (int j = 0; j < c; ++j) place += sh.list[j] > k;
+        const int place = place_of(sh.list, c, k);
         if (place < n) sh.best[place] = k;
       }
       if (tid == 0) sh.count[parity] = min(c, n);
@@ -544,8 +564,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
     float* lps = p.top_logprobs + row * n;
     for (int i = tid; i < c; i += THREADS) {
       const u64 k = sh.list[i];
-      int place = 0;
-      for (int j = 0; j < c; ++j) place += sh.list[j] > k;
+      const int place = place_of(sh.list, c, k);
       if (place < n) {
         ids[place] = key_id(k);
         lps[place] = log_prob(key_value(k), r, p.inv_t);
