@@ -72,7 +72,7 @@ def test_quantize_arguments_are_checked_on_the_host(kw, code):
 def _proj_args():
     return N.sized(N.MtrLmHeadI8Args, hidden=0x1000000, hidden_row_stride=100, weight=0x2000000, weight_row_stride=112,
                    weight_scale=0x3000000, logits=0x4000000, logits_row_stride=77, hidden_dtype=N.DTYPE_BF16,
-                   logits_dtype=N.DTYPE_BF16, rows=9, d_model=100, vocab=77, workspace=0x5000000, workspace_bytes=1 << 20)
+                   logits_dtype=N.DTYPE_BF16, rows=900, d_model=100, vocab=77, workspace=0x5000000, workspace_bytes=1 << 20)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -80,7 +80,7 @@ def _proj_args():
     (dict(d_model=0), N.ERR_BAD_SHAPE), (dict(d_model=N.MAX_I8_D_MODEL + 1), N.ERR_BAD_SHAPE), (dict(vocab=0), N.ERR_BAD_SHAPE),
     (dict(vocab=N.MAX_VOCAB + 1), N.ERR_BAD_SHAPE), (dict(hidden_dtype=3), N.ERR_BAD_PARAM), (dict(logits_dtype=-1), N.ERR_BAD_PARAM),
     (dict(weight=None), N.ERR_NULL_ARG), (dict(weight_scale=None), N.ERR_NULL_ARG), (dict(workspace=None), N.ERR_NULL_ARG),
-    (dict(workspace_bytes=9 * 112), N.ERR_BAD_SHAPE), (dict(workspace=0x5000010), N.ERR_ALIGNMENT),
+    (dict(workspace_bytes=900 * 112), N.ERR_BAD_SHAPE), (dict(rows=9, workspace=None, workspace_bytes=0), N.OK), (dict(workspace=0x5000010), N.ERR_ALIGNMENT),
     (dict(weight_row_stride=104), N.ERR_ALIGNMENT), (dict(weight=0x2000008), N.ERR_ALIGNMENT),
     (dict(weight_row_stride=96), N.ERR_BAD_SHAPE), (dict(logits_row_stride=76), N.ERR_BAD_SHAPE),
     (dict(hidden_row_stride=99), N.ERR_BAD_SHAPE), (dict(logits=0x1000000), N.ERR_BAD_PARAM),
@@ -97,11 +97,11 @@ def test_projection_arguments_are_checked_on_the_host(kw, code):
 
 def test_projection_and_sampler_must_share_the_logits():
     lm, a = _proj_args(), N.new_args()
-    a.logits, a.logits_row_stride, a.logits_dtype, a.vocab, a.num_rows = lm.logits, 77, N.DTYPE_BF16, 77, 9
+    a.logits, a.logits_row_stride, a.logits_dtype, a.vocab, a.num_rows = lm.logits, 77, N.DTYPE_BF16, 77, 900
     a.select_mode, a.out_ids = N.SELECT_ARGMAX, 0x6000000
     lib = N.load()
     for field, value, code in (("logits", 0x7000000, N.ERR_BAD_PARAM), ("logits_row_stride", 78, N.ERR_BAD_PARAM),
-                               ("logits_dtype", N.DTYPE_F16, N.ERR_BAD_PARAM), ("num_rows", 10, N.ERR_BAD_SHAPE)):
+                               ("logits_dtype", N.DTYPE_F16, N.ERR_BAD_PARAM), ("num_rows", 901, N.ERR_BAD_SHAPE)):
         b = N.MtrSamplerArgs()
         ctypes.pointer(b)[0] = a
         setattr(b, field, value)
@@ -112,7 +112,8 @@ def test_projection_and_sampler_must_share_the_logits():
 
 def test_workspace_sizes():
     assert N.lmhead_i8_workspace(0, 64) == 0 and N.lmhead_i8_workspace(4, 0) == 0
-    assert N.lmhead_i8_workspace(3, 100) == 512 + 12  # 3 rows of 112 bytes, the scales on the next 256-byte boundary
+    assert N.lmhead_i8_workspace(3, 100) == 0  # quantised by the projection itself
+    assert N.lmhead_i8_workspace(301, 100) == 33792 + 1204  # rows of 112 bytes, the scales on the next 256-byte boundary
     assert N.lmhead_i8_workspace(N.MAX_I8_ROWS, N.MAX_I8_D_MODEL) == (1 << 39) + (1 << 24)
 
 
@@ -179,7 +180,8 @@ def test_quantize_strided_rows(cuda_device):
 @gpu
 @pytest.mark.parametrize("out_dtype", DTYPES)
 @pytest.mark.parametrize("rows,d,vocab,dtype", [
-    (1, 1, 1, torch.float32), (1, 16, 8, torch.bfloat16), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
+    (1, 1, 1, torch.float32), (1, 16, 8, torch.bfloat16), (8, 2048, 1000, torch.bfloat16), (5, 1001, 300, torch.float16),
+    (8, 100, 131072, torch.float32), (1, 8192, 77, torch.bfloat16), (1, 8193, 77, torch.bfloat16), (9, 64, 20000, torch.float32), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
     (33, 100, 77, torch.float16), (129, 1001, 4099, torch.float16), (300, 64, 520, torch.float32), (256, 128, 8192, torch.bfloat16),
     (513, 2048, 1000, torch.bfloat16), (1030, 96, 264, torch.float32), (64, 3000, 131072, torch.bfloat16)])
 def test_logits_equal_the_definition(cuda_device, out_dtype, rows, d, vocab, dtype):
@@ -209,10 +211,12 @@ def test_largest_sums_are_exact(cuda_device):
 
 
 @gpu
-def test_odd_rows_and_weights(cuda_device):
+@pytest.mark.parametrize("rows", [7, 147])
+def test_odd_rows_and_weights(cuda_device, rows):
     h, w = inputs(cuda_device, 7, 200, 300, torch.bfloat16, seed=2)
     h[1], h[2, 5], h[3, 6] = 0.0, math.nan, math.inf
     w[4] = 0.0
+    h = torch.cat([h] * (rows // 7))
     weight = Int8Weight.from_weight(w)
     out = lm_head_logits_int8(h, weight.q, weight.scale)
     q, scale = quantize_rows(h)
@@ -236,6 +240,8 @@ def test_strides_and_what_lies_behind(cuda_device, out_dtype, vocab, stride, off
     got = lm_head_logits_int8(wide_h[:, 51:251], wide_w[:, :d], weight.scale, out)
     assert got is out
     assert torch.equal(out, lm_head_logits_int8(h, weight.q, weight.scale, out_dtype=out_dtype))
+    few = lm_head_logits_int8(wide_h[:7, 51:251], wide_w[:, :d], weight.scale, out_dtype=out_dtype)
+    assert torch.equal(out[:7], few)  # few rows take another way to the same bits
     rest = torch.ones_like(buf, dtype=torch.bool)
     rest[offset:].as_strided((rows, vocab), (stride, 1)).fill_(False)
     assert bool((buf[rest] == 7.0).all())  # columns behind the vocabulary and rows behind the last
@@ -290,12 +296,13 @@ def test_streams_and_graphs(cuda_device):
 def test_weight_written_just_before_its_use(cuda_device):
     # the projection is launched as a dependent of the kernels that write its operands
     for seed in range(5):
-        h, w = inputs(cuda_device, 64, 512, 2048, seed=seed)
-        torch.cuda.synchronize()
-        weight = Int8Weight.from_weight(w)
-        out = lm_head_logits_int8(h, weight.q, weight.scale)
-        torch.cuda.synchronize()
-        assert torch.equal(out, lm_head_logits_int8(h, weight.q, weight.scale))
+        for rows in (2, 64, 400):
+            h, w = inputs(cuda_device, rows, 512, 2048, seed=seed)
+            torch.cuda.synchronize()
+            weight = Int8Weight.from_weight(w)
+            out = lm_head_logits_int8(h, weight.q, weight.scale)
+            torch.cuda.synchronize()
+            assert torch.equal(out, lm_head_logits_int8(h, weight.q, weight.scale))
 
 
 @gpu
