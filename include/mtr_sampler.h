@@ -351,13 +351,12 @@ typedef struct MtrLmHeadI8Args {
   int32_t d_model;              /* 1 .. MTR_MAX_I8_D_MODEL */
   int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
   int32_t reserved0;
-  void* workspace;              /* 256-byte aligned, one call's at a time; may be NULL where 0 bytes are needed */
+  void* workspace;              /* 256-byte aligned; one call's at a time */
   int64_t workspace_bytes;      /* >= mtr_lmhead_i8_workspace(rows, d_model) */
   uint32_t* error_word;         /* device word or NULL: bits set when a bounded wait gave up */
 } MtrLmHeadI8Args;
 
-/* Workspace bytes of a call (0 for few rows, which the projection's own kernel
- * quantises, and for rows <= 0 or d_model <= 0). */
+/* Workspace bytes of a call (0 for rows <= 0 or d_model <= 0). */
 int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model);
 int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* args);
 int mtr_lmhead_i8_launch(const MtrLmHeadI8Args* args, void* stream);

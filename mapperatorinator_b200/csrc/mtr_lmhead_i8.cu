@@ -46,10 +46,6 @@ struct ProjParams {
   int32_t m_tiles, n_tiles;
   int32_t a_bytes;   // bytes of a hidden tile's copy
   int32_t store_tma; // logits rows are 16-byte aligned: tiles leave by TMA
-  const void* x;     // hidden states that the kernel quantises itself
-  int64_t x_stride;
-  int32_t x_dtype, d;
-  int32_t held;      // bytes of their int8 rows
   uint32_t* err;
 };
 
@@ -236,22 +232,29 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 constexpr int EPI = 8;  // epilogue warps
 constexpr int PROJ_THREADS = 64 + 32 * EPI;
 
-// HERE: the CTA quantises the hidden states itself (few rows): their int8 rows,
-// all of d, stay in HELD bytes at most, and the ring carries weight tiles alone.
-constexpr uint32_t HELD = 64 * 1024;
-template <int CG, int BN, bool HERE>
+template <int CG, int BN>
 struct Geo {
-  static constexpr uint32_t A_BYTES = HERE ? 0 : BM * BK, B_BYTES = BN / CG * BK, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr uint32_t BOX_BYTES = 32 * 128;                    // one epilogue warp's staging buffer
+  static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN / CG * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr uint32_t BOX_BYTES = 32 * 128;  // one epilogue warp's staging buffer
   static constexpr uint32_t OUT_BYTES = EPI * BOX_BYTES;
-  static constexpr uint32_t FIXED = 2560 + (HERE ? 4 * BM : 0);      // barriers, flags, column scales; row scales
-  static constexpr int FIT = (int)((227 * 1024 - (HERE ? HELD : 0) - OUT_BYTES - FIXED) / STAGE_BYTES);
+  static constexpr uint32_t FIXED = 2560;          // barriers, flags, column scales
+  static constexpr int FIT = (int)((227 * 1024 - OUT_BYTES - FIXED) / STAGE_BYTES);
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
-  static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + FIXED;  // + the held rows
-  static constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;        // tensor-memory columns
+  static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + FIXED;
+  static constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // tensor-memory columns
 };
-// what the held rows take: rows in eights (swizzle atoms), d in 128-byte steps
-__host__ __device__ inline int64_t held_bytes(int64_t rows, int64_t d) { return (rows + 7) / 8 * 8 * ((d + BK - 1) / BK * BK); }
+
+// A position in a ring of barriers: its slot, and the parity of its next completion.
+struct Turn {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int slots) {
+    if (++slot == slots) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
 
 __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -321,40 +324,11 @@ __device__ __forceinline__ void to_floats(uint32_t (&v)[32]) {
   }
 }
 
-// One warp quantises row r of x into the held rows: K steps of `high` rows of 128
-// bytes, 16-byte pieces XOR-swizzled as the products read them.  Returns the
-// row's scale.  (Bytes behind d in the last step meet weights that read as 0.)
-template <typename T>
-__device__ __forceinline__ float hold_row(uint8_t* held, int high, const T* x, int d, int r, int lane) {
-  constexpr int E = Vec<T>::E;
-  auto at = [&](int c) { return held + ((size_t)(c / BK) * high + r) * BK + (((c % BK) / 16) ^ (r & 7)) * 16 + c % 16; };
-  const bool vec = ((uintptr_t)x & 15u) == 0;
-  const int vecs = vec ? d / E : 0;
-  float top = 0.0f;
-#pragma unroll 4
-  for (int i = lane; i < vecs; i += 32) top = max_nan(top, magnitude(reinterpret_cast<const uint4*>(x)[i], T()));
-#pragma unroll 4
-  for (int c = vecs * E + lane; c < d; c += 32) top = max_nan(top, fabsf(to_f(x[c])));
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
-  const Divisor dv = divisor_of(top);
-#pragma unroll 4
-  for (int i = lane; i < vecs; i += 32) {
-    float f[E];
-    uint32_t b[E / 4];
-    Vec<T>::unpack(reinterpret_cast<const uint4*>(x)[i], f);
-    quotients(f, dv, b);
-    if constexpr (E == 8) *reinterpret_cast<uint2*>(at(i * E)) = make_uint2(b[0], b[1]);
-    else *reinterpret_cast<uint32_t*>(at(i * E)) = b[0];
-  }
-  for (int c = vecs * E + lane; c < d; c += 32) *at(c) = dv.zero ? (uint8_t)0 : (uint8_t)quotient(to_f(x[c]), dv);
-  return dv.s;
-}
-
-template <int CG, int BN, typename Tout, bool HERE>
+template <int CG, int BN, typename Tout>
 __global__ void __launch_bounds__(PROJ_THREADS, 1)
     lmhead_i8_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_out, const ProjParams p) {
-  typedef Geo<CG, BN, HERE> G;
+  typedef Geo<CG, BN> G;
   constexpr int S = G::STAGES;
   constexpr int CB = BN * (int)sizeof(Tout) < 128 ? BN : 128 / (int)sizeof(Tout);  // columns of a staging buffer
   constexpr int PIECES = CB * (int)sizeof(Tout) / 16;                              // 16-byte pieces of its rows
@@ -363,12 +337,10 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     uint32_t tmem_slot;
     volatile uint32_t abort_flag;
     __align__(16) float col_scale[EPI][64];
-    float row_scale[HERE ? BM : 1];
   };
   static_assert(sizeof(Fixed) <= G::FIXED, "fixed part of the shared memory");
   // the swizzle patterns of ring and staging repeat every 1024 bytes
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* const ring = smem + (HERE ? p.held : 0);
+  extern __shared__ __align__(1024) uint8_t ring[];
   Fixed& fx = *reinterpret_cast<Fixed*>(ring + (size_t)S * G::STAGE_BYTES + G::OUT_BYTES);
   uint64_t *const full = fx.full, *const empty = fx.empty, *const acc_full = fx.acc_full, *const acc_empty = fx.acc_empty;
   volatile uint32_t& abort_flag = fx.abort_flag;
@@ -379,7 +351,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   auto b_tile = [&](int s) { return ring + (size_t)s * G::STAGE_BYTES + G::A_BYTES; };
 
   if (threadIdx.x == 0) {
-    if (!HERE) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_h) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_h) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_w) : "memory");
     if (p.store_tma) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_out) : "memory");
     for (int s = 0; s < S; ++s) {
@@ -409,9 +381,10 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = fx.tmem_slot;
 
+  // The CTA's (pair's) tiles are first, first + step, ...: sixteen row tiles by all
+  // columns, rows first, so that the tiles in flight share rows and ids in L2.
   const int tiles = p.m_tiles * p.n_tiles, first = (int)(blockIdx.x / CG), step = (int)(gridDim.x / CG);
   const int KB = p.kblocks;
-  // sixteen row tiles by all columns, rows first: the tiles in flight share rows and ids in L2
   auto place = [&](int t, int& m0, int& n0) {
     constexpr int GROUP = 16;
     const int per = GROUP * p.n_tiles, g = t / per, in = t - g * per;
@@ -419,116 +392,89 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     n0 = in / high * BN;
     m0 = ((g * GROUP + in % high) * CG + cta) * BM;
   };
+  // the ids' part of a stage (CG = 2: of both CTAs, counted on the first one's barrier), with the bytes of all of it
+  auto load_ids = [&](int slot, int kb, int n0) {
+    const uint32_t bytes = (uint32_t)p.a_bytes + G::B_BYTES;
+    if (CG == 1) {
+      mbar_expect_tx(&full[slot], bytes);
+      tma_load_2d(b_tile(slot), &map_w, kb * BK, n0, &full[slot]);
+    } else {
+      if (cta == 0) mbar_expect_tx(&full[slot], 2 * bytes);
+      load_pair(b_tile(slot), &map_w, kb * BK, n0 + cta * (BN / CG), map_to(smem_u32(&full[slot]), 0));
+    }
+  };
+  uint32_t early = 0;  // stages whose ids have been asked for ahead
+  auto load_early = [&]() {
+    for (int t = first; t < tiles && early < (uint32_t)S; t += step) {
+      int m0, n0;
+      place(t, m0, n0);
+      for (int kb = 0; kb < KB && early < (uint32_t)S; ++kb, ++early) load_ids((int)early, kb, n0);
+    }
+  };
 
   // The weight tiles of the first stages are asked for before the quantisation of
   // the hidden states is waited for: that kernel lets this one in only after its
   // own wait, when whatever wrote the weight has completed.
-  uint32_t early = 0;
-  if (!HERE && warp == 0 && lane == 0) {
-    for (int t = first; t < tiles && early < (uint32_t)S; t += step) {
-      int m0, n0;
-      place(t, m0, n0);
-      for (int kb = 0; kb < KB && early < (uint32_t)S; ++kb, ++early) {
-        if (CG == 1) {
-          mbar_expect_tx(&full[early], (uint32_t)p.a_bytes + G::B_BYTES);
-          tma_load_2d(b_tile(early), &map_w, kb * BK, n0, &full[early]);
-        } else {
-          if (cta == 0) mbar_expect_tx(&full[early], 2 * ((uint32_t)p.a_bytes + G::B_BYTES));
-          load_pair(b_tile(early), &map_w, kb * BK, n0 + cta * (BN / CG), map_to(smem_u32(&full[early]), 0));
-        }
-      }
-    }
-  }
+  if (warp == 0 && lane == 0) load_early();
   wait_prior_grid();
 
-  if (HERE) {
-    // the first weight tiles travel while the rows are quantised
-    if (warp == 0 && lane == 0)
-      for (int t = first; t < tiles && early < (uint32_t)S; t += step) {
-        int m0, n0;
-        place(t, m0, n0);
-        for (int kb = 0; kb < KB && early < (uint32_t)S; ++kb, ++early) {
-          mbar_expect_tx(&full[early], G::B_BYTES);
-          tma_load_2d(b_tile(early), &map_w, kb * BK, n0, &full[early]);
-        }
-      }
-    __syncwarp();
-    const int high = (p.rows + 7) / 8 * 8;
-    for (int r = warp; r < p.rows; r += PROJ_THREADS / 32) {
-      float scale;
-      switch (p.x_dtype) {
-        case MTR_DTYPE_F32: scale = hold_row(smem, high, (const float*)p.x + r * p.x_stride, p.d, r, lane); break;
-        case MTR_DTYPE_BF16: scale = hold_row(smem, high, (const __nv_bfloat16*)p.x + r * p.x_stride, p.d, r, lane); break;
-        default: scale = hold_row(smem, high, (const __half*)p.x + r * p.x_stride, p.d, r, lane); break;
-      }
-      if (lane == 0) fx.row_scale[r] = scale;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads what was written here
-    __syncthreads();
-  }
-
   if (warp == 0 && lane == 0) {
+    // ---------------- producer
+    Turn turn;
     uint32_t it = 0;
     bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!mbar_wait(bar, parity, WAIT_NS)) {
+        abort_flag = 1u;
+        if (p.err) atomicOr(p.err, 1u);
+      }
+      return abort_flag == 0u;
+    };
     for (int t = first; t < tiles && ok; t += step) {
       int m0, n0;
       place(t, m0, n0);
-      for (int kb = 0; kb < KB; ++kb, ++it) {
-        const int s = it % S;
-        if (it >= (uint32_t)S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, WAIT_NS)) {
-          abort_flag = 1u;
-          if (p.err) atomicOr(p.err, 1u);
-        }
-        if (abort_flag) {
-          ok = false;
-          break;
-        }
-        if (CG == 1) {
-          if (it >= early) {
-            mbar_expect_tx(&full[s], (HERE ? 0u : (uint32_t)p.a_bytes) + G::B_BYTES);
-            tma_load_2d(b_tile(s), &map_w, kb * BK, n0, &full[s]);
-          }
-          if (!HERE) tma_load_2d(a_tile(s), &map_h, kb * BK, m0, &full[s]);
-        } else {
-          // the first CTA's barrier counts both CTAs' bytes
-          const uint32_t bar = map_to(smem_u32(&full[s]), 0);
-          if (it >= early) {
-            if (cta == 0) mbar_expect_tx(&full[s], 2 * ((uint32_t)p.a_bytes + G::B_BYTES));
-            load_pair(b_tile(s), &map_w, kb * BK, n0 + cta * (BN / CG), bar);
-          }
-          load_pair(a_tile(s), &map_h, kb * BK, m0, bar);
-        }
+      for (int kb = 0; kb < KB && ok; ++kb, ++it, turn.next(S)) {
+        ok = wait(&empty[turn.slot], turn.parity ^ 1);
+        if (!ok) break;
+        if (it >= early) load_ids(turn.slot, kb, n0);
+        if (CG == 1) tma_load_2d(a_tile(turn.slot), &map_h, kb * BK, m0, &full[turn.slot]);
+        else load_pair(a_tile(turn.slot), &map_h, kb * BK, m0, map_to(smem_u32(&full[turn.slot]), 0));
       }
     }
-    // the last stages are free: every copy has landed and every arrival on these barriers is in
-    for (uint32_t j = it > (uint32_t)S ? it - S : 0; ok && j < it; ++j) ok = mbar_wait(&empty[j % S], (j / S) & 1, WAIT_NS);
+    // every stage is free: its copies have landed and the arrivals on its barriers are in
+    for (int i = 0; ok && i < S; ++i, turn.next(S)) ok = wait(&empty[turn.slot], turn.parity ^ 1);
     if (!ok) {  // copies under way get time to land before the CTA may leave
       const uint64_t t0 = global_ns();
       while (global_ns() - t0 < 2000000ull) {
       }
     }
   } else if (warp == 1 && lane == 0 && cta == 0) {
+    // ---------------- products
     constexpr uint32_t idesc = idesc_i8(BM * CG, BN);
-    uint32_t it = 0, n = 0;
+    Turn turn;
+    uint32_t n = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step, ++n) {
-      const int acc = n & 1;
-      if (n >= 2 && !mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1, WAIT_NS)) {
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!mbar_wait(bar, parity, WAIT_NS)) {
         abort_flag = 1u;
         if (p.err) atomicOr(p.err, 2u);
       }
-      if (abort_flag) break;
+      return abort_flag == 0u;
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (CG == 1) tc_commit(bar);
+      else commit_pair(bar);
+    };
+    for (int t = first; t < tiles && ok; t += step, ++n) {
+      const int acc = n & 1;
+      ok = wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1);
+      if (!ok) break;
       tc_fence_after();
-      for (int kb = 0; kb < KB; ++kb, ++it) {
-        const int s = it % S;
-        if (!mbar_wait(&full[s], (it / S) & 1, WAIT_NS) || abort_flag) {
-          abort_flag = 1u;
-          if (p.err) atomicOr(p.err, 2u);
-          ok = false;
-          break;
-        }
+      for (int kb = 0; kb < KB; ++kb, turn.next(S)) {
+        ok = wait(&full[turn.slot], turn.parity);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t a0 = HERE ? smem_u32(smem) + (uint32_t)(kb * ((p.rows + 7) / 8 * 8) * BK) : smem_u32(a_tile(s)), b0 = smem_u32(b_tile(s));
+        const uint32_t a0 = smem_u32(a_tile(turn.slot)), b0 = smem_u32(b_tile(turn.slot));
 #pragma unroll
         for (int k = 0; k < BK / UK; ++k) {
           if (CG == 1)
@@ -536,12 +482,10 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
           else
             mma_i8_pair(tmem + acc * BN, sw128_desc(a0 + k * UK), sw128_desc(b0 + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
         }
-        if (CG == 1) tc_commit(&empty[s]);
-        else commit_pair(&empty[s]);
+        commit(&empty[turn.slot]);
       }
       if (!ok) break;
-      if (CG == 1) tc_commit(&acc_full[acc]);
-      else commit_pair(&acc_full[acc]);
+      commit(&acc_full[acc]);
     }
   } else if (warp >= 2) {
     // a warp's columns, a staging buffer's at a time
@@ -560,7 +504,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
         cs_next[i] = c0 < BN && col < p.vocab ? p.col_scale[col] : 0.0f;
       }
       const int row = m0 + quad * 32 + lane;
-      rs_next = row < p.rows ? (HERE ? fx.row_scale[row] : p.row_scale[row]) : 0.0f;
+      rs_next = row < p.rows ? p.row_scale[row] : 0.0f;
     };
     if (first < tiles) ask(first);
     uint32_t n = 0;
@@ -708,13 +652,13 @@ static cudaError_t launch_quantize(const void* x, int64_t x_stride, int dtype, i
   }
 }
 
-template <int CG, int BN, typename Tout, bool HERE = false>
+template <int CG, int BN, typename Tout>
 static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
-  typedef Geo<CG, BN, HERE> G;
+  typedef Geo<CG, BN> G;
   CUtensorMap mh, mw, mo;
   // a tile of fewer rows than 128 copies only those that there are, in eights
   const int high = CG == 1 && a.rows < BM ? (a.rows + 7) / 8 * 8 : BM;
-  if ((!HERE && !make_map(&mh, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, a.rows, a.d_model, q_stride, BK, high)) ||
+  if (!make_map(&mh, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, a.rows, a.d_model, q_stride, BK, high) ||
       !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.weight, a.vocab, a.d_model, a.weight_row_stride, BK, BN / CG))
     return cudaErrorInvalidValue;
   const int es = sizeof(Tout);
@@ -727,9 +671,7 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   } else {
     mo = mw;
   }
-  if (HERE) mh = mw;
-  auto kern = lmhead_i8_kernel<CG, BN, Tout, HERE>;
-  const uint32_t held = HERE ? (uint32_t)held_bytes(a.rows, a.d_model) : 0;
+  auto kern = lmhead_i8_kernel<CG, BN, Tout>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
@@ -737,7 +679,7 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&]() {
-    attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(G::DYN + (HERE ? HELD : 0)));
+    attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::DYN);
   });
   if (attr_err[dev] != cudaSuccess) return attr_err[dev];
   ProjParams p;
@@ -752,27 +694,12 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   p.n_tiles = (a.vocab + BN - 1) / BN;
   p.a_bytes = high * BK;
   p.store_tma = tma;
-  p.x = a.hidden;
-  p.x_stride = a.hidden_row_stride;
-  p.x_dtype = a.hidden_dtype;
-  p.d = a.d_model;
-  p.held = (int32_t)held;
   p.err = a.error_word;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, room = device_sms() / CG;
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
-      config(dim3((unsigned)((tiles < room ? tiles : room) * CG), 1, 1), PROJ_THREADS, G::DYN + held, CG, s, attr);
+      config(dim3((unsigned)((tiles < room ? tiles : room) * CG), 1, 1), PROJ_THREADS, G::DYN, CG, s, attr);
   return cudaLaunchKernelEx(&cfg, kern, mh, mw, mo, p);
-}
-
-// Up to 8 rows of up to 16384 values together are quantised by every CTA, in the
-// projection's own launch: one launch for the host, and as fast or faster on the
-// device although each CTA reads the rows again.  us, here / with a launch of
-// its own (148 SMs): 2 x 768 -> 4096 6.1 / 6.6, 8 x 768 -> 4096 6.2 / 7.0,
-// 8 x 2048 -> 8192 10.3 / 11.1, 4 x 4096 -> 16384 18.0 / 17.6; but
-// 16 x 768 -> 4096 7.4 / 7.1, 64 x 512 -> 8192 10.8 / 6.3.
-static bool quantised_here(int64_t rows, int64_t d) {
-  return rows <= 8 && rows * d <= 16384 && held_bytes(rows, d) <= (int64_t)HELD;
 }
 
 // The narrowest tiles that still make one round of CTAs, else pairs of CTAs on
@@ -784,10 +711,6 @@ template <typename Tout>
 static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
   const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
   auto fits = [&](int bn) { return m * ((a.vocab + bn - 1) / bn) <= sms; };
-  if (quantised_here(a.rows, a.d_model))
-    return fits(32)   ? launch_tiles<1, 32, Tout, true>(a, nullptr, 0, nullptr, s)
-           : fits(64) ? launch_tiles<1, 64, Tout, true>(a, nullptr, 0, nullptr, s)
-                      : launch_tiles<1, 128, Tout, true>(a, nullptr, 0, nullptr, s);
   if (fits(32)) return launch_tiles<1, 32, Tout>(a, q, q_stride, row_scale, s);
   if (fits(64)) return launch_tiles<1, 64, Tout>(a, q, q_stride, row_scale, s);
   if (fits(128)) return launch_tiles<1, 128, Tout>(a, q, q_stride, row_scale, s);
@@ -836,7 +759,7 @@ int mtr_quantize_rows_launch(const MtrQuantizeArgs* a, void* stream) {
 }
 
 int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model) {
-  if (rows <= 0 || d_model <= 0 || quantised_here(rows, d_model)) return 0;
+  if (rows <= 0 || d_model <= 0) return 0;
   return up((int64_t)rows * up(d_model, 16), 256) + 4ll * rows;
 }
 
@@ -849,7 +772,7 @@ int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* a) {
   if (!dtype_ok(a->hidden_dtype) || !dtype_ok(a->logits_dtype)) return MTR_ERR_BAD_PARAM;
   if (a->rows == 0) return MTR_OK;
   const int64_t need = mtr_lmhead_i8_workspace(a->rows, a->d_model);
-  if (!a->hidden || !a->weight || !a->weight_scale || !a->logits || (need > 0 && !a->workspace)) return MTR_ERR_NULL_ARG;
+  if (!a->hidden || !a->weight || !a->weight_scale || !a->logits || !a->workspace) return MTR_ERR_NULL_ARG;
   if (a->hidden_row_stride < a->d_model || a->weight_row_stride < a->d_model || a->logits_row_stride < a->vocab)
     return MTR_ERR_BAD_SHAPE;
   if (a->workspace_bytes < need) return MTR_ERR_BAD_SHAPE;
@@ -861,10 +784,9 @@ int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* a) {
   const int64_t hs = span(a->rows, a->hidden_row_stride, a->d_model, esize(a->hidden_dtype));
   const int64_t ws = span(a->vocab, a->weight_row_stride, a->d_model, 1);
   if (overlap(a->logits, ls, a->hidden, hs) || overlap(a->logits, ls, a->weight, ws) ||
-      overlap(a->logits, ls, a->weight_scale, 4ll * a->vocab))
-    return MTR_ERR_BAD_PARAM;
-  if (need > 0 && (overlap(a->logits, ls, a->workspace, need) || overlap(a->workspace, need, a->hidden, hs) ||
-                   overlap(a->workspace, need, a->weight, ws) || overlap(a->workspace, need, a->weight_scale, 4ll * a->vocab)))
+      overlap(a->logits, ls, a->weight_scale, 4ll * a->vocab) || overlap(a->logits, ls, a->workspace, need) ||
+      overlap(a->workspace, need, a->hidden, hs) || overlap(a->workspace, need, a->weight, ws) ||
+      overlap(a->workspace, need, a->weight_scale, 4ll * a->vocab))
     return MTR_ERR_BAD_PARAM;
   return MTR_OK;
 }
@@ -873,9 +795,7 @@ static int lmhead_i8_launch_impl(const MtrLmHeadI8Args* a, cudaStream_t s) {
   int8_t* q = (int8_t*)a->workspace;
   const int64_t q_stride = up(a->d_model, 16);
   float* scale = (float*)(q + up(a->rows * q_stride, 256));
-  cudaError_t e = cudaSuccess;
-  if (!quantised_here(a->rows, a->d_model))
-    e = launch_quantize(a->hidden, a->hidden_row_stride, a->hidden_dtype, a->rows, a->d_model, q, q_stride, scale, s);
+  cudaError_t e = launch_quantize(a->hidden, a->hidden_row_stride, a->hidden_dtype, a->rows, a->d_model, q, q_stride, scale, s);
   if (e == cudaSuccess) {
     switch (a->logits_dtype) {
       case MTR_DTYPE_F32: e = launch_proj<float>(*a, q, q_stride, scale, s); break;

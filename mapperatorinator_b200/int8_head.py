@@ -83,7 +83,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: torch.Tensor,
-                   out: torch.Tensor) -> tuple[N.MtrLmHeadI8Args, torch.Tensor | None]:
+                   out: torch.Tensor) -> tuple[N.MtrLmHeadI8Args, torch.Tensor]:
     """The launch arguments and the workspace they point to (to be kept until the launch)."""
     hs, ws, ls = matrix(hidden, "hidden"), matrix(weight_q, "weight_q", (torch.int8,)), matrix(out, "logits")
     device = hidden.device
@@ -99,12 +99,12 @@ def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: t
         raise ValueError("logits must be [hidden rows, vocab]")
     if vocab == 1:
         ws = (d + 15) // 16 * 16
-    need = N.lmhead_i8_workspace(rows, d)  # 0 for few rows
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    need = N.lmhead_i8_workspace(rows, d)
+    work = torch.empty(need, dtype=torch.uint8, device=device)
     a = N.sized(N.MtrLmHeadI8Args, hidden=hidden.data_ptr(), hidden_row_stride=hs, weight=weight_q.data_ptr(),
                 weight_row_stride=ws, weight_scale=weight_scale.data_ptr(), logits=out.data_ptr(), logits_row_stride=ls,
                 hidden_dtype=_DTYPES[hidden.dtype], logits_dtype=_DTYPES[out.dtype], rows=rows, d_model=d, vocab=vocab,
-                workspace=work.data_ptr() if need else None, workspace_bytes=need)
+                workspace=work.data_ptr(), workspace_bytes=need)
     return a, work
 
 

@@ -80,7 +80,7 @@ def _proj_args():
     (dict(d_model=0), N.ERR_BAD_SHAPE), (dict(d_model=N.MAX_I8_D_MODEL + 1), N.ERR_BAD_SHAPE), (dict(vocab=0), N.ERR_BAD_SHAPE),
     (dict(vocab=N.MAX_VOCAB + 1), N.ERR_BAD_SHAPE), (dict(hidden_dtype=3), N.ERR_BAD_PARAM), (dict(logits_dtype=-1), N.ERR_BAD_PARAM),
     (dict(weight=None), N.ERR_NULL_ARG), (dict(weight_scale=None), N.ERR_NULL_ARG), (dict(workspace=None), N.ERR_NULL_ARG),
-    (dict(workspace_bytes=900 * 112), N.ERR_BAD_SHAPE), (dict(rows=9, workspace=None, workspace_bytes=0), N.OK), (dict(workspace=0x5000010), N.ERR_ALIGNMENT),
+    (dict(workspace_bytes=900 * 112), N.ERR_BAD_SHAPE), (dict(workspace=0x5000010), N.ERR_ALIGNMENT),
     (dict(weight_row_stride=104), N.ERR_ALIGNMENT), (dict(weight=0x2000008), N.ERR_ALIGNMENT),
     (dict(weight_row_stride=96), N.ERR_BAD_SHAPE), (dict(logits_row_stride=76), N.ERR_BAD_SHAPE),
     (dict(hidden_row_stride=99), N.ERR_BAD_SHAPE), (dict(logits=0x1000000), N.ERR_BAD_PARAM),
@@ -112,8 +112,8 @@ def test_projection_and_sampler_must_share_the_logits():
 
 def test_workspace_sizes():
     assert N.lmhead_i8_workspace(0, 64) == 0 and N.lmhead_i8_workspace(4, 0) == 0
-    assert N.lmhead_i8_workspace(3, 100) == 0  # quantised by the projection itself
-    assert N.lmhead_i8_workspace(301, 100) == 33792 + 1204  # rows of 112 bytes, the scales on the next 256-byte boundary
+    assert N.lmhead_i8_workspace(3, 100) == 512 + 12  # 3 rows of 112 bytes, the scales on the next 256-byte boundary
+    assert N.lmhead_i8_workspace(301, 100) == 33792 + 1204
     assert N.lmhead_i8_workspace(N.MAX_I8_ROWS, N.MAX_I8_D_MODEL) == (1 << 39) + (1 << 24)
 
 
@@ -241,7 +241,7 @@ def test_strides_and_what_lies_behind(cuda_device, out_dtype, vocab, stride, off
     assert got is out
     assert torch.equal(out, lm_head_logits_int8(h, weight.q, weight.scale, out_dtype=out_dtype))
     few = lm_head_logits_int8(wide_h[:7, 51:251], wide_w[:, :d], weight.scale, out_dtype=out_dtype)
-    assert torch.equal(out[:7], few)  # few rows take another way to the same bits
+    assert torch.equal(out[:7], few)
     rest = torch.ones_like(buf, dtype=torch.bool)
     rest[offset:].as_strided((rows, vocab), (stride, 1)).fill_(False)
     assert bool((buf[rest] == 7.0).all())  # columns behind the vocabulary and rows behind the last
