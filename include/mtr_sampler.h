@@ -319,7 +319,7 @@ typedef struct MtrQuantizeArgs {
   int64_t x_row_stride;         /* elements */
   int32_t x_dtype;              /* MtrDType */
   int32_t rows;
-  int32_t cols;                 /* >= 1 */
+  int32_t cols;                 /* 1 .. MTR_MAX_I8_D_MODEL */
   int32_t reserved0;
   int8_t* q;                    /* [rows, cols] */
   int64_t q_row_stride;         /* bytes; bytes past cols are left as they are */

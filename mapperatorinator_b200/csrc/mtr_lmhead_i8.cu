@@ -736,7 +736,7 @@ using namespace mtr::i8;
 int mtr_quantize_rows_validate(const MtrQuantizeArgs* a) {
   if (!a) return MTR_ERR_NULL_ARG;
   if (a->abi_version != MTR_ABI_VERSION || a->struct_size != sizeof(MtrQuantizeArgs)) return MTR_ERR_ABI;
-  if (a->rows < 0 || a->cols < 1) return MTR_ERR_BAD_SHAPE;
+  if (a->rows < 0 || a->cols < 1 || a->cols > MTR_MAX_I8_D_MODEL) return MTR_ERR_BAD_SHAPE;
   if (!dtype_ok(a->x_dtype)) return MTR_ERR_BAD_PARAM;
   if (a->rows == 0) return MTR_OK;
   if (!a->x || !a->q || !a->scale) return MTR_ERR_NULL_ARG;

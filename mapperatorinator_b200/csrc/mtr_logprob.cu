@@ -189,7 +189,8 @@ template <int W>
 struct Shared {
   static constexpr int LIST = 64 * (W + 1);  // candidates of a row's alternatives
   u64 list[LIST];
-  u64 best[MTR_MAX_TOP_N];  // a cluster CTA's own n largest
+  u64 best[MTR_MAX_TOP_N];  // a cluster CTA's own n largest, and how many they are
+  int best_count;
   u64 bound[2];
   // by the row's parity: a warp may be a row ahead of another
   Part part[2][W];
@@ -258,8 +259,8 @@ __device__ __forceinline__ int place_of(const u64* list, int c, u64 k) {
 // of a warp, the best warp's taken, and the smallest over all warps of the r-th
 // largest lm, r n-th part of the warps (n <= r warps).  (The n-th of 32 maxima
 // is a poor bound when n is near 32; then a lane keeps two maxima.)  The larger
-// of the two leaves about n to 3 n lanes with lm >= T, whose vectors are read again (from
-// L2) for the list of candidates, which are ranked by comparing all pairs.  A
+// of the two leaves about n to 3 n lanes with lm >= T, whose vectors are read again
+// (from L2) for the list of candidates, which are ranked by comparing all pairs.  A
 // list that overflows (many equal logits) still holds more than n candidates:
 // the n-th of them is a better T, and the candidates are looked for again.
 template <typename T, int W>
@@ -546,13 +547,13 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
         const int place = place_of(sh.list, c, k);
         if (place < n) sh.best[place] = k;
       }
-      if (tid == 0) sh.count[parity] = min(c, n);
+      if (tid == 0) sh.best_count = min(c, n);
       cluster.sync();
       if (rank == 0) {
         c = 0;
         for (int k = 0; k < cs; ++k) {
           const Shared<W>* other = cluster.map_shared_rank(&sh, k);
-          const int more = other->count[parity];
+          const int more = other->best_count;
           for (int i = tid; i < more; i += THREADS) sh.list[c + i] = other->best[i];
           c += more;
         }

@@ -56,6 +56,7 @@ def _quant_args(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     ({}, N.OK), (dict(rows=0, x=None), N.OK), (dict(rows=-1), N.ERR_BAD_SHAPE), (dict(cols=0), N.ERR_BAD_SHAPE),
+    (dict(cols=N.MAX_I8_D_MODEL + 1), N.ERR_BAD_SHAPE),
     (dict(x_row_stride=63), N.ERR_BAD_SHAPE), (dict(q_row_stride=63), N.ERR_BAD_SHAPE), (dict(x_dtype=5), N.ERR_BAD_PARAM),
     (dict(q=None), N.ERR_NULL_ARG), (dict(scale=None), N.ERR_NULL_ARG), (dict(x=0x100001), N.ERR_ALIGNMENT),
     (dict(scale=0x300002), N.ERR_ALIGNMENT), (dict(q=0x100010), N.ERR_BAD_PARAM), (dict(struct_size=1), N.ERR_ABI)])

@@ -251,7 +251,8 @@ gpu = pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocab,top_n", [
     (1, 1, 0), (1, 1, 3), (3, 2, 2), (5, 7, 8), (2, 31, 5), (4, 33, 1), (3, 255, 20), (7, 257, 32), (130, 1000, 5), (64, 4096, 8),
-    (9, 4099, 20), (500, 4096, 0), (5, 8192, 32), (3, 32771, 8), (20, 65536, 1), (2, 131072, 32), (1, 131071, 5), (300, 5000, 4)])
+    (9, 4099, 20), (500, 4096, 0), (5, 8192, 32), (3, 32771, 8), (20, 65536, 1), (2, 131072, 32), (1, 131071, 5), (300, 5000, 4),
+    (2500, 300, 32), (2400, 4096, 30), (2400, 2100, 4), (1300, 9000, 28), (40, 131072, 25)])
 def test_forward(cuda_device, dtype, rows, vocab, top_n):
     logits, tokens = inputs(cuda_device, rows, vocab, dtype, seed=rows + vocab)
     check_forward(token_logprobs(logits, tokens, top_n=top_n), logits, tokens, top_n)
@@ -311,6 +312,24 @@ def test_rows_that_masks_and_values_make_odd(cuda_device, dtype, vocab, top_n):
     want[16] |= N.ROW_BAD_ID
     assert torch.equal(status.long(), want)
     assert S.row_status_report(status)["bad_id"] == [16]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,top_n", [(3, 131072, 32), (2, 65536, 3), (2400, 4096, 32), (150, 20000, 20)])
+def test_alternatives_where_candidates_crowd(cuda_device, dtype, rows, vocab, top_n):
+    # few distinct values, many ties at the bound, and rows whose largest logits all lie in one thread's vectors
+    g = torch.Generator(device=cuda_device).manual_seed(rows)
+    x = torch.randint(0, 4, (rows, vocab), generator=g, device=cuda_device).float()
+    x[1] = 0.5
+    x[0] = torch.arange(vocab, device=cuda_device) * 2.0 ** -7
+    for step in (32 * 8, 32 * 4, 128 * 8, 128 * 4, 256 * 8, 256 * 4):  # the stride of a thread's vectors, by warps and type
+        if step < vocab:
+            x[rows - 1, ::step] = 5.0
+            x[rows - 1, 1::step] = 6.0
+    x = x.to(dtype)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=cuda_device)
+    check_forward(token_logprobs(x, t, top_n=top_n), x, t, top_n)
 
 
 @gpu
