@@ -22,7 +22,7 @@ using namespace tc;
 constexpr int BM = 128;  // rows of a CTA's tile
 constexpr int BK = 128;  // int8 elements of one 128-byte swizzled row
 constexpr int UK = 32;   // K of one tcgen05.mma kind::i8
-constexpr int QUANT_THREADS = 256;
+constexpr int QUANT_THREADS = 128;
 
 struct QuantParams {
   const void* x;
@@ -107,13 +107,14 @@ __device__ __forceinline__ void quotients(const float (&x)[N], const Divisor& d,
   }
 }
 
-// Rows to int8: threads_per_row threads (a power of two, 32 .. 256) hold a row's
-// first QUANT_VECS vectors each between the two passes over it (the largest
-// magnitude, the quotients); longer rows are read again from L2.  HBM bounds it:
-// 3 bytes a bf16 value.  VEC: rows of x and q allow 16-byte loads and stores of
-// as many quotients; else every value is its own access.
-constexpr int QUANT_VECS = 4;
-template <typename T, bool VEC>
+// Rows to int8: threads_per_row threads (a power of two, 32 .. 128) hold a row's
+// first HOLD vectors each between the two passes over it (the largest magnitude,
+// the quotients); longer rows are read again from L2.  HBM bounds it: 3 bytes a
+// bf16 value.  VEC: rows of x and q allow 16-byte loads and stores of as many
+// quotients; else every value is its own access.  HOLD is 4 where a warp's 4
+// vectors a lane hold a row, else 8 (us, 4 / 8, floor): 8192 x 768 bf16 4.9 / 6.6,
+// 2.9; 8192 x 4096 bf16 20.3 / 18.8, 15.4; 131072 x 1024 fp32 119 / 94, 102.
+template <typename T, bool VEC, int HOLD>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantParams p) {
   constexpr int E = VEC ? Vec<T>::E : 1;
   __shared__ float tops[QUANT_THREADS / 32];
@@ -125,28 +126,28 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantPara
   int8_t* q = p.q + (live ? row : 0) * p.q_stride;
   const int vecs = live ? p.cols / E : 0, behind = vecs * E, rest = live ? p.cols - behind : 0;
   float top = 0.0f;
-  uint4 w[QUANT_VECS];
-  T one[QUANT_VECS];
+  uint4 w[HOLD];
+  T one[HOLD];
   if (VEC) {
 #pragma unroll
-    for (int j = 0; j < QUANT_VECS; ++j) {
+    for (int j = 0; j < HOLD; ++j) {
       w[j] = make_uint4(0u, 0u, 0u, 0u);
       const int i = tid + j * per;
       if (i < vecs) w[j] = reinterpret_cast<const uint4*>(x)[i];
     }
 #pragma unroll
-    for (int j = 0; j < QUANT_VECS; ++j) top = max_nan(top, magnitude(w[j], T()));
-    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) top = max_nan(top, magnitude(reinterpret_cast<const uint4*>(x)[i], T()));
+    for (int j = 0; j < HOLD; ++j) top = max_nan(top, magnitude(w[j], T()));
+    for (int i = tid + HOLD * per; i < vecs; i += per) top = max_nan(top, magnitude(reinterpret_cast<const uint4*>(x)[i], T()));
     if (tid < rest) top = max_nan(top, fabsf(to_f(x[behind + tid])));
   } else {
 #pragma unroll
-    for (int j = 0; j < QUANT_VECS; ++j) {
+    for (int j = 0; j < HOLD; ++j) {
       const int i = tid + j * per;
       one[j] = i < vecs ? x[i] : from_f<T>(0.0f);
     }
 #pragma unroll
-    for (int j = 0; j < QUANT_VECS; ++j) top = max_nan(top, fabsf(to_f(one[j])));
-    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) top = max_nan(top, fabsf(to_f(x[i])));
+    for (int j = 0; j < HOLD; ++j) top = max_nan(top, fabsf(to_f(one[j])));
+    for (int i = tid + HOLD * per; i < vecs; i += per) top = max_nan(top, fabsf(to_f(x[i])));
   }
   asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
   if (per > 32) {
@@ -167,15 +168,15 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantPara
       else reinterpret_cast<uint32_t*>(q)[i] = b[0];
     };
 #pragma unroll
-    for (int j = 0; j < QUANT_VECS; ++j)
+    for (int j = 0; j < HOLD; ++j)
       if (tid + j * per < vecs) put(tid + j * per, w[j]);
-    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) put(i, reinterpret_cast<const uint4*>(x)[i]);
+    for (int i = tid + HOLD * per; i < vecs; i += per) put(i, reinterpret_cast<const uint4*>(x)[i]);
     if (tid < rest) q[behind + tid] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[behind + tid]), d);
   } else {
 #pragma unroll
-    for (int j = 0; j < QUANT_VECS; ++j)
+    for (int j = 0; j < HOLD; ++j)
       if (tid + j * per < vecs) q[tid + j * per] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(one[j]), d);
-    for (int i = tid + QUANT_VECS * per; i < vecs; i += per) q[i] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[i]), d);
+    for (int i = tid + HOLD * per; i < vecs; i += per) q[i] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[i]), d);
   }
 }
 
@@ -639,16 +640,21 @@ static cudaError_t launch_quantize(const void* x, int64_t x_stride, int dtype, i
   const bool vec = (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0 && (uintptr_t)q % e == 0 && q_stride % e == 0;
   const int64_t units = vec ? cols / e : cols;
   int per = 32;
-  while (per < QUANT_THREADS && units > (int64_t)per * QUANT_VECS) per *= 2;
+  const bool wide = vec && units > 32 * 4;
+  while (per < QUANT_THREADS && units > (int64_t)per * (wide ? 8 : 4)) per *= 2;
   const QuantParams p{x, x_stride, rows, cols, per, q, q_stride, scale};
   cudaLaunchAttribute attr[2];
   const int high = QUANT_THREADS / per;
   const cudaLaunchConfig_t cfg = config(dim3((unsigned)((rows + high - 1) / high), 1, 1), QUANT_THREADS, 0, 1, s, attr);
+  auto launch = [&](auto of, auto wide_of, auto single) {
+    return cudaLaunchKernelEx(&cfg, wide ? wide_of : vec ? of : single, p);
+  };
   switch (dtype) {
-    case MTR_DTYPE_F32: return cudaLaunchKernelEx(&cfg, vec ? quantize_kernel<float, true> : quantize_kernel<float, false>, p);
+    case MTR_DTYPE_F32: return launch(quantize_kernel<float, true, 4>, quantize_kernel<float, true, 8>, quantize_kernel<float, false, 4>);
     case MTR_DTYPE_BF16:
-      return cudaLaunchKernelEx(&cfg, vec ? quantize_kernel<__nv_bfloat16, true> : quantize_kernel<__nv_bfloat16, false>, p);
-    default: return cudaLaunchKernelEx(&cfg, vec ? quantize_kernel<__half, true> : quantize_kernel<__half, false>, p);
+      return launch(quantize_kernel<__nv_bfloat16, true, 4>, quantize_kernel<__nv_bfloat16, true, 8>,
+                    quantize_kernel<__nv_bfloat16, false, 4>);
+    default: return launch(quantize_kernel<__half, true, 4>, quantize_kernel<__half, true, 8>, quantize_kernel<__half, false, 4>);
   }
 }
 
