@@ -180,13 +180,29 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantPara
   }
 }
 
-__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
-      : "memory");
+// One product, operands as the low words of their shared-memory descriptors: the
+// high word is the same for every tile of this layout (sw128_desc), and a stage
+// or a step of K moves the low word by its bytes / 16.
+template <int CG>
+__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc)
+        : "memory");
 }
 
 // Instruction descriptor of kind::i8: int32 accumulator (bits 4-5 = 2), signed A
@@ -228,8 +244,9 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 //                      in shared memory (16-byte pieces XOR-swizzled by row) and
 //                      sends them by TMA, or row by row where rows of logits are
 //                      not 16-byte aligned
-// Every wait is bounded; one that gives up sets the error word and ends the
-// CTA's loops, which then gives its copies time to land and returns.
+// Every wait is bounded; a role whose wait gives up sets the error word and stops,
+// so that the others' waits give up too; the producer then gives its copies time
+// to land, and the CTA returns.
 constexpr int EPI = 8;  // epilogue warps
 constexpr int PROJ_THREADS = 64 + 32 * EPI;
 
@@ -274,14 +291,6 @@ __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, int
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
           smem_u32(dst)),
       "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
       : "memory");
 }
 // arrives on the barrier at this offset in both CTAs of the pair
@@ -336,7 +345,6 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   struct Fixed {
     uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
     uint32_t tmem_slot;
-    volatile uint32_t abort_flag;
     __align__(16) float col_scale[EPI][64];
   };
   static_assert(sizeof(Fixed) <= G::FIXED, "fixed part of the shared memory");
@@ -344,7 +352,6 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t ring[];
   Fixed& fx = *reinterpret_cast<Fixed*>(ring + (size_t)S * G::STAGE_BYTES + G::OUT_BYTES);
   uint64_t *const full = fx.full, *const empty = fx.empty, *const acc_full = fx.acc_full, *const acc_empty = fx.acc_empty;
-  volatile uint32_t& abort_flag = fx.abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = CG > 1 ? (int)(blockIdx.x % CG) : 0;  // within the pair
@@ -363,7 +370,6 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], EPI * CG);
     }
-    abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -425,11 +431,9 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     uint32_t it = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (!mbar_wait(bar, parity, WAIT_NS)) {
-        abort_flag = 1u;
-        if (p.err) atomicOr(p.err, 1u);
-      }
-      return abort_flag == 0u;
+      if (mbar_wait(bar, parity, WAIT_NS)) return true;
+      if (p.err) atomicOr(p.err, 1u);
+      return false;
     };
     for (int t = first; t < tiles && ok; t += step) {
       int m0, n0;
@@ -456,12 +460,14 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     uint32_t n = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (!mbar_wait(bar, parity, WAIT_NS)) {
-        abort_flag = 1u;
-        if (p.err) atomicOr(p.err, 2u);
-      }
-      return abort_flag == 0u;
+      if (mbar_wait(bar, parity, WAIT_NS)) return true;
+      if (p.err) atomicOr(p.err, 2u);
+      return false;
     };
+    // this thread feeds the tensor core alone, a stage of products every 512
+    // clocks at most: everything a stage needs is an addition to these
+    const uint64_t desc = sw128_desc(smem_u32(ring));
+    const uint32_t lo0 = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
     auto commit = [&](uint64_t* bar) {
       if (CG == 1) tc_commit(bar);
       else commit_pair(bar);
@@ -474,15 +480,10 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       for (int kb = 0; kb < KB; ++kb, turn.next(S)) {
         ok = wait(&full[turn.slot], turn.parity);
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t a0 = smem_u32(a_tile(turn.slot)), b0 = smem_u32(b_tile(turn.slot));
+        const uint32_t a_lo = lo0 + (uint32_t)turn.slot * (G::STAGE_BYTES >> 4), b_lo = a_lo + (G::A_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < BK / UK; ++k) {
-          if (CG == 1)
-            mma_i8(tmem + acc * BN, sw128_desc(a0 + k * UK), sw128_desc(b0 + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
-          else
-            mma_i8_pair(tmem + acc * BN, sw128_desc(a0 + k * UK), sw128_desc(b0 + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < BK / UK; ++k)
+          mma_i8<CG>(tmem + acc * BN, a_lo + k * (UK >> 4), b_lo + k * (UK >> 4), hi, idesc, k > 0 ? 1u : (uint32_t)kb);
         commit(&empty[turn.slot]);
       }
       if (!ok) break;
@@ -522,10 +523,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       if (lane == 0) waited = mbar_wait(&acc_full[acc], (n >> 1) & 1, WAIT_NS);
       waited = __shfl_sync(FULL, waited, 0) != 0;
       if (!waited) {
-        if (lane == 0) {
-          abort_flag = 1u;
-          if (p.err) atomicOr(p.err, 4u);
-        }
+        if (lane == 0 && p.err) atomicOr(p.err, 4u);
         break;
       }
       tc_fence_after();
