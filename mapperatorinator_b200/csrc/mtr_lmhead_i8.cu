@@ -540,6 +540,11 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
         for (int h = 0; h < CB / 32; ++h) cs[h * 32 + lane] = cs_now[g / 32 + h];
         __syncwarp();
         tmem_wait_ld();
+        if (g + CB >= PART) {  // the warp's part of the accumulator is in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));
+        }
         const u64 rs2 = pk2(rs, rs);
         constexpr int EP = 16 / (int)sizeof(Tout);
         uint4 w[PIECES];
@@ -586,9 +591,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
           __syncwarp();
         }
       }
-      tc_fence_before();  // the warp's part of the accumulator has been read
-      __syncwarp();
-      if (lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));
+      if (!live && lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));  // nothing to read here
     }
     if (p.store_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
