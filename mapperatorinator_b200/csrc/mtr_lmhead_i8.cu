@@ -226,11 +226,14 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 
 // Tiles of 128 rows x BN vocabulary ids for one CTA (CG = 1), or of 256 rows x BN
 // for a pair of CTAs (CG = 2) whose products run on both tensor cores at once:
-// each CTA loads its own 128 rows and half of the ids, and each half is read
-// by both, which halves the shared-memory traffic of the ids.  At BN = 256 a
-// 128-byte step of K costs an SM 512 clocks of products; one CTA alone would
-// write 48 KB and read 48 KB of shared memory meanwhile (192 B a clock, of 128
-// there are), one of a pair 32 KB each (128).
+// each CTA loads its own 128 rows and half of the ids, and each half serves both,
+// so a pair takes 64 KB a step of K out of L2 where two CTAs alone take 96.
+//
+// What bounds it: at d = 4096 the products (8192 x 4096 -> 16384 in 331 us without
+// the quantisation; twice the measured bf16 rate gives 337); at d = 768 the
+// epilogue, which takes about as long as a 128 x 256 tile's 3072 clocks of
+// products and is not wholly hidden behind them (24 us without the quantisation
+// for 8192 x 768 -> 4096, 19 with the epilogue's work left out).
 //
 // Persistent: a CTA (pair) takes tile after tile, with two accumulators in tensor
 // memory, so that one tile is scaled and stored while the next is multiplied.
@@ -709,20 +712,25 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   return cudaLaunchKernelEx(&cfg, kern, mh, mw, mo, p);
 }
 
-// The narrowest tiles that still make one round of CTAs, else pairs of CTAs on
-// 256 x 256 (one CTA on 128 x 256 where the rows fill half a pair).  us:
-//   2 x 768 -> 4096       32 ids 6.6, 64 6.8, 128 6.9, pair 8.9
-//   333 x 1001 -> 4099    32 16.1, 64 12.9, 128 11.2, pair 15.2
-//   8192 x 768 -> 4096    32 152, 64 82, 128 48, pair 33
+// The narrowest tiles that still make one round of CTAs; up to two rounds of 128 x
+// 256 tiles, those; else pairs of CTAs on 256 x 256, unless the rows would fill
+// half a pair only.  Measured with the quantisation (us, 148 SMs), ids a tile:
+//                         32     64     128    256    pair
+//   2 x 768 -> 4096       6.1    6.5    6.5    7.3    8.3
+//   333 x 1001 -> 4099    15.4   11.8   10.2   12.4   12.0
+//   700 x 1024 -> 4096    20.4   13.0   10.8   9.3    10.2
+//   512 x 768 -> 16384    33.6   20.1   14.3   11.7   12.4
+//   1000 x 768 -> 32000   114    60.8   36.1   30.4   27.1
+//   64 x 1024 -> 65536    40.8   23.1   16.0   12.8   20.1
 template <typename Tout>
 static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
   const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
-  auto fits = [&](int bn) { return m * ((a.vocab + bn - 1) / bn) <= sms; };
-  if (fits(32)) return launch_tiles<1, 32, Tout>(a, q, q_stride, row_scale, s);
-  if (fits(64)) return launch_tiles<1, 64, Tout>(a, q, q_stride, row_scale, s);
-  if (fits(128)) return launch_tiles<1, 128, Tout>(a, q, q_stride, row_scale, s);
-  return a.rows > BM ? launch_tiles<2, 256, Tout>(a, q, q_stride, row_scale, s)
-                     : launch_tiles<1, 256, Tout>(a, q, q_stride, row_scale, s);
+  auto tiles = [&](int bn) { return m * ((a.vocab + bn - 1) / bn); };
+  if (tiles(32) <= sms) return launch_tiles<1, 32, Tout>(a, q, q_stride, row_scale, s);
+  if (tiles(64) <= sms) return launch_tiles<1, 64, Tout>(a, q, q_stride, row_scale, s);
+  if (tiles(128) <= sms) return launch_tiles<1, 128, Tout>(a, q, q_stride, row_scale, s);
+  if (m == 1 || tiles(256) <= 2 * sms) return launch_tiles<1, 256, Tout>(a, q, q_stride, row_scale, s);
+  return launch_tiles<2, 256, Tout>(a, q, q_stride, row_scale, s);
 }
 
 static bool dtype_ok(int32_t dtype) { return dtype >= MTR_DTYPE_F32 && dtype <= MTR_DTYPE_F16; }
