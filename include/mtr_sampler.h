@@ -332,7 +332,7 @@ int mtr_quantize_rows_launch(const MtrQuantizeArgs* args, void* stream);
 /*
  * logits[r, v] = RN(RN32(RN32(float(sum_k q[r, k] * weight[v, k])) * scale[r]) * weight_scale[v])
  * with q, scale the quantised hidden states (quantised by this call, into the
- * workspace) and the sum exact in int32: mtr_lmhead_launch with a quarter to a
+ * workspace where there are more than a few rows) and the sum exact in int32: mtr_lmhead_launch with a quarter to a
  * half of its weight traffic and twice its tensor rate.
  */
 typedef struct MtrLmHeadI8Args {
@@ -351,13 +351,13 @@ typedef struct MtrLmHeadI8Args {
   int32_t d_model;              /* 1 .. MTR_MAX_I8_D_MODEL */
   int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
   int32_t reserved0;
-  void* workspace;              /* 256-byte aligned; one call's at a time */
-  int64_t workspace_bytes;      /* >= mtr_lmhead_i8_workspace(rows, d_model) */
+  void* workspace;              /* 256-byte aligned; one call's at a time; may be NULL where 0 bytes are needed */
+  int64_t workspace_bytes;      /* >= mtr_lmhead_i8_workspace(rows, d_model, vocab) */
   uint32_t* error_word;         /* device word or NULL: bits set when a bounded wait gave up */
 } MtrLmHeadI8Args;
 
-/* Workspace bytes of a call (0 for rows <= 0 or d_model <= 0). */
-int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model);
+/* Workspace bytes of a call (0 for few rows, and for rows <= 0 or d_model <= 0). */
+int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model, int32_t vocab);
 int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* args);
 int mtr_lmhead_i8_launch(const MtrLmHeadI8Args* args, void* stream);
 

@@ -297,7 +297,7 @@ EXPORTS = {
                                                 c_void_p]),
     "mtr_quantize_rows_validate": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeArgs)]),
     "mtr_quantize_rows_launch": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeArgs), c_void_p]),
-    "mtr_lmhead_i8_workspace": (c_int64, [c_int32, c_int32]),
+    "mtr_lmhead_i8_workspace": (c_int64, [c_int32, c_int32, c_int32]),
     "mtr_lmhead_i8_validate": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args)]),
     "mtr_lmhead_i8_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args), c_void_p]),
     "mtr_lmhead_i8_sample_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args), ctypes.POINTER(MtrSamplerArgs),
@@ -441,8 +441,8 @@ def quantize_rows_launch(args: MtrQuantizeArgs, stream: int | None) -> None:
     check(load().mtr_quantize_rows_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_quantize_rows_launch")
 
 
-def lmhead_i8_workspace(rows: int, d_model: int) -> int:
-    return load().mtr_lmhead_i8_workspace(rows, d_model)
+def lmhead_i8_workspace(rows: int, d_model: int, vocab: int) -> int:
+    return load().mtr_lmhead_i8_workspace(rows, d_model, vocab)
 
 
 def lmhead_i8_launch(args: MtrLmHeadI8Args, stream: int | None) -> None:

@@ -20,9 +20,10 @@ CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmtr_sampler.so"
 SOURCES = [CSRC / "mtr_sampler.cu", CSRC / "mtr_stream.cu", CSRC / "mtr_stream_bf16.cu", CSRC / "mtr_stream_f16.cu",
-           CSRC / "mtr_stream_f32.cu", CSRC / "mtr_lmhead.cu", CSRC / "mtr_lmhead_i8.cu", CSRC / "mtr_logprob.cu"]
+           CSRC / "mtr_stream_f32.cu", CSRC / "mtr_lmhead.cu", CSRC / "mtr_lmhead_i8.cu",
+           CSRC / "mtr_lmhead_few.cu", CSRC / "mtr_logprob.cu"]
 HEADERS = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh", CSRC / "mtr_stream.cuh",
-           CSRC / "mtr_tc.cuh", CSRC / "mtr_vec.cuh"]
+           CSRC / "mtr_tc.cuh", CSRC / "mtr_vec.cuh", CSRC / "mtr_quant.cuh"]
 BUILD_DIR = PKG_DIR / "_build"
 
 COMPILE_FLAGS = [
@@ -50,14 +51,15 @@ def _nvcc() -> str:
 
 def _deps(src: Path) -> list:
     """Headers a translation unit includes (the stream kernel's also include mtr_stream.cuh, the
-    projections' mtr_tc.cuh, the row-streaming kernels' mtr_vec.cuh)."""
+    projections' mtr_tc.cuh, the row-streaming kernels'
+    mtr_vec.cuh and mtr_quant.cuh)."""
     deps = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh"]
     if src.name.startswith("mtr_stream"):
         deps.append(CSRC / "mtr_stream.cuh")
     if src.name.startswith("mtr_lmhead"):
         deps.append(CSRC / "mtr_tc.cuh")
-    if src.name in ("mtr_lmhead_i8.cu", "mtr_logprob.cu"):
-        deps.append(CSRC / "mtr_vec.cuh")
+    if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu", "mtr_logprob.cu"):
+        deps += [CSRC / "mtr_vec.cuh", CSRC / "mtr_quant.cuh"]
     return deps
 
 

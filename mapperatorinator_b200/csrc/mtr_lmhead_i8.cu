@@ -11,8 +11,8 @@
 // to the logits' type.
 #include <type_traits>
 
+#include "mtr_quant.cuh"
 #include "mtr_tc.cuh"
-#include "mtr_vec.cuh"
 
 namespace mtr {
 namespace i8 {
@@ -49,135 +49,20 @@ struct ProjParams {
   uint32_t* err;
 };
 
-__device__ __forceinline__ float magnitude(const uint4& w, float) {
-  return max_nan(max_nan(fabsf(__uint_as_float(w.x)), fabsf(__uint_as_float(w.y))),
-                 max_nan(fabsf(__uint_as_float(w.z)), fabsf(__uint_as_float(w.w))));
-}
-template <typename T>
-__device__ __forceinline__ float magnitude(uint4 w, T) {
-  w.x &= 0x7fff7fffu;
-  w.y &= 0x7fff7fffu;
-  w.z &= 0x7fff7fffu;
-  w.w &= 0x7fff7fffu;
-  return Vec<T>::value(Vec<T>::top(w));
-}
-
-// The divisor of a row: q(x) = the byte of RNE(RN(x / s)).  With y = RN(1 / s),
-// q0 = RN(x y), r = RN(x - q0 s) (exact) and q1 = RN(q0 + r y), q1 is the
-// correctly rounded quotient (Markstein) unless s has an all-ones significand;
-// three steps, packed two values at a time.  Those scales, and the ones so
-// small that 1 / s or r could leave the normal range, divide instead.
-struct Divisor {
-  float s, inv;
-  bool zero, divide;
-};
-__device__ __forceinline__ Divisor divisor_of(float top) {
-  Divisor d;
-  d.s = top < pos_inf() ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
-  d.zero = !(d.s > 0.0f);
-  d.divide = d.s < 0x1p-90f || (__float_as_uint(d.s) & 0x7fffffu) == 0x7fffffu;
-  d.inv = d.zero || d.divide ? 0.0f : __fdiv_rn(1.0f, d.s);
-  return d;
-}
-constexpr float WHOLE = 12582912.0f;  // 1.5 2^23: y + WHOLE holds RNE(y) in its low bits, |y| < 2^22
-__device__ __forceinline__ uint32_t quotient(float x, const Divisor& d) {
-  return __float_as_uint(__fadd_rn(__fdiv_rn(x, d.s), WHOLE));
-}
-template <int N>
-__device__ __forceinline__ void quotients(const float (&x)[N], const Divisor& d, uint32_t (&w)[N / 4]) {
-  uint32_t b[N];
-  if (d.divide) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) b[e] = quotient(x[e], d);
-  } else {
-    const u64 y2 = pk2(d.inv, d.inv), ns2 = pk2(-d.s, -d.s), whole2 = pk2(WHOLE, WHOLE);
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-      const u64 x2 = pk2(x[e], x[e + 1]), q0 = mul2(x2, y2), q1 = fma2(fma2(q0, ns2, x2), y2, q0);
-      float lo, hi;
-      up2(add2(q1, whole2), lo, hi);
-      b[e] = __float_as_uint(lo);
-      b[e + 1] = __float_as_uint(hi);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    const uint32_t lo = __byte_perm(b[4 * i], b[4 * i + 1], 0x0040), hi = __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040);
-    w[i] = d.zero ? 0u : __byte_perm(lo, hi, 0x5410);
-  }
-}
-
-// Rows to int8: threads_per_row threads (a power of two, 32 .. 128) hold a row's
-// first HOLD vectors each between the two passes over it (the largest magnitude,
-// the quotients); longer rows are read again from L2.  HBM bounds it: 3 bytes a
-// bf16 value.  VEC: rows of x and q allow 16-byte loads and stores of as many
-// quotients; else every value is its own access.  HOLD is 4 where a warp's 4
-// vectors a lane hold a row, else 8 (us, 4 / 8, floor): 8192 x 768 bf16 4.9 / 6.6,
-// 2.9; 8192 x 4096 bf16 20.3 / 18.8, 15.4; 131072 x 1024 fp32 119 / 94, 102.
+// Rows to int8: threads_per_row threads (a power of two, 32 .. 128) take a row
+// (quantize_row).  HBM bounds it: 3 bytes a bf16 value.  HOLD is 4 where a warp's
+// 4 vectors a lane hold a row, else 8 (us, 4 / 8, floor): 8192 x 768 bf16 4.9 /
+// 6.6, 2.9; 8192 x 4096 bf16 20.3 / 18.8, 15.4; 131072 x 1024 fp32 119 / 94, 102.
 template <typename T, bool VEC, int HOLD>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantParams p) {
-  constexpr int E = VEC ? Vec<T>::E : 1;
   __shared__ float tops[QUANT_THREADS / 32];
   const int per = p.threads_per_row, sub = threadIdx.x / per, tid = threadIdx.x % per;
   wait_prior_grid();
   const int64_t row = (int64_t)blockIdx.x * (QUANT_THREADS / per) + sub;
   const bool live = row < p.rows;
-  const T* x = (const T*)p.x + (live ? row : 0) * p.x_stride;
-  int8_t* q = p.q + (live ? row : 0) * p.q_stride;
-  const int vecs = live ? p.cols / E : 0, behind = vecs * E, rest = live ? p.cols - behind : 0;
-  float top = 0.0f;
-  uint4 w[HOLD];
-  T one[HOLD];
-  if (VEC) {
-#pragma unroll
-    for (int j = 0; j < HOLD; ++j) {
-      w[j] = make_uint4(0u, 0u, 0u, 0u);
-      const int i = tid + j * per;
-      if (i < vecs) w[j] = reinterpret_cast<const uint4*>(x)[i];
-    }
-#pragma unroll
-    for (int j = 0; j < HOLD; ++j) top = max_nan(top, magnitude(w[j], T()));
-    for (int i = tid + HOLD * per; i < vecs; i += per) top = max_nan(top, magnitude(reinterpret_cast<const uint4*>(x)[i], T()));
-    if (tid < rest) top = max_nan(top, fabsf(to_f(x[behind + tid])));
-  } else {
-#pragma unroll
-    for (int j = 0; j < HOLD; ++j) {
-      const int i = tid + j * per;
-      one[j] = i < vecs ? x[i] : from_f<T>(0.0f);
-    }
-#pragma unroll
-    for (int j = 0; j < HOLD; ++j) top = max_nan(top, fabsf(to_f(one[j])));
-    for (int i = tid + HOLD * per; i < vecs; i += per) top = max_nan(top, fabsf(to_f(x[i])));
-  }
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
-  if (per > 32) {
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (int k = 0; k < per / 32; ++k) top = max_nan(top, tops[sub * (per / 32) + k]);
-  }
-  const Divisor d = divisor_of(top);
-  allow_dependents();
-  if (live && tid == 0) p.scale[row] = d.s;
-  if constexpr (VEC) {
-    auto put = [&](int i, const uint4& v) {
-      float f[E];
-      uint32_t b[E / 4];
-      Vec<T>::unpack(v, f);
-      quotients(f, d, b);
-      if constexpr (E == 8) reinterpret_cast<uint2*>(q)[i] = make_uint2(b[0], b[1]);
-      else reinterpret_cast<uint32_t*>(q)[i] = b[0];
-    };
-#pragma unroll
-    for (int j = 0; j < HOLD; ++j)
-      if (tid + j * per < vecs) put(tid + j * per, w[j]);
-    for (int i = tid + HOLD * per; i < vecs; i += per) put(i, reinterpret_cast<const uint4*>(x)[i]);
-    if (tid < rest) q[behind + tid] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[behind + tid]), d);
-  } else {
-#pragma unroll
-    for (int j = 0; j < HOLD; ++j)
-      if (tid + j * per < vecs) q[tid + j * per] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(one[j]), d);
-    for (int i = tid + HOLD * per; i < vecs; i += per) q[i] = d.zero ? (int8_t)0 : (int8_t)quotient(to_f(x[i]), d);
-  }
+  const float scale = quantize_row<T, VEC, HOLD>((const T*)p.x + (live ? row : 0) * p.x_stride, live ? p.cols : 0, per, sub, tid, tops,
+                                                 p.q + (live ? row : 0) * p.q_stride, [] { allow_dependents(); });
+  if (live && tid == 0) p.scale[row] = scale;
 }
 
 // One product, operands as the low words of their shared-memory descriptors: the
@@ -773,8 +658,8 @@ int mtr_quantize_rows_launch(const MtrQuantizeArgs* a, void* stream) {
   return e == cudaSuccess ? MTR_OK : MTR_ERR_CUDA;
 }
 
-int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model) {
-  if (rows <= 0 || d_model <= 0) return 0;
+int64_t mtr_lmhead_i8_workspace(int32_t rows, int32_t d_model, int32_t vocab) {
+  if (rows <= 0 || d_model <= 0 || few_rows(rows, d_model, vocab)) return 0;
   return up((int64_t)rows * up(d_model, 16), 256) + 4ll * rows;
 }
 
@@ -786,8 +671,8 @@ int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* a) {
   if (a->vocab < 1 || a->vocab > MTR_MAX_VOCAB) return MTR_ERR_BAD_SHAPE;
   if (!dtype_ok(a->hidden_dtype) || !dtype_ok(a->logits_dtype)) return MTR_ERR_BAD_PARAM;
   if (a->rows == 0) return MTR_OK;
-  const int64_t need = mtr_lmhead_i8_workspace(a->rows, a->d_model);
-  if (!a->hidden || !a->weight || !a->weight_scale || !a->logits || !a->workspace) return MTR_ERR_NULL_ARG;
+  const int64_t need = mtr_lmhead_i8_workspace(a->rows, a->d_model, a->vocab);
+  if (!a->hidden || !a->weight || !a->weight_scale || !a->logits || (need > 0 && !a->workspace)) return MTR_ERR_NULL_ARG;
   if (a->hidden_row_stride < a->d_model || a->weight_row_stride < a->d_model || a->logits_row_stride < a->vocab)
     return MTR_ERR_BAD_SHAPE;
   if (a->workspace_bytes < need) return MTR_ERR_BAD_SHAPE;
@@ -799,14 +684,20 @@ int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* a) {
   const int64_t hs = span(a->rows, a->hidden_row_stride, a->d_model, esize(a->hidden_dtype));
   const int64_t ws = span(a->vocab, a->weight_row_stride, a->d_model, 1);
   if (overlap(a->logits, ls, a->hidden, hs) || overlap(a->logits, ls, a->weight, ws) ||
-      overlap(a->logits, ls, a->weight_scale, 4ll * a->vocab) || overlap(a->logits, ls, a->workspace, need) ||
-      overlap(a->workspace, need, a->hidden, hs) || overlap(a->workspace, need, a->weight, ws) ||
-      overlap(a->workspace, need, a->weight_scale, 4ll * a->vocab))
+      overlap(a->logits, ls, a->weight_scale, 4ll * a->vocab))
+    return MTR_ERR_BAD_PARAM;
+  if (need > 0 && (overlap(a->logits, ls, a->workspace, need) || overlap(a->workspace, need, a->hidden, hs) ||
+                   overlap(a->workspace, need, a->weight, ws) || overlap(a->workspace, need, a->weight_scale, 4ll * a->vocab)))
     return MTR_ERR_BAD_PARAM;
   return MTR_OK;
 }
 
 static int lmhead_i8_launch_impl(const MtrLmHeadI8Args* a, cudaStream_t s) {
+  if (few_rows(a->rows, a->d_model, a->vocab)) {
+    const cudaError_t e = launch_few(*a, s);
+    mtr::set_last_cuda_error((int)e);
+    return e == cudaSuccess ? MTR_OK : MTR_ERR_CUDA;
+  }
   int8_t* q = (int8_t*)a->workspace;
   const int64_t q_stride = up(a->d_model, 16);
   float* scale = (float*)(q + up(a->rows * q_stride, 256));

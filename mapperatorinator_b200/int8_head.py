@@ -36,10 +36,11 @@ def matrix(t: torch.Tensor, what: str, dtypes=_DTYPES) -> int:
         raise ValueError(f"{what} must be a CUDA tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{what} dtype {t.dtype} is not supported ({', '.join(str(d)[6:] for d in dtypes)})")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError(f"{what} must be a 2-D tensor with unit column stride")
     # a single row's stride means nothing and may be anything
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    return stride[0] if shape[0] > 1 else max(shape[1], 1)
 
 
 def _same_device(t: torch.Tensor, device: torch.device, what: str) -> None:
@@ -83,7 +84,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: torch.Tensor,
-                   out: torch.Tensor) -> tuple[N.MtrLmHeadI8Args, torch.Tensor]:
+                   out: torch.Tensor) -> tuple[N.MtrLmHeadI8Args, torch.Tensor | None]:
     """The launch arguments and the workspace they point to (to be kept until the launch)."""
     hs, ws, ls = matrix(hidden, "hidden"), matrix(weight_q, "weight_q", (torch.int8,)), matrix(out, "logits")
     device = hidden.device
@@ -99,12 +100,12 @@ def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: t
         raise ValueError("logits must be [hidden rows, vocab]")
     if vocab == 1:
         ws = (d + 15) // 16 * 16
-    need = N.lmhead_i8_workspace(rows, d)
-    work = torch.empty(need, dtype=torch.uint8, device=device)
+    need = N.lmhead_i8_workspace(rows, d, vocab)  # 0 for few rows
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     a = N.sized(N.MtrLmHeadI8Args, hidden=hidden.data_ptr(), hidden_row_stride=hs, weight=weight_q.data_ptr(),
                 weight_row_stride=ws, weight_scale=weight_scale.data_ptr(), logits=out.data_ptr(), logits_row_stride=ls,
                 hidden_dtype=_DTYPES[hidden.dtype], logits_dtype=_DTYPES[out.dtype], rows=rows, d_model=d, vocab=vocab,
-                workspace=work.data_ptr(), workspace_bytes=need)
+                workspace=work.data_ptr() if need else None, workspace_bytes=need)
     return a, work
 
 

@@ -81,7 +81,8 @@ def _proj_args():
     (dict(d_model=0), N.ERR_BAD_SHAPE), (dict(d_model=N.MAX_I8_D_MODEL + 1), N.ERR_BAD_SHAPE), (dict(vocab=0), N.ERR_BAD_SHAPE),
     (dict(vocab=N.MAX_VOCAB + 1), N.ERR_BAD_SHAPE), (dict(hidden_dtype=3), N.ERR_BAD_PARAM), (dict(logits_dtype=-1), N.ERR_BAD_PARAM),
     (dict(weight=None), N.ERR_NULL_ARG), (dict(weight_scale=None), N.ERR_NULL_ARG), (dict(workspace=None), N.ERR_NULL_ARG),
-    (dict(workspace_bytes=900 * 112), N.ERR_BAD_SHAPE), (dict(workspace=0x5000010), N.ERR_ALIGNMENT),
+    (dict(workspace_bytes=900 * 112), N.ERR_BAD_SHAPE), (dict(rows=8, workspace=None, workspace_bytes=0), N.OK),
+    (dict(workspace=0x5000010), N.ERR_ALIGNMENT),
     (dict(weight_row_stride=104), N.ERR_ALIGNMENT), (dict(weight=0x2000008), N.ERR_ALIGNMENT),
     (dict(weight_row_stride=96), N.ERR_BAD_SHAPE), (dict(logits_row_stride=76), N.ERR_BAD_SHAPE),
     (dict(hidden_row_stride=99), N.ERR_BAD_SHAPE), (dict(logits=0x1000000), N.ERR_BAD_PARAM),
@@ -112,10 +113,11 @@ def test_projection_and_sampler_must_share_the_logits():
 
 
 def test_workspace_sizes():
-    assert N.lmhead_i8_workspace(0, 64) == 0 and N.lmhead_i8_workspace(4, 0) == 0
-    assert N.lmhead_i8_workspace(3, 100) == 512 + 12  # 3 rows of 112 bytes, the scales on the next 256-byte boundary
-    assert N.lmhead_i8_workspace(301, 100) == 33792 + 1204
-    assert N.lmhead_i8_workspace(N.MAX_I8_ROWS, N.MAX_I8_D_MODEL) == (1 << 39) + (1 << 24)
+    assert N.lmhead_i8_workspace(0, 64, 100) == 0 and N.lmhead_i8_workspace(4, 0, 100) == 0
+    assert N.lmhead_i8_workspace(3, 100, 4096) == 0  # few rows
+    assert N.lmhead_i8_workspace(3, 900, 131072) == 2816 + 12  # 3 rows of 912 bytes, the scales on the next 256-byte boundary
+    assert N.lmhead_i8_workspace(301, 100, 77) == 33792 + 1204
+    assert N.lmhead_i8_workspace(N.MAX_I8_ROWS, N.MAX_I8_D_MODEL, 1) == (1 << 39) + (1 << 24)
 
 
 def test_cpu_tensors_are_refused():
@@ -182,7 +184,9 @@ def test_quantize_strided_rows(cuda_device):
 @pytest.mark.parametrize("out_dtype", DTYPES)
 @pytest.mark.parametrize("rows,d,vocab,dtype", [
     (1, 1, 1, torch.float32), (1, 16, 8, torch.bfloat16), (8, 2048, 1000, torch.bfloat16), (5, 1001, 300, torch.float16),
-    (8, 100, 131072, torch.float32), (1, 8192, 77, torch.bfloat16), (1, 8193, 77, torch.bfloat16), (9, 64, 20000, torch.float32), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
+    (8, 100, 131072, torch.float32), (1, 8192, 77, torch.bfloat16), (1, 8193, 77, torch.bfloat16), (9, 64, 20000, torch.float32),
+    (3, 15, 3, torch.bfloat16), (4, 2048, 16000, torch.float32), (8, 513, 131072, torch.bfloat16), (2, 4096, 131072, torch.bfloat16),
+    (6, 1000, 999, torch.float16), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
     (33, 100, 77, torch.float16), (129, 1001, 4099, torch.float16), (300, 64, 520, torch.float32), (256, 128, 8192, torch.bfloat16),
     (513, 2048, 1000, torch.bfloat16), (1030, 96, 264, torch.float32), (64, 3000, 131072, torch.bfloat16)])
 def test_logits_equal_the_definition(cuda_device, out_dtype, rows, d, vocab, dtype):
@@ -241,8 +245,13 @@ def test_strides_and_what_lies_behind(cuda_device, out_dtype, vocab, stride, off
     got = lm_head_logits_int8(wide_h[:, 51:251], wide_w[:, :d], weight.scale, out)
     assert got is out
     assert torch.equal(out, lm_head_logits_int8(h, weight.q, weight.scale, out_dtype=out_dtype))
-    few = lm_head_logits_int8(wide_h[:7, 51:251], wide_w[:, :d], weight.scale, out_dtype=out_dtype)
+    few_buf = torch.full((offset + 9 * stride,), 7.0, dtype=out_dtype, device=cuda_device)
+    few = few_buf[offset:].as_strided((7, vocab), (stride, 1))
+    lm_head_logits_int8(wide_h[:7, 51:251], wide_w[:, :d], weight.scale, few)  # few rows: another kernel, the same bits
     assert torch.equal(out[:7], few)
+    rest = torch.ones_like(few_buf, dtype=torch.bool)
+    rest[offset:].as_strided((7, vocab), (stride, 1)).fill_(False)
+    assert bool((few_buf[rest] == 7.0).all())
     rest = torch.ones_like(buf, dtype=torch.bool)
     rest[offset:].as_strided((rows, vocab), (stride, 1)).fill_(False)
     assert bool((buf[rest] == 7.0).all())  # columns behind the vocabulary and rows behind the last
@@ -266,10 +275,11 @@ def test_refusals(cuda_device):
 
 
 @gpu
-def test_streams_and_graphs(cuda_device):
+@pytest.mark.parametrize("rows", [2, 130])
+def test_streams_and_graphs(cuda_device, rows):
     h, w = inputs(cuda_device, 130, 768, 1000, seed=9)
     weight = Int8Weight.from_weight(w)
-    call = lambda: lm_head_logits_int8(h, weight.q, weight.scale)  # noqa: E731
+    call = lambda: lm_head_logits_int8(h[:rows], weight.q, weight.scale)  # noqa: E731
     want = call()
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
