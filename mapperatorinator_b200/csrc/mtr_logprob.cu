@@ -224,10 +224,21 @@ __device__ __forceinline__ Span<T> span_of(const FwdParams& p, int64_t row, int 
   return r;
 }
 
-constexpr int TILE = 8;  // vectors of a thread's tile
+// Vectors of a thread's tile, and warps of an SM (so its registers).  A warp that
+// has a row to itself walks a long chain a row (joins, candidates) that other
+// warps must fill: more warps with smaller tiles of 32 scores a lane.  us, tiles
+// of 8 vectors and 16 warps / 4 and 24 (4 and 20, 4 and 28 lie between): 8192 x
+// 4096 bf16 18.2 / 16.8, with 8 alternatives 29.8 / 26.3; but fp32, whose 4
+// vectors are 16 scores, 33.7 / 34.7.  Rows shared by warps want the bytes in
+// flight: 1024 x 131072 fp32 81.4 / 114, 2000 x 65533 bf16 48.9 / 54.8.
+template <typename T, int W>
+struct Plan {
+  static constexpr int TILE = W == 1 ? 32 / Vec<T>::E : 8;
+  static constexpr int WARPS = W == 1 && Vec<T>::E == 8 ? 24 : 16;
+};
 
 // tile starting at vector t0 of the CTA's run; masked scores behind its end
-template <typename T, int THREADS>
+template <int THREADS, int TILE, typename T>
 __device__ __forceinline__ void load_tile(uint4 (&w)[TILE], const Span<T>& r, int t0, int tid) {
   const uint4* b = r.body() + t0 + tid;
   if (t0 + THREADS * TILE <= r.v1) {
@@ -264,9 +275,9 @@ __device__ __forceinline__ int place_of(const u64* list, int c, u64 k) {
 // list that overflows (many equal logits) still holds more than n candidates:
 // the n-th of them is a better T, and the candidates are looked for again.
 template <typename T, int W>
-__global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams p) {
+__global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(const FwdParams p) {
   typedef Vec<T> X;
-  constexpr int E = X::E, THREADS = W * 32;
+  constexpr int E = X::E, THREADS = W * 32, TILE = Plan<T, W>::TILE;
   __shared__ Shared<W> sh;
   constexpr int LIST = Shared<W>::LIST;
   const int tid = threadIdx.x, warp = W > 1 ? tid >> 5 : 0, lane = tid & 31;
@@ -284,7 +295,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
   wait_prior_grid();
   Span<T> sp = span_of<T>(p, row, rank);
   uint4 next[TILE];
-  load_tile<T, THREADS>(next, sp, sp.v0, tid);
+  load_tile<THREADS>(next, sp, sp.v0, tid);
 
   for (int parity = 0; row < p.rows; row += step, parity ^= 1) {
     // the token and its logit, needed last, are asked for first
@@ -380,10 +391,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) logprob_kernel(const FwdParams
     // the tile behind the one at t0 - THREADS TILE: this row's, or the next row's first
     auto ask = [&](uint4 (&w)[TILE], int t0) {
       if (t0 < sp.v1) {
-        load_tile<T, THREADS>(w, sp, t0, tid);
+        load_tile<THREADS>(w, sp, t0, tid);
       } else if (row + step < p.rows) {
         after = span_of<T>(p, row + step, rank);
-        load_tile<T, THREADS>(w, after, after.v0, tid);
+        load_tile<THREADS>(w, after, after.v0, tid);
       }
     };
     for (int t0 = sp.v0 + THREADS * TILE;; t0 += THREADS * TILE) {
@@ -722,7 +733,7 @@ static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
 
 // Warps and CTAs of a row, by how many rows there are to fill the device's 16
 // warps an SM and how long they are.  Measured (us, 148 SMs):
-//   8192 x 4096 bf16      1 warp 18.0, 2 23.0, 4 44.6     enough rows: a warp each
+//   8192 x 4096 bf16      1 warp 16.8, 2 23.0, 4 44.6     enough rows: a warp each
 //   2000 x 65533 bf16     1 warp 50.4, 2 52.6, 4 48.1, 8 57.3   long rows: 4
 //   1024 x 131072 fp32    1 warp 99.1, 2 81.7, 4 80.8, 8 83.6
 //   256 x 65536 fp16      1 warp 24.6, 4 11.4, 8 10.6, 4 CTAs of 8 25.8
