@@ -147,7 +147,7 @@ struct Geo {
   static constexpr int FIT = (int)((227 * 1024 - OUT_BYTES - FIXED) / STAGE_BYTES);
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + FIXED;
-  static constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // tensor-memory columns
+  static constexpr uint32_t COLS = 2 * BN;  // tensor-memory columns
 };
 
 // A position in a ring of barriers: its slot, and the parity of its next completion.
@@ -557,7 +557,7 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
       !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.weight, a.vocab, a.d_model, a.weight_row_stride, BK, BN / CG))
     return cudaErrorInvalidValue;
   const int es = sizeof(Tout);
-  const bool tma = BN * es >= 128 && (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
+  const bool tma = (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
   const CUtensorMapDataType type = std::is_same<Tout, float>::value           ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : std::is_same<Tout, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -600,18 +600,17 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
 // The narrowest tiles that still make one round of CTAs; up to two rounds of 128 x
 // 256 tiles, those; else pairs of CTAs on 256 x 256, unless the rows would fill
 // half a pair only.  Measured with the quantisation (us, 148 SMs), ids a tile:
-//                         32     64     128    256    pair
-//   2 x 768 -> 4096       6.1    6.5    6.5    7.3    8.3
-//   333 x 1001 -> 4099    15.4   11.8   10.2   12.4   12.0
-//   700 x 1024 -> 4096    20.4   13.0   10.8   9.3    10.2
-//   512 x 768 -> 16384    33.6   20.1   14.3   11.7   12.4
-//   1000 x 768 -> 32000   114    60.8   36.1   30.4   27.1
-//   64 x 1024 -> 65536    40.8   23.1   16.0   12.8   20.1
+//                         64     128    256    pair
+//   128 x 768 -> 4096     6.9    7.3    8.2    9.2      (tiles of 32: 7.1)
+//   333 x 1001 -> 4099    11.8   10.2   12.4   12.0
+//   700 x 1024 -> 4096    13.2   10.8   9.1    10.2
+//   512 x 768 -> 16384    20.2   14.4   11.8   12.5
+//   1000 x 768 -> 32000   60.8   35.7   29.7   27.0
+//   64 x 1024 -> 65536    23.1   16.1   12.3   20.4
 template <typename Tout>
 static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
   const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
   auto tiles = [&](int bn) { return m * ((a.vocab + bn - 1) / bn); };
-  if (tiles(32) <= sms) return launch_tiles<1, 32, Tout>(a, q, q_stride, row_scale, s);
   if (tiles(64) <= sms) return launch_tiles<1, 64, Tout>(a, q, q_stride, row_scale, s);
   if (tiles(128) <= sms) return launch_tiles<1, 128, Tout>(a, q, q_stride, row_scale, s);
   if (m == 1 || tiles(256) <= 2 * sms) return launch_tiles<1, 256, Tout>(a, q, q_stride, row_scale, s);
