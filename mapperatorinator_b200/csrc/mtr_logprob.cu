@@ -23,6 +23,8 @@
 // give NaN), and a score equal to the maximum, whose d is +0 = 0, becomes -1000
 // too and so leaves the sums: it is counted in n.  NaN is found by the maximum,
 // which keeps it.
+#include <float.h>
+
 #include "mtr_vec.cuh"
 
 namespace mtr {
@@ -254,6 +256,7 @@ __device__ __forceinline__ void load_tile(uint4 (&w)[TILE], const Span<T>& r, in
 // how many of list[0 .. c) are larger than k
 __device__ __forceinline__ int place_of(const u64* list, int c, u64 k) {
   int place = 0;
+#pragma unroll 4
   for (int j = 0; j < c; ++j) place += list[j] > k;
   return place;
 }
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
     if (W > 1) __syncthreads();
     else __syncwarp();
   };
-  if (tid < 2) sh.count[tid] = 0;
+  if (W > 1 && tid < 2) sh.count[tid] = 0;
   wait_prior_grid();
   Span<T> sp = span_of<T>(p, row, rank);
   uint4 next[TILE];
@@ -486,23 +489,29 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
     // candidates: keys of the scores that reach the bound
     u64 bound = order_key(fmaxf(nth, rth), 0xffffffffu);
     int c = 0;
-    if (tid == 0) sh.count[parity ^ 1] = 0;
+    if (W > 1 && tid == 0) sh.count[parity ^ 1] = 0;
     bool again = false;
+    float least = 0.0f;  // the bound's score; of masked scores none is a candidate
     auto list = [&](float f, int id) {
-      bool hit = f >= key_value(bound) && f > neg_inf();
+      bool hit = f >= least;
       if (again) hit = hit && order_key(f, (uint32_t)id) >= bound;
       const unsigned hits = __ballot_sync(FULL, hit);
       if (hits == 0) return;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&sh.count[parity], __popc(hits));
-      at = __shfl_sync(FULL, at, 0) + __popc(hits & ((1u << lane) - 1u));
+      int at = c;
+      if (W > 1) {
+        if (lane == 0) at = atomicAdd(&sh.count[parity], __popc(hits));
+        at = __shfl_sync(FULL, at, 0);
+      } else {
+        c += __popc(hits);
+      }
+      at += __popc(hits & ((1u << lane) - 1u));
       if (hit && at < LIST) sh.list[at] = order_key(f, (uint32_t)id);
     };
     while (!r.bad && !r.none) {
-      const float least = key_value(bound);
+      least = fmaxf(key_value(bound), -FLT_MAX);
       if (warp == 0 && rank == 0 && sp.head + tail > 0) list(single, single_id);
       const float top = fmaxf(lm[0], lm[1]);
-      const bool won = top >= least && top > neg_inf();
+      const bool won = top >= least;
       const unsigned winners = __ballot_sync(FULL, won);
       if (won) sh.winner[warp][__popc(winners & ((1u << lane) - 1u))] = (uint8_t)lane;
       __syncwarp();
@@ -524,7 +533,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float most = X::value(X::top(w[j]));
-            const bool hit = most >= least && most > neg_inf();
+            const bool hit = most >= least;
             const unsigned hits = __ballot_sync(FULL, hit);
             if (hit) sh.found[warp][found + __popc(hits & ((1u << lane) - 1u))] = (uint16_t)at[j];
             found += __popc(hits);
@@ -537,7 +546,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
           __syncwarp();
         }
       cta_sync();
-      c = sh.count[parity];
+      if (W > 1) c = sh.count[parity];
       if (c <= LIST) break;
       // overflow: the list's n-th key is the new bound (LIST > n, so the count falls)
       for (int i = tid; i < LIST; i += THREADS) {
@@ -548,7 +557,8 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       cta_sync();
       bound = sh.bound[parity];
       again = true;
-      if (tid == 0) sh.count[parity] = 0;
+      c = 0;
+      if (W > 1 && tid == 0) sh.count[parity] = 0;
       cta_sync();
     }
     if (cs > 1) {
