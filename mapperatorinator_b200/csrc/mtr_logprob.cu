@@ -23,8 +23,6 @@
 // give NaN), and a score equal to the maximum, whose d is +0 = 0, becomes -1000
 // too and so leaves the sums: it is counted in n.  NaN is found by the maximum,
 // which keeps it.
-#include <float.h>
-
 #include "mtr_vec.cuh"
 
 namespace mtr {
@@ -200,7 +198,6 @@ struct Shared {
   int count[2];     // candidates found (where they pass LIST, the list is not complete)
   Part cta;         // read by the cluster's other CTAs
   float cta_nth, cta_rth;
-  uint16_t found[W][128];
   uint8_t winner[W][32];
 };
 
@@ -508,7 +505,8 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       if (hit && at < LIST) sh.list[at] = order_key(f, (uint32_t)id);
     };
     while (!r.bad && !r.none) {
-      least = fmaxf(key_value(bound), -FLT_MAX);
+      least = fmaxf(key_value(bound), X::LOWEST);
+      const typename X::Top cut = X::pattern(least);
       if (warp == 0 && rank == 0 && sp.head + tail > 0) list(single, single_id);
       const float top = fmaxf(lm[0], lm[1]);
       const bool won = top >= least;
@@ -521,29 +519,25 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       const int count = __popc(winners);
       for (int first = 0; first < count; first += 8)
         for (int i0 = 0; i0 < most_of; i0 += 16) {
+          uint32_t reach = 0;  // bits 4 j ..: the j-th vector's
+          auto vector = [&](int j) {
+            const int who = first + 2 * j + (lane >> 4);
+            return who < count ? sp.v0 + warp * 32 + sh.winner[warp][who] + (i0 + (lane & 15)) * THREADS : sp.v1;
+          };
           uint4 w[4];
-          int at[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int who = first + 2 * j + (lane >> 4), i = i0 + (lane & 15);
-            at[j] = who < count ? sp.v0 + warp * 32 + sh.winner[warp][who] + i * THREADS : sp.v1;
-            w[j] = at[j] < sp.v1 ? body[at[j]] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+            const int at = vector(j);
+            w[j] = at < sp.v1 ? body[at] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
           }
-          int found = 0;  // vectors that hold a candidate
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float most = X::value(X::top(w[j]));
-            const bool hit = most >= least;
-            const unsigned hits = __ballot_sync(FULL, hit);
-            if (hit) sh.found[warp][found + __popc(hits & ((1u << lane) - 1u))] = (uint16_t)at[j];
-            found += __popc(hits);
+          for (int j = 0; j < 4; ++j) reach |= X::reach(w[j], cut) << (4 * j);
+          while (__any_sync(FULL, reach != 0u)) {  // one score a lane
+            const int bit = reach ? __ffs(reach) - 1 : 0;
+            const int id = sp.head + vector((bit >> 2) & 3) * E + (E == 8 ? 2 * (bit & 3) + (bit >> 4) : bit & 3);
+            list(reach ? to_f(sp.x[id]) : neg_inf(), id);
+            reach &= reach - 1;
           }
-          __syncwarp();
-          for (int k = 0; k < found * E; k += 32) {  // their scores, one a lane
-            const int slot = (k + lane) / E, id = slot < found ? sp.head + sh.found[warp][slot] * E + lane % E : -1;
-            list(id >= 0 ? to_f(sp.x[id]) : neg_inf(), id);
-          }
-          __syncwarp();
         }
       cta_sync();
       if (W > 1) c = sh.count[parity];

@@ -31,13 +31,15 @@ __device__ __forceinline__ u64 add2(u64 a, u64 b) {
   return d;
 }
 
-// 16 bytes of a row: E values, their packed maximum, their fp32 values.
+// 16 bytes of a row: E values, their packed maximum, their fp32 values; reach:
+// which of them are at least `cut`, value 2 k + h in bit k + 16 h (fp32: value k in bit k).
 template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int E = 4;
   static constexpr uint32_t FILL = 0xff800000u;  // -inf
+  static constexpr float LOWEST = -0x1.fffffep127f;
   typedef float Top;                             // the largest of a vector; NaN when one is
   static __device__ __forceinline__ Top top(const uint4& w) {
     return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
@@ -46,6 +48,10 @@ struct Vec<float> {
   static __device__ __forceinline__ float value(Top t) { return t; }
   static __device__ __forceinline__ Top pattern(float m) { return m; }
   static __device__ __forceinline__ bool has(Top t, Top m) { return t == m; }
+  static __device__ __forceinline__ uint32_t reach(const uint4& w, Top cut) {
+    return (__uint_as_float(w.x) >= cut ? 1u : 0u) | (__uint_as_float(w.y) >= cut ? 2u : 0u) |
+           (__uint_as_float(w.z) >= cut ? 4u : 0u) | (__uint_as_float(w.w) >= cut ? 8u : 0u);
+  }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&f)[E]) {
     f[0] = __uint_as_float(w.x);
     f[1] = __uint_as_float(w.y);
@@ -57,6 +63,7 @@ template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int E = 8;
   static constexpr uint32_t FILL = 0xff80ff80u;
+  static constexpr float LOWEST = -0x1.fep127f;
   typedef __nv_bfloat162 Top;
   static __device__ __forceinline__ Top pair(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
   static __device__ __forceinline__ Top top(const uint4& w) {
@@ -66,6 +73,10 @@ struct Vec<__nv_bfloat16> {
   static __device__ __forceinline__ float value(Top t) { return max_nan(__low2float(t), __high2float(t)); }
   static __device__ __forceinline__ Top pattern(float m) { return __float2bfloat162_rn(m); }
   static __device__ __forceinline__ bool has(Top t, Top m) { return __heq2_mask(t, m) != 0u; }
+  static __device__ __forceinline__ uint32_t reach(const uint4& w, Top cut) {
+    return (__hge2_mask(pair(w.x), cut) & 0x10001u) | (__hge2_mask(pair(w.y), cut) & 0x20002u) |
+           (__hge2_mask(pair(w.z), cut) & 0x40004u) | (__hge2_mask(pair(w.w), cut) & 0x80008u);
+  }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&f)[E]) {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -79,6 +90,7 @@ template <>
 struct Vec<__half> {
   static constexpr int E = 8;
   static constexpr uint32_t FILL = 0xfc00fc00u;
+  static constexpr float LOWEST = -65504.0f;
   typedef __half2 Top;
   static __device__ __forceinline__ Top pair(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
   static __device__ __forceinline__ Top top(const uint4& w) {
@@ -88,6 +100,10 @@ struct Vec<__half> {
   static __device__ __forceinline__ float value(Top t) { return max_nan(__low2float(t), __high2float(t)); }
   static __device__ __forceinline__ Top pattern(float m) { return __float2half2_rn(m); }
   static __device__ __forceinline__ bool has(Top t, Top m) { return __heq2_mask(t, m) != 0u; }
+  static __device__ __forceinline__ uint32_t reach(const uint4& w, Top cut) {
+    return (__hge2_mask(pair(w.x), cut) & 0x10001u) | (__hge2_mask(pair(w.y), cut) & 0x20002u) |
+           (__hge2_mask(pair(w.z), cut) & 0x40004u) | (__hge2_mask(pair(w.w), cut) & 0x80008u);
+  }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&f)[E]) {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
