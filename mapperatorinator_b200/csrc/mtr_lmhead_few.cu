@@ -16,6 +16,10 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MOST_ROWS = 8;
+// CTAs an SM, for whose registers four trips of a lane's loads are asked for at
+// once (2 x 4096 -> 16384: 13.4 us; with 3 CTAs, 15.7; with two trips and 80
+// registers, 18.9)
+constexpr int CTAS = 2;
 constexpr int HELD = 64 * 1024;  // bytes of int8 rows in shared memory at most
 
 struct FewParams {
@@ -47,7 +51,7 @@ __device__ __forceinline__ float hold_rows(const FewParams& p, int8_t* held, flo
 
 // R: rows, or the next power of two; VB: ids a warp takes at a time
 template <int R, int VB>
-__global__ void __launch_bounds__(THREADS) few_rows_kernel(const FewParams p) {
+__global__ void __launch_bounds__(THREADS, CTAS) few_rows_kernel(const FewParams p) {
   extern __shared__ __align__(16) int8_t held[];
   __shared__ float tops[WARPS], row_scale[R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -81,7 +85,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const FewParams p) {
                              __dp4a((int)b[k].z, (int)h.z, __dp4a((int)b[k].y, (int)h.y, __dp4a((int)b[k].x, (int)h.x, acc[r][k]))));
       }
     };
-#pragma unroll 2
+#pragma unroll 4
     for (int i = lane; i < full; i += 32) {
       uint4 b[VB];
 #pragma unroll
@@ -136,8 +140,7 @@ cudaError_t launch_rows(const FewParams& p, cudaStream_t s) {
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&]() { attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD); });
   if (attr_err[dev] != cudaSuccess) return attr_err[dev];
-  // two CTAs an SM keep the loads of a large vocabulary coming; more quantise the rows more often
-  const int64_t all = (p.vocab + WARPS * VB - 1) / (WARPS * VB), room = 2ll * device_sms();
+  const int64_t all = (p.vocab + WARPS * VB - 1) / (WARPS * VB), room = (int64_t)CTAS * device_sms();
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)(all < room ? all : room), 1, 1);
@@ -152,19 +155,25 @@ cudaError_t launch_rows(const FewParams& p, cudaStream_t s) {
 
 template <int R>
 cudaError_t launch_ids(const FewParams& p, cudaStream_t s) {
+  // four ids share a row's bytes once every warp has some (2 x 768 -> 4096 4 / 1 id: 3.8 / 5.0 us, 2 x 100 -> 1000 2.7 / 2.2)
   return p.vocab >= 2 * WARPS * device_sms() ? launch_rows<R, 4>(p, s) : launch_rows<R, 1>(p, s);
 }
 
 }  // namespace
 
-// Up to 2^27 products, rows in powers of two: beyond them the tensor-core kernel's
-// deeper pipeline of larger copies wins although it launches twice.  us, here /
-// there (148 SMs): 2 x 768 -> 4096 3.1 / 6.1, 8 x 768 -> 4096 4.0 / 6.3,
-// 8 x 2048 -> 8192 6.9 / 9.5, 2 x 4096 -> 16384 8.8 / 15.1, 2 x 1024 -> 65536
-// 10.3 / 10.9; but 8 x 4096 -> 16384 17.5 / 14.9, 2 x 4096 -> 131072 113 / 88.
+// Where this kernel is the faster one.  What it does for a (row, id) beside the
+// products is dear when d is short (vocab R <= 128 d, or a small vocabulary), and
+// from 4 rows on its products cost more than the weight's way from HBM (R^2 d
+// vocab <= 2^30; R the rows, to a power of two).  us with weights that are not in
+// L2, here / there (148 SMs): 2 x 768 -> 4096 3.8 / 6.4, 8 x 768 -> 4096 4.4 /
+// 6.6, 8 x 2048 -> 8192 8.0 / 10.2, 2 x 4096 -> 16384 13.4 / 16.7, 2 x 1024 ->
+// 65536 15.6 / 16.0, 1 x 4096 -> 131072 76.8 / 85.8; and beyond the bounds
+// 2 x 300 -> 65536 17.2 / 11.7, 4 x 768 -> 32768 10.8 / 10.2, 8 x 2048 -> 16384
+// 12.5 / 11.8, 8 x 4096 -> 16384 20.9 / 16.7.
 bool few_rows(int64_t rows, int64_t d, int64_t vocab) {
   const int64_t r = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
-  return rows <= MOST_ROWS && r * ((d + 15) / 16 * 16) <= HELD && r * d * vocab <= 1ll << 27;
+  return rows <= MOST_ROWS && r * ((d + 15) / 16 * 16) <= HELD && (r * vocab <= 128 * d || r * vocab <= 1 << 15) &&
+         (r <= 2 || r * r * d * vocab <= 1ll << 30);
 }
 
 cudaError_t launch_few(const MtrLmHeadI8Args& a, cudaStream_t s) {

@@ -599,7 +599,8 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
 
 // The narrowest tiles that still make one round of CTAs; up to two rounds of 128 x
 // 256 tiles, those; else pairs of CTAs on 256 x 256, unless the rows would fill
-// half a pair only.  Measured with the quantisation (us, 148 SMs), ids a tile:
+// half a pair only.  Measured with the quantisation (us, 148 SMs, weights in L2),
+// ids a tile:
 //                         64     128    256    pair
 //   128 x 768 -> 4096     6.9    7.3    8.2    9.2      (tiles of 32: 7.1)
 //   333 x 1001 -> 4099    11.8   10.2   12.4   12.0

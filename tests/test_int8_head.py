@@ -186,7 +186,7 @@ def test_quantize_strided_rows(cuda_device):
     (1, 1, 1, torch.float32), (1, 16, 8, torch.bfloat16), (8, 2048, 1000, torch.bfloat16), (5, 1001, 300, torch.float16),
     (8, 100, 131072, torch.float32), (1, 8192, 77, torch.bfloat16), (1, 8193, 77, torch.bfloat16), (9, 64, 20000, torch.float32),
     (3, 15, 3, torch.bfloat16), (4, 2048, 16000, torch.float32), (8, 513, 131072, torch.bfloat16), (2, 4096, 131072, torch.bfloat16),
-    (6, 1000, 999, torch.float16), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
+    (6, 1000, 999, torch.float16), (1, 65536, 40, torch.bfloat16), (1, 65537, 40, torch.float32), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
     (33, 100, 77, torch.float16), (129, 1001, 4099, torch.float16), (300, 64, 520, torch.float32), (256, 128, 8192, torch.bfloat16),
     (513, 2048, 1000, torch.bfloat16), (1030, 96, 264, torch.float32), (64, 3000, 131072, torch.bfloat16)])
 def test_logits_equal_the_definition(cuda_device, out_dtype, rows, d, vocab, dtype):
