@@ -47,7 +47,6 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
     stride = matrix(logits, "logits")
     rows, vocab = logits.shape
     device = logits.device
-    tokens = _tokens(tokens, logits)
     if status is not None:
         if status.dtype != torch.int32 or status.shape != (rows,) or not status.is_contiguous():
             raise ValueError(f"status must be a contiguous int32 vector of {rows} elements")
@@ -56,12 +55,12 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
     if not 0 <= n <= N.MAX_TOP_N:
         raise ValueError(f"top_n must be 0 .. {N.MAX_TOP_N}")
     f32 = torch.float32
-    stats = torch.empty((rows, 4), dtype=f32, device=device)
+    stats = logits.new_empty((rows, 4), dtype=f32)
     entropy = torch.empty(rows, dtype=f32, device=device)
     lse = torch.empty(rows, dtype=f32, device=device)
     logprobs = torch.empty(rows, dtype=f32, device=device) if tokens is not None else None
-    top_ids = torch.empty((rows, n), dtype=torch.int64, device=device)
-    top_logprobs = torch.empty((rows, n), dtype=f32, device=device)
+    top_ids = logits.new_empty((rows, n), dtype=torch.int64)
+    top_logprobs = logits.new_empty((rows, n), dtype=f32)
     a = N.sized(N.MtrLogprobArgs, logits=logits.data_ptr(), logits_row_stride=stride, logits_dtype=_DTYPES[logits.dtype],
                 tokens_dtype=N.IDS_I32 if tokens is not None and tokens.dtype == torch.int32 else N.IDS_I64,
                 rows=rows, vocab=vocab, top_n=n, temperature=float(temperature), out_entropy=entropy.data_ptr(),
@@ -119,6 +118,12 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
         raise ValueError("out must have the logits' shape and dtype")
     out_stride = matrix(out, "out")
     _same_device(out, device, "out")
+    return _launch_backward(logits, stride, tokens, stats, top_ids, n, gl, ge, gz, gt, temperature, out, out_stride)
+
+
+def _launch_backward(logits, stride, tokens, stats, top_ids, n, gl, ge, gz, gt, temperature, out, out_stride) -> torch.Tensor:
+    """The launch of token_logprobs_backward; every argument has been checked."""
+    rows, vocab = logits.shape
     a = N.sized(N.MtrLogprobGradArgs, logits=logits.data_ptr(), logits_row_stride=stride,
                 logits_dtype=_DTYPES[logits.dtype],
                 tokens_dtype=N.IDS_I32 if tokens is not None and tokens.dtype == torch.int32 else N.IDS_I64,
@@ -134,7 +139,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
         a.g_lse = gz.data_ptr()
     if n:
         a.top_ids, a.g_top = top_ids.data_ptr(), gt.data_ptr()
-    launch_on(device, N.logprob_grad_launch, a)
+    launch_on(logits.device, N.logprob_grad_launch, a)
     return out
 
 
@@ -156,9 +161,11 @@ class _TokenLogprobs(torch.autograd.Function):
         logits, tokens, stats, top_ids = ctx.saved_tensors
         if g_logprobs is None and g_entropy is None and g_lse is None and g_top is None:
             return None, None, None, None, None, None
-        saved = TokenLogprobs(None, None, None, top_ids, None, stats)
-        grad = token_logprobs_backward(logits, tokens, saved, grad_logprobs=g_logprobs, grad_entropy=g_entropy,
-                                       grad_lse=g_lse, grad_top_logprobs=g_top, temperature=ctx.temperature)
+        # autograd has given the gradients their outputs' types and shapes
+        gl, ge, gz, gt = (g if g is None else g.contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top))
+        n = top_ids.shape[1] if gt is not None else 0
+        stride, grad = matrix(logits, "logits"), logits.new_empty(logits.shape)
+        _launch_backward(logits, stride, tokens, stats, top_ids, n, gl, ge, gz, gt, ctx.temperature, grad, logits.shape[1])
         return grad, None, None, None, None, None
 
 
@@ -183,6 +190,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     :func:`~mapperatorinator_b200.sampling.row_status_report` reads.  Gradients
     flow from ``logprobs``, ``entropy``, ``lse`` and ``top_logprobs`` to the
     logits (once; not through ``top_ids``)."""
+    tokens = _tokens(tokens, logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         hold: list = []
         logprobs, entropy, lse, top_logprobs = _TokenLogprobs.apply(logits, tokens, top_n, temperature, status, hold)
