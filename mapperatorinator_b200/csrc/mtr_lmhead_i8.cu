@@ -116,8 +116,8 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 //
 // What bounds it: at d = 4096 the products (8192 x 4096 -> 16384 in 331 us without
 // the quantisation; twice the measured bf16 rate gives 337); at d = 768 the
-// epilogue, which takes about as long as a 128 x 256 tile's 3072 clocks of
-// products and is not wholly hidden behind them (24 us without the quantisation
+// epilogue, which takes about as long as a 128 x 256 tile's products and is
+// not wholly hidden behind them (24 us without the quantisation
 // for 8192 x 768 -> 4096, 19 with the epilogue's work left out).
 //
 // Persistent: a CTA (pair) takes tile after tile, with two accumulators in tensor
