@@ -361,14 +361,10 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       if (bad || !(a.m > neg_inf())) return;
       if (mine == a.m) {
         const typename X::Top m = X::pattern(a.m);
+        uint32_t equal = 0;
 #pragma unroll
-        for (int j = 0; j < TILE; ++j)
-          if (X::has(top[j], m)) {
-            float f[E];
-            X::unpack(w[j], f);
-#pragma unroll
-            for (int e = 0; e < E; ++e) a.n += f[e] == a.m ? 1.0f : 0.0f;
-          }
+        for (int j = 0; j < TILE; ++j) equal += X::equal(w[j], m);
+        a.n += (float)X::count(equal);
       }
       const float nm = 0.0f - a.m;  // +0 for both zeros, so that equal scores differ by +0
       const u64 nm2 = pk2(nm, nm), sc2 = pk2(scale, scale);

@@ -32,7 +32,8 @@ __device__ __forceinline__ u64 add2(u64 a, u64 b) {
 }
 
 // 16 bytes of a row: E values, their packed maximum, their fp32 values; reach:
-// which of them are at least `cut`, value 2 k + h in bit k + 16 h (fp32: value k in bit k).
+// which of them are at least `cut`, value 2 k + h in bit k + 16 h (fp32: value k in
+// bit k); count of a sum of `equal`s: how many values equal m.
 template <typename T>
 struct Vec;
 template <>
@@ -47,7 +48,10 @@ struct Vec<float> {
   static __device__ __forceinline__ Top larger(Top a, Top b) { return max_nan(a, b); }
   static __device__ __forceinline__ float value(Top t) { return t; }
   static __device__ __forceinline__ Top pattern(float m) { return m; }
-  static __device__ __forceinline__ bool has(Top t, Top m) { return t == m; }
+  static __device__ __forceinline__ uint32_t equal(const uint4& w, Top m) {
+    return (__uint_as_float(w.x) == m) + (__uint_as_float(w.y) == m) + (__uint_as_float(w.z) == m) + (__uint_as_float(w.w) == m);
+  }
+  static __device__ __forceinline__ uint32_t count(uint32_t equal) { return equal; }
   static __device__ __forceinline__ uint32_t reach(const uint4& w, Top cut) {
     return (__uint_as_float(w.x) >= cut ? 1u : 0u) | (__uint_as_float(w.y) >= cut ? 2u : 0u) |
            (__uint_as_float(w.z) >= cut ? 4u : 0u) | (__uint_as_float(w.w) >= cut ? 8u : 0u);
@@ -72,7 +76,11 @@ struct Vec<__nv_bfloat16> {
   static __device__ __forceinline__ Top larger(Top a, Top b) { return __hmax2_nan(a, b); }
   static __device__ __forceinline__ float value(Top t) { return max_nan(__low2float(t), __high2float(t)); }
   static __device__ __forceinline__ Top pattern(float m) { return __float2bfloat162_rn(m); }
-  static __device__ __forceinline__ bool has(Top t, Top m) { return __heq2_mask(t, m) != 0u; }
+  static __device__ __forceinline__ uint32_t equal(const uint4& w, Top m) {
+    return (__heq2_mask(pair(w.x), m) & 0x10001u) + (__heq2_mask(pair(w.y), m) & 0x10001u) +
+           (__heq2_mask(pair(w.z), m) & 0x10001u) + (__heq2_mask(pair(w.w), m) & 0x10001u);
+  }
+  static __device__ __forceinline__ uint32_t count(uint32_t equal) { return (equal & 0xffffu) + (equal >> 16); }
   static __device__ __forceinline__ uint32_t reach(const uint4& w, Top cut) {
     return (__hge2_mask(pair(w.x), cut) & 0x10001u) | (__hge2_mask(pair(w.y), cut) & 0x20002u) |
            (__hge2_mask(pair(w.z), cut) & 0x40004u) | (__hge2_mask(pair(w.w), cut) & 0x80008u);
@@ -99,7 +107,11 @@ struct Vec<__half> {
   static __device__ __forceinline__ Top larger(Top a, Top b) { return __hmax2_nan(a, b); }
   static __device__ __forceinline__ float value(Top t) { return max_nan(__low2float(t), __high2float(t)); }
   static __device__ __forceinline__ Top pattern(float m) { return __float2half2_rn(m); }
-  static __device__ __forceinline__ bool has(Top t, Top m) { return __heq2_mask(t, m) != 0u; }
+  static __device__ __forceinline__ uint32_t equal(const uint4& w, Top m) {
+    return (__heq2_mask(pair(w.x), m) & 0x10001u) + (__heq2_mask(pair(w.y), m) & 0x10001u) +
+           (__heq2_mask(pair(w.z), m) & 0x10001u) + (__heq2_mask(pair(w.w), m) & 0x10001u);
+  }
+  static __device__ __forceinline__ uint32_t count(uint32_t equal) { return (equal & 0xffffu) + (equal >> 16); }
   static __device__ __forceinline__ uint32_t reach(const uint4& w, Top cut) {
     return (__hge2_mask(pair(w.x), cut) & 0x10001u) | (__hge2_mask(pair(w.y), cut) & 0x20002u) |
            (__hge2_mask(pair(w.z), cut) & 0x40004u) | (__hge2_mask(pair(w.w), cut) & 0x80008u);
