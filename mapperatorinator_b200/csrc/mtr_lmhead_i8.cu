@@ -46,6 +46,7 @@ struct ProjParams {
   int32_t m_tiles, n_tiles;
   int32_t a_bytes;   // bytes of a hidden tile's copy
   int32_t store_tma; // logits rows are 16-byte aligned: tiles leave by TMA
+  int32_t whole;     // ids in whole 16 bytes of a row of logits: a TMA store at an edge inside 16 bytes writes all of them
   uint32_t* err;
 };
 
@@ -463,8 +464,16 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
+            if (n0 + c0 + g < p.whole) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          // the ids behind the last whole 16 bytes, each lane its row's
+          const int edge = p.whole - (n0 + c0 + g), row = m0 + quad * 32 + lane;
+          if (edge >= 0 && edge < CB && row < p.rows) {
+            const int piece = edge * (int)sizeof(Tout) / 16 ^ (lane & (PIECES - 1));
+            const Tout* from = reinterpret_cast<const Tout*>(box + lane * (PIECES * 16) + piece * 16);
+            Tout* to = (Tout*)p.out + (int64_t)row * p.out_stride + p.whole;
+            for (int i = 0; i < p.vocab - p.whole; ++i) to[i] = from[i];
           }
         } else {
           __syncwarp();
@@ -496,7 +505,8 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
 
 // ---------------------------------------------------------------- host side
 // 2-D tensor map over a row-major [rows, cols] matrix, box of box_cols x
-// box_rows, 128-byte swizzle; reads 0 and writes nothing outside the matrix.
+// box_rows, 128-byte swizzle; reads 0 outside the matrix and writes nothing
+// behind the 16 bytes that its last column ends in.
 static bool make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes,
                      int box_cols, int box_rows) {
   auto fn = encode_fn();
@@ -557,12 +567,13 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
       !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.weight, a.vocab, a.d_model, a.weight_row_stride, BK, BN / CG))
     return cudaErrorInvalidValue;
   const int es = sizeof(Tout);
-  const bool tma = (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
+  const int whole = a.vocab / (16 / es) * (16 / es);
+  const bool tma = whole > 0 && (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
   const CUtensorMapDataType type = std::is_same<Tout, float>::value           ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : std::is_same<Tout, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (tma) {
-    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, 128 / es, 32)) return cudaErrorInvalidValue;
+    if (!make_map(&mo, type, a.logits, a.rows, whole, a.logits_row_stride * es, 128 / es, 32)) return cudaErrorInvalidValue;
   } else {
     mo = mw;
   }
@@ -589,6 +600,7 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   p.n_tiles = (a.vocab + BN - 1) / BN;
   p.a_bytes = high * BK;
   p.store_tma = tma;
+  p.whole = whole;
   p.err = a.error_word;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, room = device_sms() / CG;
   cudaLaunchAttribute attr[2];

@@ -231,7 +231,8 @@ def test_odd_rows_and_weights(cuda_device, rows):
 
 @gpu
 @pytest.mark.parametrize("out_dtype", DTYPES)
-@pytest.mark.parametrize("vocab,stride,offset", [(300, 301, 1), (256, 260, 0), (4096, 4104, 8), (4099, 4100, 2)])
+@pytest.mark.parametrize("vocab,stride,offset", [(300, 301, 1), (256, 260, 0), (4096, 4104, 8), (4099, 4100, 2), (4099, 4104, 0),
+                                                 (29, 32, 8), (4102, 4104, 0), (3, 8, 0)])
 def test_strides_and_what_lies_behind(cuda_device, out_dtype, vocab, stride, offset):
     rows, d = 140, 200
     h, w = inputs(cuda_device, rows, d, vocab, seed=6)
