@@ -46,7 +46,7 @@ struct ProjParams {
   int32_t m_tiles, n_tiles;
   int32_t a_bytes;   // bytes of a hidden tile's copy
   int32_t store_tma; // logits rows are 16-byte aligned: tiles leave by TMA
-  int32_t whole;     // ids in whole 16 bytes of a row of logits: a TMA store at an edge inside 16 bytes writes all of them
+  int32_t tma_ids;   // ids that may leave so: a TMA store at an edge inside 16 bytes would write all of them
   uint32_t* err;
 };
 
@@ -460,20 +460,12 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
 #pragma unroll
         for (int q = 0; q < PIECES; ++q)
           *reinterpret_cast<uint4*>(box + lane * (PIECES * 16) + (q ^ (lane & (PIECES - 1))) * 16) = w[q];
-        if (p.store_tma) {
+        if (n0 + c0 + g + CB <= p.tma_ids) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            if (n0 + c0 + g < p.whole) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
+            if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-          // the ids behind the last whole 16 bytes, each lane its row's
-          const int edge = p.whole - (n0 + c0 + g), row = m0 + quad * 32 + lane;
-          if (edge >= 0 && edge < CB && row < p.rows) {
-            const int piece = edge * (int)sizeof(Tout) / 16 ^ (lane & (PIECES - 1));
-            const Tout* from = reinterpret_cast<const Tout*>(box + lane * (PIECES * 16) + piece * 16);
-            Tout* to = (Tout*)p.out + (int64_t)row * p.out_stride + p.whole;
-            for (int i = 0; i < p.vocab - p.whole; ++i) to[i] = from[i];
           }
         } else {
           __syncwarp();
@@ -567,13 +559,12 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
       !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.weight, a.vocab, a.d_model, a.weight_row_stride, BK, BN / CG))
     return cudaErrorInvalidValue;
   const int es = sizeof(Tout);
-  const int whole = a.vocab / (16 / es) * (16 / es);
-  const bool tma = whole > 0 && (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
+  const bool tma = (uintptr_t)a.logits % 16 == 0 && a.logits_row_stride * es % 16 == 0;
   const CUtensorMapDataType type = std::is_same<Tout, float>::value           ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : std::is_same<Tout, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (tma) {
-    if (!make_map(&mo, type, a.logits, a.rows, whole, a.logits_row_stride * es, 128 / es, 32)) return cudaErrorInvalidValue;
+    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, 128 / es, 32)) return cudaErrorInvalidValue;
   } else {
     mo = mw;
   }
@@ -600,7 +591,8 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   p.n_tiles = (a.vocab + BN - 1) / BN;
   p.a_bytes = high * BK;
   p.store_tma = tma;
-  p.whole = whole;
+  // a last copy that ends inside the row's last 16 bytes leaves row by row instead
+  p.tma_ids = !tma ? 0 : a.vocab * es % 16 == 0 ? INT32_MAX : a.vocab;
   p.err = a.error_word;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, room = device_sms() / CG;
   cudaLaunchAttribute attr[2];
