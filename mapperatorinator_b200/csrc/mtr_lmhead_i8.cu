@@ -601,24 +601,32 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   return cudaLaunchKernelEx(&cfg, kern, mh, mw, mo, p);
 }
 
-// The narrowest tiles that still make one round of CTAs; up to two rounds of 128 x
-// 256 tiles, those; else pairs of CTAs on 256 x 256, unless the rows would fill
-// half a pair only.  Measured with the quantisation (us, 148 SMs, weights in L2),
-// ids a tile:
+// The narrowest tiles that still make one round of CTAs; beyond that 128 x 256
+// tiles, or pairs of CTAs on 256 x 256, which take less out of L2: pairs unless
+// they need more rounds (rows that fill half of the last pair) or there are only
+// one or two rounds of a short d, where a tile's start and end weigh most.
+// Measured with the quantisation (us, 148 SMs; weights in L2, in the rows with two
+// figures not; the rule's choice is starred):
 //                         64     128    256    pair
-//   128 x 768 -> 4096     6.9    7.3    8.2    9.2      (tiles of 32: 7.1)
-//   333 x 1001 -> 4099    11.8   10.2   12.4   12.0
-//   700 x 1024 -> 4096    13.2   10.8   9.1    10.2
-//   512 x 768 -> 16384    20.2   14.4   11.8   12.5
-//   1000 x 768 -> 32000   60.8   35.7   29.7   27.0
-//   64 x 1024 -> 65536    23.1   16.1   12.3   20.4
+//   128 x 768 -> 4096     6.9*   7.3    8.2    9.2      (tiles of 32: 7.1)
+//   333 x 1001 -> 4099    11.8   10.2*  12.4   12.0
+//   700 x 1024 -> 4096    13.2   10.8   9.1*   10.2
+//   512 x 768 -> 16384    20.2   14.4   11.8*  12.5
+//   512 x 4096 -> 16384                 34.4   31.5*
+//   900 x 768 -> 32000                  29.0   26.7*
+//   300 x 1024 -> 131072                54.0*  57.0
+//   64 x 1024 -> 65536    23.1   16.1   12.3*  20.4
 template <typename Tout>
 static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_t q_stride, const float* row_scale, cudaStream_t s) {
   const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
   auto tiles = [&](int bn) { return m * ((a.vocab + bn - 1) / bn); };
   if (tiles(64) <= sms) return launch_tiles<1, 64, Tout>(a, q, q_stride, row_scale, s);
   if (tiles(128) <= sms) return launch_tiles<1, 128, Tout>(a, q, q_stride, row_scale, s);
-  if (m == 1 || tiles(256) <= 2 * sms) return launch_tiles<1, 256, Tout>(a, q, q_stride, row_scale, s);
+  const int64_t n = (a.vocab + 255) / 256, pairs = sms / 2;
+  const int64_t rounds = (m * n + sms - 1) / sms, pair_rounds = ((m + 1) / 2 * n + pairs - 1) / pairs;
+  // a round of pairs takes about 12/13 of the time
+  if (m == 1 || 12 * pair_rounds > 13 * rounds || (rounds <= 2 && a.d_model <= 2048))
+    return launch_tiles<1, 256, Tout>(a, q, q_stride, row_scale, s);
   return launch_tiles<2, 256, Tout>(a, q, q_stride, row_scale, s);
 }
 
