@@ -188,7 +188,8 @@ def test_quantize_strided_rows(cuda_device):
     (3, 15, 3, torch.bfloat16), (4, 2048, 16000, torch.float32), (8, 513, 131072, torch.bfloat16), (2, 4096, 131072, torch.bfloat16),
     (6, 1000, 999, torch.float16), (1, 65536, 40, torch.bfloat16), (1, 65537, 40, torch.float32), (2, 768, 4096, torch.bfloat16), (128, 768, 4096, torch.bfloat16),
     (33, 100, 77, torch.float16), (129, 1001, 4099, torch.float16), (300, 64, 520, torch.float32), (256, 128, 8192, torch.bfloat16),
-    (513, 2048, 1000, torch.bfloat16), (1030, 96, 264, torch.float32), (64, 3000, 131072, torch.bfloat16)])
+    (513, 2048, 1000, torch.bfloat16), (1030, 96, 264, torch.float32), (64, 3000, 131072, torch.bfloat16),
+    (300, 2100, 8200, torch.bfloat16), (300, 64, 40000, torch.bfloat16)])
 def test_logits_equal_the_definition(cuda_device, out_dtype, rows, d, vocab, dtype):
     h, w = inputs(cuda_device, rows, d, vocab, dtype, seed=rows + d + vocab)
     weight = Int8Weight.from_weight(w)
