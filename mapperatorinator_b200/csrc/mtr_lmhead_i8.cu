@@ -418,67 +418,74 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       tc_fence_after();
       const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + c0);
       const bool live = c0 < BN && m0 + quad * 32 < p.rows && n0 + c0 < p.vocab;
+      auto scale_part = [&](auto tma) {
+        constexpr bool by_tma = decltype(tma)::value;
 #pragma unroll
-      for (int g = 0; g < PART; g += CB) {
-        if (!live) break;
-        uint32_t v[CB / 32][32];
+        for (int g = 0; g < PART; g += CB) {
+          uint32_t v[CB / 32][32];
 #pragma unroll
-        for (int h = 0; h < CB / 32; ++h) tmem_ld32(base + (uint32_t)(g + h * 32), v[h]);
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < CB / 32; ++h) cs[h * 32 + lane] = cs_now[g / 32 + h];
-        __syncwarp();
-        tmem_wait_ld();
-        if (g + CB >= PART) {  // the warp's part of the accumulator is in registers
-          tc_fence_before();
+          for (int h = 0; h < CB / 32; ++h) tmem_ld32(base + (uint32_t)(g + h * 32), v[h]);
           __syncwarp();
-          if (lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));
-        }
-        const u64 rs2 = pk2(rs, rs);
-        constexpr int EP = 16 / (int)sizeof(Tout);
-        uint4 w[PIECES];
 #pragma unroll
-        for (int h = 0; h < CB / 32; ++h) {
-          to_floats(v[h]);
+          for (int h = 0; h < CB / 32; ++h) cs[h * 32 + lane] = cs_now[g / 32 + h];
+          __syncwarp();
+          tmem_wait_ld();
+          if (g + CB >= PART) {  // the warp's part of the accumulator is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));
+          }
+          const u64 rs2 = pk2(rs, rs);
+          constexpr int EP = 16 / (int)sizeof(Tout);
+          uint4 w[PIECES];
 #pragma unroll
-          for (int q = 0; q < 32 / EP; ++q) {
-            float f[EP];
+          for (int h = 0; h < CB / 32; ++h) {
+            to_floats(v[h]);
 #pragma unroll
-            for (int e = 0; e < EP; e += 4) {
-              const float4 c4 = *reinterpret_cast<const float4*>(&cs[h * 32 + q * EP + e]);
-              const uint32_t* a4 = &v[h][q * EP + e];
-              up2(mul2(mul2(pk2(__uint_as_float(a4[0]), __uint_as_float(a4[1])), rs2), pk2(c4.x, c4.y)), f[e], f[e + 1]);
-              up2(mul2(mul2(pk2(__uint_as_float(a4[2]), __uint_as_float(a4[3])), rs2), pk2(c4.z, c4.w)), f[e + 2], f[e + 3]);
+            for (int q = 0; q < 32 / EP; ++q) {
+              float f[EP];
+#pragma unroll
+              for (int e = 0; e < EP; e += 4) {
+                const float4 c4 = *reinterpret_cast<const float4*>(&cs[h * 32 + q * EP + e]);
+                const uint32_t* a4 = &v[h][q * EP + e];
+                up2(mul2(mul2(pk2(__uint_as_float(a4[0]), __uint_as_float(a4[1])), rs2), pk2(c4.x, c4.y)), f[e], f[e + 1]);
+                up2(mul2(mul2(pk2(__uint_as_float(a4[2]), __uint_as_float(a4[3])), rs2), pk2(c4.z, c4.w)), f[e + 2], f[e + 3]);
+              }
+              w[h * 32 / EP + q] = pack<Tout>(f);
             }
-            w[h * 32 / EP + q] = pack<Tout>(f);
+          }
+          if (by_tma || p.store_tma) {  // the buffer's previous contents have been read
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+          }
+#pragma unroll
+          for (int q = 0; q < PIECES; ++q)
+            *reinterpret_cast<uint4*>(box + lane * (PIECES * 16) + (q ^ (lane & (PIECES - 1))) * 16) = w[q];
+          if constexpr (by_tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {
+            __syncwarp();
+            const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c0 + g));
+            Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c0 + g;
+            for (int r = 0; r < high; ++r, dst += p.out_stride)
+#pragma unroll
+              for (int x = 0; x < CB; x += 32) {
+                const int i = x + lane, in = i * (int)sizeof(Tout), piece = in / 16 ^ (r & (PIECES - 1));
+                if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(box + r * (PIECES * 16) + piece * 16 + in % 16);
+              }
+            __syncwarp();
           }
         }
-        if (p.store_tma) {  // the buffer's previous contents have been read
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
-        }
-#pragma unroll
-        for (int q = 0; q < PIECES; ++q)
-          *reinterpret_cast<uint4*>(box + lane * (PIECES * 16) + (q ^ (lane & (PIECES - 1))) * 16) = w[q];
-        if (n0 + c0 + g + CB <= p.tma_ids) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else {
-          __syncwarp();
-          const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c0 + g));
-          Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c0 + g;
-          for (int r = 0; r < high; ++r, dst += p.out_stride)
-#pragma unroll
-            for (int x = 0; x < CB; x += 32) {
-              const int i = x + lane, in = i * (int)sizeof(Tout), piece = in / 16 ^ (r & (PIECES - 1));
-              if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(box + r * (PIECES * 16) + piece * 16 + in % 16);
-            }
-          __syncwarp();
-        }
+      };
+      if (live) {
+        // two copies of the loop: chosen inside it, the way out costs every tile 1 %
+        if (n0 + c0 + PART <= p.tma_ids) scale_part(std::true_type());
+        else scale_part(std::false_type());
       }
       if (!live && lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc]), 0));  // nothing to read here
     }
