@@ -22,7 +22,7 @@
 // d = -1000, whose 2^d is 0 and whose product with d is 0 as well (-inf would
 // give NaN), and a score equal to the maximum, whose d is +0 = 0, becomes -1000
 // too and so leaves the sums: it is counted in n.  NaN is found by the maximum,
-// which keeps it.
+// which keeps it.  Terms below 2^-126 count as 0, in the sums and in the gradient.
 #include "mtr_vec.cuh"
 
 namespace mtr {
