@@ -101,7 +101,7 @@ def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: t
     if vocab == 1:
         ws = (d + 15) // 16 * 16
     need = N.lmhead_i8_workspace(rows, d, vocab)  # 0 for few rows
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = hidden.new_empty(need, dtype=torch.uint8) if need else None
     a = N.sized(N.MtrLmHeadI8Args, hidden=hidden.data_ptr(), hidden_row_stride=hs, weight=weight_q.data_ptr(),
                 weight_row_stride=ws, weight_scale=weight_scale.data_ptr(), logits=out.data_ptr(), logits_row_stride=ls,
                 hidden_dtype=_DTYPES[hidden.dtype], logits_dtype=_DTYPES[out.dtype], rows=rows, d_model=d, vocab=vocab,
@@ -119,7 +119,7 @@ def lm_head_logits_int8(hidden: torch.Tensor, weight_q: torch.Tensor, weight_sca
     if out is None:
         if out_dtype not in _DTYPES:
             raise TypeError(f"out_dtype {out_dtype} is not supported (float32, bfloat16, float16)")
-        out = torch.empty((hidden.shape[0], weight_q.shape[0]), dtype=out_dtype, device=hidden.device)
+        out = hidden.new_empty((hidden.shape[0], weight_q.shape[0]), dtype=out_dtype)
     a, work = lmhead_i8_args(hidden, weight_q, weight_scale, out)
     launch_on(hidden.device, N.lmhead_i8_launch, a)
     return out

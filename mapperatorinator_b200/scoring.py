@@ -56,9 +56,9 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
         raise ValueError(f"top_n must be 0 .. {N.MAX_TOP_N}")
     f32 = torch.float32
     stats = logits.new_empty((rows, 4), dtype=f32)
-    entropy = torch.empty(rows, dtype=f32, device=device)
-    lse = torch.empty(rows, dtype=f32, device=device)
-    logprobs = torch.empty(rows, dtype=f32, device=device) if tokens is not None else None
+    entropy = logits.new_empty(rows, dtype=f32)
+    lse = logits.new_empty(rows, dtype=f32)
+    logprobs = logits.new_empty(rows, dtype=f32) if tokens is not None else None
     top_ids = logits.new_empty((rows, n), dtype=torch.int64)
     top_logprobs = logits.new_empty((rows, n), dtype=f32)
     a = N.sized(N.MtrLogprobArgs, logits=logits.data_ptr(), logits_row_stride=stride, logits_dtype=_DTYPES[logits.dtype],
