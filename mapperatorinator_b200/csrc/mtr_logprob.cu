@@ -272,8 +272,8 @@ __device__ __forceinline__ int place_of(const u64* list, int c, u64 k) {
 // is a poor bound when n is near 32; then a lane keeps two maxima.)  The larger
 // of the two leaves about n to 3 n lanes with lm >= T, whose vectors are read again
 // (from L2) for the list of candidates, which are ranked by comparing all pairs.  A
-// list that overflows (many equal logits) still holds more than n candidates:
-// the n-th of them is a better T, and the candidates are looked for again.
+// list that overflows (many equal logits) is left at once: it holds more than n
+// candidates, the n-th of them is a better T, and they are looked for again.
 template <typename T, int W>
 __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(const FwdParams p) {
   typedef Vec<T> X;
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
     u64 bound = order_key(fmaxf(nth, rth), 0xffffffffu);
     int c = 0;
     if (W > 1 && tid == 0) sh.count[parity ^ 1] = 0;
-    bool again = false;
+    bool again = false, full = false;
     float least = 0.0f;  // the bound's score; of masked scores none is a candidate
     auto list = [&](float f, int id) {
       bool hit = f >= least;
@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       } else {
         c += __popc(hits);
       }
+      full = at + __popc(hits) > LIST;
       at += __popc(hits & ((1u << lane) - 1u));
       if (hit && at < LIST) sh.list[at] = order_key(f, (uint32_t)id);
     };
@@ -513,8 +514,8 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       const uint4* body = sp.body();
       const int most_of = (sp.v1 - sp.v0 - warp * 32 + THREADS - 1) / THREADS;  // vectors of the warp's first lane
       const int count = __popc(winners);
-      for (int first = 0; first < count; first += 8)
-        for (int i0 = 0; i0 < most_of; i0 += 16) {
+      for (int first = 0; first < count && !full; first += 8)
+        for (int i0 = 0; i0 < most_of && !full; i0 += 16) {
           uint32_t reach = 0;  // bits 4 j ..: the j-th vector's
           auto vector = [&](int j) {
             const int who = first + 2 * j + (lane >> 4);
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) reach |= X::reach(w[j], cut) << (4 * j);
-          while (__any_sync(FULL, reach != 0u)) {  // one score a lane
+          while (!full && __any_sync(FULL, reach != 0u)) {  // one score a lane
             const int bit = reach ? __ffs(reach) - 1 : 0;
             const int id = sp.head + vector((bit >> 2) & 3) * E + (E == 8 ? 2 * (bit & 3) + (bit >> 4) : bit & 3);
             list(reach ? to_f(sp.x[id]) : neg_inf(), id);
@@ -547,6 +548,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       cta_sync();
       bound = sh.bound[parity];
       again = true;
+      full = false;
       c = 0;
       if (W > 1 && tid == 0) sh.count[parity] = 0;
       cta_sync();
