@@ -308,9 +308,11 @@ int mtr_lmhead_sample_launch(const MtrLmHeadArgs* lm, const MtrSamplerArgs* samp
 /*
  * 8-bit output projection.  Rows of hidden states and of the weight are held
  * as int8 with one fp32 scale per row:
- *   scale[r] = RN32(max_k |x[r, k]| * RN32(1 / 127)),  q[r, k] = RNE(RN32(x[r, k] / scale[r]))
- * (q = 0 for a row of zeros, or one so small that its scale rounds to 0; a row
- * with a NaN or an infinity gets scale NaN and q = 0).
+ *   scale[r] = RN32(max_k |x[r, k]| * RN32(1 / 127)),  q[r, k] = RNE(RN32(x[r, k] / scale[r])),
+ * held to -127 .. 127 (a quotient passes 127 only where the scale is a subnormal
+ * of a few bits: fp32 rows below 2.3e-41).  q = 0 for a row of zeros, or one so
+ * small that its scale rounds to 0; a row with a NaN or an infinity gets scale
+ * NaN and q = 0.
  */
 typedef struct MtrQuantizeArgs {
   uint32_t abi_version;         /* = MTR_ABI_VERSION */

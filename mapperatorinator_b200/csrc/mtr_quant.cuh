@@ -25,11 +25,13 @@ __device__ __forceinline__ float magnitude(uint4 w, T) {
   return Vec<T>::value(Vec<T>::top(w));
 }
 
-// The divisor of a row: q(x) = the byte of RNE(RN(x / s)).  With y = RN(1 / s),
-// q0 = RN(x y), r = RN(x - q0 s) (exact) and q1 = RN(q0 + r y), q1 is the
-// correctly rounded quotient (Markstein) unless s has an all-ones significand;
+// The divisor of a row: q(x) = RNE(RN(x / s)), held to -127 .. 127.  With y =
+// RN(1 / s), q0 = RN(x y), r = RN(x - q0 s) (exact) and q1 = RN(q0 + r y), q1 is
+// the correctly rounded quotient (Markstein) unless s has an all-ones significand;
 // three steps, packed two values at a time.  Those scales, and the ones so
-// small that 1 / s or r could leave the normal range, divide instead.
+// small that 1 / s or r could leave the normal range, divide instead.  Only
+// those can pass 127: a scale of one step of 2^-149 may be rounded down by a
+// third, and the row's largest quotient is then 190.
 struct Divisor {
   float s, inv;
   bool zero, divide;
@@ -44,7 +46,7 @@ __device__ __forceinline__ Divisor divisor_of(float top) {
 }
 constexpr float WHOLE = 12582912.0f;  // 1.5 2^23: y + WHOLE holds RNE(y) in its low bits, |y| < 2^22
 __device__ __forceinline__ uint32_t quotient(float x, const Divisor& d) {
-  return __float_as_uint(__fadd_rn(__fdiv_rn(x, d.s), WHOLE));
+  return __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x, d.s), -127.0f), 127.0f), WHOLE));
 }
 template <int N>
 __device__ __forceinline__ void quotients(const float (&x)[N], const Divisor& d, uint32_t (&w)[N / 4]) {

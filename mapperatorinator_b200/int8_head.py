@@ -67,7 +67,8 @@ class Int8Weight(NamedTuple):
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """int8 rows and their fp32 scales: ``scale = max|x| * (1 / 127)`` of each
     row (the reciprocal and the product rounded to fp32) and ``q = round(x /
-    scale)`` (half to even).  A row of zeros gives zeros and scale
+    scale)`` (half to even), held to -127 .. 127 (only fp32 rows below 2.3e-41,
+    whose scales keep a few bits, pass that).  A row of zeros gives zeros and scale
     0; a row with a NaN or an infinity gives zeros and scale NaN.  The int8 rows
     start on 16-byte boundaries (``q`` may be a view of wider rows)."""
     stride = matrix(x, "x")

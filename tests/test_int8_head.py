@@ -370,3 +370,55 @@ def test_training_through_the_bf16_head(cuda_device):
     loss.backward()
     # one bf16 rounding (2^-8 relative) plus fp32 noise far below it
     assert float(((logits.grad.double() - x.grad).abs() - 2.0 ** -8 * x.grad.abs() - 1e-9).max()) <= 0
+
+
+# ------------------------------------------------------------------ rows whose scale is a small subnormal
+
+
+def subnormal_rows(cols, seed):
+    """fp32 rows whose largest magnitudes are a few thousand steps of 2^-149 at most: their scales keep few bits,
+    so that quotients of up to 190 come out before they are held to 127."""
+    tops = torch.tensor([1, 63, 64, 100, 127, 150, 190, 191, 318, 6000, 12000, 16000, 16129, 30000])
+    g = torch.Generator().manual_seed(seed)
+    steps = (torch.rand((len(tops), cols), generator=g) * (tops[:, None] + 1)).to(torch.int32)
+    steps[:, 0] = steps[:, 1] = tops.to(torch.int32)
+    negative = torch.rand((len(tops), cols), generator=g) < 0.5
+    negative[:, 0], negative[:, 1] = False, True
+    return torch.where(negative, steps | torch.tensor(-2 ** 31, dtype=torch.int32), steps).view(torch.float32)
+
+
+def held_quantize(x):
+    scale = x.abs().amax(1) * torch.tensor(1 / 127, dtype=torch.float32)
+    q = torch.where((scale > 0)[:, None], x / scale[:, None], 0.0)
+    return torch.round(q).clamp(-127, 127).to(torch.int8), scale
+
+
+def test_quotients_of_subnormal_scales_pass_127():
+    x = subnormal_rows(40, 0)
+    scale = x.abs().amax(1) * torch.tensor(1 / 127, dtype=torch.float32)
+    assert float((x / scale[:, None])[scale > 0].max()) == 190.0  # what the kernels must not store as -66
+
+
+@gpu
+@pytest.mark.parametrize("cols", [40, 33, 1000, 5001])
+def test_quantize_rows_of_subnormal_scales(cuda_device, cols):
+    x = subnormal_rows(cols, cols)
+    q, scale = quantize_rows(x.to(cuda_device))
+    want_q, want_s = held_quantize(x)
+    same(scale, want_s)
+    same(q, want_q)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [7, 140])
+@pytest.mark.parametrize("cols", [40, 33])
+def test_logits_of_subnormal_scales(cuda_device, rows, cols):
+    x = subnormal_rows(cols, cols)[4:11].repeat(rows // 7, 1)
+    g = torch.Generator().manual_seed(1)
+    wide = torch.zeros((50, 48), dtype=torch.int8)
+    wide[:, :cols] = torch.randint(-128, 128, (50, cols), generator=g).to(torch.int8)
+    ws = torch.full((50,), 2.0 ** 120)
+    wide_d = wide.to(cuda_device)
+    out = lm_head_logits_int8(x.to(cuda_device), wide_d[:, :cols], ws.to(cuda_device), out_dtype=torch.float32)
+    q, scale = held_quantize(x)
+    same(out, plain_logits(q, scale, wide[:, :cols], ws, torch.float32))
