@@ -305,6 +305,17 @@ int mtr_lmhead_launch(const MtrLmHeadArgs* args, void* stream);
  * stride and vocabulary) and the sampler's rows must lie inside lm->rows. */
 int mtr_lmhead_sample_launch(const MtrLmHeadArgs* lm, const MtrSamplerArgs* sampler, void* stream);
 
+/* Waits of the tensor-core projections (this one and the 8-bit one) that gave up
+ * on the current device since the library was loaded; 0 on a healthy device.
+ * Waits for `stream`, which must not be capturing (MTR_ERR_UNSUPPORTED).  Logits
+ * that such a projection did not compute are NaN, so the sampler marks their
+ * rows MTR_ROW_NONFINITE and gives them pad_id. */
+int mtr_projection_timeouts(uint32_t* count, void* stream);
+
+/* Test hook, for the whole process: while on, the epilogues of tensor-core
+ * projections that are launched take their first wait as run out. */
+void mtr_projection_test_waits(int32_t on);
+
 /*
  * 8-bit output projection.  Rows of hidden states and of the weight are held
  * as int8 with one fp32 scale per row:

@@ -295,6 +295,8 @@ EXPORTS = {
     "mtr_lmhead_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadArgs), c_void_p]),
     "mtr_lmhead_sample_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadArgs), ctypes.POINTER(MtrSamplerArgs),
                                                 c_void_p]),
+    "mtr_projection_timeouts": (ctypes.c_int, [ctypes.POINTER(c_uint32), c_void_p]),
+    "mtr_projection_test_waits": (None, [c_int32]),
     "mtr_quantize_rows_validate": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeArgs)]),
     "mtr_quantize_rows_launch": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeArgs), c_void_p]),
     "mtr_lmhead_i8_workspace": (c_int64, [c_int32, c_int32, c_int32]),
@@ -430,6 +432,16 @@ def lmhead_launch(args: MtrLmHeadArgs, stream: int | None) -> None:
 def lmhead_sample_launch(lm: MtrLmHeadArgs, args: MtrSamplerArgs, stream: int | None) -> None:
     check(load().mtr_lmhead_sample_launch(ctypes.byref(lm), ctypes.byref(args), c_void_p(stream or 0)),
           "mtr_lmhead_sample_launch")
+
+
+def projection_timeouts(stream: int | None) -> int:
+    n = c_uint32(0)
+    check(load().mtr_projection_timeouts(ctypes.byref(n), c_void_p(stream or 0)), "mtr_projection_timeouts")
+    return n.value
+
+
+def projection_test_waits(on: bool) -> None:
+    load().mtr_projection_test_waits(int(on))
 
 
 def sized(cls, **fields):

@@ -34,6 +34,8 @@
 // CTAs exit (no early launch_dependents): admitted during the epilogue, the
 // sampler's CTAs crowded onto the few SMs without a 150 KB projection CTA and
 // the pair took 1.9 us longer.
+#include <atomic>
+
 #include "mtr_tc.cuh"
 
 namespace mtr {
@@ -50,6 +52,7 @@ struct Params {
   int32_t vocab;
   int32_t kblocks;
   uint32_t* err;
+  int32_t give_up;  // test hook: the epilogue takes its wait as run out
 };
 
 using namespace tc;
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(128, 1)
       const int s = kb % S;
       if (kb >= S && !mbar_wait(&empty[s], ((kb / S) & 1) ^ 1, WAIT_NS)) {
         abort_flag = 1u;
-        if (p.err) atomicOr(p.err, 1u);
+        gave_up(p.err, 1u);
         break;
       }
       if (abort_flag) break;
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(128, 1)
       const int s = kb % S;
       if (!mbar_wait(&full[s], (kb / S) & 1, WAIT_NS) || abort_flag) {
         abort_flag = 1u;
-        if (p.err) atomicOr(p.err, 2u);
+        gave_up(p.err, 2u);
         ok = false;
         break;
       }
@@ -181,12 +184,12 @@ __global__ void __launch_bounds__(128, 1)
   // ---------------- epilogue: all four warps; one lane per warp polls the
   // barrier (128 pollers would contend with the copies' completions for it)
   bool waited = true;
-  if (lane == 0) waited = mbar_wait(&done, 0, WAIT_NS);
+  if (lane == 0) waited = mbar_wait(&done, 0, WAIT_NS) && !p.give_up;
   waited = __shfl_sync(FULL, waited, 0) != 0;
   tc_fence_after();
   // tcgen05.ld is warp-collective: the whole warp reads or none of it
   const bool go = __all_sync(FULL, waited && !abort_flag);
-  if (!waited && lane == 0 && p.err) atomicOr(p.err, 4u);
+  if (!waited && lane == 0) gave_up(p.err, 4u);
   if (go) {
     const int row = m0 + warp * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
@@ -217,6 +220,12 @@ __global__ void __launch_bounds__(128, 1)
           if (col + 8 * q < p.vocab) *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
       }
     }
+  } else {
+    // what was not computed reads NaN, which the sampler and the scores report
+    const int row = m0 + warp * 32 + lane;
+    if (row < p.rows)
+      for (int col = n0; col < n0 + BN && col < p.vocab; col += 8)
+        *reinterpret_cast<uint4*>(p.out + (int64_t)row * p.out_stride + col) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
   }
   tc_fence_before();
   __syncthreads();
@@ -272,6 +281,7 @@ static cudaError_t launch_bn(const MtrLmHeadArgs& a, cudaStream_t s) {
   p.vocab = a.vocab;
   p.kblocks = a.d_model / BK;
   p.err = a.error_word;
+  p.give_up = test_waits();
   const dim3 grid((unsigned)((a.vocab + BN - 1) / BN), (unsigned)((a.rows + BM - 1) / BM), 1);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -286,9 +296,32 @@ static cudaError_t launch_bn(const MtrLmHeadArgs& a, cudaStream_t s) {
 }
 
 }  // namespace lm
+
+namespace tc {
+static std::atomic<bool> test_waits_on{false};
+bool test_waits() { return test_waits_on.load(std::memory_order_relaxed); }
+}  // namespace tc
 }  // namespace mtr
 
 // ---------------------------------------------------------------- C ABI
+void mtr_projection_test_waits(int32_t on) { mtr::tc::test_waits_on.store(on != 0, std::memory_order_relaxed); }
+
+int mtr_projection_timeouts(uint32_t* count, void* stream) {
+  if (!count) return MTR_ERR_NULL_ARG;
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  uint32_t n[2] = {0, 0};
+  cudaError_t e = cudaStreamIsCapturing(s, &capture);
+  if (e == cudaSuccess && capture != cudaStreamCaptureStatusNone) return MTR_ERR_UNSUPPORTED;
+  if (e == cudaSuccess) e = mtr::tc::read_gave_up(&n[0], s);
+  if (e == cudaSuccess) e = mtr::tc::read_gave_up_i8(&n[1], s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  mtr::set_last_cuda_error((int)e);
+  if (e != cudaSuccess) return MTR_ERR_CUDA;
+  *count = n[0] + n[1];
+  return MTR_OK;
+}
+
 int mtr_lmhead_validate(const MtrLmHeadArgs* a) {
   if (!a) return MTR_ERR_NULL_ARG;
   if (a->abi_version != MTR_ABI_VERSION || a->struct_size != sizeof(MtrLmHeadArgs)) return MTR_ERR_ABI;

@@ -48,6 +48,7 @@ struct ProjParams {
   int32_t store_tma; // logits rows are 16-byte aligned: tiles leave by TMA
   int32_t tma_ids;   // ids that may leave so: a TMA store at an edge inside 16 bytes would write all of them
   uint32_t* err;
+  int32_t give_up;   // test hook: the epilogue takes its first wait as run out
 };
 
 // Rows to int8: threads_per_row threads (a power of two, 32 .. 128) take a row
@@ -133,9 +134,9 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 //                      in shared memory (16-byte pieces XOR-swizzled by row) and
 //                      sends them by TMA, or row by row where rows of logits are
 //                      not 16-byte aligned
-// Every wait is bounded; a role whose wait gives up sets the error word and stops,
+// Every wait is bounded; a role whose wait gives up counts it (gave_up) and stops,
 // so that the others' waits give up too; the producer then gives its copies time
-// to land, and the CTA returns.
+// to land, the epilogue writes NaN for what was not computed, and the CTA returns.
 constexpr int EPI = 8;  // epilogue warps
 constexpr int PROJ_THREADS = 64 + 32 * EPI;
 
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       if (mbar_wait(bar, parity, WAIT_NS)) return true;
-      if (p.err) atomicOr(p.err, 1u);
+      gave_up(p.err, 1u);
       return false;
     };
     for (int t = first; t < tiles && ok; t += step) {
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       if (mbar_wait(bar, parity, WAIT_NS)) return true;
-      if (p.err) atomicOr(p.err, 2u);
+      gave_up(p.err, 2u);
       return false;
     };
     // this thread feeds the tensor core alone, a stage of products every 512
@@ -409,10 +410,17 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       const float rs = rs_next;
       if (t + step < tiles) ask(t + step);
       bool waited = true;
-      if (lane == 0) waited = mbar_wait(&acc_full[acc], (n >> 1) & 1, WAIT_NS);
+      if (lane == 0) waited = mbar_wait(&acc_full[acc], (n >> 1) & 1, WAIT_NS) && !p.give_up;
       waited = __shfl_sync(FULL, waited, 0) != 0;
       if (!waited) {
-        if (lane == 0 && p.err) atomicOr(p.err, 4u);
+        if (lane == 0) gave_up(p.err, 4u);
+        // what is not computed reads NaN, which the sampler and the scores report
+        for (; t < tiles; t += step) {
+          place(t, m0, n0);
+          for (int r = m0 + quad * 32; c0 < BN && r < min(m0 + quad * 32 + 32, p.rows); ++r)
+            for (int col = n0 + c0 + lane; col < min(n0 + c0 + PART, p.vocab); col += 32)
+              ((Tout*)p.out)[r * p.out_stride + col] = from_f<Tout>(__int_as_float(0x7fc00000));
+        }
         break;
       }
       tc_fence_after();
@@ -601,6 +609,7 @@ static cudaError_t launch_tiles(const MtrLmHeadI8Args& a, const int8_t* q, int64
   // a last copy that ends inside the row's last 16 bytes leaves row by row instead
   p.tma_ids = !tma ? 0 : a.vocab * es % 16 == 0 ? INT32_MAX : a.vocab;
   p.err = a.error_word;
+  p.give_up = test_waits();
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, room = device_sms() / CG;
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
@@ -647,6 +656,8 @@ static bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
 static int64_t span(int64_t rows, int64_t stride, int64_t cols, int64_t es) { return ((rows - 1) * stride + cols) * es; }
 
 }  // namespace i8
+
+cudaError_t tc::read_gave_up_i8(uint32_t* n, cudaStream_t s) { return read_gave_up(n, s); }
 }  // namespace mtr
 
 // ---------------------------------------------------------------- C ABI

@@ -51,6 +51,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t ph, uint64_t bud
     }
   }
 }
+// Bounded waits that gave up on this device since the library was loaded (each
+// translation unit has its own count; mtr_projection_timeouts adds them), and the
+// bit of one in the caller's word.
+static __device__ uint32_t gave_up_count;
+__device__ __forceinline__ void gave_up(uint32_t* err, uint32_t bit) {
+  atomicAdd(&gave_up_count, 1u);
+  if (err) atomicOr(err, bit);
+}
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -73,6 +81,12 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
 }
 
 // ---------------------------------------------------------------- host side
+static inline cudaError_t read_gave_up(uint32_t* n, cudaStream_t s) {
+  return cudaMemcpyFromSymbolAsync(n, gave_up_count, sizeof(*n), 0, cudaMemcpyDeviceToHost, s);
+}
+cudaError_t read_gave_up_i8(uint32_t* n, cudaStream_t s);  // mtr_lmhead_i8.cu's count
+bool test_waits();                                         // mtr_projection_test_waits
+
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;

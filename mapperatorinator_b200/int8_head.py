@@ -116,7 +116,9 @@ def lm_head_logits_int8(hidden: torch.Tensor, weight_q: torch.Tensor, weight_sca
     states ``[R, d]`` (float32, bfloat16 or float16), weight rows ``[V, d]``
     whose row stride is a multiple of 16 bytes (as :func:`quantize_rows` lays
     them out) and their scales ``[V]``.  The logits are ``out``, or a new tensor
-    of ``out_dtype``; any of the three dtypes.  Not differentiable."""
+    of ``out_dtype``; any of the three dtypes.  Not differentiable.  Logits that a
+    wait that gave up left without a value are NaN
+    (:func:`~mapperatorinator_b200.sampling.projection_timeouts`)."""
     if out is None:
         if out_dtype not in _DTYPES:
             raise TypeError(f"out_dtype {out_dtype} is not supported (float32, bfloat16, float16)")

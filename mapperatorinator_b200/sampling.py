@@ -114,6 +114,17 @@ def lm_head_logits(hidden: torch.Tensor, weight: torch.Tensor, out: torch.Tensor
     return out
 
 
+def projection_timeouts(device=None) -> int:
+    """How many bounded waits of the tensor-core projections (``lm_head_logits``,
+    ``lm_head_logits_int8``, ``step_hidden``) have given up on ``device`` (default:
+    the current one) since the library was loaded: 0 on a healthy device.  One
+    host sync with the device's current stream.  Logits that such a projection did
+    not compute are NaN: the sampler marks their rows ``nonfinite`` in its status
+    and pads them, and their scores are NaN."""
+    with torch.cuda.device(device):
+        return N.projection_timeouts(torch.cuda.current_stream().cuda_stream)
+
+
 def _uniforms(n: int, device, uniforms, generator) -> torch.Tensor:
     if uniforms is None:
         return torch.rand(n, device=device, generator=generator, dtype=torch.float32)
