@@ -597,9 +597,11 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
 // two numbers (both divided by T).  One CTA owns a run of a row's vectors and
 // asks for them before anything else; the row's numbers arrive meanwhile.  The
 // few ids that are given something of their own (the token, the alternatives)
-// are written once more, in full precision, after the run: one thread for each
-// distinct id, so a token that is also an alternative is summed before the
-// rounding.  4 bytes of traffic for a bf16 score and about 6 instructions: HBM
+// are written once more after the run, one thread for each distinct id, so a
+// token that is also an alternative is summed before the rounding.  With o_v what
+// is given to v alone, the row's `a` holds -o_v p_v: v gets o_v (1 - p_v) + p_v
+// (the others' terms), 1 - p_v = -expm1(log p_v), which keeps the digits of a
+// gradient that is small because p_v is near 1.  4 bytes of traffic for a bf16 score and about 6 instructions: HBM
 // bounds it.
 struct GradRow {
   float m, log2_s, a, b;
@@ -608,6 +610,13 @@ template <typename T>
 __device__ __forceinline__ float grad_of(T x, const GradRow& r, float scale) {
   const float d = max_nan(fmaf(to_f(x) - r.m, scale, -r.log2_s), -1000.0f);
   return ex2(d) * fmaf(r.b, d, r.a);
+}
+
+// the same for an id that `own` is given to alone; `rest` is what the row's even part has from the others
+template <typename T>
+__device__ __forceinline__ float own_grad_of(T x, const GradRow& r, const GradParams& p, float log_s, float own, float rest) {
+  const float logp = fmaf(to_f(x) - r.m, p.inv_t, -log_s), d = max_nan(fmaf(to_f(x) - r.m, p.scale, -r.log2_s), -1000.0f);
+  return fmaf(-own * p.inv_t, expm1f(logp), ex2(d) * fmaf(r.b, d, rest * p.inv_t));
 }
 
 constexpr int GRAD_VECS = 4;  // vectors a thread holds
@@ -647,7 +656,8 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const GradParams p) {
   const bool has = tok >= 0 && tok < V;
   const float gt = has && p.g_logprobs ? p.g_logprobs[row] : 0.0f;
   const float gh = p.g_entropy ? p.g_entropy[row] : 0.0f;
-  float even = (p.g_lse ? p.g_lse[row] : 0.0f) - gt - gh * st.z;
+  const float gz = p.g_lse ? p.g_lse[row] : 0.0f;
+  float even = gz - gt - gh * st.z;
   const int slots = 1 + p.top_n;
   if (p.top_n > 0) {
     if (tid < p.top_n) {
@@ -701,20 +711,22 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const GradParams p) {
   if (p.top_n == 0) {
     if (!has || tok < from || tok >= to) return;
     __syncthreads();  // after the run's own store of this id
-    if (tid == 0) g[tok] = from_f<T>(fmaf(gt, p.inv_t, grad_of(x[tok], r, p.scale)));
+    if (tid == 0) g[tok] = from_f<T>(own_grad_of(x[tok], r, p, st.y, gt, gz - gh * st.z));
     return;
   }
   __syncthreads();
   if (tid < slots) {
     const int id = slot_id[tid];
     bool mine = id >= from && id < to;
-    float own = 0.0f;
+    float own = 0.0f, rest = gz - gh * st.z;
     for (int j = 0; j < slots; ++j)
       if (slot_id[j] == id) {
         if (j < tid) mine = false;  // an earlier slot writes it
         own += slot_g[j];
+      } else {
+        rest -= slot_g[j];
       }
-    if (mine) g[id] = from_f<T>(fmaf(own, p.inv_t, grad_of(x[id], r, p.scale)));
+    if (mine) g[id] = from_f<T>(own_grad_of(x[id], r, p, st.y, own, rest));
   }
 }
 

@@ -520,3 +520,40 @@ def test_sampler_scores_its_tokens(cuda_device, do_sample):
     assert bool(done.any()) and a.token_logprobs is None
     with pytest.raises(ValueError):
         S.FusedSampler(**kw, token_logprobs=40)
+
+
+# ------------------------------------------------------------------ gradients that are small beside their terms
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 0.5])
+@pytest.mark.parametrize("top_n", [0, 3])
+def test_small_gradients_keep_their_digits(cuda_device, dtype, temperature, top_n):
+    # A given token that has nearly all the mass: its gradient g (1 - p) / T is far smaller than g / T.  With 63 zeros beside
+    # logit / T = 12, 16, 20 every term is positive.  Relative errors: a term of S' 2^-22 + 3 2^-24 |d|, |d| <= 20; its sum, log1p
+    # and expm1 below 70 2^-24 more; d and its mean, products: 10 2^-24.  In all less than (4 + 60 + 70 + 10) 2^-24 < 2^-16.
+    x = torch.zeros((3, 64), device=cuda_device)
+    x[0, 5], x[1, 6], x[2, 7] = 12.0 * temperature, 16.0 * temperature, 20.0 * temperature
+    x = x.to(dtype)
+    t = torch.tensor([5, 6, 7], device=cuda_device)
+    r = token_logprobs(x, t, top_n=top_n, temperature=temperature)
+    gl = torch.full((3,), 1.5, device=cuda_device)
+    gh, gz = torch.full((3,), -0.25, device=cuda_device), torch.zeros(3, device=cuda_device)
+    gt = torch.zeros((3, top_n), device=cuda_device)
+    gt[:, :1] = 0.5  # the first alternative is the token
+    grad = token_logprobs_backward(x, t, r, grad_logprobs=gl, grad_entropy=gh, grad_lse=gz, temperature=temperature,
+                                   grad_top_logprobs=gt if top_n else None)
+    xd = x.double() / temperature
+    far = xd.amax(1)  # of each other id from the token
+    rest = 63 * torch.exp(-far)  # S - 1
+    logp = -torch.log1p(rest)
+    one_less_p = -torch.expm1(logp)
+    p = torch.exp(logp)
+    entropy = -p * logp + rest * p * (far - logp)
+    own = 1.5 + (0.5 if top_n else 0.0)
+    want = (own * one_less_p + 0.25 * p * (logp + entropy)) / temperature
+    got = grad[torch.arange(3, device=cuda_device), t].double()
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0  # the fp32 rounding is in the count above
+    err = ((got - want) / want).abs()
+    assert float(err.max()) <= 2.0 ** -16 * (1 + half) + half, err
