@@ -15,6 +15,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _native as N
 from .int8_head import _DTYPES, _same_device, launch_on, matrix
@@ -29,6 +30,12 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor          # [R, n] int64, -1 where there are fewer alternatives
     top_logprobs: torch.Tensor     # [R, n] float32
     stats: torch.Tensor            # [R, 4] float32, for token_logprobs_backward
+
+
+def _no_tangent(*tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("token log probabilities have no forward-mode derivative")
 
 
 def _tokens(tokens: torch.Tensor | None, logits: torch.Tensor) -> torch.Tensor | None:
@@ -93,7 +100,8 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
     zeros).  This is what autograd runs; called directly it needs no autograd
     graph, so it can be captured in a CUDA graph.  ``logits``, ``tokens`` and
     ``temperature`` are the forward call's; ``out`` has the logits' shape and
-    dtype and must not overlap them."""
+    dtype and must not overlap them.  Itself not differentiable."""
+    _no_tangent(logits, grad_logprobs, grad_entropy, grad_lse, grad_top_logprobs)
     stride = matrix(logits, "logits")
     rows, vocab = logits.shape
     device = logits.device
@@ -189,7 +197,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     ``status`` (int32 ``[R]``) receives the row bits that
     :func:`~mapperatorinator_b200.sampling.row_status_report` reads.  Gradients
     flow from ``logprobs``, ``entropy``, ``lse`` and ``top_logprobs`` to the
-    logits (once; not through ``top_ids``)."""
+    logits (once, in reverse mode; not through ``top_ids``)."""
+    _no_tangent(logits)
     tokens = _tokens(tokens, logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         hold: list = []

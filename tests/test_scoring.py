@@ -557,3 +557,40 @@ def test_small_gradients_keep_their_digits(cuda_device, dtype, temperature, top_
     half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0  # the fp32 rounding is in the count above
     err = ((got - want) / want).abs()
     assert float(err.max()) <= 2.0 ** -16 * (1 + half) + half, err
+
+
+# ------------------------------------------------------------------ forward-mode derivatives
+
+
+def _refuses_tangents(device):
+    import torch.autograd.forward_ad as fwd
+
+    x, t = torch.randn((3, 20), device=device), torch.tensor([1, 2, 3], device=device)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            token_logprobs(dual, t)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            token_logprobs(dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            token_logprobs(dual, t)
+        result = TokenLogprobs(None, x[:, 0], x[:, 0], t[:, None][:, :0], x[:, :0], x[:, :4].contiguous())
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            token_logprobs_backward(dual, t, result, grad_lse=x[:, 0].contiguous())
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            token_logprobs_backward(x, t, result, grad_lse=fwd.make_dual(x[:, 0].contiguous(), torch.ones(3, device=device)))
+
+
+def test_forward_mode_is_refused():
+    _refuses_tangents("cpu")
+
+
+@gpu
+def test_forward_mode_is_refused_and_plain_tensors_pass(cuda_device):
+    import torch.autograd.forward_ad as fwd
+
+    _refuses_tangents(cuda_device)
+    x, t = inputs(cuda_device, 5, 70, torch.float32)
+    want = token_logprobs(x, t)
+    with fwd.dual_level():
+        assert torch.equal(token_logprobs(x, t).logprobs, want.logprobs)
