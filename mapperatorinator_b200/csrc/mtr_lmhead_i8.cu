@@ -550,7 +550,7 @@ static cudaError_t launch_quantize(const void* x, int64_t x_stride, int dtype, i
   while (per < QUANT_THREADS && units > (int64_t)per * (wide ? 8 : 4)) per *= 2;
   const QuantParams p{x, x_stride, rows, cols, per, q, q_stride, scale};
   cudaLaunchAttribute attr[2];
-  const int high = QUANT_THREADS / per;
+  const int64_t high = QUANT_THREADS / per;
   const cudaLaunchConfig_t cfg = config(dim3((unsigned)((rows + high - 1) / high), 1, 1), QUANT_THREADS, 0, 1, s, attr);
   auto launch = [&](auto of, auto wide_of, auto single) {
     return cudaLaunchKernelEx(&cfg, wide ? wide_of : vec ? of : single, p);

@@ -422,3 +422,21 @@ def test_logits_of_subnormal_scales(cuda_device, rows, cols):
     out = lm_head_logits_int8(x.to(cuda_device), wide_d[:, :cols], ws.to(cuda_device), out_dtype=torch.float32)
     q, scale = held_quantize(x)
     same(out, plain_logits(q, scale, wide[:, :cols], ws, torch.float32))
+
+
+# ------------------------------------------------------------------ the largest row count
+
+
+@gpu
+def test_quantize_as_many_rows_as_the_count_holds(cuda_device):
+    rows = 2 ** 31 - 1
+    x = torch.full((rows,), 3.0, dtype=torch.bfloat16, device=cuda_device)
+    x[-1], x[-2] = -3.0, 0.0
+    q = torch.zeros(rows, dtype=torch.int8, device=cuda_device)
+    scale = torch.empty(rows, device=cuda_device)
+    a = N.sized(N.MtrQuantizeArgs, x=x.data_ptr(), x_row_stride=1, x_dtype=N.DTYPE_BF16, rows=rows, cols=1, q=q.data_ptr(),
+                q_row_stride=1, scale=scale.data_ptr())
+    N.quantize_rows_launch(a, torch.cuda.current_stream().cuda_stream)
+    want = float(torch.tensor(3.0) * torch.tensor(1 / 127, dtype=torch.float32))
+    assert q[-1] == -127 and q[-2] == 0 and scale[-2] == 0 and scale[-1] == want
+    assert bool((q[:-2] == 127).all()) and bool((scale[:-2] == want).all())
