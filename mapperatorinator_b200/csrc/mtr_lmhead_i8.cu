@@ -648,12 +648,7 @@ static cudaError_t launch_proj(const MtrLmHeadI8Args& a, const int8_t* q, int64_
 
 static bool dtype_ok(int32_t dtype) { return dtype >= MTR_DTYPE_F32 && dtype <= MTR_DTYPE_F16; }
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
-// bytes [p, p + n) and [q, q + m) share one
-static bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
-  return (uintptr_t)p < (uintptr_t)q + (uintptr_t)m && (uintptr_t)q < (uintptr_t)p + (uintptr_t)n;
-}
-static int64_t span(int64_t rows, int64_t stride, int64_t cols, int64_t es) { return ((rows - 1) * stride + cols) * es; }
+static mtr::Bytes run_of(const void* at, int64_t n) { return {at, 1, n, n}; }
 
 }  // namespace i8
 
@@ -672,9 +667,9 @@ int mtr_quantize_rows_validate(const MtrQuantizeArgs* a) {
   if (!a->x || !a->q || !a->scale) return MTR_ERR_NULL_ARG;
   if (a->x_row_stride < a->cols || a->q_row_stride < a->cols) return MTR_ERR_BAD_SHAPE;
   if ((uintptr_t)a->x % esize(a->x_dtype) || (uintptr_t)a->scale % 4) return MTR_ERR_ALIGNMENT;
-  const int64_t xs = span(a->rows, a->x_row_stride, a->cols, esize(a->x_dtype)), qs = span(a->rows, a->q_row_stride, a->cols, 1);
-  if (overlap(a->x, xs, a->q, qs) || overlap(a->x, xs, a->scale, 4ll * a->rows) || overlap(a->q, qs, a->scale, 4ll * a->rows))
-    return MTR_ERR_BAD_PARAM;
+  const mtr::Bytes x = mtr::bytes_of(a->x, a->rows, a->x_row_stride, a->cols, esize(a->x_dtype));
+  const mtr::Bytes q = mtr::bytes_of(a->q, a->rows, a->q_row_stride, a->cols, 1), scale = run_of(a->scale, 4ll * a->rows);
+  if (overlap(x, q) || overlap(x, scale) || overlap(q, scale)) return MTR_ERR_BAD_PARAM;
   return MTR_OK;
 }
 
@@ -710,14 +705,12 @@ int mtr_lmhead_i8_validate(const MtrLmHeadI8Args* a) {
       (uintptr_t)a->weight_scale % 4 || (uintptr_t)a->logits % esize(a->logits_dtype) || (uintptr_t)a->workspace % 256 ||
       (uintptr_t)a->error_word % 4)
     return MTR_ERR_ALIGNMENT;
-  const int64_t ls = span(a->rows, a->logits_row_stride, a->vocab, esize(a->logits_dtype));
-  const int64_t hs = span(a->rows, a->hidden_row_stride, a->d_model, esize(a->hidden_dtype));
-  const int64_t ws = span(a->vocab, a->weight_row_stride, a->d_model, 1);
-  if (overlap(a->logits, ls, a->hidden, hs) || overlap(a->logits, ls, a->weight, ws) ||
-      overlap(a->logits, ls, a->weight_scale, 4ll * a->vocab))
-    return MTR_ERR_BAD_PARAM;
-  if (need > 0 && (overlap(a->logits, ls, a->workspace, need) || overlap(a->workspace, need, a->hidden, hs) ||
-                   overlap(a->workspace, need, a->weight, ws) || overlap(a->workspace, need, a->weight_scale, 4ll * a->vocab)))
+  const mtr::Bytes logits = mtr::bytes_of(a->logits, a->rows, a->logits_row_stride, a->vocab, esize(a->logits_dtype));
+  const mtr::Bytes hidden = mtr::bytes_of(a->hidden, a->rows, a->hidden_row_stride, a->d_model, esize(a->hidden_dtype));
+  const mtr::Bytes weight = mtr::bytes_of(a->weight, a->vocab, a->weight_row_stride, a->d_model, 1);
+  const mtr::Bytes scale = run_of(a->weight_scale, 4ll * a->vocab), work = run_of(a->workspace, need);
+  if (overlap(logits, hidden) || overlap(logits, weight) || overlap(logits, scale)) return MTR_ERR_BAD_PARAM;
+  if (need > 0 && (overlap(logits, work) || overlap(work, hidden) || overlap(work, weight) || overlap(work, scale)))
     return MTR_ERR_BAD_PARAM;
   return MTR_OK;
 }

@@ -801,13 +801,6 @@ static cudaError_t launch_grad(const GradParams& p, cudaStream_t s) {
                : launch(logprob_grad_kernel<T, false>, p, grid, threads, 1, s);
 }
 
-// whether two row-strided matrices share a byte
-static bool overlap(const void* a, int64_t sa, const void* b, int64_t sb, int64_t rows, int64_t cols, int64_t es) {
-  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-  const uintptr_t a1 = a0 + (uintptr_t)(((rows - 1) * sa + cols) * es), b1 = b0 + (uintptr_t)(((rows - 1) * sb + cols) * es);
-  return a0 < b1 && b0 < a1;
-}
-
 template <typename A>
 static int check_common(const A* a) {
   if (!a) return MTR_ERR_NULL_ARG;
@@ -888,7 +881,9 @@ int mtr_logprob_grad_validate(const MtrLogprobGradArgs* a) {
       (uintptr_t)a->g_entropy % 4 || (uintptr_t)a->g_lse % 4 || (uintptr_t)a->g_top % 4 ||
       (uintptr_t)a->grad_logits % esize(a->logits_dtype))
     return MTR_ERR_ALIGNMENT;
-  if (overlap(a->logits, a->logits_row_stride, a->grad_logits, a->grad_row_stride, a->rows, a->vocab, esize(a->logits_dtype)))
+  const int64_t es = esize(a->logits_dtype);
+  if (overlap(mtr::bytes_of(a->logits, a->rows, a->logits_row_stride, a->vocab, es),
+              mtr::bytes_of(a->grad_logits, a->rows, a->grad_row_stride, a->vocab, es)))
     return MTR_ERR_BAD_PARAM;
   return MTR_OK;
 }

@@ -18,6 +18,22 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// ---------------------------------------------------------------- host side
+// A row-strided matrix as bytes: `rows` rows of `width`, `stride` apart.
+struct Bytes {
+  const void* at;
+  int64_t rows, stride, width;
+};
+inline Bytes bytes_of(const void* at, int64_t rows, int64_t stride, int64_t cols, int64_t es) { return {at, rows, stride * es, cols * es}; }
+// Whether two share a byte: their spans overlap, and they do not lie side by side in rows of one width.
+inline bool overlap(const Bytes& a, const Bytes& b) {
+  const uintptr_t a0 = (uintptr_t)a.at, b0 = (uintptr_t)b.at;
+  if (a0 >= b0 + (uintptr_t)((b.rows - 1) * b.stride + b.width) || b0 >= a0 + (uintptr_t)((a.rows - 1) * a.stride + a.width)) return false;
+  if (a.stride != b.stride) return true;
+  const int64_t off = (int64_t)(b0 - a0) % a.stride, behind = off < 0 ? off + a.stride : off;  // from a row of a to the next of b
+  return behind < a.width || behind + b.width > a.stride;
+}
+
 // max that gives NaN when an operand is NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;

@@ -440,3 +440,37 @@ def test_quantize_as_many_rows_as_the_count_holds(cuda_device):
     want = float(torch.tensor(3.0) * torch.tensor(1 / 127, dtype=torch.float32))
     assert q[-1] == -127 and q[-2] == 0 and scale[-2] == 0 and scale[-1] == want
     assert bool((q[:-2] == 127).all()) and bool((scale[:-2] == want).all())
+
+
+# ------------------------------------------------------------------ matrices side by side in one buffer
+
+
+@pytest.mark.parametrize("at,code", [(100, N.OK), (99, N.ERR_BAD_PARAM), (300 - 77, N.OK), (300 - 76, N.ERR_BAD_PARAM),
+                                     (300 + 100, N.OK), (-77, N.OK), (-76, N.ERR_BAD_PARAM), (0, N.ERR_BAD_PARAM)])
+def test_hidden_and_logits_may_share_a_buffer_of_wider_rows(at, code):
+    a = _proj_args()
+    a.hidden_row_stride = a.logits_row_stride = 300
+    a.logits = a.hidden + 2 * at
+    lib = N.load()
+    assert lib.mtr_lmhead_i8_validate(ctypes.byref(a)) == code
+    a.logits_row_stride = 301  # rows that drift against each other may meet
+    assert lib.mtr_lmhead_i8_validate(ctypes.byref(a)) == N.ERR_BAD_PARAM
+
+
+@pytest.mark.parametrize("at,code", [(128, N.OK), (127, N.ERR_BAD_PARAM), (256 - 64, N.OK), (256 - 63, N.ERR_BAD_PARAM)])
+def test_rows_and_their_int8_may_share_a_buffer_of_wider_rows(at, code):
+    a = _quant_args(x_row_stride=128, q_row_stride=256)
+    a.q = a.x + at
+    assert N.load().mtr_quantize_rows_validate(ctypes.byref(a)) == code
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 150])
+def test_hidden_and_logits_in_one_buffer(cuda_device, rows):
+    h, w = inputs(cuda_device, rows, 200, 301, seed=21)
+    weight = Int8Weight.from_weight(w)
+    both = torch.full((rows, 520), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    both[:, :200] = h
+    lm_head_logits_int8(both[:, :200], weight.q, weight.scale, both[:, 204:505])
+    assert torch.equal(both[:, 204:505], lm_head_logits_int8(h, weight.q, weight.scale))
+    assert torch.equal(both[:, :200], h) and bool((both[:, 200:204] == 7.0).all()) and bool((both[:, 505:] == 7.0).all())

@@ -594,3 +594,30 @@ def test_forward_mode_is_refused_and_plain_tensors_pass(cuda_device):
     want = token_logprobs(x, t)
     with fwd.dual_level():
         assert torch.equal(token_logprobs(x, t).logprobs, want.logprobs)
+
+
+# ------------------------------------------------------------------ logits and gradient side by side in one buffer
+
+
+@pytest.mark.parametrize("at,code", [(64, N.OK), (63, N.ERR_BAD_PARAM), (150 - 64, N.OK), (150 - 63, N.ERR_BAD_PARAM), (-64, N.OK)])
+def test_logits_and_gradient_may_share_a_buffer_of_wider_rows(at, code):
+    import ctypes
+
+    a = N.sized(N.MtrLogprobGradArgs, logits=0x10000, logits_row_stride=150, tokens=0x20000, logits_dtype=N.DTYPE_BF16,
+                tokens_dtype=N.IDS_I64, rows=4, vocab=64, top_n=0, temperature=1.0, stats=0x35000, g_logprobs=0x36000,
+                grad_logits=0x10000 + 2 * at, grad_row_stride=150)
+    assert N.load().mtr_logprob_grad_validate(ctypes.byref(a)) == code
+
+
+@gpu
+@pytest.mark.parametrize("gap", [0, 3])
+def test_logits_and_gradient_in_one_buffer(cuda_device, gap):
+    rows, vocab = 40, 1000
+    x, t = inputs(cuda_device, rows, vocab, torch.bfloat16, seed=22)
+    both = torch.full((rows, 2 * vocab + gap), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    both[:, :vocab] = x
+    g = torch.rand(rows, device=cuda_device)
+    logits, grad = both[:, :vocab], both[:, vocab + gap:]
+    token_logprobs_backward(logits, t, token_logprobs(logits, t), grad_logprobs=g, grad_lse=g, out=grad)
+    assert torch.equal(grad, token_logprobs_backward(x, t, token_logprobs(x, t), grad_logprobs=g, grad_lse=g))
+    assert torch.equal(logits, x) and bool((both[:, vocab:vocab + gap] == 7.0).all())
