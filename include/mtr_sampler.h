@@ -59,6 +59,7 @@ extern "C" {
 #define MTR_MAX_I8_ROWS (1 << 22)
 #define MTR_MAX_SCORE_ROWS (1 << 27)
 #define MTR_MAX_TOP_N 32
+#define MTR_MAX_TEMPERATURE 0x1p100f /* of the scores: e^((x - max) / T) is 0 where x - max passes the fp32 range */
 
 /* Return codes of every entry point. */
 typedef enum MtrStatus {
@@ -401,7 +402,7 @@ typedef struct MtrLogprobArgs {
   int32_t rows;                 /* 0 .. MTR_MAX_SCORE_ROWS */
   int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
   int32_t top_n;                /* 0 .. MTR_MAX_TOP_N */
-  float temperature;            /* > 0, finite, with a finite reciprocal */
+  float temperature;            /* > 0, with a finite reciprocal, <= MTR_MAX_TEMPERATURE */
   float* out_logprobs;          /* [rows] or NULL */
   float* out_entropy;           /* [rows] or NULL */
   float* out_lse;               /* [rows] or NULL */

@@ -30,6 +30,7 @@ MAX_I8_D_MODEL = 131072
 MAX_I8_ROWS = 1 << 22
 MAX_SCORE_ROWS = 1 << 27
 MAX_TOP_N = 32
+MAX_TEMPERATURE = 2.0 ** 100  # of the scores
 
 # MtrStatus
 OK = 0

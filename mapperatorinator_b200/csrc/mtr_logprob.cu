@@ -22,7 +22,9 @@
 // d = -1000, whose 2^d is 0 and whose product with d is 0 as well (-inf would
 // give NaN), and a score equal to the maximum, whose d is +0 = 0, becomes -1000
 // too and so leaves the sums: it is counted in n.  NaN is found by the maximum,
-// which keeps it.  Terms below 2^-126 count as 0, in the sums and in the gradient.
+// which keeps it.  Terms below 2^-126 count as 0, in the sums and in the gradient;
+// so do those whose x - m passes the fp32 range (T <= 2^100 leaves less than
+// -2^27 of it), but their log probabilities are finite again (log_prob).
 #include "mtr_vec.cuh"
 
 namespace mtr {
@@ -161,7 +163,10 @@ __device__ __forceinline__ Row row_of(const Part& p, float inv_t) {
 __device__ __forceinline__ float log_prob(float x, const Row& r, float inv_t) {
   if (r.bad) return qnan();
   if (r.none || x == neg_inf()) return neg_inf();
-  return (x - r.m) * inv_t - r.log_s;
+  const float away = x - r.m;
+  // beyond the range, where T > 1 may bring it back: by halves
+  if (!(away > neg_inf())) return (0.5f * x - 0.5f * r.m) * inv_t * 2.0f - r.log_s;
+  return away * inv_t - r.log_s;
 }
 
 __device__ __forceinline__ float warp_max_nan(float v) {
@@ -809,7 +814,7 @@ static int check_common(const A* a) {
   if (a->logits_dtype < MTR_DTYPE_F32 || a->logits_dtype > MTR_DTYPE_F16) return MTR_ERR_BAD_PARAM;
   if (a->tokens_dtype != MTR_IDS_I64 && a->tokens_dtype != MTR_IDS_I32) return MTR_ERR_BAD_PARAM;
   if (a->top_n < 0 || a->top_n > MTR_MAX_TOP_N) return MTR_ERR_BAD_PARAM;
-  if (!(a->temperature > 0.0f) || !(a->temperature < INFINITY) || !(1.4426950408889634f / a->temperature < INFINITY))
+  if (!(a->temperature > 0.0f) || !(a->temperature <= MTR_MAX_TEMPERATURE) || !(1.4426950408889634f / a->temperature < INFINITY))
     return MTR_ERR_BAD_PARAM;
   if (a->rows == 0) return MTR_OK;
   if (!a->logits) return MTR_ERR_NULL_ARG;

@@ -184,7 +184,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
 
     ``logits`` is ``[R, V]`` (float32, bfloat16 or float16, any row stride >= V),
     ``tokens`` ``[R]`` int64 or int32, or None for the entropy, log-sum-exp and
-    alternatives alone; ``top_n`` is at most 32.  Results are float32.
+    alternatives alone; ``top_n`` is at most 32, ``temperature`` at most 2^100.
+    Results are float32.
 
     - Masked ids (-inf) have probability 0, add nothing to the entropy and are
       never alternatives: where a row has fewer ids left the missing ones read

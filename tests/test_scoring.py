@@ -621,3 +621,47 @@ def test_logits_and_gradient_in_one_buffer(cuda_device, gap):
     token_logprobs_backward(logits, t, token_logprobs(logits, t), grad_logprobs=g, grad_lse=g, out=grad)
     assert torch.equal(grad, token_logprobs_backward(x, t, token_logprobs(x, t), grad_logprobs=g, grad_lse=g))
     assert torch.equal(logits, x) and bool((both[:, vocab:vocab + gap] == 7.0).all())
+
+
+# ------------------------------------------------------------------ logits further apart than the type's largest value
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 2.0 ** 100])
+@pytest.mark.parametrize("vocab", [5, 700, 70000])
+def test_logits_at_both_ends_of_the_range(cuda_device, dtype, temperature, vocab):
+    # x - max passes the range before the division by T brings it back
+    x = torch.zeros((4, vocab), device=cuda_device)
+    x[0, 0], x[0, 1], x[0, 2] = 3.0e38, -3.0e38, 2.0e38
+    x[1] = -3.0e38
+    x[1, vocab - 1] = 3.0e38
+    x[2, ::2] = 1.0e38
+    x[2, 1::2] = -2.5e38
+    x[3, 3] = -math.inf
+    x[3, 4] = torch.finfo(dtype).max
+    x = x.to(dtype)
+    t = torch.tensor([1, 0, 1, 4], device=cuda_device)
+    r = token_logprobs(x, t, top_n=4, temperature=temperature)
+    ref = reference(x, t, 4, temperature)
+    f32 = lambda v: v.float().double()  # noqa: E731  a log probability below the fp32 range reads -inf
+    es, eh = bounds(ref, vocab)
+    close(r.logprobs, f32(ref["logprobs"]), es + 4 * U * ref["logprobs"].abs(), "logprobs")
+    close(r.entropy, ref["entropy"], eh, "entropy")
+    close(r.lse, ref["lse"], es + 2 * U * ref["lse"].abs(), "lse")
+    assert torch.equal(r.top_ids, ref["top_ids"])
+    close(r.top_logprobs, f32(ref["top_logprobs"]), es[:, None] + 4 * U * ref["top_logprobs"].abs().nan_to_num(0, 0, 0), "top")
+    g = torch.tensor([1.0, -2.0, 0.5, 3.0], device=cuda_device) * temperature
+    grad = token_logprobs_backward(x, t, r, grad_logprobs=g, grad_entropy=g, grad_lse=-g, temperature=temperature)
+    dx, tol = plain_gradient(ref, t, vocab, temperature, g.double(), g.double(), -g.double(), None, None)
+    check_gradient(grad, dx, tol, dtype)
+
+
+@pytest.mark.parametrize("temperature,code", [(2.0 ** 100, N.OK), (2.0 ** 100 * (1 + 2.0 ** -23), N.ERR_BAD_PARAM), (3.0e38, N.ERR_BAD_PARAM)])
+def test_largest_temperature(temperature, code):
+    import ctypes
+
+    a = _args(temperature=temperature)
+    assert N.load().mtr_logprob_validate(ctypes.byref(a)) == code
+    if code != N.OK:
+        assert N.load().mtr_logprob_launch(ctypes.byref(a), None) == code
