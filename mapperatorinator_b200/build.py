@@ -51,15 +51,17 @@ def _nvcc() -> str:
 
 def _deps(src: Path) -> list:
     """Headers a translation unit includes (the stream kernel's also include mtr_stream.cuh, the
-    projections' mtr_tc.cuh, the row-streaming kernels'
-    mtr_vec.cuh and mtr_quant.cuh)."""
+    tensor-core projections' mtr_tc.cuh, the row-streaming kernels' mtr_vec.cuh, those that
+    quantise mtr_quant.cuh)."""
     deps = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh"]
     if src.name.startswith("mtr_stream"):
         deps.append(CSRC / "mtr_stream.cuh")
-    if src.name.startswith("mtr_lmhead"):
+    if src.name in ("mtr_lmhead.cu", "mtr_lmhead_i8.cu"):
         deps.append(CSRC / "mtr_tc.cuh")
     if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu", "mtr_logprob.cu"):
-        deps += [CSRC / "mtr_vec.cuh", CSRC / "mtr_quant.cuh"]
+        deps.append(CSRC / "mtr_vec.cuh")
+    if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu"):
+        deps.append(CSRC / "mtr_quant.cuh")
     return deps
 
 

@@ -18,7 +18,7 @@ import torch
 
 from . import _native as N
 
-_DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
+DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
 
 
 def launch_on(device: torch.device, launch, *args) -> None:
@@ -30,7 +30,7 @@ def launch_on(device: torch.device, launch, *args) -> None:
             launch(*args, torch._C._cuda_getCurrentRawStream(device.index))
 
 
-def matrix(t: torch.Tensor, what: str, dtypes=_DTYPES) -> int:
+def matrix(t: torch.Tensor, what: str, dtypes=DTYPES) -> int:
     """Checks a 2-D CUDA tensor with unit column stride; returns its row stride in elements."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
@@ -43,7 +43,7 @@ def matrix(t: torch.Tensor, what: str, dtypes=_DTYPES) -> int:
     return stride[0] if shape[0] > 1 else max(shape[1], 1)
 
 
-def _same_device(t: torch.Tensor, device: torch.device, what: str) -> None:
+def same_device(t: torch.Tensor, device: torch.device, what: str) -> None:
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, not on {device}")
 
@@ -78,7 +78,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     wide = (cols + 15) // 16 * 16
     q = torch.empty((rows, wide), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    a = N.sized(N.MtrQuantizeArgs, x=x.data_ptr(), x_row_stride=stride, x_dtype=_DTYPES[x.dtype], rows=rows, cols=cols,
+    a = N.sized(N.MtrQuantizeArgs, x=x.data_ptr(), x_row_stride=stride, x_dtype=DTYPES[x.dtype], rows=rows, cols=cols,
                 q=q.data_ptr(), q_row_stride=wide, scale=scale.data_ptr())
     launch_on(x.device, N.quantize_rows_launch, a)
     return q[:, :cols], scale
@@ -92,7 +92,7 @@ def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: t
     rows, d = hidden.shape
     vocab = weight_q.shape[0]
     for t, what in ((weight_q, "weight_q"), (weight_scale, "weight_scale"), (out, "logits")):
-        _same_device(t, device, what)
+        same_device(t, device, what)
     if weight_q.shape[1] != d:
         raise ValueError(f"hidden d_model {d} != weight d_model {weight_q.shape[1]}")
     if weight_scale.dtype != torch.float32 or weight_scale.shape != (vocab,) or (vocab > 1 and weight_scale.stride(0) != 1):
@@ -105,7 +105,7 @@ def lmhead_i8_args(hidden: torch.Tensor, weight_q: torch.Tensor, weight_scale: t
     work = hidden.new_empty(need, dtype=torch.uint8) if need else None
     a = N.sized(N.MtrLmHeadI8Args, hidden=hidden.data_ptr(), hidden_row_stride=hs, weight=weight_q.data_ptr(),
                 weight_row_stride=ws, weight_scale=weight_scale.data_ptr(), logits=out.data_ptr(), logits_row_stride=ls,
-                hidden_dtype=_DTYPES[hidden.dtype], logits_dtype=_DTYPES[out.dtype], rows=rows, d_model=d, vocab=vocab,
+                hidden_dtype=DTYPES[hidden.dtype], logits_dtype=DTYPES[out.dtype], rows=rows, d_model=d, vocab=vocab,
                 workspace=work.data_ptr() if need else None, workspace_bytes=need)
     return a, work
 
@@ -120,7 +120,7 @@ def lm_head_logits_int8(hidden: torch.Tensor, weight_q: torch.Tensor, weight_sca
     wait that gave up left without a value are NaN
     (:func:`~mapperatorinator_b200.sampling.projection_timeouts`)."""
     if out is None:
-        if out_dtype not in _DTYPES:
+        if out_dtype not in DTYPES:
             raise TypeError(f"out_dtype {out_dtype} is not supported (float32, bfloat16, float16)")
         out = hidden.new_empty((hidden.shape[0], weight_q.shape[0]), dtype=out_dtype)
     a, work = lmhead_i8_args(hidden, weight_q, weight_scale, out)

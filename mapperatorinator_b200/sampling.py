@@ -477,7 +477,8 @@ class FusedSampler:
         ``hidden`` has the logits' rows ([2B, d] with CFG).  The logits stay
         readable in ``self.lm_logits`` until the next call.  An
         :class:`~mapperatorinator_b200.int8_head.Int8Weight` takes the 8-bit
-        projection (``lm_head_logits_int8``) instead."""
+        projection (``lm_head_logits_int8``) instead; ``tile_n`` is the bf16
+        projection's alone."""
         _require_cuda(hidden, "hidden")
         i8 = isinstance(weight, Int8Weight)
         rows = hidden.shape[0]

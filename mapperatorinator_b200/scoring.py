@@ -18,7 +18,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from . import _native as N
-from .int8_head import _DTYPES, _same_device, launch_on, matrix
+from .int8_head import DTYPES, same_device, launch_on, matrix
 
 
 class TokenLogprobs(NamedTuple):
@@ -45,7 +45,7 @@ def _tokens(tokens: torch.Tensor | None, logits: torch.Tensor) -> torch.Tensor |
         raise TypeError(f"tokens dtype {tokens.dtype} is not supported (int64, int32)")
     if tokens.shape != logits.shape[:1]:
         raise ValueError(f"tokens must have one id per row ({logits.shape[0]})")
-    _same_device(tokens, logits.device, "tokens")
+    same_device(tokens, logits.device, "tokens")
     return tokens.contiguous()
 
 
@@ -57,7 +57,7 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
     if status is not None:
         if status.dtype != torch.int32 or status.shape != (rows,) or not status.is_contiguous():
             raise ValueError(f"status must be a contiguous int32 vector of {rows} elements")
-        _same_device(status, device, "status")
+        same_device(status, device, "status")
     n = int(top_n)
     if not 0 <= n <= N.MAX_TOP_N:
         raise ValueError(f"top_n must be 0 .. {N.MAX_TOP_N}")
@@ -68,7 +68,7 @@ def _forward(logits: torch.Tensor, tokens: torch.Tensor | None, top_n: int, temp
     logprobs = logits.new_empty(rows, dtype=f32) if tokens is not None else None
     top_ids = logits.new_empty((rows, n), dtype=torch.int64)
     top_logprobs = logits.new_empty((rows, n), dtype=f32)
-    a = N.sized(N.MtrLogprobArgs, logits=logits.data_ptr(), logits_row_stride=stride, logits_dtype=_DTYPES[logits.dtype],
+    a = N.sized(N.MtrLogprobArgs, logits=logits.data_ptr(), logits_row_stride=stride, logits_dtype=DTYPES[logits.dtype],
                 tokens_dtype=N.IDS_I32 if tokens is not None and tokens.dtype == torch.int32 else N.IDS_I64,
                 rows=rows, vocab=vocab, top_n=n, temperature=float(temperature), out_entropy=entropy.data_ptr(),
                 out_lse=lse.data_ptr(), out_stats=stats.data_ptr())
@@ -87,7 +87,7 @@ def _grad_input(g: torch.Tensor | None, shape, device, what: str) -> torch.Tenso
         return None
     if g.dtype != torch.float32 or tuple(g.shape) != tuple(shape):
         raise ValueError(f"{what} must be float32 of shape {tuple(shape)}")
-    _same_device(g, device, what)
+    same_device(g, device, what)
     return g.contiguous()  # sums and means hand in expanded scalars
 
 
@@ -113,7 +113,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
     if n and (top_ids.dtype != torch.int64 or top_ids.shape[0] != rows or not top_ids.is_contiguous()):
         raise ValueError(f"result.top_ids must be a contiguous int64 tensor of {rows} rows")
     for t, what in ((stats, "result.stats"), (top_ids, "result.top_ids")):
-        _same_device(t, device, what)
+        same_device(t, device, what)
     if grad_logprobs is not None and tokens is None:
         raise ValueError("grad_logprobs needs the tokens")
     gl = _grad_input(grad_logprobs, (rows,), device, "grad_logprobs")
@@ -125,7 +125,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
     elif out.dtype != logits.dtype or out.shape != logits.shape:
         raise ValueError("out must have the logits' shape and dtype")
     out_stride = matrix(out, "out")
-    _same_device(out, device, "out")
+    same_device(out, device, "out")
     return _launch_backward(logits, stride, tokens, stats, top_ids, n, gl, ge, gz, gt, temperature, out, out_stride)
 
 
@@ -133,7 +133,7 @@ def _launch_backward(logits, stride, tokens, stats, top_ids, n, gl, ge, gz, gt, 
     """The launch of token_logprobs_backward; every argument has been checked."""
     rows, vocab = logits.shape
     a = N.sized(N.MtrLogprobGradArgs, logits=logits.data_ptr(), logits_row_stride=stride,
-                logits_dtype=_DTYPES[logits.dtype],
+                logits_dtype=DTYPES[logits.dtype],
                 tokens_dtype=N.IDS_I32 if tokens is not None and tokens.dtype == torch.int32 else N.IDS_I64,
                 rows=rows, vocab=vocab, top_n=n, temperature=float(temperature), stats=stats.data_ptr(),
                 grad_logits=out.data_ptr(), grad_row_stride=out_stride)

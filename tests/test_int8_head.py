@@ -474,3 +474,16 @@ def test_hidden_and_logits_in_one_buffer(cuda_device, rows):
     lm_head_logits_int8(both[:, :200], weight.q, weight.scale, both[:, 204:505])
     assert torch.equal(both[:, 204:505], lm_head_logits_int8(h, weight.q, weight.scale))
     assert torch.equal(both[:, :200], h) and bool((both[:, 200:204] == 7.0).all()) and bool((both[:, 505:] == 7.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dequantized_weight(cuda_device, dtype):
+    _, w = inputs(cuda_device, 1, 203, 37, seed=30)
+    w[4] = 0.0
+    w = w.to(dtype)
+    back = Int8Weight.from_weight(w).dequantize()
+    assert back.shape == w.shape and back.dtype == torch.float32 and bool((back[4] == 0).all())
+    # half a step of the row's scale, and the roundings of the scale, the quotient and the product
+    step = w.float().abs().amax(1, keepdim=True) / 127
+    assert bool(((back - w.float()).abs() <= 0.5 * step + 4 * 2.0 ** -24 * 127 * step).all())
