@@ -44,6 +44,7 @@ struct FwdParams {
   int32_t cluster;  // CTAs of a row
   float scale;      // log2(e) / T
   float inv_t;      // 1 / T
+  float part, part_inv_t;  // 1/2 and 2 / T where T > 1, which may bring back what x - m takes out of the range; else 1 and 1 / T
   float* logprobs;
   float* entropy;
   float* lse;
@@ -160,13 +161,10 @@ __device__ __forceinline__ Row row_of(const Part& p, float inv_t) {
   }
   return r;
 }
-__device__ __forceinline__ float log_prob(float x, const Row& r, float inv_t) {
+__device__ __forceinline__ float log_prob(float x, const Row& r, const FwdParams& p) {
   if (r.bad) return qnan();
   if (r.none || x == neg_inf()) return neg_inf();
-  const float away = x - r.m;
-  // beyond the range, where T > 1 may bring it back: by halves
-  if (!(away > neg_inf())) return (0.5f * x - 0.5f * r.m) * inv_t * 2.0f - r.log_s;
-  return away * inv_t - r.log_s;
+  return fmaf(fmaf(x, p.part, -(r.m * p.part)), p.part_inv_t, -r.log_s);
 }
 
 __device__ __forceinline__ float warp_max_nan(float v) {
@@ -471,7 +469,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       uint32_t st = r.bad ? MTR_ROW_NONFINITE : r.none ? MTR_ROW_ALL_MASKED : 0u;
       if (p.tokens) {
         if (token >= V) st |= MTR_ROW_BAD_ID;
-        if (p.logprobs) p.logprobs[row] = (token < 0 || token >= V) ? 0.0f : log_prob(token_x, r, p.inv_t);
+        if (p.logprobs) p.logprobs[row] = (token < 0 || token >= V) ? 0.0f : log_prob(token_x, r, p);
       }
       if (p.entropy) p.entropy[row] = r.entropy;
       if (p.lse) p.lse[row] = r.lse;
@@ -586,7 +584,7 @@ __global__ void __launch_bounds__(W * 32, Plan<T, W>::WARPS / W) logprob_kernel(
       const int place = place_of(sh.list, c, k);
       if (place < n) {
         ids[place] = key_id(k);
-        lps[place] = log_prob(key_value(k), r, p.inv_t);
+        lps[place] = log_prob(key_value(k), r, p);
       }
     }
     for (int j = c + tid; j < n; j += THREADS) {
@@ -856,6 +854,8 @@ int mtr_logprob_launch(const MtrLogprobArgs* a, void* stream) {
   p.top_n = a->top_n;
   p.scale = (float)(1.4426950408889634 / (double)a->temperature);
   p.inv_t = (float)(1.0 / (double)a->temperature);
+  p.part = a->temperature > 1.0f ? 0.5f : 1.0f;
+  p.part_inv_t = p.inv_t / p.part;
   p.logprobs = a->out_logprobs;
   p.entropy = a->out_entropy;
   p.lse = a->out_lse;
