@@ -33,6 +33,8 @@ class TokenLogprobs(NamedTuple):
 
 
 def _no_tangent(*tensors: torch.Tensor | None) -> None:
+    if forward_ad._current_level < 0:  # no dual level is open: nothing carries a tangent
+        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError("token log probabilities have no forward-mode derivative")
