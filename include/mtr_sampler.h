@@ -347,7 +347,7 @@ int mtr_quantize_rows_launch(const MtrQuantizeArgs* args, void* stream);
  * logits[r, v] = RN(RN32(RN32(float(sum_k q[r, k] * weight[v, k])) * scale[r]) * weight_scale[v])
  * with q, scale the quantised hidden states (quantised by this call, into the
  * workspace where there are more than a few rows) and the sum exact in int32:
- * mtr_lmhead_launch with half its weight traffic and twice its tensor rate.
+ * mtr_lmhead_launch with half the weight bytes and 8-bit products.
  */
 typedef struct MtrLmHeadI8Args {
   uint32_t abi_version;         /* = MTR_ABI_VERSION */

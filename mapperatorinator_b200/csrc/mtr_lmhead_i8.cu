@@ -53,8 +53,9 @@ struct ProjParams {
 
 // Rows to int8: threads_per_row threads (a power of two, 32 .. 128) take a row
 // (quantize_row).  HBM bounds it: 3 bytes a bf16 value.  HOLD is 4 where a warp's
-// 4 vectors a lane hold a row, else 8 (us, 4 / 8, floor): 8192 x 768 bf16 4.9 /
-// 6.6, 2.9; 8192 x 4096 bf16 20.3 / 18.8, 15.4; 131072 x 1024 fp32 119 / 94, 102.
+// 4 vectors a lane hold a row, else 8 (us, 4 / 8, its bytes at the measured copy
+// rate): 8192 x 768 bf16 4.9 / 6.6, 2.9; 8192 x 4096 bf16 20.3 / 18.8, 15.4;
+// 131072 x 1024 fp32 119 / 94, 102 (mostly reads, which run faster than a copy).
 template <typename T, bool VEC, int HOLD>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_kernel(const QuantParams p) {
   __shared__ float tops[QUANT_THREADS / 32];
@@ -117,10 +118,11 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 // so a pair takes 64 KB a step of K out of L2 where two CTAs alone take 96.
 //
 // What bounds it: at d = 4096 the products (8192 x 4096 -> 16384 in 331 us without
-// the quantisation; twice the measured bf16 rate gives 337); at d = 768 the
-// epilogue, which takes about as long as a 128 x 256 tile's products and is
-// not wholly hidden behind them (24 us without the quantisation
-// for 8192 x 768 -> 4096, 19 with the epilogue's work left out).
+// the quantisation, 3.3 POP/s: 2.03 times the measured bf16 rate).  At d = 768
+// neither side alone: 8192 x 768 -> 4096 takes 25 us without the quantisation,
+// 20 with one step of K (the epilogue and its stores), 19 with the epilogue's
+// work left out (six steps of K, starts and ends of 512 tiles); an accumulator is
+// free only when all of it has been read, so the two overlap in part.
 //
 // Persistent: a CTA (pair) takes tile after tile, with two accumulators in tensor
 // memory, so that one tile is scaled and stored while the next is multiplied.
