@@ -59,6 +59,7 @@ extern "C" {
 #define MTR_MAX_I8_ROWS (1 << 22)
 #define MTR_MAX_SCORE_ROWS (1 << 27)
 #define MTR_MAX_TOP_N 32
+#define MTR_MAX_TEACHER_IDS 128
 #define MTR_MAX_TEMPERATURE 0x1p100f /* of the scores: e^((x - max) / T) is 0 where x - max passes the fp32 range */
 
 /* Return codes of every entry point. */
@@ -449,6 +450,54 @@ typedef struct MtrLogprobGradArgs {
 
 int mtr_logprob_grad_validate(const MtrLogprobGradArgs* args);
 int mtr_logprob_grad_launch(const MtrLogprobGradArgs* args, void* stream);
+
+/*
+ * Loss of a student's logits against the top ids of a teacher, row by row, and
+ * its gradient.  With q = softmax(logits / temperature), l_j the teacher's log
+ * probabilities of the n ids of a row and S the set of these ids:
+ *   tail = 0: p_j = e^(l_j) / sum_i e^(l_i) (so l may be logits too),
+ *             loss = sum_j p_j (log p_j - log q_{id_j})
+ *   tail = 1: p_j = e^(l_j), p_t = 1 - sum_j p_j, q_t = 1 - sum_{v in S} q_v,
+ *             loss = sum_j p_j (log p_j - log q_{id_j}) + p_t (log p_t - log q_t);
+ *             a p_t below 2^-20 is the rounding of the l_j and counts as 0
+ *   grad_v = g [ q_v (P + p_t) - sum_j [v = id_j] p_j ] / temperature          (v in S)
+ *            g [ q_v P - p_t (1 - q_t) q_v / q_t ] / temperature               (the others)
+ * with P = sum_j p_j, and p_t = 0 where tail = 0; rounded once.
+ * An id below 0 is no entry, one >= vocab neither (and sets MTR_ROW_BAD_ID); an
+ * l of -inf is probability 0.  A row without entries (tail = 0: without one of
+ * probability above 0) has loss 0 and gradient 0, whatever its logits.  An id that
+ * is given twice is two entries.  A row with NaN or +inf in the logits or its l
+ * (MTR_ROW_NONFINITE) reads NaN; one whose logits are all -inf
+ * (MTR_ROW_ALL_MASKED), or without mass where the teacher has some, +inf, the
+ * former with gradient 0.
+ */
+typedef struct MtrDistillArgs {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrDistillArgs) */
+  const void* logits;           /* [rows, vocab] */
+  int64_t logits_row_stride;    /* elements */
+  const void* teacher_ids;      /* [rows, n] */
+  int64_t ids_row_stride;       /* elements */
+  const float* teacher_logprobs; /* [rows, n] */
+  int64_t logprobs_row_stride;  /* elements */
+  int32_t logits_dtype;         /* MtrDType */
+  int32_t ids_dtype;            /* MtrIdType */
+  int32_t rows;                 /* 0 .. MTR_MAX_SCORE_ROWS */
+  int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
+  int32_t n;                    /* 1 .. MTR_MAX_TEACHER_IDS */
+  int32_t tail;                 /* 0 or 1 */
+  double temperature;           /* > 0, with a finite fp32 reciprocal, <= MTR_MAX_TEMPERATURE */
+  float* out_loss;              /* [rows]; NULL: the gradient alone, from an earlier call's stats */
+  double* stats;                /* [rows, 2] or NULL, 16-byte aligned: the largest logit outside S and the sum of
+                                   e^((logit - largest) / temperature) there; written with out_loss, read without it */
+  const float* g_loss;          /* [rows] gradients of the losses, or NULL (ones) */
+  void* grad_logits;            /* [rows, vocab], logits_dtype, or NULL; must not overlap the logits */
+  int64_t grad_row_stride;      /* elements */
+  uint32_t* out_status;         /* [rows] MTR_ROW_* bits or NULL; written with out_loss */
+} MtrDistillArgs;
+
+int mtr_distill_validate(const MtrDistillArgs* args);
+int mtr_distill_launch(const MtrDistillArgs* args, void* stream);
 
 /* ABI identity: MTR_ABI_VERSION and sizeof(MtrSamplerArgs) of the library. */
 int mtr_abi_version(void);

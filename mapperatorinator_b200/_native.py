@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_float, c_int32, c_int64, c_uint32, c_void_p
+from ctypes import c_double, c_float, c_int32, c_int64, c_uint32, c_void_p
 from pathlib import Path
 
 from . import build as _build
@@ -30,6 +30,7 @@ MAX_I8_D_MODEL = 131072
 MAX_I8_ROWS = 1 << 22
 MAX_SCORE_ROWS = 1 << 27
 MAX_TOP_N = 32
+MAX_TEACHER_IDS = 128
 MAX_TEMPERATURE = 2.0 ** 100  # of the scores
 
 # MtrStatus
@@ -281,6 +282,34 @@ class MtrLogprobGradArgs(ctypes.Structure):
     ]
 
 
+class MtrDistillArgs(ctypes.Structure):
+    """include/mtr_sampler.h MtrDistillArgs: losses against a teacher's top ids and their gradient."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("logits", c_void_p),
+        ("logits_row_stride", c_int64),
+        ("teacher_ids", c_void_p),
+        ("ids_row_stride", c_int64),
+        ("teacher_logprobs", c_void_p),
+        ("logprobs_row_stride", c_int64),
+        ("logits_dtype", c_int32),
+        ("ids_dtype", c_int32),
+        ("rows", c_int32),
+        ("vocab", c_int32),
+        ("n", c_int32),
+        ("tail", c_int32),
+        ("temperature", c_double),
+        ("out_loss", c_void_p),
+        ("stats", c_void_p),
+        ("g_loss", c_void_p),
+        ("grad_logits", c_void_p),
+        ("grad_row_stride", c_int64),
+        ("out_status", c_void_p),
+    ]
+
+
 # Every symbol include/mtr_sampler.h declares: (name, restype, argtypes).
 EXPORTS = {
     "mtr_abi_version": (ctypes.c_int, []),
@@ -309,6 +338,8 @@ EXPORTS = {
     "mtr_logprob_launch": (ctypes.c_int, [ctypes.POINTER(MtrLogprobArgs), c_void_p]),
     "mtr_logprob_grad_validate": (ctypes.c_int, [ctypes.POINTER(MtrLogprobGradArgs)]),
     "mtr_logprob_grad_launch": (ctypes.c_int, [ctypes.POINTER(MtrLogprobGradArgs), c_void_p]),
+    "mtr_distill_validate": (ctypes.c_int, [ctypes.POINTER(MtrDistillArgs)]),
+    "mtr_distill_launch": (ctypes.c_int, [ctypes.POINTER(MtrDistillArgs), c_void_p]),
 }
 
 
@@ -473,3 +504,7 @@ def logprob_launch(args: MtrLogprobArgs, stream: int | None) -> None:
 
 def logprob_grad_launch(args: MtrLogprobGradArgs, stream: int | None) -> None:
     check(load().mtr_logprob_grad_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_logprob_grad_launch")
+
+
+def distill_launch(args: MtrDistillArgs, stream: int | None) -> None:
+    check(load().mtr_distill_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_distill_launch")
