@@ -60,6 +60,9 @@ extern "C" {
 #define MTR_MAX_SCORE_ROWS (1 << 27)
 #define MTR_MAX_TOP_N 32
 #define MTR_MAX_TEACHER_IDS 128
+#define MTR_MAX_DRAFTS 128
+#define MTR_MAX_VERIFY_BATCH (1 << 20)
+#define MTR_VERIFY_MAX_RUNS 16
 #define MTR_MAX_TEMPERATURE 0x1p100f /* of the scores: e^((x - max) / T) is 0 where x - max passes the fp32 range */
 
 /* Return codes of every entry point. */
@@ -498,6 +501,61 @@ typedef struct MtrDistillArgs {
 
 int mtr_distill_validate(const MtrDistillArgs* args);
 int mtr_distill_launch(const MtrDistillArgs* args, void* stream);
+
+/*
+ * Drafted tokens accepted or replaced under the target's distribution.  For each
+ * of `batch` sequences: target logits of drafts + 1 positions, the tokens that
+ * were drafted for the first of them, the logits that they were drawn from
+ * (NULL: no distribution, all mass on the token) and drafts + 1 uniforms.  With
+ *   p_j = softmax(target_j / temperature), q_j = softmax(draft_j / draft_temperature),
+ * draft j is accepted while u_j q_j(t_j) < p_j(t_j).  At the first position that is
+ * not, the token is the smallest id v with sum_{i <= v} w_i > u_drafts sum_i w_i,
+ * w = max(p - q, 0) (w = p where that is 0 everywhere), and behind the last draft
+ * w = p.  do_sample = 0: draft j is accepted while it is the largest target logit
+ * (the lowest id of equal ones), and the token is that id.
+ * The tokens are what real arithmetic decides, but for borders within double's
+ * rounding.
+ * A draft id below 0 ends a sequence's drafts (so does one >= vocab, which sets
+ * MTR_ROW_BAD_ID).  A uniform outside [0, 1) is clamped (MTR_ROW_BAD_UNIFORM).  A
+ * target row with NaN or +inf (MTR_ROW_NONFINITE) or of -inf alone
+ * (MTR_ROW_ALL_MASKED) at the position that decides gives pad_id; such a draft
+ * row refuses its token and is drawn from p (same bits).  Positions behind the
+ * one that decides are not looked at.
+ */
+typedef struct MtrVerifyArgs {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrVerifyArgs) */
+  const void* target_logits;    /* [batch, drafts + 1, vocab] */
+  int64_t target_batch_stride;  /* elements */
+  int64_t target_pos_stride;    /* elements, >= vocab */
+  const void* draft_logits;     /* [batch, drafts, vocab], logits_dtype, or NULL */
+  int64_t draft_batch_stride;
+  int64_t draft_pos_stride;
+  const void* draft_ids;        /* [batch, drafts] */
+  int64_t ids_row_stride;
+  const float* uniforms;        /* [batch, drafts + 1]; required when do_sample */
+  int64_t uniforms_row_stride;
+  int32_t logits_dtype;         /* MtrDType */
+  int32_t ids_dtype;            /* MtrIdType */
+  int32_t batch;                /* 0 .. MTR_MAX_VERIFY_BATCH */
+  int32_t drafts;               /* 0 .. MTR_MAX_DRAFTS */
+  int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
+  int32_t do_sample;            /* 0 or 1 */
+  double temperature;           /* > 0, with a finite fp32 reciprocal, <= MTR_MAX_TEMPERATURE */
+  double draft_temperature;     /* likewise */
+  int64_t pad_id;
+  int64_t* out_tokens;          /* [batch, drafts + 1]: the accepted drafts, the new token, pad_id */
+  int32_t* out_accepted;        /* [batch]: accepted drafts */
+  float* out_logprobs;          /* [batch, drafts + 1] or NULL: log p of the tokens, 0 for padding */
+  uint32_t* out_status;         /* [batch] MTR_ROW_* bits or NULL */
+  void* workspace;              /* 16-byte aligned; one call's at a time */
+  int64_t workspace_bytes;      /* >= mtr_verify_workspace(...) */
+} MtrVerifyArgs;
+
+/* Workspace bytes of a call (0 for batch <= 0). */
+int64_t mtr_verify_workspace(int32_t batch, int32_t drafts, int32_t vocab, int32_t logits_dtype);
+int mtr_verify_validate(const MtrVerifyArgs* args);
+int mtr_verify_launch(const MtrVerifyArgs* args, void* stream);
 
 /* ABI identity: MTR_ABI_VERSION and sizeof(MtrSamplerArgs) of the library. */
 int mtr_abi_version(void);

@@ -31,6 +31,8 @@ MAX_I8_ROWS = 1 << 22
 MAX_SCORE_ROWS = 1 << 27
 MAX_TOP_N = 32
 MAX_TEACHER_IDS = 128
+MAX_DRAFTS = 128
+MAX_VERIFY_BATCH = 1 << 20
 MAX_TEMPERATURE = 2.0 ** 100  # of the scores
 
 # MtrStatus
@@ -310,6 +312,40 @@ class MtrDistillArgs(ctypes.Structure):
     ]
 
 
+class MtrVerifyArgs(ctypes.Structure):
+    """include/mtr_sampler.h MtrVerifyArgs: drafted tokens accepted or replaced."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("target_logits", c_void_p),
+        ("target_batch_stride", c_int64),
+        ("target_pos_stride", c_int64),
+        ("draft_logits", c_void_p),
+        ("draft_batch_stride", c_int64),
+        ("draft_pos_stride", c_int64),
+        ("draft_ids", c_void_p),
+        ("ids_row_stride", c_int64),
+        ("uniforms", c_void_p),
+        ("uniforms_row_stride", c_int64),
+        ("logits_dtype", c_int32),
+        ("ids_dtype", c_int32),
+        ("batch", c_int32),
+        ("drafts", c_int32),
+        ("vocab", c_int32),
+        ("do_sample", c_int32),
+        ("temperature", c_double),
+        ("draft_temperature", c_double),
+        ("pad_id", c_int64),
+        ("out_tokens", c_void_p),
+        ("out_accepted", c_void_p),
+        ("out_logprobs", c_void_p),
+        ("out_status", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
 # Every symbol include/mtr_sampler.h declares: (name, restype, argtypes).
 EXPORTS = {
     "mtr_abi_version": (ctypes.c_int, []),
@@ -340,6 +376,9 @@ EXPORTS = {
     "mtr_logprob_grad_launch": (ctypes.c_int, [ctypes.POINTER(MtrLogprobGradArgs), c_void_p]),
     "mtr_distill_validate": (ctypes.c_int, [ctypes.POINTER(MtrDistillArgs)]),
     "mtr_distill_launch": (ctypes.c_int, [ctypes.POINTER(MtrDistillArgs), c_void_p]),
+    "mtr_verify_workspace": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "mtr_verify_validate": (ctypes.c_int, [ctypes.POINTER(MtrVerifyArgs)]),
+    "mtr_verify_launch": (ctypes.c_int, [ctypes.POINTER(MtrVerifyArgs), c_void_p]),
 }
 
 
@@ -508,3 +547,11 @@ def logprob_grad_launch(args: MtrLogprobGradArgs, stream: int | None) -> None:
 
 def distill_launch(args: MtrDistillArgs, stream: int | None) -> None:
     check(load().mtr_distill_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_distill_launch")
+
+
+def verify_workspace(batch: int, drafts: int, vocab: int, logits_dtype: int) -> int:
+    return load().mtr_verify_workspace(batch, drafts, vocab, logits_dtype)
+
+
+def verify_launch(args: MtrVerifyArgs, stream: int | None) -> None:
+    check(load().mtr_verify_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_verify_launch")

@@ -21,7 +21,8 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmtr_sampler.so"
 SOURCES = [CSRC / "mtr_sampler.cu", CSRC / "mtr_stream.cu", CSRC / "mtr_stream_bf16.cu", CSRC / "mtr_stream_f16.cu",
            CSRC / "mtr_stream_f32.cu", CSRC / "mtr_lmhead.cu", CSRC / "mtr_lmhead_i8.cu",
-           CSRC / "mtr_lmhead_few.cu", CSRC / "mtr_logprob.cu", CSRC / "mtr_distill.cu"]
+           CSRC / "mtr_lmhead_few.cu", CSRC / "mtr_logprob.cu", CSRC / "mtr_distill.cu",
+           CSRC / "mtr_verify.cu"]
 HEADERS = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh", CSRC / "mtr_stream.cuh",
            CSRC / "mtr_tc.cuh", CSRC / "mtr_vec.cuh", CSRC / "mtr_quant.cuh"]
 BUILD_DIR = PKG_DIR / "_build"
@@ -58,7 +59,7 @@ def _deps(src: Path) -> list:
         deps.append(CSRC / "mtr_stream.cuh")
     if src.name in ("mtr_lmhead.cu", "mtr_lmhead_i8.cu"):
         deps.append(CSRC / "mtr_tc.cuh")
-    if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu", "mtr_logprob.cu", "mtr_distill.cu"):
+    if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu", "mtr_logprob.cu", "mtr_distill.cu", "mtr_verify.cu"):
         deps.append(CSRC / "mtr_vec.cuh")
     if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu"):
         deps.append(CSRC / "mtr_quant.cuh")

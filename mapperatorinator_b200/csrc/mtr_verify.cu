@@ -1,0 +1,690 @@
+// mtr_verify.cu -- drafted tokens accepted or replaced under the target's
+// distribution (speculative sampling).
+//
+// With p_j the target's softmax(logits / T) of position j, q_j the draft's (or all
+// mass on the drafted token t_j where no draft logits are given) and u the caller's
+// uniforms, draft j is accepted while u_j q_j(t_j) < p_j(t_j).  At the first that is
+// not, j = a, a token is drawn from w = max(p_a - q_a, 0): the smallest id v with
+// sum_{i <= v} w_i > u_K sum w; behind the last draft from w = p.
+//
+// Tokens are decisions, so each is what real arithmetic decides (but for borders
+// nearer than double's rounding):
+//   rows_kernel   reads every row that may count once and keeps its largest
+//                 logit and the sum of e^((x - max) / T) about it, fp32 terms, within
+//                 E = 2^-15 relative (below).  HBM bounds it.
+//   pick_kernel   decides the drafts in turn: log u + log q - log p in double from
+//                 these sums, clear when it is further than 2 E from 0; else (about
+//                 once in 10^4 drafts) both sums are formed again in double.  Then it
+//                 draws from the one position that counts, all in double.
+// The bound E: ex2.approx is within 2^-22, its argument within 3 2^-24 |d| of d, and
+// the mean of |d| under the softmax is at most log V < 12; a thread adds at most 16
+// pairs in fp32 before double takes over, and its sum moves to a larger maximum at
+// most 36 times, within 2^-22 each: 2.4e-7 + 2.2e-6 + 1e-6 + 8.6e-6 < 2^-15 = 3.1e-5.
+#include "mtr_vec.cuh"
+
+namespace mtr {
+namespace vf {
+
+constexpr double BORDER = 0x1p-14;  // 2 E: two sums
+
+struct Part {  // of a run of a row
+  float m;
+  int32_t id;  // the first id of the largest logit (greedy only)
+  double s;    // NaN: a NaN or +inf
+};
+
+struct Params {
+  const void* target;
+  int64_t t_batch, t_pos;
+  const void* draft;  // NULL: one-hot
+  int64_t d_batch, d_pos;
+  const void* ids;
+  int64_t ids_stride;
+  int32_t ids32;
+  const float* uniforms;
+  int64_t u_stride;
+  int32_t batch, drafts, vocab;
+  int32_t runs;     // of a row, a CTA each
+  int32_t run;      // vectors of a run
+  int32_t greedy;
+  int32_t cluster;
+  float t_scale, d_scale;    // log2(e) / T
+  double t_inv, d_inv;       // 1 / T
+  int64_t pad_id;
+  Part* parts;               // [batch (2 drafts + 1)] rows of runs: the targets, then the drafts
+  int64_t* tokens;
+  int32_t* accepted;
+  float* logprobs;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ double nan_d() { return __longlong_as_double(0x7ff8000000000000LL); }
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  return v;
+}
+__device__ __forceinline__ int64_t draft_id(const Params& p, int64_t b, int j) {
+  const int64_t at = b * p.ids_stride + j;
+  return p.ids32 ? (int64_t)((const int32_t*)p.ids)[at] : ((const int64_t*)p.ids)[at];
+}
+
+constexpr int HOLD = 4;  // vectors of a thread's tile
+
+// One run of one row: its largest logit and the sum about it.
+template <typename T, int THREADS, bool GREEDY>
+__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+  typedef Vec<T> X;
+  constexpr int E = X::E, WARPS = THREADS / 32;
+  __shared__ float sh_m[WARPS];
+  __shared__ double sh_s[WARPS];
+  __shared__ int sh_id[WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int K = p.drafts, V = p.vocab;
+  const int64_t row = blockIdx.x, targets = (int64_t)p.batch * (K + 1);
+  const bool draft = row >= targets;
+  const int64_t b = draft ? (row - targets) / K : row / (K + 1);
+  const int j = (int)(draft ? (row - targets) % K : row % (K + 1));
+  wait_prior_grid();
+  // a position counts only behind drafts that are ids
+  for (int i = 0; i < (draft ? j + 1 : j); ++i) {
+    const int64_t id = draft_id(p, b, i);
+    if (id < 0 || id >= V) return;
+  }
+  const T* x = draft ? (const T*)p.draft + b * p.d_batch + j * p.d_pos : (const T*)p.target + b * p.t_batch + j * p.t_pos;
+  const float scale = draft ? p.d_scale : p.t_scale;
+  const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
+  const int head = min(off ? E - off : 0, V), vecs = (V - head) / E, behind = V - head - vecs * E;
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  const int v0 = min((int)blockIdx.y * p.run, vecs), v1 = blockIdx.y == gridDim.y - 1 ? vecs : min(v0 + p.run, vecs);
+
+  float m = neg_inf();
+  double s = 0.0;
+  bool bad = false;
+  int at = 0x7fffffff;
+  auto rise = [&](float v) {
+    if (!(v < pos_inf())) bad = true;
+    if (v > m) {
+      s *= (double)ex2((m - v) * scale);  // m = -inf: 0
+      m = v;
+    }
+  };
+  // the single logits before the first boundary and behind the last, of the first run
+  const int single = blockIdx.y > 0 ? -1 : tid < head ? tid : tid >= 32 && tid < 32 + behind ? V - behind + tid - 32 : -1;
+  const float one = single >= 0 ? to_f(x[single]) : neg_inf();
+  for (int i0 = v0 + tid; i0 < v1; i0 += HOLD * THREADS) {
+    uint4 w[HOLD];
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k) {
+      const int i = i0 + k * THREADS;
+      w[k] = i < v1 ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+    }
+    if constexpr (GREEDY) {
+      float best = m;
+#pragma unroll
+      for (int k = 0; k < HOLD; ++k) {
+        const float v = X::value(X::top(w[k]));
+        if (v > best) {
+          best = v;
+          at = i0 + k * THREADS;
+        }
+      }
+    }
+    typename X::Top top = X::top(w[0]);
+#pragma unroll
+    for (int k = 1; k < HOLD; ++k) top = X::larger(top, X::top(w[k]));
+    rise(X::value(top));
+    if (bad || !(m > neg_inf())) continue;
+    const u64 nm2 = pk2(-m, -m), sc2 = pk2(scale, scale);
+    u64 s2 = 0;
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k) {
+      float f[E];
+      X::unpack(w[k], f);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        float d0, d1;
+        up2(mul2(add2(pk2(f[e], f[e + 1]), nm2), sc2), d0, d1);
+        s2 = add2(s2, pk2(ex2(d0), ex2(d1)));
+      }
+    }
+    float lo, hi;
+    up2(s2, lo, hi);
+    s += (double)lo + (double)hi;
+  }
+  float vector_m = m;  // what `at` holds
+  if (single >= 0) {
+    rise(one);
+    if (!bad && m > neg_inf()) s += (double)ex2((one - m) * scale);
+  }
+  const float most = warp_max(bad ? neg_inf() : m);
+  if (!bad && m > neg_inf()) s *= (double)ex2((m - most) * scale);
+  if (bad) s = nan_d();
+  s = warp_sum(s);
+  if (lane == 0) {
+    sh_m[warp] = most;
+    sh_s[warp] = s;
+  }
+  __syncthreads();
+  float all = sh_m[0];
+#pragma unroll
+  for (int k = 1; k < WARPS; ++k) all = fmaxf(all, sh_m[k]);
+  int id = 0x7fffffff;
+  if constexpr (GREEDY) {
+    // the first id whose logit is the largest
+    if (single >= 0 && one == all) id = single;
+    if (vector_m == all && at < vecs) {
+      float f[E];
+      X::unpack(body[at], f);
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (f[e] == all) id = min(id, head + at * E + e);
+    }
+    id = __reduce_min_sync(FULL, id);
+    if (lane == 0) sh_id[warp] = id;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      sum += sh_m[k] > neg_inf() ? sh_s[k] * (double)ex2((sh_m[k] - all) * scale) : sh_s[k];
+      if constexpr (GREEDY) id = min(id, sh_id[k]);
+    }
+    p.parts[row * p.runs + blockIdx.y] = Part{all, id, sum};
+  }
+}
+
+constexpr int PICK = 512, PICK_WARPS = PICK / 32;
+
+struct Sums {
+  double t, d;
+};
+
+struct PickShared {
+  double warp_t[PICK_WARPS], warp_d[PICK_WARPS];
+  Sums cta;                      // read by the cluster's other CTAs
+  double weight;                 // likewise
+  double piece[PICK_WARPS];
+  int stop, unclear, bad_draft;
+  uint32_t status;
+  float t_m, d_m;
+  double t_s, d_s;
+  int token;
+};
+
+// A row's parts joined; every lane the same.
+__device__ __forceinline__ Part join(const Part* parts, int runs, float scale) {
+  Part r = parts[0];
+  for (int i = 1; i < runs; ++i) {
+    const Part q = parts[i];
+    const float m = fmaxf(r.m, q.m);
+    if (q.m > r.m || (q.m == r.m && q.id < r.id)) r.id = q.id;
+    r.s = (r.m > neg_inf() ? r.s * (double)ex2((r.m - m) * scale) : r.s) + (q.m > neg_inf() ? q.s * (double)ex2((q.m - m) * scale) : q.s);
+    r.m = m;
+  }
+  return r;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
+  __shared__ PickShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cs = p.cluster, rank = cs > 1 ? (int)(blockIdx.x % cs) : 0;
+  const int64_t b = cs > 1 ? blockIdx.x / cs : blockIdx.x;
+  const int K = p.drafts, V = p.vocab;
+  wait_prior_grid();
+
+  const Part* t_parts = p.parts + b * (K + 1) * p.runs;
+  const Part* d_parts = p.parts + ((int64_t)p.batch * (K + 1) + b * K) * p.runs;
+  auto t_row = [&](int j) { return (const T*)p.target + b * p.t_batch + j * p.t_pos; };
+  auto d_row = [&](int j) { return (const T*)p.draft + b * p.d_batch + j * p.d_pos; };
+  auto uniform = [&](int j, uint32_t& st) {
+    float u = p.uniforms[b * p.u_stride + j];
+    if (!(u >= 0.0f)) {
+      u = 0.0f;
+      st |= MTR_ROW_BAD_UNIFORM;
+    } else if (u >= 1.0f) {
+      u = 0x1.fffffep-1f;
+      st |= MTR_ROW_BAD_UNIFORM;
+    }
+    return (double)u;
+  };
+  auto cluster_sync = [&]() {
+    if (cs > 1) cluster.sync();
+    else __syncthreads();
+  };
+  // this CTA's ids, a warp's of them
+  const int share = (V + cs - 1) / cs, c0 = min(rank * share, V), c1 = min(c0 + share, V);
+  auto piece_of = [&](int from, int to, int k, int& a, int& z) {
+    const int each = (to - from + PICK_WARPS - 1) / PICK_WARPS;
+    a = min(from + k * each, to);
+    z = min(a + each, to);
+  };
+  // sums of e^((x - m) / T) over the whole row(s) in double; the same in every thread of the cluster
+  auto exact_sums = [&](const T* t, float tm, const T* d, float dm) {
+    int a, z;
+    piece_of(c0, c1, warp, a, z);
+    Sums s{0.0, 0.0};
+    for (int v = a + lane; v < z; v += 32) {
+      s.t += exp(((double)to_f(t[v]) - (double)tm) * p.t_inv);
+      if (d) s.d += exp(((double)to_f(d[v]) - (double)dm) * p.d_inv);
+    }
+    s.t = warp_sum(s.t);
+    s.d = warp_sum(s.d);
+    if (lane == 0) {
+      sh.warp_t[warp] = s.t;
+      sh.warp_d[warp] = s.d;
+    }
+    __syncthreads();
+    s = Sums{0.0, 0.0};
+    for (int k = 0; k < PICK_WARPS; ++k) {
+      s.t += sh.warp_t[k];
+      s.d += sh.warp_d[k];
+    }
+    if (cs > 1) {
+      if (tid == 0) sh.cta = s;
+      cluster.sync();
+      s = Sums{0.0, 0.0};
+      for (int k = 0; k < cs; ++k) {
+        const Sums o = cluster.map_shared_rank(&sh, k)->cta;
+        s.t += o.t;
+        s.d += o.d;
+      }
+      cluster.sync();  // read before it is written again
+    } else {
+      __syncthreads();
+    }
+    return s;
+  };
+
+  // The drafts in turn, 32 at a time: lane l decides draft first + l.
+  uint32_t status = 0;
+  int stop = 0;          // accepted so far
+  bool open = true;
+  while (open) {
+    if (warp == 0) {
+      const int j = stop + lane;
+      int verdict = 2;  // 0 accepted, 1 refused (or no draft), 2 unclear
+      uint32_t st = 0;
+      const int64_t id = j < K ? draft_id(p, b, j) : -1;
+      if (id < 0 || id >= V) {
+        verdict = 1;
+        if (id >= V) st |= MTR_ROW_BAD_ID;
+      }
+      // positions behind the first that is no draft have no parts
+      const unsigned ends = __ballot_sync(FULL, verdict == 1);
+      const int known = ends ? __ffs(ends) - 1 : 32;
+      if (lane < known) {
+        const Part t = join(t_parts + (int64_t)j * p.runs, p.runs, p.t_scale);
+        const bool t_bad = !(t.s < (double)pos_inf()), t_none = !t_bad && !(t.m > neg_inf());
+        if (t_bad || t_none) {
+          verdict = 1;  // the draw reports it
+        } else if (p.greedy) {
+          verdict = t.id == (int)id ? 0 : 1;
+        } else {
+          const float xt = to_f(t_row(j)[id]);
+          const double u = uniform(j, st);
+          bool q_zero = false, q_bad = false;
+          double lq = 0.0;
+          if (p.draft) {
+            const Part d = join(d_parts + (int64_t)j * p.runs, p.runs, p.d_scale);
+            if (!(d.s < (double)pos_inf())) {
+              st |= MTR_ROW_NONFINITE;
+              q_bad = true;
+            } else if (!(d.m > neg_inf())) {
+              st |= MTR_ROW_ALL_MASKED;
+              q_bad = true;
+            } else {
+              const float xd = to_f(d_row(j)[id]);
+              q_zero = xd == neg_inf();
+              lq = ((double)xd - (double)d.m) * p.d_inv - log(d.s);
+            }
+          }
+          if (q_bad || xt == neg_inf()) verdict = 1;
+          else if (q_zero || u == 0.0) verdict = 0;
+          else {
+            const double far = log(u) + lq - (((double)xt - (double)t.m) * p.t_inv - log(t.s));
+            verdict = far < -BORDER ? 0 : far > BORDER ? 1 : 2;
+          }
+        }
+      }
+      const unsigned not_yes = __ballot_sync(FULL, verdict != 0);
+      const int n = not_yes ? __ffs(not_yes) - 1 : 32;
+      // the bits of the positions that were looked at in earnest
+      status |= __reduce_or_sync(FULL, lane <= n ? st : 0u);
+      const int what = n < 32 ? __shfl_sync(FULL, verdict, n) : 3;
+      if (lane == 0) {
+        sh.stop = stop + n;
+        sh.unclear = what;
+      }
+    }
+    __syncthreads();
+    stop = sh.stop;
+    const int what = sh.unclear;
+    __syncthreads();
+    if (what == 1) {
+      open = false;
+    } else if (what == 2) {
+      const int j = stop;
+      const Part t = join(t_parts + (int64_t)j * p.runs, p.runs, p.t_scale);
+      const Part d = p.draft ? join(d_parts + (int64_t)j * p.runs, p.runs, p.d_scale) : Part{0.0f, 0, 1.0};
+      const Sums s = exact_sums(t_row(j), t.m, p.draft ? d_row(j) : nullptr, d.m);
+      const int64_t id = draft_id(p, b, j);
+      uint32_t st = 0;
+      const double pt = exp(((double)to_f(t_row(j)[id]) - (double)t.m) * p.t_inv) / s.t;
+      const double qd = p.draft ? exp(((double)to_f(d_row(j)[id]) - (double)d.m) * p.d_inv) / s.d : 1.0;
+      if (uniform(j, st) * qd < pt) ++stop;
+      else open = false;
+    }
+  }
+
+  // The draw from position `stop`.
+  const int64_t drafted = stop < K ? draft_id(p, b, stop) : -1;
+  const bool refused = drafted >= 0 && drafted < V;
+  const Part t = join(t_parts + (int64_t)stop * p.runs, p.runs, p.t_scale);
+  const bool t_bad = !(t.s < (double)pos_inf()), t_none = !t_bad && !(t.m > neg_inf());
+  const T* x = t_row(stop);
+  int token = -1;
+  double token_s = t.s;
+  if (t_bad || t_none) {
+    status |= t_bad ? MTR_ROW_NONFINITE : MTR_ROW_ALL_MASKED;
+  } else if (p.greedy) {
+    token = t.id;
+  } else {
+    const T* y = nullptr;
+    float dm = 0.0f;
+    if (refused && p.draft) {
+      const Part d = join(d_parts + (int64_t)stop * p.runs, p.runs, p.d_scale);
+      if (d.s < (double)pos_inf() && d.m > neg_inf()) {
+        y = d_row(stop);
+        dm = d.m;
+      }
+    }
+    const int hot = refused && !p.draft ? (int)drafted : -1;
+    const Sums s = exact_sums(x, t.m, y, dm);
+    token_s = s.t;
+    const double over_t = 1.0 / s.t, over_d = y ? 1.0 / s.d : 0.0;
+    bool from_p = false;
+    auto weight = [&](int v) {
+      const double pt = exp(((double)to_f(x[v]) - (double)t.m) * p.t_inv) * over_t;
+      if (from_p) return pt;
+      if (y) return fmax(pt - exp(((double)to_f(y[v]) - (double)dm) * p.d_inv) * over_d, 0.0);
+      return v == hot ? 0.0 : pt;
+    };
+    // the weight of [from, to) by pieces of a warp each, in sh.piece; the sum
+    auto weigh = [&](int from, int to) {
+      int a, z;
+      piece_of(from, to, warp, a, z);
+      double w = 0.0;
+      for (int v = a + lane; v < z; v += 32) w += weight(v);
+      w = warp_sum(w);
+      __syncthreads();
+      if (lane == 0) sh.piece[warp] = w;
+      __syncthreads();
+      w = 0.0;
+      for (int k = 0; k < PICK_WARPS; ++k) w += sh.piece[k];
+      return w;
+    };
+    // first piece of n whose running sum passes u: its index, and the sum before it
+    auto choose = [&](auto piece, int n, double u, double& before) {
+      double run = before;
+      int last = -1;
+      double at = before;
+      for (int k = 0; k < n; ++k) {
+        const double w = piece(k);
+        if (w > 0.0) {
+          last = k;
+          at = run;
+        }
+        run += w;
+        if (run > u) break;
+      }
+      before = at;
+      return last;
+    };
+    double mine = weigh(c0, c1), all = mine;
+    if (cs > 1) {
+      if (tid == 0) sh.weight = mine;
+      cluster.sync();
+      all = 0.0;
+      for (int k = 0; k < cs; ++k) all += cluster.map_shared_rank(&sh, k)->weight;
+    }
+    if (!(all > 0.0)) {  // target and draft are the same: draw from the target
+      from_p = true;
+      cluster_sync();
+      mine = all = weigh(c0, c1);
+      if (cs > 1) {
+        if (tid == 0) sh.weight = mine;
+        cluster.sync();
+        all = 0.0;
+        for (int k = 0; k < cs; ++k) all += cluster.map_shared_rank(&sh, k)->weight;
+      }
+    }
+    const double u = uniform(K, status) * all;
+    double before = 0.0;
+    int owner = 0;
+    if (cs > 1) {
+      owner = choose([&](int k) { return cluster.map_shared_rank(&sh, k)->weight; }, cs, u, before);
+      cluster.sync();
+    }
+    if (rank == owner) {
+      int a, z;
+      int k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
+      piece_of(c0, c1, max(k, 0), a, z);
+      weigh(a, z);
+      k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
+      int from, to;
+      piece_of(a, z, max(k, 0), from, to);
+      if (warp == 0) {
+        int last = -1;
+        double run = before;
+        for (int v0 = from; v0 < to; v0 += 32) {
+          const int v = v0 + lane;
+          const double w = v < to ? weight(v) : 0.0;
+          double up = w;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double q = __shfl_up_sync(FULL, up, o);
+            if (lane >= o) up += q;
+          }
+          const unsigned past = __ballot_sync(FULL, w > 0.0 && run + up > u), some = __ballot_sync(FULL, w > 0.0);
+          if (past) {
+            last = v0 + __ffs(past) - 1;
+            break;
+          }
+          if (some) last = v0 + 31 - __clz(some);
+          run += __shfl_sync(FULL, up, 31);
+        }
+        if (lane == 0) sh.token = last;
+      }
+      __syncthreads();
+      token = sh.token;
+    } else {
+      return;
+    }
+  }
+  if (p.greedy || t_bad || t_none) {
+    if (rank != 0) return;
+  }
+
+  for (int j = tid; j <= K; j += PICK) {
+    int64_t out = p.pad_id;
+    float lp = 0.0f;
+    const int64_t id = j < stop ? draft_id(p, b, j) : j == stop && token >= 0 ? token : -1;
+    if (id >= 0) {
+      out = id;
+      const Part r = j < stop ? join(t_parts + (int64_t)j * p.runs, p.runs, p.t_scale) : t;
+      lp = (float)(((double)to_f(t_row(j)[id]) - (double)r.m) * p.t_inv - log(j < stop ? r.s : token_s));
+    }
+    p.tokens[b * (K + 1) + j] = out;
+    if (p.logprobs) p.logprobs[b * (K + 1) + j] = lp;
+  }
+  if (tid == 0) {
+    p.accepted[b] = stop;
+    if (p.status) p.status[b] = status;
+  }
+}
+
+static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
+
+// Runs of a row (a CTA each), and vectors of a run: rows are split until there are
+// four CTAs an SM (148 SMs) or a run is a tile.  The workspace goes by it, so it
+// asks no device.
+constexpr int64_t ENOUGH = 4 * 148;
+struct Shape {
+  int threads, runs, run;
+};
+static Shape shape_for(int64_t rows, int vocab, int es) {
+  const int64_t vecs = ((int64_t)vocab * es + 15) / 16;
+  const int threads = vecs <= 128 * HOLD ? 128 : 256;
+  const int64_t tile = (int64_t)threads * HOLD, tiles = (vecs + tile - 1) / tile;
+  int64_t runs = 1;
+  while (runs < MTR_VERIFY_MAX_RUNS && runs < tiles && rows * runs < ENOUGH) runs *= 2;
+  const int64_t each = (tiles + runs - 1) / runs;
+  runs = (tiles + each - 1) / each;
+  return {threads, (int)(runs > 0 ? runs : 1), (int)(each * tile)};
+}
+static int64_t rows_of(const MtrVerifyArgs& a) {
+  return (int64_t)a.batch * (a.drafts + 1) + (a.draft_logits && a.do_sample ? (int64_t)a.batch * a.drafts : 0);
+}
+
+template <typename K>
+static cudaError_t launch(K kern, const Params& p, dim3 grid, int threads, int cluster, cudaStream_t s) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  cfg.numAttrs = launch_attrs(attr, cluster, true);
+  cfg.attrs = attr;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+template <typename T>
+static cudaError_t launch_all(Params p, int64_t rows, cudaStream_t s) {
+  const Shape g = shape_for(rows, p.vocab, sizeof(T));
+  p.runs = g.runs;
+  p.run = g.run;
+  const dim3 grid((unsigned)rows, (unsigned)g.runs, 1);
+  cudaError_t e;
+  if (g.threads == 128)
+    e = p.greedy ? launch(rows_kernel<T, 128, true>, p, grid, 128, 1, s) : launch(rows_kernel<T, 128, false>, p, grid, 128, 1, s);
+  else
+    e = p.greedy ? launch(rows_kernel<T, 256, true>, p, grid, 256, 1, s) : launch(rows_kernel<T, 256, false>, p, grid, 256, 1, s);
+  if (e != cudaSuccess) return e;
+  int cluster = 1;
+  while (!p.greedy && cluster < 8 && p.batch * cluster * 2 <= device_sms() && p.vocab >= 4096 * cluster) cluster *= 2;
+  p.cluster = cluster;
+  return launch(pick_kernel<T>, p, dim3((unsigned)(p.batch * cluster), 1, 1), PICK, cluster, s);
+}
+
+}  // namespace vf
+}  // namespace mtr
+
+// ---------------------------------------------------------------- C ABI
+using namespace mtr::vf;
+
+int64_t mtr_verify_workspace(int32_t batch, int32_t drafts, int32_t vocab, int32_t logits_dtype) {
+  if (batch <= 0 || drafts < 0 || vocab <= 0) return 0;
+  const int es = esize(logits_dtype);
+  const int64_t targets = (int64_t)batch * (drafts + 1), both = targets + (int64_t)batch * drafts;
+  const int64_t a = targets * shape_for(targets, vocab, es).runs, b = both * shape_for(both, vocab, es).runs;
+  return (a > b ? a : b) * (int64_t)sizeof(Part);
+}
+
+int mtr_verify_validate(const MtrVerifyArgs* a) {
+  if (!a) return MTR_ERR_NULL_ARG;
+  if (a->abi_version != MTR_ABI_VERSION || a->struct_size != sizeof(MtrVerifyArgs)) return MTR_ERR_ABI;
+  if (a->batch < 0 || a->batch > MTR_MAX_VERIFY_BATCH || a->drafts < 0 || a->drafts > MTR_MAX_DRAFTS) return MTR_ERR_BAD_SHAPE;
+  if (a->vocab < 1 || a->vocab > MTR_MAX_VOCAB) return MTR_ERR_BAD_SHAPE;
+  if (a->logits_dtype < MTR_DTYPE_F32 || a->logits_dtype > MTR_DTYPE_F16) return MTR_ERR_BAD_PARAM;
+  if (a->ids_dtype != MTR_IDS_I64 && a->ids_dtype != MTR_IDS_I32) return MTR_ERR_BAD_PARAM;
+  if (a->do_sample != 0 && a->do_sample != 1) return MTR_ERR_BAD_PARAM;
+  const double temps[2] = {a->temperature, a->draft_temperature};
+  for (double t : temps)
+    if (!(t > 0.0) || !(t <= (double)MTR_MAX_TEMPERATURE) || !((float)(1.4426950408889634 / t) < INFINITY)) return MTR_ERR_BAD_PARAM;
+  if (a->batch == 0) return MTR_OK;
+  if (!a->target_logits || !a->out_tokens || !a->out_accepted || !a->workspace) return MTR_ERR_NULL_ARG;
+  if ((a->drafts > 0 && !a->draft_ids) || (a->do_sample && !a->uniforms)) return MTR_ERR_NULL_ARG;
+  if (a->target_pos_stride < a->vocab || a->target_batch_stride < 0) return MTR_ERR_BAD_SHAPE;
+  if (a->draft_logits && (a->draft_pos_stride < a->vocab || a->draft_batch_stride < 0)) return MTR_ERR_BAD_SHAPE;
+  if (a->ids_row_stride < 0 || a->uniforms_row_stride < 0) return MTR_ERR_BAD_SHAPE;
+  const int64_t need = mtr_verify_workspace(a->batch, a->drafts, a->vocab, a->logits_dtype);
+  if (a->workspace_bytes < need) return MTR_ERR_BAD_SHAPE;
+  const int es = esize(a->logits_dtype);
+  if ((uintptr_t)a->target_logits % es || (uintptr_t)a->draft_logits % es || (uintptr_t)a->draft_ids % (a->ids_dtype == MTR_IDS_I64 ? 8 : 4) ||
+      (uintptr_t)a->uniforms % 4 || (uintptr_t)a->out_tokens % 8 || (uintptr_t)a->out_accepted % 4 || (uintptr_t)a->out_logprobs % 4 ||
+      (uintptr_t)a->out_status % 4 || (uintptr_t)a->workspace % 16)
+    return MTR_ERR_ALIGNMENT;
+  const int64_t more = a->drafts + 1, all = a->batch * more;
+  auto run = [](const void* at, int64_t n) { return mtr::Bytes{at, 1, n, n}; };
+  const mtr::Bytes work = run(a->workspace, need), outs[4] = {run(a->out_tokens, 8 * all), run(a->out_accepted, 4ll * a->batch),
+                                                              run(a->out_logprobs, 4 * all), run(a->out_status, 4ll * a->batch)};
+  for (const mtr::Bytes& o : outs) {
+    if (!o.at) continue;
+    if (overlap(o, work)) return MTR_ERR_BAD_PARAM;
+    if (a->drafts > 0 && overlap(o, mtr::bytes_of(a->draft_ids, a->ids_row_stride ? a->batch : 1, a->ids_row_stride ? a->ids_row_stride : a->drafts,
+                                                  a->drafts, a->ids_dtype == MTR_IDS_I64 ? 8 : 4)))
+      return MTR_ERR_BAD_PARAM;
+    if (a->do_sample && overlap(o, mtr::bytes_of(a->uniforms, a->uniforms_row_stride ? a->batch : 1,
+                                                 a->uniforms_row_stride ? a->uniforms_row_stride : more, more, 4)))
+      return MTR_ERR_BAD_PARAM;
+  }
+  return MTR_OK;
+}
+
+int mtr_verify_launch(const MtrVerifyArgs* a, void* stream) {
+  const int v = mtr_verify_validate(a);
+  if (v != MTR_OK) return v;
+  if (a->batch == 0) return MTR_OK;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.target = a->target_logits;
+  p.t_batch = a->target_batch_stride;
+  p.t_pos = a->target_pos_stride;
+  p.draft = a->do_sample ? a->draft_logits : nullptr;
+  p.d_batch = a->draft_batch_stride;
+  p.d_pos = a->draft_pos_stride;
+  p.ids = a->draft_ids;
+  p.ids_stride = a->ids_row_stride;
+  p.ids32 = a->ids_dtype == MTR_IDS_I32;
+  p.uniforms = a->uniforms;
+  p.u_stride = a->uniforms_row_stride;
+  p.batch = a->batch;
+  p.drafts = a->drafts;
+  p.vocab = a->vocab;
+  p.greedy = !a->do_sample;
+  p.t_scale = (float)(1.4426950408889634 / a->temperature);
+  p.d_scale = (float)(1.4426950408889634 / a->draft_temperature);
+  p.t_inv = 1.0 / a->temperature;
+  p.d_inv = 1.0 / a->draft_temperature;
+  p.pad_id = a->pad_id;
+  p.parts = (Part*)a->workspace;
+  p.tokens = a->out_tokens;
+  p.accepted = a->out_accepted;
+  p.logprobs = a->out_logprobs;
+  p.status = a->out_status;
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t rows = rows_of(*a);
+  cudaError_t e;
+  switch (a->logits_dtype) {
+    case MTR_DTYPE_F32: e = launch_all<float>(p, rows, s); break;
+    case MTR_DTYPE_BF16: e = launch_all<__nv_bfloat16>(p, rows, s); break;
+    default: e = launch_all<__half>(p, rows, s); break;
+  }
+  mtr::set_last_cuda_error((int)e);
+  return e == cudaSuccess ? MTR_OK : MTR_ERR_CUDA;
+}
