@@ -57,6 +57,8 @@ extern "C" {
 #define MTR_MAX_LB_EOS 8
 #define MTR_MAX_I8_D_MODEL 131072 /* 127 * 128 * 131072 < 2^31: the int32 sums cannot wrap */
 #define MTR_MAX_I8_ROWS (1 << 22)
+#define MTR_MAX_F8_D_MODEL 131072
+#define MTR_MAX_F8_ROWS (1 << 22)
 #define MTR_MAX_SCORE_ROWS (1 << 27)
 #define MTR_MAX_TOP_N 32
 #define MTR_MAX_TEACHER_IDS 128
@@ -310,7 +312,7 @@ int mtr_lmhead_launch(const MtrLmHeadArgs* args, void* stream);
  * stride and vocabulary) and the sampler's rows must lie inside lm->rows. */
 int mtr_lmhead_sample_launch(const MtrLmHeadArgs* lm, const MtrSamplerArgs* sampler, void* stream);
 
-/* Waits of the tensor-core projections (this one and the 8-bit one) that gave up
+/* Waits of the tensor-core projections (this one and the 8-bit ones) that gave up
  * on the current device since the library was loaded; 0 on a healthy device.
  * Waits for `stream`, which must not be capturing (MTR_ERR_UNSUPPORTED).  Logits
  * that such a projection did not compute are NaN, so the sampler marks their
@@ -382,6 +384,70 @@ int mtr_lmhead_i8_launch(const MtrLmHeadI8Args* args, void* stream);
 /* As mtr_lmhead_sample_launch, with the 8-bit projection (the sampler's
  * logits_dtype must be the projection's). */
 int mtr_lmhead_i8_sample_launch(const MtrLmHeadI8Args* lm, const MtrSamplerArgs* sampler, void* stream);
+
+/*
+ * Output projection in 8-bit floating point (e4m3) with one fp32 scale for each
+ * block of 128 values of d: of a row (block_rows = 1: hidden states) or of 128 rows
+ * (block_rows = 128: weights, as checkpoints of this format hold them).  The last
+ * block of a row, and the last rows, may be shorter.
+ *   scale = RN32(max |x| * RN32(1 / 448)) over the block,  q = e4m3(RN32(x / scale)),
+ * rounded to nearest even and held to -448 .. 448.  q = 0 in a block of zeros, or
+ * one so small that its scale rounds to 0; a block with a NaN or an infinity gets
+ * scale NaN and q = 0.
+ */
+typedef struct MtrQuantizeBlocksArgs {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrQuantizeBlocksArgs) */
+  const void* x;                /* [rows, cols], x_dtype */
+  int64_t x_row_stride;         /* elements */
+  int32_t x_dtype;              /* MtrDType */
+  int32_t rows;                 /* 0 .. MTR_MAX_F8_ROWS */
+  int32_t cols;                 /* 1 .. MTR_MAX_F8_D_MODEL */
+  int32_t block_rows;           /* 1 or 128 */
+  uint8_t* q;                   /* [rows, cols] e4m3, 4-byte aligned */
+  int64_t q_row_stride;         /* bytes, multiple of 4; bytes past cols are left as they are */
+  float* scale;                 /* [ceil(rows / block_rows), ceil(cols / 128)] */
+  int64_t scale_row_stride;     /* elements */
+} MtrQuantizeBlocksArgs;
+
+int mtr_quantize_blocks_validate(const MtrQuantizeBlocksArgs* args);
+int mtr_quantize_blocks_launch(const MtrQuantizeBlocksArgs* args, void* stream);
+
+/*
+ * logits[r, v] = RN(sum_b scale[r, b] * weight_scale[v / 128, b] * sum_{k in block b} q[r, k] * weight[v, k])
+ * with q, scale the hidden states quantised by this call (into the workspace where
+ * there are more than a few rows); sums in fp32.
+ */
+typedef struct MtrLmHeadF8Args {
+  uint32_t abi_version;         /* = MTR_ABI_VERSION */
+  uint32_t struct_size;         /* = sizeof(MtrLmHeadF8Args) */
+  const void* hidden;           /* [rows, d_model], hidden_dtype */
+  int64_t hidden_row_stride;    /* elements */
+  const uint8_t* weight;        /* [vocab, d_model] e4m3, 16-byte aligned */
+  int64_t weight_row_stride;    /* bytes, multiple of 16 */
+  const float* weight_scale;    /* [ceil(vocab / 128), ceil(d_model / 128)] */
+  int64_t scale_row_stride;     /* elements */
+  void* logits;                 /* [rows, vocab], logits_dtype; must not overlap the inputs */
+  int64_t logits_row_stride;    /* elements */
+  int32_t hidden_dtype;         /* MtrDType */
+  int32_t logits_dtype;         /* MtrDType */
+  int32_t rows;                 /* 0 .. MTR_MAX_F8_ROWS */
+  int32_t d_model;              /* 1 .. MTR_MAX_F8_D_MODEL */
+  int32_t vocab;                /* 1 .. MTR_MAX_VOCAB */
+  int32_t reserved0;
+  void* workspace;              /* 256-byte aligned; one call's at a time; may be NULL where 0 bytes are needed */
+  int64_t workspace_bytes;      /* >= mtr_lmhead_f8_workspace(rows, d_model, vocab) */
+  uint32_t* error_word;         /* device word or NULL: bits set when a bounded wait gave up */
+} MtrLmHeadF8Args;
+
+/* Workspace bytes of a call (0 for few rows, and for rows <= 0 or d_model <= 0). */
+int64_t mtr_lmhead_f8_workspace(int32_t rows, int32_t d_model, int32_t vocab);
+int mtr_lmhead_f8_validate(const MtrLmHeadF8Args* args);
+int mtr_lmhead_f8_launch(const MtrLmHeadF8Args* args, void* stream);
+
+/* As mtr_lmhead_sample_launch, with this projection (the sampler's logits_dtype
+ * must be the projection's). */
+int mtr_lmhead_f8_sample_launch(const MtrLmHeadF8Args* lm, const MtrSamplerArgs* sampler, void* stream);
 
 /*
  * Log probabilities of given tokens, entropy, log-sum-exp and top alternatives

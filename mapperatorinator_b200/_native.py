@@ -28,6 +28,8 @@ MAX_EOS_RANGES = 2
 MAX_LB_EOS = 8
 MAX_I8_D_MODEL = 131072
 MAX_I8_ROWS = 1 << 22
+MAX_F8_D_MODEL = 131072
+MAX_F8_ROWS = 1 << 22
 MAX_SCORE_ROWS = 1 << 27
 MAX_TOP_N = 32
 MAX_TEACHER_IDS = 128
@@ -233,6 +235,51 @@ class MtrLmHeadI8Args(ctypes.Structure):
     ]
 
 
+class MtrQuantizeBlocksArgs(ctypes.Structure):
+    """include/mtr_sampler.h MtrQuantizeBlocksArgs: blocks of 128 values to e4m3 with a scale each."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("x", c_void_p),
+        ("x_row_stride", c_int64),
+        ("x_dtype", c_int32),
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("block_rows", c_int32),
+        ("q", c_void_p),
+        ("q_row_stride", c_int64),
+        ("scale", c_void_p),
+        ("scale_row_stride", c_int64),
+    ]
+
+
+class MtrLmHeadF8Args(ctypes.Structure):
+    """include/mtr_sampler.h MtrLmHeadF8Args: the output projection in 8-bit floating point."""
+
+    _fields_ = [
+        ("abi_version", c_uint32),
+        ("struct_size", c_uint32),
+        ("hidden", c_void_p),
+        ("hidden_row_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_row_stride", c_int64),
+        ("weight_scale", c_void_p),
+        ("scale_row_stride", c_int64),
+        ("logits", c_void_p),
+        ("logits_row_stride", c_int64),
+        ("hidden_dtype", c_int32),
+        ("logits_dtype", c_int32),
+        ("rows", c_int32),
+        ("d_model", c_int32),
+        ("vocab", c_int32),
+        ("reserved0", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("error_word", c_void_p),
+    ]
+
+
 class MtrLogprobArgs(ctypes.Structure):
     """include/mtr_sampler.h MtrLogprobArgs: log probabilities of given tokens."""
 
@@ -369,6 +416,13 @@ EXPORTS = {
     "mtr_lmhead_i8_validate": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args)]),
     "mtr_lmhead_i8_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args), c_void_p]),
     "mtr_lmhead_i8_sample_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadI8Args), ctypes.POINTER(MtrSamplerArgs),
+                                                   c_void_p]),
+    "mtr_quantize_blocks_validate": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeBlocksArgs)]),
+    "mtr_quantize_blocks_launch": (ctypes.c_int, [ctypes.POINTER(MtrQuantizeBlocksArgs), c_void_p]),
+    "mtr_lmhead_f8_workspace": (c_int64, [c_int32, c_int32, c_int32]),
+    "mtr_lmhead_f8_validate": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadF8Args)]),
+    "mtr_lmhead_f8_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadF8Args), c_void_p]),
+    "mtr_lmhead_f8_sample_launch": (ctypes.c_int, [ctypes.POINTER(MtrLmHeadF8Args), ctypes.POINTER(MtrSamplerArgs),
                                                    c_void_p]),
     "mtr_logprob_validate": (ctypes.c_int, [ctypes.POINTER(MtrLogprobArgs)]),
     "mtr_logprob_launch": (ctypes.c_int, [ctypes.POINTER(MtrLogprobArgs), c_void_p]),
@@ -535,6 +589,23 @@ def lmhead_i8_launch(args: MtrLmHeadI8Args, stream: int | None) -> None:
 def lmhead_i8_sample_launch(lm: MtrLmHeadI8Args, args: MtrSamplerArgs, stream: int | None) -> None:
     check(load().mtr_lmhead_i8_sample_launch(ctypes.byref(lm), ctypes.byref(args), c_void_p(stream or 0)),
           "mtr_lmhead_i8_sample_launch")
+
+
+def quantize_blocks_launch(args: MtrQuantizeBlocksArgs, stream: int | None) -> None:
+    check(load().mtr_quantize_blocks_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_quantize_blocks_launch")
+
+
+def lmhead_f8_workspace(rows: int, d_model: int, vocab: int) -> int:
+    return load().mtr_lmhead_f8_workspace(rows, d_model, vocab)
+
+
+def lmhead_f8_launch(args: MtrLmHeadF8Args, stream: int | None) -> None:
+    check(load().mtr_lmhead_f8_launch(ctypes.byref(args), c_void_p(stream or 0)), "mtr_lmhead_f8_launch")
+
+
+def lmhead_f8_sample_launch(lm: MtrLmHeadF8Args, args: MtrSamplerArgs, stream: int | None) -> None:
+    check(load().mtr_lmhead_f8_sample_launch(ctypes.byref(lm), ctypes.byref(args), c_void_p(stream or 0)),
+          "mtr_lmhead_f8_sample_launch")
 
 
 def logprob_launch(args: MtrLogprobArgs, stream: int | None) -> None:

@@ -22,9 +22,9 @@ LIB_PATH = LIB_DIR / "libmtr_sampler.so"
 SOURCES = [CSRC / "mtr_sampler.cu", CSRC / "mtr_stream.cu", CSRC / "mtr_stream_bf16.cu", CSRC / "mtr_stream_f16.cu",
            CSRC / "mtr_stream_f32.cu", CSRC / "mtr_lmhead.cu", CSRC / "mtr_lmhead_i8.cu",
            CSRC / "mtr_lmhead_few.cu", CSRC / "mtr_logprob.cu", CSRC / "mtr_distill.cu",
-           CSRC / "mtr_verify.cu"]
+           CSRC / "mtr_verify.cu", CSRC / "mtr_lmhead_f8.cu", CSRC / "mtr_lmhead_f8_few.cu"]
 HEADERS = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh", CSRC / "mtr_stream.cuh",
-           CSRC / "mtr_tc.cuh", CSRC / "mtr_vec.cuh", CSRC / "mtr_quant.cuh"]
+           CSRC / "mtr_tc.cuh", CSRC / "mtr_vec.cuh", CSRC / "mtr_quant.cuh", CSRC / "mtr_f8.cuh"]
 BUILD_DIR = PKG_DIR / "_build"
 
 COMPILE_FLAGS = [
@@ -53,16 +53,20 @@ def _nvcc() -> str:
 def _deps(src: Path) -> list:
     """Headers a translation unit includes (the stream kernel's also include mtr_stream.cuh, the
     tensor-core projections' mtr_tc.cuh, the row-streaming kernels' mtr_vec.cuh, those that
-    quantise mtr_quant.cuh)."""
+    quantise mtr_quant.cuh, the 8-bit float projection's mtr_f8.cuh)."""
     deps = [REPO_DIR / "include" / "mtr_sampler.h", CSRC / "mtr_common.cuh"]
     if src.name.startswith("mtr_stream"):
         deps.append(CSRC / "mtr_stream.cuh")
-    if src.name in ("mtr_lmhead.cu", "mtr_lmhead_i8.cu"):
+    if src.name in ("mtr_lmhead.cu", "mtr_lmhead_i8.cu", "mtr_lmhead_f8.cu"):
         deps.append(CSRC / "mtr_tc.cuh")
-    if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu", "mtr_logprob.cu", "mtr_distill.cu", "mtr_verify.cu"):
+    f8 = src.name in ("mtr_lmhead_f8.cu", "mtr_lmhead_f8_few.cu")
+    i8 = src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu")
+    if f8 or i8 or src.name in ("mtr_logprob.cu", "mtr_distill.cu", "mtr_verify.cu"):
         deps.append(CSRC / "mtr_vec.cuh")
-    if src.name in ("mtr_lmhead_i8.cu", "mtr_lmhead_few.cu"):
+    if f8 or i8:
         deps.append(CSRC / "mtr_quant.cuh")
+    if f8:
+        deps.append(CSRC / "mtr_f8.cuh")
     return deps
 
 

@@ -310,15 +310,16 @@ int mtr_projection_timeouts(uint32_t* count, void* stream) {
   if (!count) return MTR_ERR_NULL_ARG;
   cudaStream_t s = (cudaStream_t)stream;
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  uint32_t n[2] = {0, 0};
+  uint32_t n[3] = {0, 0, 0};
   cudaError_t e = cudaStreamIsCapturing(s, &capture);
   if (e == cudaSuccess && capture != cudaStreamCaptureStatusNone) return MTR_ERR_UNSUPPORTED;
   if (e == cudaSuccess) e = mtr::tc::read_gave_up(&n[0], s);
   if (e == cudaSuccess) e = mtr::tc::read_gave_up_i8(&n[1], s);
+  if (e == cudaSuccess) e = mtr::tc::read_gave_up_f8(&n[2], s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   mtr::set_last_cuda_error((int)e);
   if (e != cudaSuccess) return MTR_ERR_CUDA;
-  *count = n[0] + n[1];
+  *count = n[0] + n[1] + n[2];
   return MTR_OK;
 }
 

@@ -36,9 +36,9 @@ struct Divisor {
   float s, inv;
   bool zero, divide;
 };
-__device__ __forceinline__ Divisor divisor_of(float top) {
+__device__ __forceinline__ Divisor divisor_of(float top, float reciprocal = 1.0f / 127.0f) {
   Divisor d;
-  d.s = top < pos_inf() ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fc00000);
+  d.s = top < pos_inf() ? __fmul_rn(top, reciprocal) : __int_as_float(0x7fc00000);
   d.zero = !(d.s > 0.0f);
   d.divide = d.s < 0x1p-90f || (__float_as_uint(d.s) & 0x7fffffu) == 0x7fffffu;
   d.inv = d.zero || d.divide ? 0.0f : __fdiv_rn(1.0f, d.s);

@@ -23,6 +23,7 @@ from typing import Sequence
 import torch
 
 from . import _native as N
+from .fp8_head import Fp8Weight, lmhead_f8_args
 from .int8_head import Int8Weight, launch_on, lmhead_i8_args
 from .scoring import TokenLogprobs, token_logprobs as score_tokens
 
@@ -116,7 +117,7 @@ def lm_head_logits(hidden: torch.Tensor, weight: torch.Tensor, out: torch.Tensor
 
 def projection_timeouts(device=None) -> int:
     """How many bounded waits of the tensor-core projections (``lm_head_logits``,
-    ``lm_head_logits_int8``, ``step_hidden``) have given up on ``device`` (default:
+    ``lm_head_logits_int8``, ``lm_head_logits_fp8``, ``step_hidden``) have given up on ``device`` (default:
     the current one) since the library was loaded: 0 on a healthy device.  One
     host sync with the device's current stream.  Logits that such a projection did
     not compute are NaN: the sampler marks their rows ``nonfinite`` in its status
@@ -468,7 +469,7 @@ class FusedSampler:
         ids = self.out_ids if finished is None else self.out_ids.masked_fill(finished, -1)
         self.token_logprobs = score_tokens(self.scores, ids, top_n=self._score_top)
 
-    def step_hidden(self, hidden: torch.Tensor, weight: torch.Tensor | Int8Weight, input_ids: torch.Tensor | None = None,
+    def step_hidden(self, hidden: torch.Tensor, weight: torch.Tensor | Int8Weight | Fp8Weight, input_ids: torch.Tensor | None = None,
                     uniforms: torch.Tensor | None = None, generator: torch.Generator | None = None, *,
                     id_buffer: torch.Tensor | None = None, cur_len=None, tile_n: int = 0) -> torch.Tensor:
         """The decoder's last hidden states to the next tokens: the tensor-core
@@ -477,14 +478,15 @@ class FusedSampler:
         ``hidden`` has the logits' rows ([2B, d] with CFG).  The logits stay
         readable in ``self.lm_logits`` until the next call.  An
         :class:`~mapperatorinator_b200.int8_head.Int8Weight` takes the 8-bit
-        projection (``lm_head_logits_int8``) instead; ``tile_n`` is the bf16
-        projection's alone."""
+        projection (``lm_head_logits_int8``) instead, an
+        :class:`~mapperatorinator_b200.fp8_head.Fp8Weight` the one in 8-bit floating
+        point (``lm_head_logits_fp8``); ``tile_n`` is the bf16 projection's alone."""
         _require_cuda(hidden, "hidden")
-        i8 = isinstance(weight, Int8Weight)
+        i8, f8 = isinstance(weight, Int8Weight), isinstance(weight, Fp8Weight)
         rows = hidden.shape[0]
         if rows != (2 * self.num_rows if self._base.cfg_enabled else self.num_rows):
             raise ValueError(f"hidden has {rows} rows")
-        vocab = (weight.q if i8 else weight).shape[0]
+        vocab = (weight.q if i8 or f8 else weight).shape[0]
         if vocab != self.vocab_size:
             raise ValueError(f"weight vocabulary {vocab} != {self.vocab_size}")
         buf = getattr(self, "lm_logits", None)
@@ -493,6 +495,8 @@ class FusedSampler:
             self.lm_logits = buf
         if i8:
             lm, work = lmhead_i8_args(hidden, weight.q, weight.scale, buf)
+        elif f8:
+            lm, work = lmhead_f8_args(hidden, weight.q, weight.scale, buf)
         else:
             lm = _lmhead_args(hidden, weight, buf, tile_n)
         if self._base.select_mode == N.SELECT_SAMPLE:
@@ -501,6 +505,8 @@ class FusedSampler:
         finished = self._finished_before()
         if i8:
             launch_on(hidden.device, N.lmhead_i8_sample_launch, lm, a)
+        elif f8:
+            launch_on(hidden.device, N.lmhead_f8_sample_launch, lm, a)
         else:
             N.lmhead_sample_launch(lm, a, torch.cuda.current_stream(hidden.device).cuda_stream)
         self._score(finished)
