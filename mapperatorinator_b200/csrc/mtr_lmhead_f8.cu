@@ -164,25 +164,39 @@ __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
 //   warp 0, one lane   producer: TMA loads into a ring of STAGES stages
 //   warp 1, one lane   issues the products (of a pair: the first CTA's only);
 //                      the whole warp allocates and frees the tensor memory
-//   warps 2-9          epilogue: warp w owns tensor memory lanes 32 (w % 4) ..,
-//                      tile rows, and half of the columns, whose logits it holds
-//                      in registers over the tile's blocks (128 a lane at most);
-//                      at the tile's end it rounds them, stages 32 rows x 128 bytes
+//   warp 2             copies the blocks' scales into a ring of their own: a trip to
+//                      L2 takes longer than a block's products
+//   warps 4 ..         epilogue: warp w owns tensor memory lanes 32 (w % 4) ..,
+//                      tile rows, and some of the columns, whose logits it holds
+//                      in registers over the tile's blocks (64 a lane);
+//                      at the tile's end it rounds them, stages 32 rows x 64 or 128 bytes
 //                      in shared memory (16-byte pieces XOR-swizzled by row) and
 //                      sends them by TMA, or row by row where rows of logits are
 //                      not 16-byte aligned
 // Every wait is bounded; a role whose wait gives up counts it (gave_up) and stops,
 // so that the others' waits give up too; the producer then gives its copies time
 // to land, the epilogue writes NaN for what was not computed, and the CTA returns.
-constexpr int EPI = 8;  // epilogue warps
-constexpr int PROJ_THREADS = 64 + 32 * EPI;
+constexpr int RING = 4;  // blocks whose scales are in shared memory
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
 
 template <int CG, int BN>
 struct Geo {
+  static constexpr int EPI = 8, THREADS = 128 + 32 * EPI;  // epilogue warps
+  // Registers a thread.  384 threads have 168 each at launch; where the epilogue
+  // holds 128 sums a lane the control group's four warps leave most of theirs to
+  // it: 128 * 56 + 256 * 224 = 384 * 168.
+  static constexpr bool SPLIT = BN == 256;
+  static constexpr int LAUNCH_REGS = 168, CONTROL_REGS = 56, EPI_REGS = 224;
+  static_assert(!SPLIT || 128 * CONTROL_REGS + 32 * EPI * EPI_REGS <= THREADS * LAUNCH_REGS, "registers of the launch");
   static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN / CG * BK, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr uint32_t BOX_BYTES = 32 * 128;  // one epilogue warp's staging buffer
+  static constexpr uint32_t ROW_BYTES = 128;                   // of a staging buffer
+  static constexpr uint32_t BOX_BYTES = 32 * ROW_BYTES;        // one epilogue warp's
   static constexpr uint32_t OUT_BYTES = EPI * BOX_BYTES;
-  static constexpr uint32_t FIXED = 512;           // barriers
+  static constexpr uint32_t FIXED = 2816;                      // barriers, scales
   static constexpr int FIT = (int)((227 * 1024 - OUT_BYTES - FIXED) / STAGE_BYTES);
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr uint32_t DYN = STAGES * STAGE_BYTES + OUT_BYTES + FIXED;
@@ -191,18 +205,20 @@ struct Geo {
 };
 
 template <int CG, int BN, typename Tout>
-__global__ void __launch_bounds__(PROJ_THREADS, 1)
+__global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
     lmhead_f8_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_out, const ProjParams p) {
   typedef Geo<CG, BN> G;
   constexpr int S = G::STAGES, NACC = G::NACC;
-  constexpr int CB = 128 / (int)sizeof(Tout);           // columns of a staging buffer
-  constexpr int PIECES = 8;                             // 16-byte pieces of its rows
-  constexpr int PART = BN / 2 < CB ? CB : BN / 2;       // a warp's columns
-  constexpr int ACTIVE = 4 * (BN / PART);               // warps that have some
+  constexpr int ROW = G::ROW_BYTES, PIECES = ROW / 16;      // bytes and 16-byte pieces of a staged row
+  constexpr int CB = ROW / (int)sizeof(Tout);               // columns of a staging buffer
+  constexpr int MIN_PART = CB > 32 ? CB : 32;
+  constexpr int EACH = BN / (G::EPI / 4), PART = EACH < MIN_PART ? MIN_PART : EACH;  // a warp's columns
+  constexpr int ACTIVE = 4 * (BN / PART);                   // warps that have some
   struct Fixed {
-    uint64_t full[S], empty[S], acc_full[NACC], acc_empty[NACC];
+    uint64_t full[S], empty[S], acc_full[NACC], acc_empty[NACC], sc_full[RING], sc_empty[RING];
     uint32_t tmem_slot;
+    __align__(16) float rows[RING][BM], ids[RING][4];  // scales of a block: of the rows, of each 128 ids
   };
   static_assert(sizeof(Fixed) <= G::FIXED, "fixed part of the shared memory");
   static_assert(BN <= 256 && BLOCK % PART == 0, "a warp's columns share a weight block");
@@ -231,7 +247,14 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&fx.sc_full[i], 32);
+      mbar_init(&fx.sc_empty[i], ACTIVE);
+    }
+  }
   if (warp == 1) {
+    __syncwarp();
     if (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&fx.tmem_slot)), "r"(G::COLS) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -283,181 +306,204 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
   if (warp == 0 && lane == 0) load_early();
   wait_prior_grid();
 
-  if (warp == 0 && lane == 0) {
-    // ---------------- producer
-    Turn turn;
-    uint32_t it = 0;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (mbar_wait(bar, parity, WAIT_NS)) return true;
-      gave_up(p.err, 1u);
-      return false;
-    };
-    for (int t = first; t < tiles && ok; t += step) {
-      int m0, n0;
-      place(t, m0, n0);
-      for (int kb = 0; kb < KB && ok; ++kb, ++it, turn.next(S)) {
-        ok = wait(&empty[turn.slot], turn.parity ^ 1);
-        if (!ok) break;
-        if (it >= early) load_ids(turn.slot, kb, n0);
-        if (CG == 1) tma_load_2d(a_tile(turn.slot), &map_h, kb * BK, m0, &full[turn.slot]);
-        else load_pair(a_tile(turn.slot), &map_h, kb * BK, m0, map_to(smem_u32(&full[turn.slot]), 0));
+  if (warp < 4) {
+    if constexpr (G::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::CONTROL_REGS));
+    if (warp == 0 && lane == 0) {
+      // ---------------- producer
+      Turn turn;
+      uint32_t it = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait(bar, parity, WAIT_NS)) return true;
+        gave_up(p.err, 1u);
+        return false;
+      };
+      for (int t = first; t < tiles && ok; t += step) {
+        int m0, n0;
+        place(t, m0, n0);
+        for (int kb = 0; kb < KB && ok; ++kb, ++it, turn.next(S)) {
+          ok = wait(&empty[turn.slot], turn.parity ^ 1);
+          if (!ok) break;
+          if (it >= early) load_ids(turn.slot, kb, n0);
+          if (CG == 1) tma_load_2d(a_tile(turn.slot), &map_h, kb * BK, m0, &full[turn.slot]);
+          else load_pair(a_tile(turn.slot), &map_h, kb * BK, m0, map_to(smem_u32(&full[turn.slot]), 0));
+        }
       }
-    }
-    // every stage is free: its copies have landed and the arrivals on its barriers are in
-    for (int i = 0; ok && i < S; ++i, turn.next(S)) ok = wait(&empty[turn.slot], turn.parity ^ 1);
-    if (!ok) {  // copies under way get time to land before the CTA may leave
-      const uint64_t t0 = global_ns();
-      while (global_ns() - t0 < 2000000ull) {
+      // every stage is free: its copies have landed and the arrivals on its barriers are in
+      for (int i = 0; ok && i < S; ++i, turn.next(S)) ok = wait(&empty[turn.slot], turn.parity ^ 1);
+      if (!ok) {  // copies under way get time to land before the CTA may leave
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2000000ull) {
+        }
       }
-    }
-  } else if (warp == 1 && lane == 0 && cta == 0) {
-    // ---------------- products
-    constexpr uint32_t idesc = idesc_f8(BM * CG, BN);
-    Turn turn, acc;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (mbar_wait(bar, parity, WAIT_NS)) return true;
-      gave_up(p.err, 2u);
-      return false;
-    };
-    // this thread feeds the tensor core alone, a stage of products every 512
-    // clocks at most: everything a stage needs is an addition to these
-    const uint64_t desc = sw128_desc(smem_u32(ring));
-    const uint32_t lo0 = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
-    auto commit = [&](uint64_t* bar) {
-      if (CG == 1) tc_commit(bar);
-      else commit_pair(bar);
-    };
-    for (int t = first; t < tiles && ok; t += step) {
-      for (int kb = 0; kb < KB; ++kb, turn.next(S), acc.next(NACC)) {
-        ok = wait(&acc_empty[acc.slot], acc.parity ^ 1) && wait(&full[turn.slot], turn.parity);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t a_lo = lo0 + (uint32_t)turn.slot * (G::STAGE_BYTES >> 4), b_lo = a_lo + (G::A_BYTES >> 4);
+    } else if (warp == 1 && cta == 0) {
+      // ---------------- products: the warp in step, one elected lane issues
+      constexpr uint32_t idesc = idesc_f8(BM * CG, BN);
+      Turn turn, acc;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (__all_sync(FULL, mbar_wait(bar, parity, WAIT_NS))) return true;
+        if (lane == 0) gave_up(p.err, 2u);
+        return false;
+      };
+      // this warp feeds the tensor core alone, a stage of products every 512
+      // clocks at most: everything a stage needs is an addition to these
+      const uint64_t desc = sw128_desc(smem_u32(ring));
+      const uint32_t lo0 = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
+      for (int t = first; t < tiles && ok; t += step) {
+        for (int kb = 0; kb < KB; ++kb, turn.next(S), acc.next(NACC)) {
+          const uint32_t a_lo = lo0 + (uint32_t)turn.slot * (G::STAGE_BYTES >> 4), b_lo = a_lo + (G::A_BYTES >> 4);
+          // the stage first: its copies are there before the accumulator is free
+          ok = wait(&full[turn.slot], turn.parity) && wait(&acc_empty[acc.slot], acc.parity ^ 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < BK / UK; ++k)
-          mma_f8<CG>(tmem + acc.slot * BN, a_lo + k * (UK >> 4), b_lo + k * (UK >> 4), hi, idesc, k > 0 ? 1u : 0u);
-        commit(&empty[turn.slot]);
-        commit(&acc_full[acc.slot]);
-      }
-    }
-  } else if (warp >= 2 && (warp - 2) / 4 * PART < BN) {
-    const int quad = warp & 3, c0 = (warp - 2) / 4 * PART;
-    uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 2) * G::BOX_BYTES;
-    // The scales of the lane's row and the warp's columns are asked for two blocks
-    // ahead, over tile borders: a trip to L2 takes longer than a block.
-    int ask_t = first, ask_kb = 0;
-    auto ask = [&](float& rs, float& ws) {
-      rs = ws = 0.0f;
-      if (ask_t >= tiles) return;
-      int m0, n0;
-      place(ask_t, m0, n0);
-      const int row = m0 + quad * 32 + lane;
-      if (row < p.rows) rs = p.row_scale[ask_kb * p.row_pitch + row];
-      if (n0 + c0 < p.vocab) ws = p.w_scale[(int64_t)((n0 + c0) / BLOCK) * p.w_pitch + ask_kb];
-      if (++ask_kb == KB) {
-        ask_kb = 0;
-        ask_t += step;
-      }
-    };
-    float rs0, ws0, rs1, ws1;
-    ask(rs0, ws0);
-    ask(rs1, ws1);
-    Turn acc;
-    bool first_wait = true;
-    for (int t = first; t < tiles; t += step) {
-      int m0, n0;
-      place(t, m0, n0);
-      const bool live = m0 + quad * 32 < p.rows && n0 + c0 < p.vocab;
-      u64 sum[PART / 2];
-#pragma unroll
-      for (int i = 0; i < PART / 2; ++i) sum[i] = 0;
-      bool waited = true;
-      for (int kb = 0; kb < KB; ++kb, acc.next(NACC)) {
-        const float f = __fmul_rn(rs0, ws0);
-        rs0 = rs1;
-        ws0 = ws1;
-        ask(rs1, ws1);
-        if (lane == 0) waited = mbar_wait(&acc_full[acc.slot], acc.parity, WAIT_NS) && !(p.give_up && first_wait);
-        first_wait = false;
-        waited = __shfl_sync(FULL, waited, 0) != 0;
-        if (!waited) break;
-        tc_fence_after();
-        if (live) {
-          const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc.slot * BN + c0);
-          const u64 f2 = pk2(f, f);
-#pragma unroll
-          for (int g = 0; g < PART / 32; ++g) {
-            uint32_t v[32];
-            tmem_ld32(base + (uint32_t)(g * 32), v);
-            tmem_wait_ld();
-            if (g == PART / 32 - 1) {  // the warp's part of the accumulator is in registers
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) arrive_at(map_to(smem_u32(&acc_empty[acc.slot]), 0));
+            for (int k = 0; k < BK / UK; ++k)
+              mma_f8<CG>(tmem + acc.slot * BN, a_lo + k * (UK >> 4), b_lo + k * (UK >> 4), hi, idesc, k > 0 ? 1u : 0u);
+            if (CG == 1) {
+              tc_commit(&empty[turn.slot]);
+              tc_commit(&acc_full[acc.slot]);
+            } else {
+              commit_pair(&empty[turn.slot]);
+              commit_pair(&acc_full[acc.slot]);
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              sum[g * 16 + i] = fma2(pk2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2, sum[g * 16 + i]);
           }
-        } else if (lane == 0) {
-          arrive_at(map_to(smem_u32(&acc_empty[acc.slot]), 0));  // nothing to read here
-        }
-      }
-      if (!waited) {
-        if (lane == 0) gave_up(p.err, 4u);
-        // what is not computed reads NaN, which the sampler and the scores report
-        for (; t < tiles; t += step) {
-          place(t, m0, n0);
-          for (int r = m0 + quad * 32; r < min(m0 + quad * 32 + 32, p.rows); ++r)
-            for (int col = n0 + c0 + lane; col < min(n0 + c0 + PART, p.vocab); col += 32)
-              ((Tout*)p.out)[r * p.out_stride + col] = from_f<Tout>(__int_as_float(0x7fc00000));
-        }
-        break;
-      }
-      if (!live) continue;
-      const bool by_tma = n0 + c0 + PART <= p.tma_ids;
-#pragma unroll
-      for (int g = 0; g < PART; g += CB) {
-        constexpr int EP = 16 / (int)sizeof(Tout);
-        uint4 w[PIECES];
-#pragma unroll
-        for (int q = 0; q < PIECES; ++q) {
-          float f[EP];
-#pragma unroll
-          for (int e = 0; e < EP; e += 2) up2(sum[(g + q * EP + e) / 2], f[e], f[e + 1]);
-          w[q] = pack<Tout>(f);
-        }
-        if (p.store_tma) {  // the buffer's previous contents have been read
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
-        }
-#pragma unroll
-        for (int q = 0; q < PIECES; ++q)
-          *reinterpret_cast<uint4*>(box + lane * (PIECES * 16) + (q ^ (lane & (PIECES - 1))) * 16) = w[q];
-        if (by_tma) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else {
-          __syncwarp();
-          const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c0 + g));
-          Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c0 + g;
-          for (int r = 0; r < high; ++r, dst += p.out_stride)
-#pragma unroll
-            for (int x = 0; x < CB; x += 32) {
-              const int i = x + lane, in = i * (int)sizeof(Tout), piece = in / 16 ^ (r & (PIECES - 1));
-              if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(box + r * (PIECES * 16) + piece * 16 + in % 16);
-            }
           __syncwarp();
         }
       }
+    } else if (warp == 2) {
+      // ---------------- scales: RING blocks ahead of the epilogue, past tile borders
+      Turn turn;
+      for (int t = first; t < tiles; t += step) {
+        int m0, n0;
+        place(t, m0, n0);
+        // four rows a lane; behind the last row and the last id any scale does
+        const float* r = p.row_scale + min(m0 + 4 * lane, (p.rows - 1) & ~3);
+        const float* w = p.w_scale + (int64_t)(min(n0 + lane * BLOCK, p.vocab - 1) / BLOCK) * p.w_pitch;
+        bool ok = true;
+        for (int kb = 0; kb < KB; ++kb, turn.next(RING), r += p.row_pitch, ++w) {
+          ok = __all_sync(FULL, mbar_wait(&fx.sc_empty[turn.slot], turn.parity ^ 1, WAIT_NS));
+          if (!ok) break;
+          copy_async<16>(&fx.rows[turn.slot][4 * lane], r);
+          if (lane * BLOCK < BN) copy_async<4>(&fx.ids[turn.slot][lane], w);
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&fx.sc_full[turn.slot])) : "memory");
+        }
+        if (!ok) {
+          if (lane == 0) gave_up(p.err, 1u);
+          break;
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    if (p.store_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  } else {
+    if constexpr (G::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::EPI_REGS));
+    if ((warp - 4) / 4 * PART < BN) {
+      const int quad = warp & 3, c0 = (warp - 4) / 4 * PART;
+      uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 4) * G::BOX_BYTES;
+      constexpr int LD = 32, BUFS = 2;
+      const uint32_t tmem_at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0, empty_at = map_to(smem_u32(acc_empty), 0);
+      const float *const row_scale = &fx.rows[0][quad * 32 + lane], *const id_scale = &fx.ids[0][c0 / BLOCK];
+      Turn acc, sc;
+      bool hook = p.give_up != 0;
+      for (int t = first; t < tiles; t += step) {
+        int m0, n0;
+        place(t, m0, n0);
+        const bool live = m0 + quad * 32 < p.rows && n0 + c0 < p.vocab;
+        float sum[PART];
+#pragma unroll
+        for (int i = 0; i < PART; ++i) sum[i] = 0.0f;
+        bool waited = true;
+        for (int kb = 0; kb < KB; ++kb, acc.next(NACC), sc.next(RING)) {
+          if (lane == 0)
+            waited = mbar_wait(&fx.sc_full[sc.slot], sc.parity, WAIT_NS) && mbar_wait(&acc_full[acc.slot], acc.parity, WAIT_NS) && !hook;
+          hook = false;
+          waited = __shfl_sync(FULL, waited, 0) != 0;
+          if (!waited) break;
+          tc_fence_after();
+          const uint32_t base = tmem_at + (uint32_t)(acc.slot * BN);
+          uint32_t v[BUFS][LD];
+          if (live) tmem_ld(base, v[0]);
+          const float f = __fmul_rn(row_scale[sc.slot * BM], id_scale[sc.slot * 4]);
+          auto release = [&]() {  // the warp's part of the accumulator is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              arrive_here(&fx.sc_empty[sc.slot]);
+              if (CG == 1) arrive_here(&acc_empty[acc.slot]);
+              else arrive_at(empty_at + (uint32_t)(acc.slot * 8));
+            }
+          };
+          if (live) {
+#pragma unroll
+            for (int g = 0; g < PART / LD; ++g) {
+              uint32_t(&now)[LD] = v[g % BUFS];
+              tmem_wait_ld(now);
+              if (g + 1 == PART / LD) release();
+              else if (BUFS > 1) tmem_ld(base + (uint32_t)((g + 1) * LD), v[(g + 1) % BUFS]);
+#pragma unroll
+              for (int i = 0; i < LD; ++i) sum[g * LD + i] = fmaf(__uint_as_float(now[i]), f, sum[g * LD + i]);
+              if (BUFS == 1 && g + 1 < PART / LD) tmem_ld(base + (uint32_t)((g + 1) * LD), v[0]);
+            }
+          } else {
+            release();  // nothing to read here
+          }
+        }
+        if (!waited) {
+          if (lane == 0) gave_up(p.err, 4u);
+          // what is not computed reads NaN, which the sampler and the scores report
+          for (; t < tiles; t += step) {
+            place(t, m0, n0);
+            for (int r = m0 + quad * 32; r < min(m0 + quad * 32 + 32, p.rows); ++r)
+              for (int col = n0 + c0 + lane; col < min(n0 + c0 + PART, p.vocab); col += 32)
+                ((Tout*)p.out)[r * p.out_stride + col] = from_f<Tout>(__int_as_float(0x7fc00000));
+          }
+          break;
+        }
+        if (!live) continue;
+        const bool by_tma = n0 + c0 + PART <= p.tma_ids;
+        auto swizzle = [](int r) { return ROW == 128 ? r & 7 : (r >> 1) & 3; };  // of TMA's 128- and 64-byte patterns
+#pragma unroll
+        for (int g = 0; g < PART; g += CB) {
+          constexpr int EP = 16 / (int)sizeof(Tout);
+          uint4 w[PIECES];
+#pragma unroll
+          for (int q = 0; q < PIECES; ++q) {
+            float f[EP];
+#pragma unroll
+            for (int e = 0; e < EP; ++e) f[e] = sum[g + q * EP + e];
+            w[q] = pack<Tout>(f);
+          }
+          if (p.store_tma) {  // the buffer's previous contents have been read
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+          }
+#pragma unroll
+          for (int q = 0; q < PIECES; ++q)
+            *reinterpret_cast<uint4*>(box + lane * ROW + (q ^ swizzle(lane)) * 16) = w[q];
+          if (by_tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (n0 + c0 + g < p.vocab) store_2d(&map_out, box, n0 + c0 + g, m0 + quad * 32);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {
+            __syncwarp();
+            const int high = min(32, p.rows - (m0 + quad * 32)), wide = min(CB, p.vocab - (n0 + c0 + g));
+            Tout* dst = (Tout*)p.out + (int64_t)(m0 + quad * 32) * p.out_stride + n0 + c0 + g;
+            for (int r = 0; r < high; ++r, dst += p.out_stride)
+#pragma unroll
+              for (int x = 0; x < CB; x += 32) {
+                const int i = x + lane, in = i * (int)sizeof(Tout), piece = in / 16 ^ swizzle(r);
+                if (i < wide) dst[i] = *reinterpret_cast<const Tout*>(box + r * ROW + piece * 16 + in % 16);
+              }
+            __syncwarp();
+          }
+        }
+      }
+      if (p.store_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -528,7 +574,7 @@ static cudaError_t launch_tiles(const MtrLmHeadF8Args& a, const Held& h, cudaStr
                                    : std::is_same<Tout, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (tma) {
-    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, 128 / es, 32)) return cudaErrorInvalidValue;
+    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, (int)G::ROW_BYTES / es, 32, G::ROW_BYTES == 64)) return cudaErrorInvalidValue;
   } else {
     mo = mw;
   }
@@ -564,7 +610,7 @@ static cudaError_t launch_tiles(const MtrLmHeadF8Args& a, const Held& h, cudaStr
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, room = device_sms() / CG;
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
-      config(dim3((unsigned)((tiles < room ? tiles : room) * CG), 1, 1), PROJ_THREADS, G::DYN, CG, s, attr);
+      config(dim3((unsigned)((tiles < room ? tiles : room) * CG), 1, 1), G::THREADS, G::DYN, CG, s, attr);
   return cudaLaunchKernelEx(&cfg, kern, mh, mw, mo, p);
 }
 
@@ -625,7 +671,7 @@ int mtr_quantize_blocks_launch(const MtrQuantizeBlocksArgs* a, void* stream) {
 
 int64_t mtr_lmhead_f8_workspace(int32_t rows, int32_t d_model, int32_t vocab) {
   if (rows <= 0 || d_model <= 0 || few_rows(rows, d_model, vocab)) return 0;
-  return up((int64_t)rows * up(d_model, 16), 256) + 4ll * rows * blocks_of(d_model);
+  return up((int64_t)rows * up(d_model, 16), 256) + 4ll * up(rows, 4) * blocks_of(d_model);
 }
 
 int mtr_lmhead_f8_validate(const MtrLmHeadF8Args* a) {
@@ -666,7 +712,7 @@ static int lmhead_f8_launch_impl(const MtrLmHeadF8Args* a, cudaStream_t s) {
   h.q = (uint8_t*)a->workspace;
   h.q_stride = up(a->d_model, 16);
   h.scale = (float*)(h.q + up(a->rows * h.q_stride, 256));
-  h.pitch = a->rows;  // a block's scales of all rows side by side, as the epilogue's lanes read them
+  h.pitch = up(a->rows, 4);  // a block's scales of all rows side by side, 16 bytes a lane
   const QuantParams p{a->hidden, a->hidden_row_stride, a->rows, a->d_model, h.q, h.q_stride, h.scale, 1, h.pitch};
   cudaError_t e = launch_quantize(p, a->hidden_dtype, false, s);
   if (e == cudaSuccess) {

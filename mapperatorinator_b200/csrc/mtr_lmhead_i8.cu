@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
         for (int g = 0; g < PART; g += CB) {
           uint32_t v[CB / 32][32];
 #pragma unroll
-          for (int h = 0; h < CB / 32; ++h) tmem_ld32(base + (uint32_t)(g + h * 32), v[h]);
+          for (int h = 0; h < CB / 32; ++h) tmem_ld(base + (uint32_t)(g + h * 32), v[h]);
           __syncwarp();
 #pragma unroll
           for (int h = 0; h < CB / 32; ++h) cs[h * 32 + lane] = cs_now[g / 32 + h];

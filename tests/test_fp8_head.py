@@ -142,7 +142,7 @@ def test_projection_and_sampler_must_share_the_logits():
 def test_workspace_sizes():
     assert N.lmhead_f8_workspace(0, 64, 100) == 0 and N.lmhead_f8_workspace(4, 0, 100) == 0
     assert N.lmhead_f8_workspace(3, 100, 4096) == 0  # few rows
-    assert N.lmhead_f8_workspace(301, 200, 77) == 62720 + 301 * 8  # 301 rows of 208 bytes, the scales on the next 256-byte boundary
+    assert N.lmhead_f8_workspace(301, 200, 77) == 62720 + 304 * 8  # 301 rows of 208 bytes, the scales of 304 on the next 256-byte boundary
     assert N.lmhead_f8_workspace(N.MAX_F8_ROWS, N.MAX_F8_D_MODEL, 1) == (1 << 39) + (1 << 34)
 
 
