@@ -341,20 +341,22 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
       constexpr uint32_t idesc = idesc_f8(BM * CG, BN);
       Turn turn, acc;
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
+      auto wait = [&](uint32_t bar, uint32_t parity) {
         if (__all_sync(FULL, mbar_wait(bar, parity, WAIT_NS))) return true;
         if (lane == 0) gave_up(p.err, 2u);
         return false;
       };
       // this warp feeds the tensor core alone, a stage of products every 512
       // clocks at most: everything a stage needs is an addition to these
+      const uint32_t full_at = held(smem_u32(full)), stage_empty_at = held(smem_u32(empty));
+      const uint32_t acc_full_at = held(smem_u32(acc_full)), acc_empty_at = held(smem_u32(acc_empty));
       const uint64_t desc = sw128_desc(smem_u32(ring));
       const uint32_t lo0 = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
       for (int t = first; t < tiles && ok; t += step) {
         for (int kb = 0; kb < KB; ++kb, turn.next(S), acc.next(NACC)) {
           const uint32_t a_lo = lo0 + (uint32_t)turn.slot * (G::STAGE_BYTES >> 4), b_lo = a_lo + (G::A_BYTES >> 4);
           // the stage first: its copies are there before the accumulator is free
-          ok = wait(&full[turn.slot], turn.parity) && wait(&acc_empty[acc.slot], acc.parity ^ 1);
+          ok = wait(full_at + 8 * turn.slot, turn.parity) && wait(acc_empty_at + 8 * acc.slot, acc.parity ^ 1);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -362,11 +364,11 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
             for (int k = 0; k < BK / UK; ++k)
               mma_f8<CG>(tmem + acc.slot * BN, a_lo + k * (UK >> 4), b_lo + k * (UK >> 4), hi, idesc, k > 0 ? 1u : 0u);
             if (CG == 1) {
-              tc_commit(&empty[turn.slot]);
-              tc_commit(&acc_full[acc.slot]);
+              tc_commit(stage_empty_at + 8 * turn.slot);
+              tc_commit(acc_full_at + 8 * acc.slot);
             } else {
-              commit_pair(&empty[turn.slot]);
-              commit_pair(&acc_full[acc.slot]);
+              commit_pair(stage_empty_at + 8 * turn.slot);
+              commit_pair(acc_full_at + 8 * acc.slot);
             }
           }
           __syncwarp();
@@ -402,8 +404,11 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
       const int quad = warp & 3, c0 = (warp - 4) / 4 * PART;
       uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 4) * G::BOX_BYTES;
       constexpr int LD = 32, BUFS = 2;
-      const uint32_t tmem_at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0, empty_at = map_to(smem_u32(acc_empty), 0);
-      const float *const row_scale = &fx.rows[0][quad * 32 + lane], *const id_scale = &fx.ids[0][c0 / BLOCK];
+      const uint32_t tmem_at = held(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0);
+      const uint32_t full_at = held(smem_u32(acc_full)), empty_at = held(CG == 1 ? smem_u32(acc_empty) : map_to(smem_u32(acc_empty), 0));
+      const uint32_t sc_full_at = held(smem_u32(fx.sc_full)), sc_empty_at = held(smem_u32(fx.sc_empty));
+      const uint32_t rows_at = held(smem_u32(&fx.rows[0][quad * 32 + lane])), ids_at = held(smem_u32(&fx.ids[0][c0 / BLOCK]));
+      const bool first_lane = held(lane) == 0;
       Turn acc, sc;
       bool hook = p.give_up != 0;
       for (int t = first; t < tiles; t += step) {
@@ -415,8 +420,8 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
         for (int i = 0; i < PART; ++i) sum[i] = 0.0f;
         bool waited = true;
         for (int kb = 0; kb < KB; ++kb, acc.next(NACC), sc.next(RING)) {
-          if (lane == 0)
-            waited = mbar_wait(&fx.sc_full[sc.slot], sc.parity, WAIT_NS) && mbar_wait(&acc_full[acc.slot], acc.parity, WAIT_NS) && !hook;
+          if (first_lane)
+            waited = mbar_wait(sc_full_at + 8 * sc.slot, sc.parity, WAIT_NS) && mbar_wait(full_at + 8 * acc.slot, acc.parity, WAIT_NS) && !hook;
           hook = false;
           waited = __shfl_sync(FULL, waited, 0) != 0;
           if (!waited) break;
@@ -424,14 +429,14 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
           const uint32_t base = tmem_at + (uint32_t)(acc.slot * BN);
           uint32_t v[BUFS][LD];
           if (live) tmem_ld(base, v[0]);
-          const float f = __fmul_rn(row_scale[sc.slot * BM], id_scale[sc.slot * 4]);
+          const float f = __fmul_rn(load_shared(rows_at + sc.slot * (BM * 4)), load_shared(ids_at + sc.slot * 16));
           auto release = [&]() {  // the warp's part of the accumulator is in registers
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              arrive_here(&fx.sc_empty[sc.slot]);
-              if (CG == 1) arrive_here(&acc_empty[acc.slot]);
-              else arrive_at(empty_at + (uint32_t)(acc.slot * 8));
+            if (first_lane) {
+              arrive_here(sc_empty_at + 8 * sc.slot);
+              if (CG == 1) arrive_here(empty_at + 8 * acc.slot);
+              else arrive_at(empty_at + 8 * acc.slot);
             }
           };
           if (live) {

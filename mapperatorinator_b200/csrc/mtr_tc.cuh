@@ -43,8 +43,7 @@ __device__ __forceinline__ uint64_t global_ns() {
 // Waits for the phase with parity `ph` to complete; false after `budget_ns`
 // nanoseconds (0: a single poll).  The clock is read only every 4096 polls:
 // a healthy hand-off completes long before the first read.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t ph, uint64_t budget_ns) {
-  const uint32_t a = smem_u32(b);
+__device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t ph, uint64_t budget_ns) {
   uint64_t t0 = 0;
   for (uint32_t i = 1;; ++i) {
     uint32_t done;
@@ -64,6 +63,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t ph, uint64_t bud
     }
   }
 }
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t ph, uint64_t budget_ns) { return mbar_wait(smem_u32(b), ph, budget_ns); }
+// A value that the compiler keeps in a register: it would form a shared-memory
+// address anew, from the CTA's place in the cluster, wherever it is used.
+__device__ __forceinline__ uint32_t held(uint32_t v) {
+  asm volatile("mov.b32 %0, %0;" : "+r"(v));
+  return v;
+}
+__device__ __forceinline__ float load_shared(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
 // Bounded waits that gave up on this device since the library was loaded (each
 // translation unit has its own count; mtr_projection_timeouts adds them), and the
 // bit of one in the caller's word.
@@ -81,10 +92,10 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) { tc_commit(smem_u32(bar)); }
 // Shared-memory matrix descriptor of a K-major tile with the 128-byte swizzle:
 // rows of 128 bytes, 8-row atoms 1024 bytes apart (stride byte offset), leading
 // byte offset 16 (unused by this layout), descriptor version 1, layout type 2.
@@ -157,8 +168,8 @@ __device__ __forceinline__ void arrive_at(uint32_t addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // the same on a barrier of this CTA: no trip through the cluster's network
-__device__ __forceinline__ void arrive_here(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void arrive_here(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -168,12 +179,12 @@ __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, int
       : "memory");
 }
 // arrives on the barrier at this offset in both CTAs of the pair
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                   smem_u32(bar)),
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                "h"((uint16_t)3)
                : "memory");
 }
+__device__ __forceinline__ void commit_pair(uint64_t* bar) { commit_pair(smem_u32(bar)); }
 __device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
                "r"(smem_u32(src))
