@@ -96,17 +96,28 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   const int64_t b = draft ? (row - targets) / K : row / (K + 1);
   const int j = (int)(draft ? (row - targets) % K : row % (K + 1));
   wait_prior_grid();
-  // a position counts only behind drafts that are ids
-  for (int i = 0; i < (draft ? j + 1 : j); ++i) {
-    const int64_t id = draft_id(p, b, i);
-    if (id < 0 || id >= V) return;
-  }
   const T* x = draft ? (const T*)p.draft + b * p.d_batch + j * p.d_pos : (const T*)p.target + b * p.t_batch + j * p.t_pos;
   const float scale = draft ? p.d_scale : p.t_scale;
   const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
   const int head = min(off ? E - off : 0, V), vecs = (V - head) / E, behind = V - head - vecs * E;
   const uint4* body = reinterpret_cast<const uint4*>(x + head);
   const int v0 = min((int)blockIdx.y * p.run, vecs), v1 = blockIdx.y == gridDim.y - 1 ? vecs : min(v0 + p.run, vecs);
+
+  // the first tile is asked for before it is known whether the row counts
+  uint4 w[HOLD];
+  auto ask = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k) {
+      const int i = i0 + k * THREADS;
+      w[k] = i < v1 ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+    }
+  };
+  ask(v0 + tid);
+  // a position counts only behind drafts that are ids
+  for (int i0 = 0, n = draft ? j + 1 : j; i0 < n; i0 += 32) {
+    const int64_t id = i0 + lane < n ? draft_id(p, b, i0 + lane) : 0;
+    if (__any_sync(FULL, id < 0 || id >= V)) return;
+  }
 
   float m = neg_inf();
   double s = 0.0;
@@ -123,12 +134,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   const int single = blockIdx.y > 0 ? -1 : tid < head ? tid : tid >= 32 && tid < 32 + behind ? V - behind + tid - 32 : -1;
   const float one = single >= 0 ? to_f(x[single]) : neg_inf();
   for (int i0 = v0 + tid; i0 < v1; i0 += HOLD * THREADS) {
-    uint4 w[HOLD];
-#pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      const int i = i0 + k * THREADS;
-      w[k] = i < v1 ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
-    }
+    if (i0 != v0 + tid) ask(i0);
     if constexpr (GREEDY) {
       float best = m;
 #pragma unroll
@@ -206,21 +212,38 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 }
 
 constexpr int PICK = 512, PICK_WARPS = PICK / 32;
+constexpr int KEPT = 8;  // ids of a thread whose terms stay in registers
+constexpr int MOST = 16; // ids of a thread in the last search: V / (16 warps) / 512 threads
+
+// e^((x - m) / T) in double, x <= m finite or -inf: with c = 64 log2(e) / T,
+// z = x c - m c = k + r, k whole and |r| <= 1/2, the value is 2^(k / 64) 2^(r / 64): a
+// table of 64 powers, an exponent, and the series of e^(r ln2 / 64) to r^4 (within
+// 4e-14).  Nine double operations, which bound the kernel (64 a clock and SM); the
+// library's exp has about twice as many.  Where z is at most -64000, 2^-1000, the value is 0.
+struct Exp {
+  double c, mc;
+};
+__device__ __forceinline__ double term(float x, const Exp& e, const double* powers) {
+  constexpr double STEP = 0.69314718055994530942 / 64.0, MAGIC = 6755399441055744.0;  // 1.5 2^52
+  const double z = fma((double)x, e.c, -e.mc), y = z + MAGIC, r = z - (y - MAGIC);
+  const int k = __double2loint(y);
+  double v = fma(fma(fma(fma(STEP * STEP * STEP * STEP / 24.0, r, STEP * STEP * STEP / 6.0), r, STEP * STEP / 2.0), r, STEP), r, 1.0) *
+             powers[k & 63];
+  v = __hiloint2double(__double2hiint(v) + ((k >> 6) << 20), __double2loint(v));
+  return (uint32_t)__double2hiint(z) >= 0xc0ef4000u ? 0.0 : v;  // z <= -64000
+}
 
 struct Sums {
   double t, d;
 };
 
 struct PickShared {
+  double powers[64];
   double warp_t[PICK_WARPS], warp_d[PICK_WARPS];
   Sums cta;                      // read by the cluster's other CTAs
   double weight;                 // likewise
   double piece[PICK_WARPS];
-  int stop, unclear, bad_draft;
-  uint32_t status;
-  float t_m, d_m;
-  double t_s, d_s;
-  int token;
+  int stop, unclear, token;
 };
 
 // A row's parts joined; every lane the same.
@@ -237,7 +260,7 @@ __device__ __forceinline__ Part join(const Part* parts, int runs, float scale) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
+__global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
   __shared__ PickShared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -261,26 +284,22 @@ __global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
     }
     return (double)u;
   };
-  auto cluster_sync = [&]() {
-    if (cs > 1) cluster.sync();
-    else __syncthreads();
-  };
-  // this CTA's ids, a warp's of them
+  if (tid < 64) sh.powers[tid] = exp2(tid / 64.0);
+  __syncthreads();
+  const double* powers = sh.powers;
+  constexpr double LOG2E_64 = 64.0 * 1.4426950408889634074;
+  auto exp_of = [&](float m, double inv) { return Exp{LOG2E_64 * inv, (double)m * (LOG2E_64 * inv)}; };
+  // this CTA's ids [c0, c1); `kept`: a thread has KEPT of them, one after another, at most
   const int share = (V + cs - 1) / cs, c0 = min(rank * share, V), c1 = min(c0 + share, V);
-  auto piece_of = [&](int from, int to, int k, int& a, int& z) {
-    const int each = (to - from + PICK_WARPS - 1) / PICK_WARPS;
+  const bool kept = share <= PICK * KEPT;
+  // part `k` of [from, to) cut into n
+  auto part_of = [](int from, int to, int n, int k, int& a, int& z) {
+    const int each = (to - from + n - 1) / n;
     a = min(from + k * each, to);
     z = min(a + each, to);
   };
-  // sums of e^((x - m) / T) over the whole row(s) in double; the same in every thread of the cluster
-  auto exact_sums = [&](const T* t, float tm, const T* d, float dm) {
-    int a, z;
-    piece_of(c0, c1, warp, a, z);
-    Sums s{0.0, 0.0};
-    for (int v = a + lane; v < z; v += 32) {
-      s.t += exp(((double)to_f(t[v]) - (double)tm) * p.t_inv);
-      if (d) s.d += exp(((double)to_f(d[v]) - (double)dm) * p.d_inv);
-    }
+  // sums over the CTA, then over the cluster; the same in every thread
+  auto total = [&](Sums s) {
     s.t = warp_sum(s.t);
     s.d = warp_sum(s.d);
     if (lane == 0) {
@@ -307,6 +326,33 @@ __global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
       __syncthreads();
     }
     return s;
+  };
+  // a warp's ids [a, z) of two rows (y may be missing), 32 in step: f(x, y)
+  auto stream = [&](const T* x, const T* y, int a, int z, auto f) {
+    constexpr int U = 8;
+    for (int v0 = a + lane; v0 < z; v0 += 32 * U) {
+      float xs[U], ys[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int v = v0 + 32 * i;
+        xs[i] = v < z ? to_f(x[v]) : neg_inf();
+        ys[i] = y && v < z ? to_f(y[v]) : neg_inf();
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (v0 + 32 * i < z) f(v0 + 32 * i, xs[i], ys[i]);
+    }
+  };
+  // sums of e^((x - m) / T) over the whole row(s)
+  auto exact_sums = [&](const T* t, const Exp& te, const T* d, const Exp& de) {
+    int a, z;
+    part_of(c0, c1, PICK_WARPS, warp, a, z);
+    Sums s{0.0, 0.0};
+    stream(t, d, a, z, [&](int, float x, float y) {
+      s.t += term(x, te, powers);
+      if (d) s.d += term(y, de, powers);
+    });
+    return total(s);
   };
 
   // The drafts in turn, 32 at a time: lane l decides draft first + l.
@@ -380,11 +426,12 @@ __global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
       const int j = stop;
       const Part t = join(t_parts + (int64_t)j * p.runs, p.runs, p.t_scale);
       const Part d = p.draft ? join(d_parts + (int64_t)j * p.runs, p.runs, p.d_scale) : Part{0.0f, 0, 1.0};
-      const Sums s = exact_sums(t_row(j), t.m, p.draft ? d_row(j) : nullptr, d.m);
+      const Exp te = exp_of(t.m, p.t_inv), de = exp_of(d.m, p.d_inv);
+      const Sums s = exact_sums(t_row(j), te, p.draft ? d_row(j) : nullptr, de);
       const int64_t id = draft_id(p, b, j);
       uint32_t st = 0;
-      const double pt = exp(((double)to_f(t_row(j)[id]) - (double)t.m) * p.t_inv) / s.t;
-      const double qd = p.draft ? exp(((double)to_f(d_row(j)[id]) - (double)d.m) * p.d_inv) / s.d : 1.0;
+      const double pt = term(to_f(t_row(j)[id]), te, powers) / s.t;
+      const double qd = p.draft ? term(to_f(d_row(j)[id]), de, powers) / s.d : 1.0;
       if (uniform(j, st) * qd < pt) ++stop;
       else open = false;
     }
@@ -413,35 +460,67 @@ __global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
       }
     }
     const int hot = refused && !p.draft ? (int)drafted : -1;
-    const Sums s = exact_sums(x, t.m, y, dm);
+    const Exp te = exp_of(t.m, p.t_inv), de = exp_of(dm, p.d_inv);
+    int a, z;  // the thread's run of ids, where terms are kept
+    part_of(c0, c1, PICK, tid, a, z);
+    double et[KEPT], ed[KEPT];
+    Sums s;
+    if (kept) {
+      float xs[KEPT], ys[KEPT];
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i) {
+        xs[i] = a + i < z ? to_f(x[a + i]) : neg_inf();
+        ys[i] = y && a + i < z ? to_f(y[a + i]) : neg_inf();
+      }
+      s = Sums{0.0, 0.0};
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i) {
+        et[i] = term(xs[i], te, powers);
+        ed[i] = y ? term(ys[i], de, powers) : 0.0;
+        s.t += et[i];
+        s.d += ed[i];
+      }
+      s = total(s);
+    } else {
+      s = exact_sums(x, te, y, de);
+    }
     token_s = s.t;
     const double over_t = 1.0 / s.t, over_d = y ? 1.0 / s.d : 0.0;
     bool from_p = false;
-    auto weight = [&](int v) {
-      const double pt = exp(((double)to_f(x[v]) - (double)t.m) * p.t_inv) * over_t;
-      if (from_p) return pt;
-      if (y) return fmax(pt - exp(((double)to_f(y[v]) - (double)dm) * p.d_inv) * over_d, 0.0);
-      return v == hot ? 0.0 : pt;
+    auto weight = [&](int v, double e, double q) {  // of id v from its two terms
+      if (from_p) return e * over_t;
+      return v == hot ? 0.0 : fmax(fma(e, over_t, -(q * over_d)), 0.0);
     };
-    // the weight of [from, to) by pieces of a warp each, in sh.piece; the sum
-    auto weigh = [&](int from, int to) {
-      int a, z;
-      piece_of(from, to, warp, a, z);
+    // the CTA's weight by pieces of a warp each, in sh.piece; the sum over the cluster
+    auto weigh = [&]() {
       double w = 0.0;
-      for (int v = a + lane; v < z; v += 32) w += weight(v);
+      if (kept) {
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i) w += a + i < z ? weight(a + i, et[i], ed[i]) : 0.0;
+      } else {
+        int from, to;
+        part_of(c0, c1, PICK_WARPS, warp, from, to);
+        stream(x, y, from, to, [&](int v, float xv, float yv) { w += weight(v, term(xv, te, powers), y ? term(yv, de, powers) : 0.0); });
+      }
       w = warp_sum(w);
       __syncthreads();
       if (lane == 0) sh.piece[warp] = w;
       __syncthreads();
       w = 0.0;
       for (int k = 0; k < PICK_WARPS; ++k) w += sh.piece[k];
+      if (cs > 1) {
+        cluster.sync();  // an earlier weight has been read
+        if (tid == 0) sh.weight = w;
+        cluster.sync();
+        w = 0.0;
+        for (int k = 0; k < cs; ++k) w += cluster.map_shared_rank(&sh, k)->weight;
+      }
       return w;
     };
-    // first piece of n whose running sum passes u: its index, and the sum before it
-    auto choose = [&](auto piece, int n, double u, double& before) {
-      double run = before;
-      int last = -1;
-      double at = before;
+    // first piece of n whose running sum passes u (or the last that has any): its index, and the sum before it
+    auto choose = [](auto piece, int n, double u, double& before) {
+      double run = before, at = before;
+      int last = 0;
       for (int k = 0; k < n; ++k) {
         const double w = piece(k);
         if (w > 0.0) {
@@ -454,23 +533,10 @@ __global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
       before = at;
       return last;
     };
-    double mine = weigh(c0, c1), all = mine;
-    if (cs > 1) {
-      if (tid == 0) sh.weight = mine;
-      cluster.sync();
-      all = 0.0;
-      for (int k = 0; k < cs; ++k) all += cluster.map_shared_rank(&sh, k)->weight;
-    }
+    double all = weigh();
     if (!(all > 0.0)) {  // target and draft are the same: draw from the target
       from_p = true;
-      cluster_sync();
-      mine = all = weigh(c0, c1);
-      if (cs > 1) {
-        if (tid == 0) sh.weight = mine;
-        cluster.sync();
-        all = 0.0;
-        for (int k = 0; k < cs; ++k) all += cluster.map_shared_rank(&sh, k)->weight;
-      }
+      all = weigh();
     }
     const double u = uniform(K, status) * all;
     double before = 0.0;
@@ -478,42 +544,60 @@ __global__ void __launch_bounds__(PICK) pick_kernel(const Params p) {
     if (cs > 1) {
       owner = choose([&](int k) { return cluster.map_shared_rank(&sh, k)->weight; }, cs, u, before);
       cluster.sync();
+      if (rank != owner) return;
     }
-    if (rank == owner) {
-      int a, z;
-      int k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
-      piece_of(c0, c1, max(k, 0), a, z);
-      weigh(a, z);
-      k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
-      int from, to;
-      piece_of(a, z, max(k, 0), from, to);
-      if (warp == 0) {
-        int last = -1;
-        double run = before;
-        for (int v0 = from; v0 < to; v0 += 32) {
-          const int v = v0 + lane;
-          const double w = v < to ? weight(v) : 0.0;
-          double up = w;
+    // the piece that decides: a warp's, where terms are kept; else one that is weighed again by runs of a thread
+    int k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
+    double w[MOST], mine = 0.0;
+    if (kept) {
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double q = __shfl_up_sync(FULL, up, o);
-            if (lane >= o) up += q;
-          }
-          const unsigned past = __ballot_sync(FULL, w > 0.0 && run + up > u), some = __ballot_sync(FULL, w > 0.0);
-          if (past) {
-            last = v0 + __ffs(past) - 1;
-            break;
-          }
-          if (some) last = v0 + 31 - __clz(some);
-          run += __shfl_sync(FULL, up, 31);
-        }
-        if (lane == 0) sh.token = last;
-      }
-      __syncthreads();
-      token = sh.token;
+      for (int i = 0; i < MOST; ++i) w[i] = i < KEPT && a + i < z ? weight(a + i, et[i % KEPT], ed[i % KEPT]) : 0.0;
     } else {
-      return;
+      int from, to;
+      part_of(c0, c1, PICK_WARPS, k, from, to);
+      part_of(from, to, PICK, tid, a, z);
+      float xs[MOST], ys[MOST];
+#pragma unroll
+      for (int i = 0; i < MOST; ++i) {
+        xs[i] = a + i < z ? to_f(x[a + i]) : neg_inf();
+        ys[i] = y && a + i < z ? to_f(y[a + i]) : neg_inf();
+      }
+#pragma unroll
+      for (int i = 0; i < MOST; ++i) w[i] = a + i < z ? weight(a + i, term(xs[i], te, powers), y ? term(ys[i], de, powers) : 0.0) : 0.0;
     }
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) mine += w[i];
+    if (!kept) {
+      const double sum = warp_sum(mine);
+      __syncthreads();
+      if (lane == 0) sh.piece[warp] = sum;
+      __syncthreads();
+      k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
+    }
+    if (warp == k) {
+      double up = mine;  // running sums of the lanes
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double q = __shfl_up_sync(FULL, up, o);
+        if (lane >= o) up += q;
+      }
+      const unsigned past = __ballot_sync(FULL, mine > 0.0 && before + up > u), some = __ballot_sync(FULL, mine > 0.0);
+      const int who = past ? __ffs(past) - 1 : some ? 31 - __clz(some) : 0;
+      if (lane == who) {
+        double run = before + (up - mine);
+        int last = -1;
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+          run += w[i];
+          if (open && w[i] > 0.0) last = a + i;
+          if (run > u) open = false;
+        }
+        sh.token = last;
+      }
+    }
+    __syncthreads();
+    token = sh.token;
   }
   if (p.greedy || t_bad || t_none) {
     if (rank != 0) return;
