@@ -211,39 +211,59 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   }
 }
 
-constexpr int PICK = 512, PICK_WARPS = PICK / 32;
+// Threads of a CTA that draws: fewer, whose terms stay in registers, where a CTA has
+// few ids; else many, which hide the double operations' latency.
+constexpr int FEW = 512, MANY = 512;
 constexpr int KEPT = 8;  // ids of a thread whose terms stay in registers
-constexpr int MOST = 16; // ids of a thread in the last search: V / (16 warps) / 512 threads
+constexpr int NEAR = 64; // ids of a warp next to the border between p > q and p < q
+constexpr double NOTHING = 0x1p-900;  // a sum of ids without weight stays below it
 
 // e^((x - m) / T) in double, x <= m finite or -inf: with c = 64 log2(e) / T,
-// z = x c - m c = k + r, k whole and |r| <= 1/2, the value is 2^(k / 64) 2^(r / 64): a
+// z = (x - m) c = k + r, k whole and |r| <= 1/2, the value is 2^(k / 64) 2^(r / 64): a
 // table of 64 powers, an exponent, and the series of e^(r ln2 / 64) to r^4 (within
-// 4e-14).  Nine double operations, which bound the kernel (64 a clock and SM); the
-// library's exp has about twice as many.  Where z is at most -64000, 2^-1000, the value is 0.
+// 4e-14).  Ten double operations, which bound the kernel (64 a clock and SM); the
+// library's exp has about twice as many.  z is held to -64000, where the value is
+// 2^-1000 (one unsigned minimum of high words): far and masked ids then add next to
+// nothing to a sum of at least 1, and term_or_0 gives them nothing.
 struct Exp {
-  double c, mc;
+  double m, c;
 };
-__device__ __forceinline__ double term(float x, const Exp& e, const double* powers) {
+constexpr uint32_t FAR = 0xc0ef4000u;  // the high word of -64000.0
+__device__ __forceinline__ Exp exp_of(float m, double inv) { return Exp{(double)m, 64.0 * 1.4426950408889634074 * inv}; }
+__device__ __forceinline__ double term(float x, const Exp& e, const double* powers, bool& far) {
   constexpr double STEP = 0.69314718055994530942 / 64.0, MAGIC = 6755399441055744.0;  // 1.5 2^52
-  const double z = fma((double)x, e.c, -e.mc), y = z + MAGIC, r = z - (y - MAGIC);
+  const double d = ((double)x - e.m) * e.c;
+  far = (uint32_t)__double2hiint(d) >= FAR;
+  const double z = __hiloint2double((int)min((uint32_t)__double2hiint(d), FAR), __double2loint(d)), y = z + MAGIC, r = z - (y - MAGIC);
   const int k = __double2loint(y);
-  double v = fma(fma(fma(fma(STEP * STEP * STEP * STEP / 24.0, r, STEP * STEP * STEP / 6.0), r, STEP * STEP / 2.0), r, STEP), r, 1.0) *
-             powers[k & 63];
-  v = __hiloint2double(__double2hiint(v) + ((k >> 6) << 20), __double2loint(v));
-  return (uint32_t)__double2hiint(z) >= 0xc0ef4000u ? 0.0 : v;  // z <= -64000
+  const double v = fma(fma(fma(fma(STEP * STEP * STEP * STEP / 24.0, r, STEP * STEP * STEP / 6.0), r, STEP * STEP / 2.0), r, STEP), r, 1.0) *
+                   powers[k & 63];
+  return __hiloint2double(__double2hiint(v) + ((k >> 6) << 20), __double2loint(v));
+}
+__device__ __forceinline__ double term(float x, const Exp& e, const double* powers) {
+  bool far;
+  return term(x, e, powers, far);
+}
+__device__ __forceinline__ double term_or_0(float x, const Exp& e, const double* powers) {
+  bool far;
+  const double v = term(x, e, powers, far);
+  return far ? 0.0 : v;
 }
 
 struct Sums {
   double t, d;
+  double over;  // ids next to the border that a list had no room for
 };
 
+template <int PICK_WARPS>
 struct PickShared {
   double powers[64];
-  double warp_t[PICK_WARPS], warp_d[PICK_WARPS];
+  double warp_t[PICK_WARPS], warp_d[PICK_WARPS], warp_over[PICK_WARPS];
   Sums cta;                      // read by the cluster's other CTAs
   double weight;                 // likewise
   double piece[PICK_WARPS];
   int stop, unclear, token;
+  int32_t near[PICK_WARPS][NEAR];
 };
 
 // A row's parts joined; every lane the same.
@@ -259,9 +279,12 @@ __device__ __forceinline__ Part join(const Part* parts, int runs, float scale) {
   return r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
-  __shared__ PickShared sh;
+template <typename T, bool kept>
+__global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params p) {
+  constexpr int PICK = kept ? FEW : MANY, PICK_WARPS = PICK / 32;
+  constexpr int PIECE = (MTR_MAX_VOCAB + PICK_WARPS - 1) / PICK_WARPS;         // a warp's ids at most
+  constexpr int MOST = kept ? KEPT : (PIECE + PICK - 1) / PICK;               // and a thread's in the last search
+  __shared__ PickShared<PICK_WARPS> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = p.cluster, rank = cs > 1 ? (int)(blockIdx.x % cs) : 0;
@@ -287,11 +310,8 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
   if (tid < 64) sh.powers[tid] = exp2(tid / 64.0);
   __syncthreads();
   const double* powers = sh.powers;
-  constexpr double LOG2E_64 = 64.0 * 1.4426950408889634074;
-  auto exp_of = [&](float m, double inv) { return Exp{LOG2E_64 * inv, (double)m * (LOG2E_64 * inv)}; };
-  // this CTA's ids [c0, c1); `kept`: a thread has KEPT of them, one after another, at most
+  // this CTA's ids [c0, c1); kept: a thread has KEPT of them, one after another, at most
   const int share = (V + cs - 1) / cs, c0 = min(rank * share, V), c1 = min(c0 + share, V);
-  const bool kept = share <= PICK * KEPT;
   // part `k` of [from, to) cut into n
   auto part_of = [](int from, int to, int n, int k, int& a, int& z) {
     const int each = (to - from + n - 1) / n;
@@ -305,21 +325,24 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
     if (lane == 0) {
       sh.warp_t[warp] = s.t;
       sh.warp_d[warp] = s.d;
+      sh.warp_over[warp] = s.over;
     }
     __syncthreads();
-    s = Sums{0.0, 0.0};
+    s = Sums{0.0, 0.0, 0.0};
     for (int k = 0; k < PICK_WARPS; ++k) {
       s.t += sh.warp_t[k];
       s.d += sh.warp_d[k];
+      s.over += sh.warp_over[k];
     }
     if (cs > 1) {
       if (tid == 0) sh.cta = s;
       cluster.sync();
-      s = Sums{0.0, 0.0};
+      s = Sums{0.0, 0.0, 0.0};
       for (int k = 0; k < cs; ++k) {
         const Sums o = cluster.map_shared_rank(&sh, k)->cta;
         s.t += o.t;
         s.d += o.d;
+        s.over += o.over;
       }
       cluster.sync();  // read before it is written again
     } else {
@@ -327,31 +350,59 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
     }
     return s;
   };
-  // a warp's ids [a, z) of two rows (y may be missing), 32 in step: f(x, y)
+  // A warp's ids [a, z) of two rows (y may be missing): f(id, x, y);
+  // the warp is in step, ids behind the end are z and their values -inf.  Rows that lie
+  // alike about the 16-byte boundaries are read in vectors, the next ones under way
+  // while these are summed; else every value is its own access.
   auto stream = [&](const T* x, const T* y, int a, int z, auto f) {
-    constexpr int U = 8;
-    for (int v0 = a + lane; v0 < z; v0 += 32 * U) {
-      float xs[U], ys[U];
+    constexpr int E = Vec<T>::E;
+    auto singles = [&](int from, int to) {
+      constexpr int U = 8;
+      for (int v0 = from + lane; v0 - lane < to; v0 += 32 * U) {
+        float xs[U], ys[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int v = v0 + 32 * i;
-        xs[i] = v < z ? to_f(x[v]) : neg_inf();
-        ys[i] = y && v < z ? to_f(y[v]) : neg_inf();
+        for (int i = 0; i < U; ++i) {
+          const int v = v0 + 32 * i;
+          xs[i] = v < to ? to_f(x[v]) : neg_inf();
+          ys[i] = y && v < to ? to_f(y[v]) : neg_inf();
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) f(min(v0 + 32 * i, to), xs[i], ys[i]);
       }
+    };
+    if (y && (((uintptr_t)x ^ (uintptr_t)y) & 15u)) {
+      singles(a, z);
+      return;
+    }
+    const int off = (int)(((uintptr_t)(x + a) & 15u) / sizeof(T)), head = min(off ? E - off : 0, z - a), vecs = (z - a - head) / E;
+    const uint4 *xv = reinterpret_cast<const uint4*>(x + a + head), *yv = reinterpret_cast<const uint4*>(y + a + head);
+    const uint4 fill = make_uint4(Vec<T>::FILL, Vec<T>::FILL, Vec<T>::FILL, Vec<T>::FILL);
+    uint4 nx = lane < vecs ? xv[lane] : fill, ny = y && lane < vecs ? yv[lane] : fill;
+    singles(a, a + head);
+    singles(a + head + vecs * E, z);
+    for (int i = lane; i - lane < vecs; i += 32) {
+      float xs[E], ys[E];
+      Vec<T>::unpack(nx, xs);
+      Vec<T>::unpack(ny, ys);
+      nx = i + 32 < vecs ? xv[i + 32] : fill;
+      ny = y && i + 32 < vecs ? yv[i + 32] : fill;
+      const int v = i < vecs ? a + head + i * E : z;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v0 + 32 * i < z) f(v0 + 32 * i, xs[i], ys[i]);
+      for (int e = 0; e < E; ++e) f(v + e, xs[e], ys[e]);
     }
   };
   // sums of e^((x - m) / T) over the whole row(s)
   auto exact_sums = [&](const T* t, const Exp& te, const T* d, const Exp& de) {
     int a, z;
     part_of(c0, c1, PICK_WARPS, warp, a, z);
-    Sums s{0.0, 0.0};
-    stream(t, d, a, z, [&](int, float x, float y) {
-      s.t += term(x, te, powers);
-      if (d) s.d += term(y, de, powers);
-    });
+    Sums s{0.0, 0.0, 0.0};
+    if (d)
+      stream(t, d, a, z, [&](int, float x, float y) {
+        s.t += term(x, te, powers);
+        s.d += term(y, de, powers);
+      });
+    else
+      stream(t, d, a, z, [&](int, float x, float) { s.t += term(x, te, powers); });
     return total(s);
   };
 
@@ -430,8 +481,8 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
       const Sums s = exact_sums(t_row(j), te, p.draft ? d_row(j) : nullptr, de);
       const int64_t id = draft_id(p, b, j);
       uint32_t st = 0;
-      const double pt = term(to_f(t_row(j)[id]), te, powers) / s.t;
-      const double qd = p.draft ? term(to_f(d_row(j)[id]), de, powers) / s.d : 1.0;
+      const double pt = term_or_0(to_f(t_row(j)[id]), te, powers) / s.t;
+      const double qd = p.draft ? term_or_0(to_f(d_row(j)[id]), de, powers) / s.d : 1.0;
       if (uniform(j, st) * qd < pt) ++stop;
       else open = false;
     }
@@ -463,27 +514,69 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
     const Exp te = exp_of(t.m, p.t_inv), de = exp_of(dm, p.d_inv);
     int a, z;  // the thread's run of ids, where terms are kept
     part_of(c0, c1, PICK, tid, a, z);
-    double et[KEPT], ed[KEPT];
+    int from = 0, to = 0;  // or the warp's piece
+    double et[KEPT], ed[KEPT], above_t = 0.0, above_d = 0.0;
+    int listed = 0;
     Sums s;
-    if (kept) {
+    if constexpr (kept) {
       float xs[KEPT], ys[KEPT];
 #pragma unroll
       for (int i = 0; i < KEPT; ++i) {
         xs[i] = a + i < z ? to_f(x[a + i]) : neg_inf();
         ys[i] = y && a + i < z ? to_f(y[a + i]) : neg_inf();
       }
-      s = Sums{0.0, 0.0};
+      s = Sums{0.0, 0.0, 0.0};
 #pragma unroll
       for (int i = 0; i < KEPT; ++i) {
-        et[i] = term(xs[i], te, powers);
-        ed[i] = y ? term(ys[i], de, powers) : 0.0;
+        et[i] = term_or_0(xs[i], te, powers);
+        ed[i] = y ? term_or_0(ys[i], de, powers) : 0.0;
         s.t += et[i];
         s.d += ed[i];
       }
       s = total(s);
     } else {
-      s = exact_sums(x, te, y, de);
+      // One pass: the sums, and of the warp's piece those of the ids whose p is above
+      // q.  Which they are is clear from the fp32 sums but for ids with |p - q| <
+      // 2^-12 p or so, which are listed and looked at when the sums are known.
+      part_of(c0, c1, PICK_WARPS, warp, from, to);
+      s = Sums{0.0, 0.0, 0.0};
+      if (y) {
+        const Part d = join(d_parts + (int64_t)stop * p.runs, p.runs, p.d_scale);
+        const double ratio = t.s / d.s;
+        stream(x, y, from, to, [&](int v, float xv, float yv) {
+          const double e = term(xv, te, powers), q = term(yv, de, powers), over = fma(-q, ratio, e);
+          s.t += e;
+          s.d += q;
+          // |over| against 2^-12 of the larger term, by exponents: within a factor of two
+          const int high = __double2hiint(over), size = max(__double2hiint(e), __double2hiint(q * ratio));
+          const bool close = (high & 0x7fffffff) + (12 << 20) < size && size > (40 << 20);  // not both far
+          if (high >= 0 && !close) {
+            above_t += e;
+            above_d += q;
+          }
+          const unsigned some = __ballot_sync(FULL, close && v < to);
+          if (some) {
+            const int at = listed + __popc(some & ((1u << lane) - 1u));
+            if (close && v < to && at < NEAR) sh.near[warp][at] = v;
+            listed += __popc(some);
+          }
+        });
+        if (listed > NEAR) s.over = 1.0;
+        __syncwarp();
+      } else {
+        auto add = [&](int, float xv, float) { above_t += term(xv, te, powers); };
+        if (hot >= from && hot < to) {  // the drafted token has no part in the draw
+          stream(x, nullptr, from, hot, add);
+          stream(x, nullptr, hot + 1, to, add);
+          if (lane == 0) s.t = term(to_f(x[hot]), te, powers);
+        } else {
+          stream(x, nullptr, from, to, add);
+        }
+        s.t += above_t;
+      }
+      s = total(s);
     }
+    const bool summed = s.over == 0.0;  // the pieces' sums are complete
     token_s = s.t;
     const double over_t = 1.0 / s.t, over_d = y ? 1.0 / s.d : 0.0;
     bool from_p = false;
@@ -494,13 +587,31 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
     // the CTA's weight by pieces of a warp each, in sh.piece; the sum over the cluster
     auto weigh = [&]() {
       double w = 0.0;
-      if (kept) {
+      if constexpr (kept) {
 #pragma unroll
         for (int i = 0; i < KEPT; ++i) w += a + i < z ? weight(a + i, et[i], ed[i]) : 0.0;
+      } else if (summed && !from_p) {
+        w = above_t * over_t - above_d * over_d;
+        for (int i = lane; i < listed; i += 32) {
+          const int v = sh.near[warp][i];
+          w += weight(v, term(to_f(x[v]), te, powers), term(to_f(y[v]), de, powers));
+        }
       } else {
-        int from, to;
-        part_of(c0, c1, PICK_WARPS, warp, from, to);
-        stream(x, y, from, to, [&](int v, float xv, float yv) { w += weight(v, term(xv, te, powers), y ? term(yv, de, powers) : 0.0); });
+        if (y && !from_p) {
+          stream(x, y, from, to, [&](int, float xv, float yv) {
+            const double one = fma(term(xv, te, powers), over_t, -(term(yv, de, powers) * over_d));
+            if (__double2hiint(one) >= 0) w += one;
+          });
+        } else {
+          auto add = [&](int, float xv, float) { w += term(xv, te, powers); };
+          if (!from_p && hot >= from && hot < to) {  // the drafted token has no part
+            stream(x, nullptr, from, hot, add);
+            stream(x, nullptr, hot + 1, to, add);
+          } else {
+            stream(x, nullptr, from, to, add);
+          }
+          w *= over_t;
+        }
       }
       w = warp_sum(w);
       __syncthreads();
@@ -523,7 +634,7 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
       int last = 0;
       for (int k = 0; k < n; ++k) {
         const double w = piece(k);
-        if (w > 0.0) {
+        if (w > NOTHING) {
           last = k;
           at = run;
         }
@@ -534,7 +645,7 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
       return last;
     };
     double all = weigh();
-    if (!(all > 0.0)) {  // target and draft are the same: draw from the target
+    if (!(all > NOTHING)) {  // target and draft are the same: draw from the target
       from_p = true;
       all = weigh();
     }
@@ -549,11 +660,10 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
     // the piece that decides: a warp's, where terms are kept; else one that is weighed again by runs of a thread
     int k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
     double w[MOST], mine = 0.0;
-    if (kept) {
+    if constexpr (kept) {
 #pragma unroll
-      for (int i = 0; i < MOST; ++i) w[i] = i < KEPT && a + i < z ? weight(a + i, et[i % KEPT], ed[i % KEPT]) : 0.0;
+      for (int i = 0; i < MOST; ++i) w[i] = a + i < z ? weight(a + i, et[i % KEPT], ed[i % KEPT]) : 0.0;
     } else {
-      int from, to;
       part_of(c0, c1, PICK_WARPS, k, from, to);
       part_of(from, to, PICK, tid, a, z);
       float xs[MOST], ys[MOST];
@@ -563,11 +673,11 @@ __global__ void __launch_bounds__(PICK, 1) pick_kernel(const Params p) {
         ys[i] = y && a + i < z ? to_f(y[a + i]) : neg_inf();
       }
 #pragma unroll
-      for (int i = 0; i < MOST; ++i) w[i] = a + i < z ? weight(a + i, term(xs[i], te, powers), y ? term(ys[i], de, powers) : 0.0) : 0.0;
+      for (int i = 0; i < MOST; ++i) w[i] = a + i < z ? weight(a + i, term_or_0(xs[i], te, powers), y ? term_or_0(ys[i], de, powers) : 0.0) : 0.0;
     }
 #pragma unroll
     for (int i = 0; i < MOST; ++i) mine += w[i];
-    if (!kept) {
+    if constexpr (!kept) {
       const double sum = warp_sum(mine);
       __syncthreads();
       if (lane == 0) sh.piece[warp] = sum;
@@ -670,9 +780,11 @@ static cudaError_t launch_all(Params p, int64_t rows, cudaStream_t s) {
     e = p.greedy ? launch(rows_kernel<T, 256, true>, p, grid, 256, 1, s) : launch(rows_kernel<T, 256, false>, p, grid, 256, 1, s);
   if (e != cudaSuccess) return e;
   int cluster = 1;
-  while (!p.greedy && cluster < 8 && p.batch * cluster * 2 <= device_sms() && p.vocab >= 4096 * cluster) cluster *= 2;
+  while (!p.greedy && cluster < 8 && p.batch * cluster * 2 <= device_sms() && p.vocab > FEW * KEPT * cluster) cluster *= 2;
   p.cluster = cluster;
-  return launch(pick_kernel<T>, p, dim3((unsigned)(p.batch * cluster), 1, 1), PICK, cluster, s);
+  const dim3 ctas((unsigned)(p.batch * cluster), 1, 1);
+  if (p.greedy || (p.vocab + cluster - 1) / cluster <= FEW * KEPT) return launch(pick_kernel<T, true>, p, ctas, FEW, cluster, s);
+  return launch(pick_kernel<T, false>, p, ctas, MANY, cluster, s);
 }
 
 }  // namespace vf
