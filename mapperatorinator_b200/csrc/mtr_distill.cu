@@ -38,6 +38,7 @@ struct Params {
   int32_t vocab;
   int32_t n;
   int32_t tail;
+  int32_t cluster; // CTAs of a row
   int32_t alike;  // logits and gradient rows lie alike about the 16-byte boundaries
   float scale;    // log2(e) / T
   double inv_t;
@@ -85,42 +86,52 @@ __device__ __forceinline__ void drop(uint4& w, uint32_t bits, T) {
   half(w.w, bits >> 6);
 }
 
-constexpr int HOLD = 4;      // vectors a thread keeps
+constexpr int MOST_THREADS = 512;  // whose CTAs may share a row
 
 template <int WARPS>
 struct Shared {
   float m[WARPS];    // a warp's largest logit outside S
   double s[WARPS];   // and its sum about it; NaN: a NaN or +inf
   float row_m, row_c;
+  float cta_m;       // read by the cluster's other CTAs
+  double cta_s;
   int dup;
   int32_t id[MTR_MAX_TEACHER_IDS];
   double p[MTR_MAX_TEACHER_IDS];
 };
 
-// SLOTS: entries a lane of the first warp has (1 or 4)
-template <typename T, int THREADS, int SLOTS, bool SCAN, bool GRAD>
-__global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
+// HOLD: vectors a thread keeps; CTAS: CTAs of an SM; SLOTS: entries a lane of the
+// first warp has (1 or 4)
+template <typename T, int THREADS, int HOLD, int CTAS, int SLOTS, bool SCAN, bool GRAD>
+__global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const Params p) {
   typedef Vec<T> X;
   constexpr int E = X::E, WARPS = THREADS / 32;
   extern __shared__ __align__(16) uint32_t bits[];  // bit 8 + id - head
   __shared__ Shared<WARPS> sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int V = p.vocab;
-  const int64_t row = blockIdx.x;
+  const int cs = THREADS == MOST_THREADS ? p.cluster : 1, rank = cs > 1 ? (int)(blockIdx.x % cs) : 0;
+  const int64_t row = cs > 1 ? blockIdx.x / cs : blockIdx.x;
+  cg::cluster_group cluster = cg::this_cluster();
+  auto sync = [] {
+    if constexpr (THREADS > 32) __syncthreads();
+    else __syncwarp();
+  };
   wait_prior_grid();
 
   const T* x = (const T*)p.logits + row * p.stride;
   const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
   const int head = min(off ? E - off : 0, V), vecs = (V - head) / E, behind = V - head - vecs * E;
   const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  // the CTA's vectors [v0, v1); the first one has the single logits before the first 16-byte boundary and behind the last too
+  const int run = cs > 1 ? (vecs + cs - 1) / cs : vecs, v0 = min(rank * run, vecs), v1 = min(v0 + run, vecs);
   uint4 w[HOLD];
 #pragma unroll
   for (int j = 0; j < HOLD; ++j) {
-    const int i = tid + j * THREADS;
-    w[j] = i < vecs ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+    const int i = v0 + tid + j * THREADS;
+    w[j] = i < v1 ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
   }
-  // single logits before the first 16-byte boundary and behind the last
-  const int single = tid < head ? tid : tid >= 32 && tid < 32 + behind ? V - behind + tid - 32 : -1;
+  const int single = rank > 0 ? -1 : tid < head ? tid : tid >= 16 && tid < 16 + behind ? V - behind + tid - 16 : -1;
   float one = single >= 0 ? to_f(x[single]) : neg_inf();
 
   // the teacher's entries, of the first warp: entry lane + 32 k
@@ -148,7 +159,7 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
   }
   for (int i = tid; i < (V + 8 + 31) / 32; i += THREADS) bits[i] = 0u;
   if (tid == 0) sh.dup = 0;
-  __syncthreads();
+  sync();
   bool lead[SLOTS];  // the first of equal ids
   if (warp == 0) {
 #pragma unroll
@@ -161,20 +172,23 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
       }
     }
   }
-  __syncthreads();
+  sync();
 
   auto listed = [&](int i) {  // which values of vector i are of S
     if constexpr (E == 8) return (uint32_t) reinterpret_cast<const uint8_t*>(bits)[i + 1];
     else return ((uint32_t) reinterpret_cast<const uint8_t*>(bits)[(i + 2) >> 1] >> ((i & 1) * 4)) & 15u;
   };
+  // the ids of S leave the vectors i0, i0 + THREADS, ...: few batches have any
+  auto leave = [&](uint4 (&v)[HOLD], int i0) {
+    uint32_t b[HOLD], any = 0;
 #pragma unroll
-  for (int j = 0; j < HOLD; ++j) {
-    const int i = tid + j * THREADS;
-    if (i < vecs) {
-      const uint32_t b = listed(i);
-      if (b) drop(w[j], b, T());
+    for (int j = 0; j < HOLD; ++j) any |= b[j] = i0 + j * THREADS < v1 ? listed(i0 + j * THREADS) : 0u;
+    if (any) {
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j) drop(v[j], b[j], T());
     }
-  }
+  };
+  leave(w, v0 + tid);
   if (single >= 0) {
     const int b = 8 + single - head;
     if (bits[b >> 5] >> (b & 31) & 1u) one = neg_inf();
@@ -216,19 +230,14 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
       s += (double)lo + (double)hi;
     };
     take(w);
-    for (int i0 = tid + HOLD * THREADS; i0 < vecs; i0 += HOLD * THREADS) {
+    for (int i0 = v0 + tid + HOLD * THREADS; i0 < v1; i0 += HOLD * THREADS) {
       uint4 v[HOLD];
 #pragma unroll
       for (int j = 0; j < HOLD; ++j) {
         const int i = i0 + j * THREADS;
-        v[j] = i < vecs ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
+        v[j] = i < v1 ? body[i] : make_uint4(X::FILL, X::FILL, X::FILL, X::FILL);
       }
-#pragma unroll
-      for (int j = 0; j < HOLD; ++j) {
-        const int i = i0 + j * THREADS;
-        const uint32_t b = i < vecs ? listed(i) : 0u;
-        if (b) drop(v[j], b, T());
-      }
+      leave(v, i0);
       take(v);
     }
     if (single >= 0) {
@@ -245,119 +254,143 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
     }
   }
 
-  // the teacher's numbers, by the first warp
-  double pj[SLOTS], mass = 0.0, log_mass = 0.0, rest = 0.0;
-  bool empty = false, odd = false;
+  // What needs no sum, by the first warp: the teacher's probabilities, and the terms
+  // of S about its largest logit x_s.
+  constexpr double NAN_D = 0.0 / 0.0;
+  double pj[SLOTS], ej[SLOTS], mass = 0.0, rest = 0.0, in = 0.0, cross = 0.0;
+  float x_s = neg_inf();
+  bool empty = false, odd = false, bad_s = false;
   if (warp == 0) {
     bool any = false;
     float lp_top = neg_inf();
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
-      if (32 * k >= p.n) break;
       any |= id[k] >= 0;
-      if (id[k] >= 0 && !(lp[k] < pos_inf())) odd = true;
+      if (id[k] >= 0) {
+        odd |= !(lp[k] < pos_inf());
+        bad_s |= !(xs[k] < pos_inf());
+      }
       lp_top = fmaxf(lp_top, lp[k]);
+      x_s = fmaxf(x_s, xs[k]);
     }
     any = __any_sync(FULL, any);
     odd = __any_sync(FULL, odd);
+    bad_s = __any_sync(FULL, bad_s);
     lp_top = warp_max(lp_top);
+    x_s = warp_max(x_s);
     empty = !any || (!p.tail && lp_top == neg_inf() && !odd);
-    const double shift = p.tail || odd || empty ? 0.0 : (double)lp_top;
+    const double shift = p.tail || odd || empty ? 0.0 : (double)lp_top, about = x_s > neg_inf() && !bad_s ? (double)x_s : 0.0;
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
-      pj[k] = 0.0;
-      if (32 * k < p.n) {
-        if (id[k] >= 0) pj[k] = exp((double)lp[k] - shift);
-        mass += pj[k];
+      pj[k] = ej[k] = 0.0;
+      if (id[k] >= 0) {
+        pj[k] = exp((double)lp[k] - shift);
+        ej[k] = exp(((double)xs[k] - about) * p.inv_t);
+        if (lead[k]) in += ej[k];
       }
+      mass += pj[k];
     }
     mass = warp_sum(mass);
+    in = warp_sum(in);
+    double log_mass = 0.0;
     if (p.tail) {
       rest = 1.0 - mass;
       if (rest < LEAST_REST) rest = 0.0;
     } else if (!empty) {
       log_mass = shift + log(mass);
+      const double over = 1.0 / mass;
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (32 * k < p.n) pj[k] /= mass;
+      for (int k = 0; k < SLOTS; ++k) pj[k] *= over;
       mass = 1.0;
     }
+    if (SCAN && p.loss) {
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (pj[k] > 0.0) cross += pj[k] * (((double)lp[k] - log_mass) - ((double)xs[k] - about) * p.inv_t);
+      cross = warp_sum(cross);
+    }
   }
-  __syncthreads();
+  sync();
+
+  // the warps' sums joined, then the CTAs'
+  float m_all = neg_inf();
+  double s_all = 0.0;
+  auto join = [&](float m, double s) {  // of the lanes
+    m_all = warp_max(m);
+    if (m > neg_inf()) s *= (double)ex2((m - m_all) * p.scale);
+    s_all = warp_sum(s);
+  };
+  if constexpr (SCAN) {
+    if (WARPS == 1) {
+      m_all = sh.m[0];
+      s_all = sh.s[0];
+    } else if (warp == 0) {
+      join(lane < WARPS ? sh.m[lane] : neg_inf(), lane < WARPS ? sh.s[lane] : 0.0);
+    }
+    if (cs > 1) {
+      if (tid == 0) {
+        sh.cta_m = m_all;
+        sh.cta_s = s_all;
+      }
+      cluster.sync();
+      if (warp == 0) {
+        const Shared<WARPS>* other = cluster.map_shared_rank(&sh, lane % cs);
+        join(lane < cs ? other->cta_m : neg_inf(), lane < cs ? other->cta_s : 0.0);
+      }
+      cluster.sync();  // this CTA's have been read
+    }
+  }
 
   // the row's
-  double ej[SLOTS], q_scale = 0.0, own_scale = 0.0;
+  double q_scale = 0.0, own_scale = 0.0;
   if (warp == 0) {
-    const double nan = __longlong_as_double(0x7ff8000000000000LL);
     double sum_rest;
     float m_rest;
     if constexpr (SCAN) {
-      m_rest = warp_max(lane < WARPS ? sh.m[lane] : neg_inf());
-      double part = lane < WARPS ? sh.s[lane] : 0.0;
-      if (lane < WARPS && sh.m[lane] > neg_inf()) part *= (double)ex2((sh.m[lane] - m_rest) * p.scale);
-      sum_rest = warp_sum(part);
+      m_rest = m_all;
+      sum_rest = s_all;
     } else {
       const double2 st = p.stats[row];
       m_rest = (float)st.x;
       sum_rest = st.y;
     }
-    bool bad = !(sum_rest < (double)pos_inf());
-    float x_top = m_rest;
-#pragma unroll
-    for (int k = 0; k < SLOTS; ++k)
-      if (32 * k < p.n && id[k] >= 0) {
-        if (!(xs[k] < pos_inf())) bad = true;
-        x_top = fmaxf(x_top, xs[k]);
-      }
-    bad = __any_sync(FULL, bad);
-    x_top = warp_max(x_top);
-    const bool none = !bad && !(x_top > neg_inf());
-    const double top = none ? 0.0 : (double)x_top;
-    const double rest_part = m_rest > neg_inf() ? sum_rest * exp(((double)m_rest - top) * p.inv_t) : 0.0;
-    double in = 0.0;
-#pragma unroll
-    for (int k = 0; k < SLOTS; ++k) {
-      ej[k] = 0.0;
-      if (32 * k < p.n && id[k] >= 0) {
-        ej[k] = exp(((double)xs[k] - top) * p.inv_t);
-        if (lead[k]) in += ej[k];
-      }
-    }
-    in = warp_sum(in);
-    const double all = in + rest_part;
-    if (SCAN && p.loss) {
-      const double log_all = none ? 0.0 : log(all);
-      double loss = 0.0;
-#pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (32 * k < p.n && pj[k] > 0.0) loss += pj[k] * (((double)lp[k] - log_mass) - ((double)xs[k] - top) * p.inv_t + log_all);
-      loss = warp_sum(loss);
-      if (lane == 0) {
-        if (rest > 0.0)
-          loss += m_rest > neg_inf() ? rest * (log(rest) - (log(sum_rest) + ((double)m_rest - top) * p.inv_t - log_all)) : (double)pos_inf();
-        p.loss[row] = empty ? 0.0f : bad || odd ? (float)nan : (float)loss;
-      }
-    }
-    if (SCAN && lane == 0 && p.stats) p.stats[row] = make_double2((double)m_rest, sum_rest);
-    if (SCAN && p.status) {
-      wrong = __any_sync(FULL, wrong);
-      uint32_t st = wrong ? MTR_ROW_BAD_ID : 0u;
-      if (!empty) st |= bad || odd ? MTR_ROW_NONFINITE : none ? MTR_ROW_ALL_MASKED : 0u;
-      if (lane == 0) p.status[row] = st;
-    }
+    const bool bad = bad_s || !(sum_rest < (double)pos_inf());
+    const bool some = m_rest > neg_inf(), none = !bad && !some && !(x_s > neg_inf());
+    // both sums about the larger of m_rest and x_s
+    const double apart = some && x_s > neg_inf() ? ((double)m_rest - (double)x_s) * p.inv_t : 0.0, shrink = exp(-fabs(apart));
+    const double in_part = apart > 0.0 ? in * shrink : in, rest_part = some ? (apart < 0.0 ? sum_rest * shrink : sum_rest) : 0.0;
+    const double all = in_part + rest_part, over_all = 1.0 / all;
     if constexpr (GRAD) {
       const double g = (p.g_loss ? (double)p.g_loss[row] : 1.0) * p.inv_t;
       // e = 2^((x - m_rest) scale): q = e rest_part / (sum_rest all), q / q_t = e / sum_rest
       double c = 0.0;
-      if (!empty && !none && m_rest > neg_inf()) c = g * (mass * (rest_part / all) - rest * (in / all)) / sum_rest;
-      if (!empty && (bad || odd)) c = nan;
-      q_scale = empty || none ? 0.0 : g * (mass + rest) / all;
+      if (!empty && !none && some) c = g * (mass * (rest_part * over_all) - rest * (in_part * over_all)) / sum_rest;
+      if (!empty && (bad || odd)) c = NAN_D;
+      q_scale = empty || none ? 0.0 : g * (mass + rest) * over_all * (apart > 0.0 ? shrink : 1.0);
       own_scale = empty || none ? 0.0 : g;
-      if (bad || odd) q_scale = empty ? 0.0 : nan;
+      if (bad || odd) q_scale = empty ? 0.0 : NAN_D;
       if (lane == 0) {
-        sh.row_m = m_rest > neg_inf() && !empty && !bad ? m_rest : 0.0f;
+        sh.row_m = some && !empty && !bad ? m_rest : 0.0f;
         sh.row_c = (float)c;
       }
+    }
+    if constexpr (GRAD && THREADS > 32) sync();  // the others go on with the gradient
+    if (SCAN && p.loss && lane == 0 && rank == 0) {
+      // log sum about x_s: log q_j = (x_j - x_s) / T - log_s
+      const double log_s = none ? 0.0 : log(all) + (apart > 0.0 ? apart : 0.0);
+      double loss = cross + mass * log_s;
+      if (!(x_s > neg_inf()) && mass > 0.0) loss = (double)pos_inf();
+      if (rest > 0.0) loss += some ? rest * (log(rest) - (log(sum_rest) - log(all) + fmin(apart, 0.0))) : (double)pos_inf();
+      p.loss[row] = empty ? 0.0f : bad || odd ? (float)NAN_D : (float)loss;
+    }
+    if (SCAN && lane == 0 && rank == 0 && p.stats) p.stats[row] = make_double2((double)m_rest, sum_rest);
+    if (SCAN && p.status) {
+      wrong = __any_sync(FULL, wrong);
+      uint32_t st = wrong ? MTR_ROW_BAD_ID : 0u;
+      if (!empty) st |= bad || odd ? MTR_ROW_NONFINITE : none ? MTR_ROW_ALL_MASKED : 0u;
+      if (lane == 0 && rank == 0) p.status[row] = st;
+    }
+    if constexpr (GRAD) {
       if (sh.dup) {  // equal ids: the leading one gets all of their probability
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
@@ -377,15 +410,25 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
             pj[k] = sum;
           }
       }
+      __syncwarp();
     }
+  } else if constexpr (GRAD) {
+    sync();
   }
   if constexpr (!GRAD) return;
-  __syncthreads();
   const float rm = sh.row_m, rc = sh.row_c;
   T* g = (T*)p.grad + row * p.grad_stride;
   const u64 nm2 = pk2(-rm, -rm), sc2 = pk2(p.scale, p.scale), c2 = pk2(rc, rc);
   // a row of gradient 0 may hold NaN, which has no gradient then
   const bool zero = rc == 0.0f;
+  auto store = [&](int i, const uint4& packed, const float (&f)[E]) {
+    if (p.alike) {
+      reinterpret_cast<uint4*>(g + head)[i] = packed;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) g[head + i * E + e] = from_f<T>(f[e]);
+    }
+  };
   auto put = [&](int i, const uint4& v) {
     float f[E];
     X::unpack(v, f);
@@ -394,58 +437,84 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const Params p) {
       float d0, d1;
       up2(mul2(add2(pk2(f[e], f[e + 1]), nm2), sc2), d0, d1);
       up2(mul2(pk2(ex2(d0), ex2(d1)), c2), f[e], f[e + 1]);
-      if (zero) f[e] = f[e + 1] = 0.0f;
     }
-    if (p.alike) {
-      reinterpret_cast<uint4*>(g + head)[i] = pack<T>(f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) g[head + i * E + e] = from_f<T>(f[e]);
-    }
+    store(i, pack<T>(f), f);
   };
+  if (zero) {
+    const float f[E] = {};
+    for (int i = v0 + tid; i < v1; i += THREADS) store(i, make_uint4(0u, 0u, 0u, 0u), f);
+  } else {
 #pragma unroll
-  for (int j = 0; j < HOLD; ++j)
-    if (tid + j * THREADS < vecs) put(tid + j * THREADS, w[j]);
-  for (int i = tid + HOLD * THREADS; i < vecs; i += THREADS) put(i, body[i]);
+    for (int j = 0; j < HOLD; ++j)
+      if (v0 + tid + j * THREADS < v1) put(v0 + tid + j * THREADS, w[j]);
+    for (int i0 = v0 + tid + HOLD * THREADS; i0 < v1; i0 += HOLD * THREADS) {
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j)
+        if (i0 + j * THREADS < v1) w[j] = body[i0 + j * THREADS];
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j)
+        if (i0 + j * THREADS < v1) put(i0 + j * THREADS, w[j]);
+    }
+  }
   if (single >= 0) g[single] = from_f<T>(zero ? 0.0f : ex2((one - rm) * p.scale) * rc);
-  __syncthreads();  // the entries of S are written over
+  sync();  // the entries of S are written over, by the CTA that wrote there
+  const int from = rank == 0 ? 0 : head + v0 * E, to = head + v1 * E, last = rank == 0 ? V - behind : V;
   if (warp == 0) {
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
-      if (32 * k < p.n && id[k] >= 0 && lead[k]) g[id[k]] = from_f<T>((float)(ej[k] * q_scale - pj[k] * own_scale));
+      if (lead[k] && ((id[k] >= from && id[k] < to) || id[k] >= last)) g[id[k]] = from_f<T>((float)(ej[k] * q_scale - pj[k] * own_scale));
   }
 }
 
 static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
 
-template <typename T, int THREADS, int SLOTS>
+// vectors of a thread in registers: more warps pay more than longer runs (8192 x 4096 bf16: 16 vectors 51.1 us, 4 35.1)
+constexpr int HELD = 4;
+template <typename T, int THREADS, int CTAS, int SLOTS>
 static cudaError_t launch_of(const Params& p, int64_t rows, bool scan, cudaStream_t s) {
   const int dyn = (p.vocab + 8 + 31) / 32 * 4;  // at most 16.4 KB
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)rows, 1, 1);
+  cfg.gridDim = dim3((unsigned)(rows * p.cluster), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = (size_t)dyn;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
-  cfg.numAttrs = launch_attrs(attr, 1, true);
+  cfg.numAttrs = launch_attrs(attr, p.cluster, true);
   cfg.attrs = attr;
-  if (!p.grad) return cudaLaunchKernelEx(&cfg, distill_kernel<T, THREADS, SLOTS, true, false>, p);
-  return scan ? cudaLaunchKernelEx(&cfg, distill_kernel<T, THREADS, SLOTS, true, true>, p)
-              : cudaLaunchKernelEx(&cfg, distill_kernel<T, THREADS, SLOTS, false, true>, p);
+  if (!p.grad) return cudaLaunchKernelEx(&cfg, distill_kernel<T, THREADS, HELD, CTAS, SLOTS, true, false>, p);
+  return scan ? cudaLaunchKernelEx(&cfg, distill_kernel<T, THREADS, HELD, CTAS, SLOTS, true, true>, p)
+              : cudaLaunchKernelEx(&cfg, distill_kernel<T, THREADS, HELD, CTAS, SLOTS, false, true>, p);
+}
+template <typename T, int THREADS, int CTAS>
+static cudaError_t launch(const Params& p, int64_t rows, bool scan, cudaStream_t s) {
+  return p.n <= 32 ? launch_of<T, THREADS, CTAS, 1>(p, rows, scan, s) : launch_of<T, THREADS, CTAS, MTR_MAX_TEACHER_IDS / 32>(p, rows, scan, s);
 }
 
-template <typename T, int THREADS>
-static cudaError_t launch(const Params& p, int64_t rows, bool scan, cudaStream_t s) {
-  return p.n <= 32 ? launch_of<T, THREADS, 1>(p, rows, scan, s) : launch_of<T, THREADS, MTR_MAX_TEACHER_IDS / 32>(p, rows, scan, s);
-}
+// Threads of a row, by how many rows there are to fill the device's 16 warps an SM
+// and how long they are; CTAs share a row only where they give idle SMs work.
+// Loss and gradient together, with 20 ids (us, 32 / 128 / 256 threads, 148 SMs):
+//   8192 x 1000 bf16    17.3 / 44.8 / 73.3     enough rows: a warp each
+//   8192 x 4096 bf16    35.1 /      /
+//   3000 x 4096 fp32    23.8 / 25.4 / 34.0
+//   1000 x 4096 bf16    10.8 /  8.6 / 13.6     few rows: more warps each
+//   2000 x 16384 bf16   44.3 / 33.1 / 39.8     long rows: 128 threads, then 256
+//   300 x 16384 fp32    38.7 / 15.7 / 12.5
+//   2000 x 65533 bf16               / 125.6, 512 threads 123.8
 template <typename T>
-static cudaError_t launch(const Params& p, int64_t rows, bool scan, cudaStream_t s) {
-  const int64_t vecs = (int64_t)p.vocab * (int)sizeof(T) / 16;
-  if (vecs <= 64 * HOLD) return launch<T, 64>(p, rows, scan, s);
-  if (vecs <= 128 * HOLD) return launch<T, 128>(p, rows, scan, s);
-  if (vecs <= 256 * HOLD) return launch<T, 256>(p, rows, scan, s);
-  return launch<T, 512>(p, rows, scan, s);
+static cudaError_t launch(Params p, int64_t rows, bool scan, cudaStream_t s) {
+  const int64_t vecs = (int64_t)p.vocab * (int)sizeof(T) / 16, sms = device_sms();
+  int threads = vecs > 4096 ? 256 : vecs > 1024 ? 128 : 32;
+  while (threads < MOST_THREADS && rows * threads < 16 * 32 * sms && vecs >= 8 * threads) threads *= threads == 32 ? 4 : 2;
+  p.cluster = 1;
+  while (threads == MOST_THREADS && p.cluster < 8 && scan && vecs >= 2ll * HELD * MOST_THREADS * p.cluster && rows * p.cluster * 2 <= sms)
+    p.cluster *= 2;
+  switch (threads) {
+    case 32: return launch<T, 32, 28>(p, rows, scan, s);
+    case 128: return launch<T, 128, 7>(p, rows, scan, s);
+    case 256: return launch<T, 256, 4>(p, rows, scan, s);
+    default: return launch<T, 512, 2>(p, rows, scan, s);
+  }
 }
 
 }  // namespace ds
