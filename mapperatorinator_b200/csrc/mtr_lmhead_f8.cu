@@ -47,9 +47,9 @@ __device__ __forceinline__ void store4(uint8_t* q, int c, int cols, uint32_t w) 
 }
 
 // A row's blocks of 128, a warp for UNITS of them: four values a lane and block.
-// HBM bounds it: 3 bytes a bf16 value.
-constexpr int UNITS = 8;
-template <typename T, bool VEC>
+// HBM bounds it: 3 bytes a bf16 value.  Fewer units where rows are few, so that there
+// are warps for all SMs.
+template <typename T, bool VEC, int UNITS>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const QuantParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int blocks = (p.cols + BLOCK - 1) / BLOCK, runs = (blocks + UNITS - 1) / UNITS;
@@ -59,16 +59,27 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const Quan
   if (row >= p.rows) return;
   const int b0 = (int)(unit % runs) * UNITS;
   const T* x = (const T*)p.x + row * p.x_stride;
-  float v[UNITS][4];
+  float v[UNITS][4], top[UNITS];
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) load4<T, VEC>(x, (b0 + i) * BLOCK + 4 * lane, p.cols, v[i]);
 #pragma unroll
+  for (int i = 0; i < UNITS; ++i) top[i] = largest(magnitude(v[i]));
+  // lane i has block i's scale and its reciprocal
+  float mine = top[0];
+#pragma unroll
+  for (int i = 1; i < UNITS; ++i) mine = lane == i ? top[i] : mine;
+  const i8::Divisor own = i8::divisor_of(mine, RECIPROCAL);
+  if (lane < UNITS && b0 + lane < blocks) p.scale[row * p.scale_row + (b0 + lane) * p.scale_col] = own.s;
+  const uint32_t flags = (own.zero ? 1u : 0u) | (own.divide ? 2u : 0u);
+#pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const int b = b0 + i;
-    if (b >= blocks) return;
-    const i8::Divisor d = i8::divisor_of(largest(magnitude(v[i])), RECIPROCAL);
-    store4(p.q + row * p.q_stride, b * BLOCK + 4 * lane, p.cols, quotients(v[i], d));
-    if (lane == 0) p.scale[row * p.scale_row + b * p.scale_col] = d.s;
+    i8::Divisor d;
+    d.s = __shfl_sync(FULL, own.s, i);
+    d.inv = __shfl_sync(FULL, own.inv, i);
+    const uint32_t f = __shfl_sync(FULL, flags, i);
+    d.zero = f & 1u;
+    d.divide = f & 2u;
+    if (b0 + i < blocks) store4(p.q + row * p.q_stride, (b0 + i) * BLOCK + 4 * lane, p.cols, quotients(v[i], d));
   }
 }
 
@@ -168,8 +179,8 @@ __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
 //                      L2 takes longer than a block's products
 //   warps 4 ..         epilogue: warp w owns tensor memory lanes 32 (w % 4) ..,
 //                      tile rows, and some of the columns, whose logits it holds
-//                      in registers over the tile's blocks (64 a lane);
-//                      at the tile's end it rounds them, stages 32 rows x 64 or 128 bytes
+//                      in registers over the tile's blocks (128 a lane at most);
+//                      at the tile's end it rounds them, stages 32 rows x 128 bytes
 //                      in shared memory (16-byte pieces XOR-swizzled by row) and
 //                      sends them by TMA, or row by row where rows of logits are
 //                      not 16-byte aligned
@@ -216,7 +227,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
   constexpr int EACH = BN / (G::EPI / 4), PART = EACH < MIN_PART ? MIN_PART : EACH;  // a warp's columns
   constexpr int ACTIVE = 4 * (BN / PART);                   // warps that have some
   struct Fixed {
-    uint64_t full[S], empty[S], acc_full[NACC], acc_empty[NACC], sc_full[RING], sc_empty[RING];
+    uint64_t full[S], done[S], acc_empty[NACC], sc_full[RING], sc_empty[RING];
     uint32_t tmem_slot;
     __align__(16) float rows[RING][BM], ids[RING][4];  // scales of a block: of the rows, of each 128 ids
   };
@@ -225,7 +236,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
   // the swizzle patterns of ring and staging repeat every 1024 bytes
   extern __shared__ __align__(1024) uint8_t ring[];
   Fixed& fx = *reinterpret_cast<Fixed*>(ring + (size_t)S * G::STAGE_BYTES + G::OUT_BYTES);
-  uint64_t *const full = fx.full, *const empty = fx.empty, *const acc_full = fx.acc_full, *const acc_empty = fx.acc_empty;
+  uint64_t *const full = fx.full, *const done = fx.done, *const acc_empty = fx.acc_empty;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = CG > 1 ? (int)(blockIdx.x % CG) : 0;  // within the pair
@@ -238,12 +249,9 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
     if (p.store_tma) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_out) : "memory");
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&done[s], 1);
     }
-    for (int i = 0; i < NACC; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], ACTIVE * CG);
-    }
+    for (int i = 0; i < NACC; ++i) mbar_init(&acc_empty[i], ACTIVE * CG);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -322,7 +330,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
         int m0, n0;
         place(t, m0, n0);
         for (int kb = 0; kb < KB && ok; ++kb, ++it, turn.next(S)) {
-          ok = wait(&empty[turn.slot], turn.parity ^ 1);
+          ok = wait(&done[turn.slot], turn.parity ^ 1);
           if (!ok) break;
           if (it >= early) load_ids(turn.slot, kb, n0);
           if (CG == 1) tma_load_2d(a_tile(turn.slot), &map_h, kb * BK, m0, &full[turn.slot]);
@@ -330,7 +338,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
         }
       }
       // every stage is free: its copies have landed and the arrivals on its barriers are in
-      for (int i = 0; ok && i < S; ++i, turn.next(S)) ok = wait(&empty[turn.slot], turn.parity ^ 1);
+      for (int i = 0; ok && i < S; ++i, turn.next(S)) ok = wait(&done[turn.slot], turn.parity ^ 1);
       if (!ok) {  // copies under way get time to land before the CTA may leave
         const uint64_t t0 = global_ns();
         while (global_ns() - t0 < 2000000ull) {
@@ -348,28 +356,26 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
       };
       // this warp feeds the tensor core alone, a stage of products every 512
       // clocks at most: everything a stage needs is an addition to these
-      const uint32_t full_at = held(smem_u32(full)), stage_empty_at = held(smem_u32(empty));
-      const uint32_t acc_full_at = held(smem_u32(acc_full)), acc_empty_at = held(smem_u32(acc_empty));
+      const uint32_t full_at = held(smem_u32(full)), done_at = held(smem_u32(done));
+      const uint32_t acc_empty_at = held(smem_u32(acc_empty));
       const uint64_t desc = sw128_desc(smem_u32(ring));
       const uint32_t lo0 = (uint32_t)desc, hi = (uint32_t)(desc >> 32);
       for (int t = first; t < tiles && ok; t += step) {
         for (int kb = 0; kb < KB; ++kb, turn.next(S), acc.next(NACC)) {
           const uint32_t a_lo = lo0 + (uint32_t)turn.slot * (G::STAGE_BYTES >> 4), b_lo = a_lo + (G::A_BYTES >> 4);
-          // the stage first: its copies are there before the accumulator is free
-          ok = wait(full_at + 8 * turn.slot, turn.parity) && wait(acc_empty_at + 8 * acc.slot, acc.parity ^ 1);
-          if (!ok) break;
+          const uint32_t full_bar = full_at + 8 * turn.slot, empty_bar = acc_empty_at + 8 * acc.slot;
+          if (!both_complete(lane == 0, full_bar, turn.parity, empty_bar, acc.parity ^ 1)) {
+            ok = wait(full_bar, turn.parity) && wait(empty_bar, acc.parity ^ 1);
+            if (!ok) break;
+          }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < BK / UK; ++k)
               mma_f8<CG>(tmem + acc.slot * BN, a_lo + k * (UK >> 4), b_lo + k * (UK >> 4), hi, idesc, k > 0 ? 1u : 0u);
-            if (CG == 1) {
-              tc_commit(stage_empty_at + 8 * turn.slot);
-              tc_commit(acc_full_at + 8 * acc.slot);
-            } else {
-              commit_pair(stage_empty_at + 8 * turn.slot);
-              commit_pair(acc_full_at + 8 * acc.slot);
-            }
+            // the stage is free for the producer and the accumulator full for the epilogue
+            if (CG == 1) tc_commit(done_at + 8 * turn.slot);
+            else commit_pair(done_at + 8 * turn.slot);
           }
           __syncwarp();
         }
@@ -405,11 +411,11 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
       uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 4) * G::BOX_BYTES;
       constexpr int LD = 32, BUFS = 2;
       const uint32_t tmem_at = held(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0);
-      const uint32_t full_at = held(smem_u32(acc_full)), empty_at = held(CG == 1 ? smem_u32(acc_empty) : map_to(smem_u32(acc_empty), 0));
+      const uint32_t done_at = held(smem_u32(done)), empty_at = held(map_to(smem_u32(acc_empty), 0));
       const uint32_t sc_full_at = held(smem_u32(fx.sc_full)), sc_empty_at = held(smem_u32(fx.sc_empty));
       const uint32_t rows_at = held(smem_u32(&fx.rows[0][quad * 32 + lane])), ids_at = held(smem_u32(&fx.ids[0][c0 / BLOCK]));
       const bool first_lane = held(lane) == 0;
-      Turn acc, sc;
+      Turn acc, sc, turn;
       bool hook = p.give_up != 0;
       for (int t = first; t < tiles; t += step) {
         int m0, n0;
@@ -419,12 +425,14 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < PART; ++i) sum[i] = 0.0f;
         bool waited = true;
-        for (int kb = 0; kb < KB; ++kb, acc.next(NACC), sc.next(RING)) {
-          if (first_lane)
-            waited = mbar_wait(sc_full_at + 8 * sc.slot, sc.parity, WAIT_NS) && mbar_wait(full_at + 8 * acc.slot, acc.parity, WAIT_NS) && !hook;
-          hook = false;
-          waited = __shfl_sync(FULL, waited, 0) != 0;
-          if (!waited) break;
+        for (int kb = 0; kb < KB; ++kb, acc.next(NACC), sc.next(RING), turn.next(S)) {
+          const uint32_t sc_bar = sc_full_at + 8 * sc.slot, done_bar = done_at + 8 * turn.slot;
+          if (hook || !both_complete(first_lane, sc_bar, sc.parity, done_bar, turn.parity)) {
+            if (lane == 0) waited = mbar_wait(sc_bar, sc.parity, WAIT_NS) && mbar_wait(done_bar, turn.parity, WAIT_NS) && !hook;
+            hook = false;
+            waited = __shfl_sync(FULL, waited, 0) != 0;
+            if (!waited) break;
+          }
           tc_fence_after();
           const uint32_t base = tmem_at + (uint32_t)(acc.slot * BN);
           uint32_t v[BUFS][LD];
@@ -433,11 +441,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
           auto release = [&]() {  // the warp's part of the accumulator is in registers
             tc_fence_before();
             __syncwarp();
-            if (first_lane) {
-              arrive_here(sc_empty_at + 8 * sc.slot);
-              if (CG == 1) arrive_here(empty_at + 8 * acc.slot);
-              else arrive_at(empty_at + 8 * acc.slot);
-            }
+            arrive_both(first_lane, sc_empty_at + 8 * sc.slot, empty_at + 8 * acc.slot);
           };
           if (live) {
 #pragma unroll
@@ -467,7 +471,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
         }
         if (!live) continue;
         const bool by_tma = n0 + c0 + PART <= p.tma_ids;
-        auto swizzle = [](int r) { return ROW == 128 ? r & 7 : (r >> 1) & 3; };  // of TMA's 128- and 64-byte patterns
+        auto swizzle = [](int r) { return r & 7; };  // of TMA's 128-byte pattern
 #pragma unroll
         for (int g = 0; g < PART; g += CB) {
           constexpr int EP = 16 / (int)sizeof(Tout);
@@ -545,9 +549,14 @@ static cudaError_t launch_quantize(const QuantParams& p, bool tiles, cudaStream_
     const cudaLaunchConfig_t cfg = config(dim3((unsigned)blocks, (unsigned)((p.rows + BLOCK - 1) / BLOCK), 1), QUANT_THREADS, 0, 1, s, attr);
     return vec ? cudaLaunchKernelEx(&cfg, quantize_tiles_kernel<T, true>, p) : cudaLaunchKernelEx(&cfg, quantize_tiles_kernel<T, false>, p);
   }
-  const int64_t units = p.rows * ((blocks + UNITS - 1) / UNITS), warps = QUANT_THREADS / 32;
-  const cudaLaunchConfig_t cfg = config(dim3((unsigned)((units + warps - 1) / warps), 1, 1), QUANT_THREADS, 0, 1, s, attr);
-  return vec ? cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, true>, p) : cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, false>, p);
+  auto rows = [&](auto kern, int64_t each) {
+    const int64_t units = p.rows * ((blocks + each - 1) / each), warps = QUANT_THREADS / 32;
+    const cudaLaunchConfig_t cfg = config(dim3((unsigned)((units + warps - 1) / warps), 1, 1), QUANT_THREADS, 0, 1, s, attr);
+    return cudaLaunchKernelEx(&cfg, kern, p);
+  };
+  if (p.rows * blocks < 8ll * 16 * device_sms())
+    return vec ? rows(quantize_rows_kernel<T, true, 2>, 2) : rows(quantize_rows_kernel<T, false, 2>, 2);
+  return vec ? rows(quantize_rows_kernel<T, true, 8>, 8) : rows(quantize_rows_kernel<T, false, 8>, 8);
 }
 static cudaError_t launch_quantize(const QuantParams& p, int dtype, bool tiles, cudaStream_t s) {
   switch (dtype) {
@@ -579,7 +588,7 @@ static cudaError_t launch_tiles(const MtrLmHeadF8Args& a, const Held& h, cudaStr
                                    : std::is_same<Tout, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (tma) {
-    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, (int)G::ROW_BYTES / es, 32, G::ROW_BYTES == 64)) return cudaErrorInvalidValue;
+    if (!make_map(&mo, type, a.logits, a.rows, a.vocab, a.logits_row_stride * es, (int)G::ROW_BYTES / es, 32)) return cudaErrorInvalidValue;
   } else {
     mo = mw;
   }

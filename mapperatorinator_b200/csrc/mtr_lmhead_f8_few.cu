@@ -39,22 +39,23 @@ struct FewParams {
 // bytes between hidden rows: two neighbours' 64 bytes of a fragment load lie in different halves of the banks
 __host__ __device__ constexpr int row_bytes(int blocks) { return blocks * BLOCK + 64; }
 
-// The rows' blocks, a warp each; rows up to ROWS that are not there are 0.
+// The rows' blocks, a warp each.  What rows up to ROWS that are not there hold does
+// not matter: theirs are sums of their own, which nobody reads.
 template <int ROWS, typename T, bool VEC>
 __device__ __forceinline__ void hold_rows(const FewParams& p, uint8_t* held, float* scale) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = ROWS * p.blocks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = p.rows * p.blocks;
   constexpr int U = 4;  // blocks under way
   for (int u0 = warp; u0 < units; u0 += WARPS * U) {
     float v[U][4];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = u0 + i * WARPS, r = u % ROWS, b = u / ROWS;
-      if (u < units && r < p.rows) load4<T, VEC>((const T*)p.x + r * p.x_stride, b * BLOCK + 4 * lane, p.d, v[i]);
+      const int u = u0 + i * WARPS, r = u / p.blocks, b = u - r * p.blocks;
+      if (u < units) load4<T, VEC>((const T*)p.x + r * p.x_stride, b * BLOCK + 4 * lane, p.d, v[i]);
       else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = u0 + i * WARPS, r = u % ROWS, b = u / ROWS;
+      const int u = u0 + i * WARPS, r = u / p.blocks, b = u - r * p.blocks;
       if (u < units) {
         const i8::Divisor d = i8::divisor_of(largest(magnitude(v[i])), RECIPROCAL);
         *reinterpret_cast<uint32_t*>(held + r * row_bytes(p.blocks) + b * BLOCK + 4 * lane) = quotients(v[i], d);

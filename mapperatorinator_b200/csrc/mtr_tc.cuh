@@ -64,6 +64,25 @@ __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t ph, uint64_t budg
   }
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t ph, uint64_t budget_ns) { return mbar_wait(smem_u32(b), ph, budget_ns); }
+// Whether two phases have completed, polled once, by the lanes with `mine` (one of
+// the warp) and without a branch: what waits finds its barriers complete more often
+// than not, and a loop that the warp leaves and joins again costs it 150 clocks each.
+__device__ __forceinline__ bool both_complete(bool mine, uint32_t a, uint32_t pa, uint32_t b, uint32_t pb) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred m, p, q;\n\t"
+      "setp.ne.b32 m, %1, 0;\n\t"
+      "setp.ne.b32 p, 0, 0;\n\t"
+      "setp.ne.b32 q, 0, 0;\n\t"
+      "@m mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
+      "@m mbarrier.try_wait.parity.shared::cta.b64 q, [%4], %5;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"((uint32_t)mine), "r"(a), "r"(pa), "r"(b), "r"(pb)
+      : "memory");
+  return __any_sync(FULL, ok != 0u);
+}
 // A value that the compiler keeps in a register: it would form a shared-memory
 // address anew, from the CTA's place in the cluster, wherever it is used.
 __device__ __forceinline__ uint32_t held(uint32_t v) {
@@ -167,9 +186,15 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void arrive_at(uint32_t addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// the same on a barrier of this CTA: no trip through the cluster's network
-__device__ __forceinline__ void arrive_here(uint32_t addr) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(addr) : "memory");
+// arrivals of the lanes with `mine` on a barrier of this CTA and on one of the cluster
+__device__ __forceinline__ void arrive_both(bool mine, uint32_t here, uint32_t there) {
+  asm volatile(
+      "{\n\t.reg .pred m;\n\t"
+      "setp.ne.b32 m, %0, 0;\n\t"
+      "@m mbarrier.arrive.shared::cta.b64 _, [%1];\n\t"
+      "@m mbarrier.arrive.shared::cluster.b64 _, [%2];\n\t}" ::"r"((uint32_t)mine),
+      "r"(here), "r"(there)
+      : "memory");
 }
 __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -216,10 +241,10 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // 2-D tensor map over a row-major [rows, cols] matrix, box of box_cols x
-// box_rows, 128-byte (64-byte) swizzle; reads 0 outside the matrix and writes nothing
+// box_rows, 128-byte swizzle; reads 0 outside the matrix and writes nothing
 // behind the 16 bytes that its last column ends in.
 inline bool make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes,
-                     int box_cols, int box_rows, bool swizzle64 = false) {
+                     int box_cols, int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -227,7 +252,7 @@ inline bool make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base,
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tc
