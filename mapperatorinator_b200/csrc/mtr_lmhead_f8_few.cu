@@ -19,7 +19,7 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int CTAS = 2;           // an SM
-constexpr int HELD = 100 * 1024;  // bytes of rows and scales in shared memory at most
+constexpr int ROWS = 8;           // of a fragment
 
 struct FewParams {
   const void* x;
@@ -39,9 +39,9 @@ struct FewParams {
 // bytes between hidden rows: two neighbours' 64 bytes of a fragment load lie in different halves of the banks
 __host__ __device__ constexpr int row_bytes(int blocks) { return blocks * BLOCK + 64; }
 
-// The rows' blocks, a warp each.  What rows up to ROWS that are not there hold does
-// not matter: theirs are sums of their own, which nobody reads.
-template <int ROWS, typename T, bool VEC>
+// The rows' blocks, a warp each.  (In the place of rows that are not there the products
+// take the last one, whose sums there nobody reads.)
+template <typename T, bool VEC>
 __device__ __forceinline__ void hold_rows(const FewParams& p, uint8_t* held, float* scale) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = p.rows * p.blocks;
   constexpr int U = 4;  // blocks under way
@@ -64,10 +64,10 @@ __device__ __forceinline__ void hold_rows(const FewParams& p, uint8_t* held, flo
     }
   }
 }
-template <int ROWS, typename T>
+template <typename T>
 __device__ __forceinline__ void hold_rows(const FewParams& p, uint8_t* held, float* scale) {
-  if (p.vec) hold_rows<ROWS, T, true>(p, held, scale);
-  else hold_rows<ROWS, T, false>(p, held, scale);
+  if (p.vec) hold_rows<T, true>(p, held, scale);
+  else hold_rows<T, false>(p, held, scale);
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -77,12 +77,12 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT, int SPLIT>
+template <int SPLIT>
 __global__ void __launch_bounds__(THREADS, CTAS) few_rows_kernel(const FewParams p) {
-  constexpr int ROWS = 8 * NT, GP = WARPS / SPLIT;
+  constexpr int GP = WARPS / SPLIT;
   extern __shared__ __align__(16) uint8_t held[];
-  __shared__ float joined[SPLIT > 1 ? WARPS : 1][SPLIT > 1 ? NT * 4 * 32 : 1];
-  float* scale = reinterpret_cast<float*>(held + ROWS * row_bytes(p.blocks));  // [blocks][ROWS]
+  __shared__ float joined[SPLIT > 1 ? WARPS : 1][SPLIT > 1 ? 4 * 32 : 1];
+  float* scale = reinterpret_cast<float*>(held + p.rows * row_bytes(p.blocks));  // [blocks][ROWS]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % SPLIT, sub = warp / SPLIT;
   const int KB = p.blocks, V = p.vocab, groups = (V + 15) / 16;
   const int g = lane >> 2, t = lane & 3;
@@ -112,17 +112,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) few_rows_kernel(const FewParams
   uint4 next[2][4];
   if ((int)blockIdx.x * GP + sub < groups) load(next, blockIdx.x * GP + sub, part);
   switch (p.x_dtype) {
-    case MTR_DTYPE_F32: hold_rows<ROWS, float>(p, held, scale); break;
-    case MTR_DTYPE_BF16: hold_rows<ROWS, __nv_bfloat16>(p, held, scale); break;
-    default: hold_rows<ROWS, __half>(p, held, scale); break;
+    case MTR_DTYPE_F32: hold_rows<float>(p, held, scale); break;
+    case MTR_DTYPE_BF16: hold_rows<__nv_bfloat16>(p, held, scale); break;
+    default: hold_rows<__half>(p, held, scale); break;
   }
   __syncthreads();
 
   for (int base = blockIdx.x * GP; base < groups; base += step) {
     const int group = base + sub;
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (group < groups) {
       const float* ws = p.w_scale + (int64_t)(group / 8) * p.ws_stride;
       for (int kb = part; kb < KB; kb += 2 * SPLIT) {
@@ -139,103 +137,88 @@ __global__ void __launch_bounds__(THREADS, CTAS) few_rows_kernel(const FewParams
         for (int i = 0; i < 2; ++i) {
           const int b = kb + i * SPLIT;
           if (b >= KB) break;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint8_t* h = held + (n * 8 + g) * row_bytes(KB) + b * BLOCK + 16 * t;
-            const uint4 h0 = *reinterpret_cast<const uint4*>(h), h1 = *reinterpret_cast<const uint4*>(h + 64);
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma(c, w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, h0.x, h0.y);
-            mma(c, w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, h0.z, h0.w);
-            mma(c, w[i][2].x, w[i][3].x, w[i][2].y, w[i][3].y, h1.x, h1.y);
-            mma(c, w[i][2].z, w[i][3].z, w[i][2].w, w[i][3].w, h1.z, h1.w);
-            const float2 hs = *reinterpret_cast<const float2*>(scale + b * ROWS + n * 8 + 2 * t);
-            const float f0 = __fmul_rn(hs.x, i ? s1 : s0), f1 = __fmul_rn(hs.y, i ? s1 : s0);
-            acc[n][0] = fmaf(c[0], f0, acc[n][0]);
-            acc[n][1] = fmaf(c[1], f1, acc[n][1]);
-            acc[n][2] = fmaf(c[2], f0, acc[n][2]);
-            acc[n][3] = fmaf(c[3], f1, acc[n][3]);
-          }
+          const uint8_t* h = held + min(g, p.rows - 1) * row_bytes(KB) + b * BLOCK + 16 * t;
+          const uint4 h0 = *reinterpret_cast<const uint4*>(h), h1 = *reinterpret_cast<const uint4*>(h + 64);
+          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma(c, w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, h0.x, h0.y);
+          mma(c, w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, h0.z, h0.w);
+          mma(c, w[i][2].x, w[i][3].x, w[i][2].y, w[i][3].y, h1.x, h1.y);
+          mma(c, w[i][2].z, w[i][3].z, w[i][2].w, w[i][3].w, h1.z, h1.w);
+          const float2 hs = *reinterpret_cast<const float2*>(scale + b * ROWS + 2 * t);
+          const float f0 = __fmul_rn(hs.x, i ? s1 : s0), f1 = __fmul_rn(hs.y, i ? s1 : s0);
+          acc[0] = fmaf(c[0], f0, acc[0]);
+          acc[1] = fmaf(c[1], f1, acc[1]);
+          acc[2] = fmaf(c[2], f0, acc[2]);
+          acc[3] = fmaf(c[3], f1, acc[3]);
         }
       }
     }
     if constexpr (SPLIT > 1) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) joined[warp][(n * 4 + e) * 32 + lane] = acc[n][e];
+      for (int e = 0; e < 4; ++e) joined[warp][e * 32 + lane] = acc[e];
       __syncthreads();
       if (part == 0)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int k = 1; k < SPLIT; ++k) acc[n][e] += joined[warp + k][(n * 4 + e) * 32 + lane];
+          for (int k = 1; k < SPLIT; ++k) acc[e] += joined[warp + k][e * 32 + lane];
     }
     if (part == 0 && group < groups) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = n * 8 + 2 * t + (e & 1), v = group * 16 + g + (e >> 1) * 8;
-          if (r < p.rows && v < V) {
-            const int64_t at = r * p.out_stride + v;
-            switch (p.out_dtype) {
-              case MTR_DTYPE_F32: ((float*)p.out)[at] = acc[n][e]; break;
-              case MTR_DTYPE_BF16: ((__nv_bfloat16*)p.out)[at] = from_f<__nv_bfloat16>(acc[n][e]); break;
-              default: ((__half*)p.out)[at] = from_f<__half>(acc[n][e]); break;
-            }
+      for (int e = 0; e < 4; ++e) {
+        const int r = 2 * t + (e & 1), v = group * 16 + g + (e >> 1) * 8;
+        if (r < p.rows && v < V) {
+          const int64_t at = r * p.out_stride + v;
+          switch (p.out_dtype) {
+            case MTR_DTYPE_F32: ((float*)p.out)[at] = acc[e]; break;
+            case MTR_DTYPE_BF16: ((__nv_bfloat16*)p.out)[at] = from_f<__nv_bfloat16>(acc[e]); break;
+            default: ((__half*)p.out)[at] = from_f<__half>(acc[e]); break;
           }
         }
+      }
     }
     if (SPLIT > 1) __syncthreads();  // the parts have been read
   }
 }
 
-int held_bytes(int rows, int64_t blocks) { return (int)(rows * row_bytes((int)blocks) + blocks * rows * 4); }
-
-template <int NT, int SPLIT>
+template <int SPLIT>
 cudaError_t launch_split(const FewParams& p, cudaStream_t s) {
-  auto kern = few_rows_kernel<NT, SPLIT>;
-  static std::once_flag once[64];
-  static cudaError_t attr_err[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  std::call_once(once[dev], [&]() { attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD); });
-  if (attr_err[dev] != cudaSuccess) return attr_err[dev];
   const int64_t groups = (p.vocab + 15) / 16, all = (groups * SPLIT + WARPS - 1) / WARPS, room = (int64_t)CTAS * device_sms();
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)(all < room ? all : room), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)held_bytes(8 * NT, p.blocks);
+  cfg.dynamicSmemBytes = (size_t)(p.rows * row_bytes(p.blocks) + p.blocks * ROWS * 4);  // few_rows: 48 blocks, 8.2 KB at most
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   cfg.numAttrs = launch_attrs(attr, 1, true);
   cfg.attrs = attr;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  return cudaLaunchKernelEx(&cfg, few_rows_kernel<SPLIT>, p);
 }
 
-template <int NT>
 cudaError_t launch_rows(const FewParams& p, cudaStream_t s) {
   const int64_t groups = (p.vocab + 15) / 16, warps = (int64_t)CTAS * device_sms() * WARPS;
   int split = 1;
   while (split < 8 && groups * split * 2 <= warps && split * 2 <= p.blocks) split *= 2;
   switch (split) {
-    case 1: return launch_split<NT, 1>(p, s);
-    case 2: return launch_split<NT, 2>(p, s);
-    case 4: return launch_split<NT, 4>(p, s);
-    default: return launch_split<NT, 8>(p, s);
+    case 1: return launch_split<1>(p, s);
+    case 2: return launch_split<2>(p, s);
+    case 4: return launch_split<4>(p, s);
+    default: return launch_split<8>(p, s);
   }
 }
 
 }  // namespace
 
+// Where this kernel is the faster one: every CTA quantises all rows, so their blocks
+// must be few, the fewer the more the vocabulary's own time weighs.  us with weights
+// that are not in L2, here / there (148 SMs): 1 x 768 -> 4096 3.3 / 6.0, 8 x 768 ->
+// 4096 5.5 / 6.2, 8 x 300 -> 65536 12.0 / 12.8, 1 x 1024 -> 65536 16.5 / 16.7; and
+// beyond the bounds 4 x 1024 -> 65536 18.3 / 16.6, 1 x 4096 -> 16384 18.6 / 17.3, 8 x
+// 4096 -> 131072 116 / 93, 16 x 768 -> 4096 (two fragments of rows) 8.0 / 6.2.
 bool few_rows(int64_t rows, int64_t d, int64_t vocab) {
   const int64_t blocks = (d + BLOCK - 1) / BLOCK;
-  return rows <= 8 && blocks <= 64 && held_bytes(8, blocks) <= HELD;
+  return rows <= ROWS && rows * blocks <= (vocab <= 8192 ? 48 : 24);
 }
 
 cudaError_t launch_few(const MtrLmHeadF8Args& a, cudaStream_t s) {
@@ -256,7 +239,7 @@ cudaError_t launch_few(const MtrLmHeadF8Args& a, cudaStream_t s) {
   p.vocab = a.vocab;
   const int es = a.hidden_dtype == MTR_DTYPE_F32 ? 4 : 2;
   p.vec = (uintptr_t)a.hidden % (4 * es) == 0 && a.hidden_row_stride % 4 == 0;
-  return launch_rows<1>(p, s);
+  return launch_rows(p, s);
 }
 
 }  // namespace f8

@@ -138,12 +138,12 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, 
     a = _args(logits, teacher_ids, teacher_logprobs, temperature, tail, status)
     g = _grad_losses(grad_losses, logits)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
     elif out.dtype != logits.dtype or out.shape != logits.shape:
         raise ValueError("out must have the logits' shape and dtype")
     a.grad_row_stride = matrix(out, "out")
     same_device(out, logits.device, "out")
-    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    loss = logits.new_empty(logits.shape[0], dtype=torch.float32)
     a.out_loss, a.grad_logits = loss.data_ptr(), out.data_ptr()
     if g is not None:
         a.g_loss = g.data_ptr()

@@ -113,11 +113,11 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
             raise ValueError(f"status must be a contiguous int32 vector of {batch} elements")
         same_device(status, device, "status")
         a.out_status = status.data_ptr()
-    tokens = torch.empty((batch, more), dtype=torch.int64, device=device)
-    accepted = torch.empty(batch, dtype=torch.int32, device=device)
-    logprobs = torch.empty((batch, more), dtype=torch.float32, device=device)
+    new = target_logits.new_empty
+    tokens, accepted = new((batch, more), dtype=torch.int64), new(batch, dtype=torch.int32)
+    logprobs = new((batch, more), dtype=torch.float32)
     need = N.verify_workspace(batch, drafts, vocab, a.logits_dtype)
-    work = torch.empty(need, dtype=torch.uint8, device=device)
+    work = new(need, dtype=torch.uint8)
     a.out_tokens, a.out_accepted, a.out_logprobs = tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr()
     a.workspace, a.workspace_bytes = work.data_ptr(), need
     launch_on(device, N.verify_launch, a)
