@@ -55,7 +55,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     """Accepts or replaces the drafted tokens of B sequences.
 
     ``target_logits`` is ``[B, K + 1, V]`` (float32, bfloat16 or float16, any batch
-    and position strides): the target's logits -- processed scores, if a chain
+    stride, position stride >= V): the target's logits -- processed scores, if a chain
     applies -- after the prefix and after each draft.  ``draft_ids`` is ``[B, K]``
     int64 or int32, ``draft_logits`` ``[B, K, V]`` of the target's dtype: what the
     drafts were drawn from, or None for drafts without a distribution (looked up,

@@ -337,6 +337,18 @@ def test_one_teacher_row_for_all_and_no_rows(cuda_device):
 
 
 @gpu
+@pytest.mark.parametrize("rows,vocab,n,dtype", [(9000, 600, 8, torch.bfloat16), (5000, 4097, 20, torch.float16), (2600, 2100, 40, torch.float32),
+                                                (1, 131072, 32, torch.float32), (20, 70001, 5, torch.bfloat16), (700, 33000, 16, torch.bfloat16)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_many_rows_and_few(cuda_device, tail, rows, vocab, n, dtype):
+    """The number of threads and CTAs that share a row goes by both sizes."""
+    logits, ids, lps, w = inputs(cuda_device, rows, vocab, n, dtype, seed=rows)
+    logits[rows // 2, vocab // 3] = math.nan
+    logits[rows - 1, : vocab - 3] = -math.inf
+    check(logits, ids, lps, tail, 1.3, w)
+
+
+@gpu
 def test_refusals(cuda_device):
     logits, ids, lps, w = inputs(cuda_device, 6, 50, 4, torch.float32)
     for bad in (ids[:5], ids.float(), ids[:, :0], ids[:, :3], ids.cpu(), ids.t()):

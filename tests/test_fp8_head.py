@@ -327,6 +327,31 @@ def test_streams_and_graphs(cuda_device, rows):
 
 
 @gpu
+def test_weight_written_just_before_its_use(cuda_device):
+    # the projection is launched as a dependent of the kernels that write its operands
+    for seed in range(5):
+        for rows in (2, 64, 400):
+            h, w = inputs(cuda_device, rows, 512, 2048, seed=seed)
+            torch.cuda.synchronize()
+            weight = Fp8Weight.from_weight(w)
+            out = lm_head_logits_fp8(h, weight.q, weight.scale)
+            torch.cuda.synchronize()
+            assert torch.equal(out, lm_head_logits_fp8(h, weight.q, weight.scale))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("d,vocab", [(128, 16), (768, 4097), (1001, 8192), (6000, 40), (385, 70001), (2900, 8192)])
+def test_few_rows(cuda_device, rows, d, vocab):
+    h, w = inputs(cuda_device, 8, d, vocab, seed=rows + d)
+    weight = Fp8Weight.from_weight(w)
+    out = lm_head_logits_fp8(h[:rows], weight.q, weight.scale, out_dtype=torch.float32)
+    check(out, h[:rows], weight)
+    alone = torch.cat([lm_head_logits_fp8(h[r:r + 1], weight.q, weight.scale, out_dtype=torch.float32) for r in range(rows)])
+    check(alone, h[:rows], weight)
+
+
+@gpu
 @pytest.mark.parametrize("pairs", [1, 40])
 def test_sampler_takes_the_weight(cuda_device, pairs):
     d, vocab = 320, 1000

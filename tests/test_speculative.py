@@ -290,6 +290,22 @@ def test_uniforms_next_to_the_borders(cuda_device, dtype, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("noise", [1e-3, 0.05])
+@pytest.mark.parametrize("batch,vocab", [(2, 131072), (3, 100003), (40, 20000), (80, 5000)])
+def test_distributions_nearly_alike(cuda_device, dtype, noise, batch, vocab):
+    """Refused drafts where p and q are next to each other at many ids, or at nearly all of them."""
+    target, ids, _, u = inputs(cuda_device, batch, 2, vocab, torch.float32, seed=vocab)
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    draft = target[:, :2] + noise * torch.randn((batch, 2, vocab), generator=g, device=cuda_device)
+    target, draft = target.to(dtype), draft.to(dtype)
+    ids[:, 0] = (draft[:, 0].float() - target[:, 0].float()).argmax(1)  # an id that the draft gives too much
+    u[:, 0] = 1.0 - 2.0 ** -20
+    r = check(target, ids, draft, u)
+    assert int((r.accepted == 0).sum()) > batch // 2
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("with_draft", [True, False])
 @pytest.mark.parametrize("vocab", [5, 4096, 20001])
