@@ -187,6 +187,14 @@ __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
 // Every wait is bounded; a role whose wait gives up counts it (gave_up) and stops,
 // so that the others' waits give up too; the producer then gives its copies time
 // to land, the epilogue writes NaN for what was not computed, and the CTA returns.
+//
+// What bounds it (8192 x 4096 -> 16384: 530 us, quantisation included; clock stamps): a
+// block takes about 890 clocks, of which its products need 590.  Two accumulators of
+// 256 columns are all that tensor memory holds; from the issue of a pair's products to
+// the epilogue's seeing them done pass 1250 clocks, then 220 to read and add them and
+// 340 until the next products are issued: 1800 for two blocks.  With a quarter of the
+// products it still takes 441 us.  A CTA alone sees its products done in 850 clocks, but
+// takes 48 KB a block out of L2 instead of 32: 563 us.
 constexpr int RING = 4;  // blocks whose scales are in shared memory
 
 template <int BYTES>
@@ -629,7 +637,17 @@ static cudaError_t launch_tiles(const MtrLmHeadF8Args& a, const Held& h, cudaStr
 }
 
 // The narrowest tiles that still make one round of CTAs; beyond that 128 x 256
-// tiles, or pairs of CTAs on 256 x 256, which take less out of L2.
+// tiles, or pairs of CTAs on 256 x 256, which take less out of L2.  Measured with the
+// quantisation (us, 148 SMs, weights not in L2; the rule's choice is starred):
+//                         64     128    256    pair
+//   128 x 768 -> 4096     6.2*   7.0    8.8    9.5
+//   333 x 1001 -> 4099    11.4   9.7*   14.7   15.2
+//   700 x 1024 -> 4096    14.1   12.8   11.9*  13.0
+//   512 x 768 -> 16384    21.0   16.6   15.6*  16.8
+//   64 x 4096 -> 16384    25.4   18.4*  22.6   24.9
+//   300 x 1024 -> 131072  116    73.1   66.1*  80.6
+//   1024 x 2048 -> 32768  144    89.7   77.1   74.8*
+//   8192 x 768 -> 4096    69.0   47.6   43.3   43.6*
 template <typename Tout>
 static cudaError_t launch_proj(const MtrLmHeadF8Args& a, const Held& h, cudaStream_t s) {
   const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;
@@ -638,7 +656,7 @@ static cudaError_t launch_proj(const MtrLmHeadF8Args& a, const Held& h, cudaStre
   if (tiles(128) <= sms) return launch_tiles<1, 128, Tout>(a, h, s);
   const int64_t n = (a.vocab + 255) / 256, pairs = sms / 2;
   const int64_t rounds = (m * n + sms - 1) / sms, pair_rounds = ((m + 1) / 2 * n + pairs - 1) / pairs;
-  // a round of pairs takes about 12/13 of the time
+  // a round of pairs was taken to need 12/13 of the time; the two are within 3 % where they are close
   if (m == 1 || 12 * pair_rounds > 13 * rounds || (rounds <= 2 && a.d_model <= 2048)) return launch_tiles<1, 256, Tout>(a, h, s);
   return launch_tiles<2, 256, Tout>(a, h, s);
 }

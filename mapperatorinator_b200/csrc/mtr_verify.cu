@@ -15,7 +15,11 @@
 //   pick_kernel   decides the drafts in turn: log u + log q - log p in double from
 //                 these sums, clear when it is further than 2 E from 0; else (about
 //                 once in 10^4 drafts) both sums are formed again in double.  Then it
-//                 draws from the one position that counts, all in double.
+//                 draws from the one position that counts, all in double.  It reads
+//                 short rows itself, and one launch does it all.
+// rows_kernel reads 571 MB (128 x 17 rows of 131072 bf16) in 102 us, 5.6 TB/s; the draw
+// of 128 sequences there takes 62: 69 instructions for an id's two terms, at 0.56 a
+// clock and scheduler, 41 % of the double rate.
 // The bound E: ex2.approx is within 2^-22, its argument within 3 2^-24 |d| of d, and
 // the mean of |d| under the softmax is at most log V < 12; a thread adds at most 16
 // pairs in fp32 before double takes over, and its sum moves to a larger maximum at
@@ -81,29 +85,32 @@ __device__ __forceinline__ int64_t draft_id(const Params& p, int64_t b, int j) {
 
 constexpr int HOLD = 4;  // vectors of a thread's tile
 
-// One run of one row: its largest logit and the sum about it.
-template <typename T, int THREADS, bool GREEDY>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+// A row's parts joined; every lane the same.
+__device__ __forceinline__ Part join(const Part* parts, int runs, float scale) {
+  Part r = parts[0];
+  for (int i = 1; i < runs; ++i) {
+    const Part q = parts[i];
+    const float m = fmaxf(r.m, q.m);
+    if (q.m > r.m || (q.m == r.m && q.id < r.id)) r.id = q.id;
+    r.s = (r.m > neg_inf() ? r.s * (double)ex2((r.m - m) * scale) : r.s) + (q.m > neg_inf() ? q.s * (double)ex2((q.m - m) * scale) : q.s);
+    r.m = m;
+  }
+  return r;
+}
+
+// A warp's part of the vectors [v0, v1) of a row, which THREADS threads take 32 by 32
+// (tid of them); `singles`: with the single logits before the first 16-byte boundary
+// and behind the last.  The first tile is asked for before `counts` says whether the
+// row does; nothing is returned where it does not.
+template <typename T, int THREADS, bool GREEDY, typename F>
+__device__ __forceinline__ bool warp_run(const T* x, int V, int v0, int v1, bool singles, float scale, int tid, F counts, Part& part) {
   typedef Vec<T> X;
-  constexpr int E = X::E, WARPS = THREADS / 32;
-  __shared__ float sh_m[WARPS];
-  __shared__ double sh_s[WARPS];
-  __shared__ int sh_id[WARPS];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int K = p.drafts, V = p.vocab;
-  const int64_t row = blockIdx.x, targets = (int64_t)p.batch * (K + 1);
-  const bool draft = row >= targets;
-  const int64_t b = draft ? (row - targets) / K : row / (K + 1);
-  const int j = (int)(draft ? (row - targets) % K : row % (K + 1));
-  wait_prior_grid();
-  const T* x = draft ? (const T*)p.draft + b * p.d_batch + j * p.d_pos : (const T*)p.target + b * p.t_batch + j * p.t_pos;
-  const float scale = draft ? p.d_scale : p.t_scale;
+  constexpr int E = X::E;
   const int off = (int)(((uintptr_t)x & 15u) / sizeof(T));
   const int head = min(off ? E - off : 0, V), vecs = (V - head) / E, behind = V - head - vecs * E;
   const uint4* body = reinterpret_cast<const uint4*>(x + head);
-  const int v0 = min((int)blockIdx.y * p.run, vecs), v1 = blockIdx.y == gridDim.y - 1 ? vecs : min(v0 + p.run, vecs);
-
-  // the first tile is asked for before it is known whether the row counts
+  v0 = min(v0, vecs);
+  v1 = min(v1, vecs);
   uint4 w[HOLD];
   auto ask = [&](int i0) {
 #pragma unroll
@@ -113,11 +120,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     }
   };
   ask(v0 + tid);
-  // a position counts only behind drafts that are ids
-  for (int i0 = 0, n = draft ? j + 1 : j; i0 < n; i0 += 32) {
-    const int64_t id = i0 + lane < n ? draft_id(p, b, i0 + lane) : 0;
-    if (__any_sync(FULL, id < 0 || id >= V)) return;
-  }
+  if (!counts()) return false;
 
   float m = neg_inf();
   double s = 0.0;
@@ -130,8 +133,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
       m = v;
     }
   };
-  // the single logits before the first boundary and behind the last, of the first run
-  const int single = blockIdx.y > 0 ? -1 : tid < head ? tid : tid >= 32 && tid < 32 + behind ? V - behind + tid - 32 : -1;
+  const int single = !singles ? -1 : tid < head ? tid : tid >= 16 && tid < 16 + behind ? V - behind + tid - 16 : -1;
   const float one = single >= 0 ? to_f(x[single]) : neg_inf();
   for (int i0 = v0 + tid; i0 < v1; i0 += HOLD * THREADS) {
     if (i0 != v0 + tid) ask(i0);
@@ -168,51 +170,66 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     up2(s2, lo, hi);
     s += (double)lo + (double)hi;
   }
-  float vector_m = m;  // what `at` holds
+  const float vector_m = m;  // what `at` holds
   if (single >= 0) {
     rise(one);
     if (!bad && m > neg_inf()) s += (double)ex2((one - m) * scale);
   }
-  const float most = warp_max(bad ? neg_inf() : m);
-  if (!bad && m > neg_inf()) s *= (double)ex2((m - most) * scale);
+  part.m = warp_max(bad ? neg_inf() : m);
+  if (!bad && m > neg_inf()) s *= (double)ex2((m - part.m) * scale);
   if (bad) s = nan_d();
-  s = warp_sum(s);
-  if (lane == 0) {
-    sh_m[warp] = most;
-    sh_s[warp] = s;
-  }
-  __syncthreads();
-  float all = sh_m[0];
-#pragma unroll
-  for (int k = 1; k < WARPS; ++k) all = fmaxf(all, sh_m[k]);
-  int id = 0x7fffffff;
+  part.s = warp_sum(s);
+  part.id = 0x7fffffff;
   if constexpr (GREEDY) {
     // the first id whose logit is the largest
-    if (single >= 0 && one == all) id = single;
-    if (vector_m == all && at < vecs) {
+    int id = single >= 0 && one == part.m ? single : 0x7fffffff;
+    if (vector_m == part.m && at < vecs) {
       float f[E];
       X::unpack(body[at], f);
 #pragma unroll
       for (int e = E - 1; e >= 0; --e)
-        if (f[e] == all) id = min(id, head + at * E + e);
+        if (f[e] == part.m) id = min(id, head + at * E + e);
     }
-    id = __reduce_min_sync(FULL, id);
-    if (lane == 0) sh_id[warp] = id;
-    __syncthreads();
+    part.id = __reduce_min_sync(FULL, id);
   }
-  if (tid == 0) {
-    double sum = 0.0;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) {
-      sum += sh_m[k] > neg_inf() ? sh_s[k] * (double)ex2((sh_m[k] - all) * scale) : sh_s[k];
-      if constexpr (GREEDY) id = min(id, sh_id[k]);
-    }
-    p.parts[row * p.runs + blockIdx.y] = Part{all, id, sum};
+  return true;
+}
+// a position counts only behind drafts that are ids: whether the first n are
+__device__ __forceinline__ bool drafts_are_ids(const Params& p, int64_t b, int n) {
+  const int lane = threadIdx.x & 31;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int64_t id = i0 + lane < n ? draft_id(p, b, i0 + lane) : 0;
+    if (__any_sync(FULL, id < 0 || id >= p.vocab)) return false;
   }
+  return true;
 }
 
-// Threads of a CTA that draws: fewer, whose terms stay in registers, where a CTA has
-// few ids; else many, which hide the double operations' latency.
+// One run of one row: its largest logit and the sum about it.
+template <typename T, int THREADS, bool GREEDY>
+__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ Part parts[WARPS];
+  const int tid = threadIdx.x, K = p.drafts;
+  const int64_t row = blockIdx.x, targets = (int64_t)p.batch * (K + 1);
+  const bool draft = row >= targets;
+  const int64_t b = draft ? (row - targets) / K : row / (K + 1);
+  const int j = (int)(draft ? (row - targets) % K : row % (K + 1));
+  wait_prior_grid();
+  const T* x = draft ? (const T*)p.draft + b * p.d_batch + j * p.d_pos : (const T*)p.target + b * p.t_batch + j * p.t_pos;
+  const float scale = draft ? p.d_scale : p.t_scale;
+  const int v0 = (int)blockIdx.y * p.run;
+  Part part;
+  if (!warp_run<T, THREADS, GREEDY>(x, p.vocab, v0, blockIdx.y == gridDim.y - 1 ? p.vocab : v0 + p.run, blockIdx.y == 0, scale, tid,
+                                    [&] { return drafts_are_ids(p, b, draft ? j + 1 : j); }, part))
+    return;
+  if ((tid & 31) == 0) parts[tid >> 5] = part;
+  __syncthreads();
+  if (tid == 0) p.parts[row * p.runs + blockIdx.y] = join(parts, WARPS, scale);
+}
+
+// Threads of a CTA that draws.  Where it has few ids (kept) a thread's terms stay in
+// registers.  640, 768 and 1024 threads for the others: 172, 177 and 169 us where 512
+// take 167 (128 x 8, V = 131072 bf16).
 constexpr int FEW = 512, MANY = 512;
 constexpr int KEPT = 8;  // ids of a thread whose terms stay in registers
 constexpr int NEAR = 64; // ids of a warp next to the border between p > q and p < q
@@ -264,20 +281,8 @@ struct PickShared {
   double piece[PICK_WARPS];
   int stop, unclear, token;
   int32_t near[PICK_WARPS][NEAR];
+  Part parts[2 * MTR_MAX_DRAFTS + 1];  // where the rows are read here
 };
-
-// A row's parts joined; every lane the same.
-__device__ __forceinline__ Part join(const Part* parts, int runs, float scale) {
-  Part r = parts[0];
-  for (int i = 1; i < runs; ++i) {
-    const Part q = parts[i];
-    const float m = fmaxf(r.m, q.m);
-    if (q.m > r.m || (q.m == r.m && q.id < r.id)) r.id = q.id;
-    r.s = (r.m > neg_inf() ? r.s * (double)ex2((r.m - m) * scale) : r.s) + (q.m > neg_inf() ? q.s * (double)ex2((q.m - m) * scale) : q.s);
-    r.m = m;
-  }
-  return r;
-}
 
 template <typename T, bool kept>
 __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params p) {
@@ -292,8 +297,8 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
   const int K = p.drafts, V = p.vocab;
   wait_prior_grid();
 
-  const Part* t_parts = p.parts + b * (K + 1) * p.runs;
-  const Part* d_parts = p.parts + ((int64_t)p.batch * (K + 1) + b * K) * p.runs;
+  const Part* t_parts = kept && !p.parts ? sh.parts : p.parts + b * (K + 1) * p.runs;
+  const Part* d_parts = kept && !p.parts ? sh.parts + K + 1 : p.parts + ((int64_t)p.batch * (K + 1) + b * K) * p.runs;
   auto t_row = [&](int j) { return (const T*)p.target + b * p.t_batch + j * p.t_pos; };
   auto d_row = [&](int j) { return (const T*)p.draft + b * p.d_batch + j * p.d_pos; };
   auto uniform = [&](int j, uint32_t& st) {
@@ -307,6 +312,22 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
     }
     return (double)u;
   };
+  if constexpr (kept) {
+    if (!p.parts) {  // short rows: a warp each, the targets, then the drafts
+      const int rows = p.draft ? 2 * K + 1 : K + 1;
+      for (int r = warp; r < rows; r += PICK_WARPS) {
+        const bool of_draft = r > K;
+        const int j = of_draft ? r - K - 1 : r;
+        const T* x = of_draft ? d_row(j) : t_row(j);
+        const float scale = of_draft ? p.d_scale : p.t_scale;
+        auto counts = [&] { return drafts_are_ids(p, b, of_draft ? j + 1 : j); };
+        Part part;
+        const bool some = p.greedy ? warp_run<T, 32, true>(x, V, 0, V, true, scale, lane, counts, part)
+                                   : warp_run<T, 32, false>(x, V, 0, V, true, scale, lane, counts, part);
+        if (some && lane == 0) sh.parts[r] = part;
+      }
+    }
+  }
   if (tid < 64) sh.powers[tid] = exp2(tid / 64.0);
   __syncthreads();
   const double* powers = sh.powers;
@@ -754,6 +775,16 @@ static int64_t rows_of(const MtrVerifyArgs& a) {
   return (int64_t)a.batch * (a.drafts + 1) + (a.draft_logits && a.do_sample ? (int64_t)a.batch * a.drafts : 0);
 }
 
+// Whether one launch does it all: there is a CTA for each sequence at once, and its
+// rows are short enough for it.  On the GPU that is up to 2 us slower, but a call costs
+// the host 2 us less, and such calls are bound by it (us on the GPU, one launch / two;
+// a call from Python takes 20.6 / 22.7): 1 x 4 drafts, V = 4096 fp32 11.4 / 10.6, 64 x
+// 8, 4096 bf16 16.3 / 14.2, 1 x 8, 600 bf16 9.3 / 10.3; more rows than that pay there
+// too: 256 x 8, 4096 bf16 32.0 / 29.9.
+static bool in_one(int64_t batch, int64_t rows, int vocab, int es) {
+  return batch <= device_sms() && vocab <= FEW * KEPT && rows * vocab * es <= 160 * 1024;
+}
+
 template <typename K>
 static cudaError_t launch(K kern, const Params& p, dim3 grid, int threads, int cluster, cudaStream_t s) {
   cudaLaunchConfig_t cfg;
@@ -774,6 +805,12 @@ static cudaError_t launch_all(Params p, int64_t rows, cudaStream_t s) {
   p.run = g.run;
   const dim3 grid((unsigned)rows, (unsigned)g.runs, 1);
   cudaError_t e;
+  if (in_one(p.batch, rows / p.batch, p.vocab, sizeof(T))) {
+    p.parts = nullptr;
+    p.runs = 1;
+    p.cluster = 1;
+    return launch(pick_kernel<T, true>, p, dim3((unsigned)p.batch, 1, 1), FEW, 1, s);
+  }
   if (g.threads == 128)
     e = p.greedy ? launch(rows_kernel<T, 128, true>, p, grid, 128, 1, s) : launch(rows_kernel<T, 128, false>, p, grid, 128, 1, s);
   else

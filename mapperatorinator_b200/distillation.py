@@ -138,7 +138,7 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, 
     a = _args(logits, teacher_ids, teacher_logprobs, temperature, tail, status)
     g = _grad_losses(grad_losses, logits)
     if out is None:
-        out = logits.new_empty(logits.shape)
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
     elif out.dtype != logits.dtype or out.shape != logits.shape:
         raise ValueError("out must have the logits' shape and dtype")
     a.grad_row_stride = matrix(out, "out")
