@@ -188,13 +188,15 @@ __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
 // so that the others' waits give up too; the producer then gives its copies time
 // to land, the epilogue writes NaN for what was not computed, and the CTA returns.
 //
-// What bounds it (8192 x 4096 -> 16384: 530 us, quantisation included; clock stamps): a
-// block takes about 890 clocks, of which its products need 590.  Two accumulators of
-// 256 columns are all that tensor memory holds; from the issue of a pair's products to
-// the epilogue's seeing them done pass 1250 clocks, then 220 to read and add them and
-// 340 until the next products are issued: 1800 for two blocks.  With a quarter of the
-// products it still takes 441 us.  A CTA alone sees its products done in 850 clocks, but
-// takes 48 KB a block out of L2 instead of 32: 563 us.
+// What bounds it (8192 x 4096 -> 16384: 530 .. 577 us by the clock that power leaves,
+// quantisation included; clock stamps): a block takes 875 clocks, of which the tensor
+// core is busy 55 %.  The epilogue's own chain of a block -- see it done 140 at least,
+// read, add and hand over 470, the rest of its loop 155 -- takes 730 even where no
+// product is issued, and two accumulators of 256 columns are all that tensor memory
+// holds.  Sums are scalar: packed ones cost a move each (750 -> 605 us with the scales'
+// ring).  Not faster: 16 epilogue warps of 64 columns (700; no registers left), tiles of
+// 128 columns and four accumulators (763), halves of a product handed over one by one
+// (685: N = 128 waits for shared memory), one warp that polls for all (757).
 constexpr int RING = 4;  // blocks whose scales are in shared memory
 
 template <int BYTES>
@@ -656,7 +658,7 @@ static cudaError_t launch_proj(const MtrLmHeadF8Args& a, const Held& h, cudaStre
   if (tiles(128) <= sms) return launch_tiles<1, 128, Tout>(a, h, s);
   const int64_t n = (a.vocab + 255) / 256, pairs = sms / 2;
   const int64_t rounds = (m * n + sms - 1) / sms, pair_rounds = ((m + 1) / 2 * n + pairs - 1) / pairs;
-  // a round of pairs was taken to need 12/13 of the time; the two are within 3 % where they are close
+  // pairs where they need no more rounds than 13/12 of the others'; near that the two are within 3 %
   if (m == 1 || 12 * pair_rounds > 13 * rounds || (rounds <= 2 && a.d_model <= 2048)) return launch_tiles<1, 256, Tout>(a, h, s);
   return launch_tiles<2, 256, Tout>(a, h, s);
 }
