@@ -614,11 +614,11 @@ typedef struct MtrVerifyArgs {
   int32_t* out_accepted;        /* [batch]: accepted drafts */
   float* out_logprobs;          /* [batch, drafts + 1] or NULL: log p of the tokens, 0 for padding */
   uint32_t* out_status;         /* [batch] MTR_ROW_* bits or NULL */
-  void* workspace;              /* 16-byte aligned; one call's at a time */
+  void* workspace;              /* 16-byte aligned; one call's at a time; may be NULL where 0 bytes are needed */
   int64_t workspace_bytes;      /* >= mtr_verify_workspace(...) */
 } MtrVerifyArgs;
 
-/* Workspace bytes of a call (0 for batch <= 0). */
+/* Workspace bytes of a call (0 for few short rows, and for batch <= 0). */
 int64_t mtr_verify_workspace(int32_t batch, int32_t drafts, int32_t vocab, int32_t logits_dtype);
 int mtr_verify_validate(const MtrVerifyArgs* args);
 int mtr_verify_launch(const MtrVerifyArgs* args, void* stream);

@@ -755,9 +755,9 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
 static int esize(int32_t dtype) { return dtype == MTR_DTYPE_F32 ? 4 : 2; }
 
 // Runs of a row (a CTA each), and vectors of a run: rows are split until there are
-// four CTAs an SM (148 SMs) or a run is a tile.  The workspace goes by it, so it
-// asks no device.
-constexpr int64_t ENOUGH = 4 * 148;
+// four CTAs an SM or a run is a tile.  The workspace goes by this and by in_one, so
+// they ask no device.
+constexpr int64_t SMS = 148, ENOUGH = 4 * SMS;
 struct Shape {
   int threads, runs, run;
 };
@@ -777,12 +777,12 @@ static int64_t rows_of(const MtrVerifyArgs& a) {
 
 // Whether one launch does it all: there is a CTA for each sequence at once, and its
 // rows are short enough for it.  On the GPU that is up to 2 us slower, but a call costs
-// the host 2 us less, and such calls are bound by it (us on the GPU, one launch / two;
-// a call from Python takes 20.6 / 22.7): 1 x 4 drafts, V = 4096 fp32 11.4 / 10.6, 64 x
-// 8, 4096 bf16 16.3 / 14.2, 1 x 8, 600 bf16 9.3 / 10.3; more rows than that pay there
-// too: 256 x 8, 4096 bf16 32.0 / 29.9.
+// the host 4 us less (a launch, and no workspace), and such calls are bound by it (us
+// on the GPU, one launch / two; a call from Python takes 18.9 / 22.7): 1 x 4 drafts, V =
+// 4096 fp32 11.4 / 10.6, 64 x 8, 4096 bf16 16.3 / 14.2, 1 x 8, 600 bf16 9.3 / 10.3; more
+// rows than that pay there too: 256 x 8, 4096 bf16 32.0 / 29.9.
 static bool in_one(int64_t batch, int64_t rows, int vocab, int es) {
-  return batch <= device_sms() && vocab <= FEW * KEPT && rows * vocab * es <= 160 * 1024;
+  return batch <= SMS && vocab <= FEW * KEPT && rows * vocab * es <= 160 * 1024;
 }
 
 template <typename K>
@@ -833,6 +833,7 @@ using namespace mtr::vf;
 int64_t mtr_verify_workspace(int32_t batch, int32_t drafts, int32_t vocab, int32_t logits_dtype) {
   if (batch <= 0 || drafts < 0 || vocab <= 0) return 0;
   const int es = esize(logits_dtype);
+  if (in_one(batch, 2 * (int64_t)drafts + 1, vocab, es)) return 0;
   const int64_t targets = (int64_t)batch * (drafts + 1), both = targets + (int64_t)batch * drafts;
   const int64_t a = targets * shape_for(targets, vocab, es).runs, b = both * shape_for(both, vocab, es).runs;
   return (a > b ? a : b) * (int64_t)sizeof(Part);
@@ -850,12 +851,12 @@ int mtr_verify_validate(const MtrVerifyArgs* a) {
   for (double t : temps)
     if (!(t > 0.0) || !(t <= (double)MTR_MAX_TEMPERATURE) || !((float)(1.4426950408889634 / t) < INFINITY)) return MTR_ERR_BAD_PARAM;
   if (a->batch == 0) return MTR_OK;
-  if (!a->target_logits || !a->out_tokens || !a->out_accepted || !a->workspace) return MTR_ERR_NULL_ARG;
+  const int64_t need = mtr_verify_workspace(a->batch, a->drafts, a->vocab, a->logits_dtype);
+  if (!a->target_logits || !a->out_tokens || !a->out_accepted || (need > 0 && !a->workspace)) return MTR_ERR_NULL_ARG;
   if ((a->drafts > 0 && !a->draft_ids) || (a->do_sample && !a->uniforms)) return MTR_ERR_NULL_ARG;
   if (a->target_pos_stride < a->vocab || a->target_batch_stride < 0) return MTR_ERR_BAD_SHAPE;
   if (a->draft_logits && (a->draft_pos_stride < a->vocab || a->draft_batch_stride < 0)) return MTR_ERR_BAD_SHAPE;
   if (a->ids_row_stride < 0 || a->uniforms_row_stride < 0) return MTR_ERR_BAD_SHAPE;
-  const int64_t need = mtr_verify_workspace(a->batch, a->drafts, a->vocab, a->logits_dtype);
   if (a->workspace_bytes < need) return MTR_ERR_BAD_SHAPE;
   const int es = esize(a->logits_dtype);
   if ((uintptr_t)a->target_logits % es || (uintptr_t)a->draft_logits % es || (uintptr_t)a->draft_ids % (a->ids_dtype == MTR_IDS_I64 ? 8 : 4) ||
@@ -868,7 +869,7 @@ int mtr_verify_validate(const MtrVerifyArgs* a) {
                                                               run(a->out_logprobs, 4 * all), run(a->out_status, 4ll * a->batch)};
   for (const mtr::Bytes& o : outs) {
     if (!o.at) continue;
-    if (overlap(o, work)) return MTR_ERR_BAD_PARAM;
+    if (need > 0 && overlap(o, work)) return MTR_ERR_BAD_PARAM;
     if (a->drafts > 0 && overlap(o, mtr::bytes_of(a->draft_ids, a->ids_row_stride ? a->batch : 1, a->ids_row_stride ? a->ids_row_stride : a->drafts,
                                                   a->drafts, a->ids_dtype == MTR_IDS_I64 ? 8 : 4)))
       return MTR_ERR_BAD_PARAM;

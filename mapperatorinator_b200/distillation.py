@@ -111,7 +111,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
     ``status`` (int32 ``[R]``) receives the row bits that
     :func:`~mapperatorinator_b200.sampling.row_status_report` reads.  Gradients flow
-    to the logits (once, in reverse mode)."""
+    to the logits (once, in reverse mode).  A step that is to be captured in a CUDA
+    graph takes :func:`distillation_loss_and_grad`: autograd's backward must not be
+    captured while an eager graph of the same leaves is alive."""
     _no_tangent(logits, teacher_logprobs)
     if torch.is_grad_enabled():
         if teacher_logprobs.requires_grad:

@@ -116,9 +116,10 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     new = target_logits.new_empty
     tokens, accepted = new((batch, more), dtype=torch.int64), new(batch, dtype=torch.int32)
     logprobs = new((batch, more), dtype=torch.float32)
-    need = N.verify_workspace(batch, drafts, vocab, a.logits_dtype)
-    work = new(need, dtype=torch.uint8)
     a.out_tokens, a.out_accepted, a.out_logprobs = tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr()
-    a.workspace, a.workspace_bytes = work.data_ptr(), need
+    need = N.verify_workspace(batch, drafts, vocab, a.logits_dtype)  # 0 for few short rows
+    if need:
+        work = new(need, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
     launch_on(device, N.verify_launch, a)
     return Verified(tokens, accepted, logprobs)

@@ -160,12 +160,13 @@ def _args(**kw):
     (dict(temperature=0.0), N.ERR_BAD_PARAM), (dict(temperature=math.nan), N.ERR_BAD_PARAM), (dict(draft_temperature=-1.0), N.ERR_BAD_PARAM),
     (dict(draft_temperature=math.inf), N.ERR_BAD_PARAM), (dict(temperature=1e-40), N.ERR_BAD_PARAM),
     (dict(target_logits=None), N.ERR_NULL_ARG), (dict(draft_ids=None), N.ERR_NULL_ARG), (dict(uniforms=None), N.ERR_NULL_ARG),
-    (dict(out_tokens=None), N.ERR_NULL_ARG), (dict(out_accepted=None), N.ERR_NULL_ARG), (dict(workspace=None), N.ERR_NULL_ARG),
+    (dict(out_tokens=None), N.ERR_NULL_ARG), (dict(out_accepted=None), N.ERR_NULL_ARG), (dict(workspace=None, workspace_bytes=0), N.OK),
+    (dict(batch=149, workspace=None), N.ERR_NULL_ARG),
     (dict(target_pos_stride=99), N.ERR_BAD_SHAPE), (dict(draft_pos_stride=99), N.ERR_BAD_SHAPE), (dict(target_batch_stride=-1), N.ERR_BAD_SHAPE),
-    (dict(workspace_bytes=10 * 9 * 16 - 1), N.ERR_BAD_SHAPE), (dict(workspace_bytes=10 * 9 * 16), N.OK), (dict(workspace=0x5000008), N.ERR_ALIGNMENT),
+    (dict(batch=149, workspace_bytes=149 * 9 * 16 - 1), N.ERR_BAD_SHAPE), (dict(batch=149, workspace_bytes=149 * 9 * 16), N.OK), (dict(workspace=0x5000008), N.ERR_ALIGNMENT),
     (dict(target_logits=0x1000001), N.ERR_ALIGNMENT), (dict(draft_ids=0x3000004), N.ERR_ALIGNMENT), (dict(uniforms=0x3100002), N.ERR_ALIGNMENT),
     (dict(out_tokens=0x4000004), N.ERR_ALIGNMENT), (dict(out_tokens=0x3000000), N.ERR_BAD_PARAM), (dict(out_tokens=0x3100000), N.ERR_BAD_PARAM),
-    (dict(out_logprobs=0x5000000), N.ERR_BAD_PARAM), (dict(struct_size=8), N.ERR_ABI), (dict(abi_version=1), N.ERR_ABI)])
+    (dict(batch=149, out_logprobs=0x5000000), N.ERR_BAD_PARAM), (dict(struct_size=8), N.ERR_ABI), (dict(abi_version=1), N.ERR_ABI)])
 def test_arguments_are_checked_on_the_host(kw, code):
     a = _args(**{k: v for k, v in kw.items() if k not in ("struct_size", "abi_version")})
     for k, v in kw.items():
@@ -178,7 +179,8 @@ def test_arguments_are_checked_on_the_host(kw, code):
 
 def test_workspace_sizes():
     assert N.verify_workspace(0, 4, 100, 0) == 0 and N.verify_workspace(3, -1, 100, 0) == 0
-    assert N.verify_workspace(64, 4, 4096, N.DTYPE_BF16) == 64 * 9 * 16  # a run a row
+    assert N.verify_workspace(64, 4, 4096, N.DTYPE_BF16) == 0             # one launch for all
+    assert N.verify_workspace(64, 8, 8192, N.DTYPE_BF16) == 64 * 17 * 16  # a run a row
     assert N.verify_workspace(1, 0, 131072, N.DTYPE_F32) == 16 * 16      # 16 runs
     assert N.verify_workspace(N.MAX_VERIFY_BATCH, N.MAX_DRAFTS, 131072, 0) == (257 << 20) * 16
 
