@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const Params p) 
   if (warp == 0) {
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
-      if (lead[k] && ((id[k] >= from && id[k] < to) || id[k] >= last)) g[id[k]] = from_f<T>((float)(ej[k] * q_scale - pj[k] * own_scale));
+      if (lead[k] && ((id[k] >= from && id[k] < to) || id[k] >= last)) g[id[k]] = from_f<T>(empty ? 0.0f : (float)(ej[k] * q_scale - pj[k] * own_scale));
   }
 }
 

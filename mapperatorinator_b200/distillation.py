@@ -104,8 +104,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
       below 2^-20 is the rounding of the given log probabilities and counts as 0.)
     - An id below 0 is no entry; so is one >= V, which also sets the row's ``bad_id``
       bit; a log probability of -inf is probability 0.  A row without entries (a
-      padded position) has loss 0 and gradient 0, whatever its logits hold.  An id
-      that is given twice is two entries.
+      padded position; with ``tail=False`` also one whose entries all have probability
+      0) has loss 0 and gradient 0, whatever its logits hold.  An id that is given
+      twice is two entries.
     - Where the student has no mass and the teacher has some the loss is +inf; a row
       with a NaN or +inf reads NaN; one with every logit masked has gradient 0.
 

@@ -273,6 +273,23 @@ def test_rows_that_masks_and_values_make_odd(cuda_device, dtype, tail, vocab, n)
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [3, 40])
+def test_entries_without_probability_whatever_the_logits_hold(cuda_device, dtype, n):
+    logits, ids, lps, w = inputs(cuda_device, 4, 500, n, dtype)
+    lps[:3] = -math.inf
+    logits[0, ids[0, 1]] = math.nan
+    logits[1, ids[1, 0]] = math.inf
+    logits[2] = math.nan
+    loss, grad = distillation_loss_and_grad(logits, ids, lps, w)
+    leaf = logits.clone().requires_grad_(True)
+    (distillation_loss(leaf, ids, lps) * w).sum().backward()
+    for g in (grad, leaf.grad):
+        assert torch.equal(g[:3], torch.zeros_like(g[:3])) and g[3].any()
+    assert torch.equal(loss[:3], torch.zeros_like(loss[:3])) and loss[3].isfinite()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("n", [4, 32, 70])
 def test_ids_given_twice(cuda_device, dtype, tail, n):
