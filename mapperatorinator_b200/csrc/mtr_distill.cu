@@ -23,8 +23,9 @@
 // work of S in double goes on in the first warp while the row is under way.  Losses
 // alone run at 5.9 TB/s (1024 x 131072 fp32, 90.8 us); with gradients of 2-byte rows
 // the instructions bound it (two exponentials, an unpacking and a packing a logit):
-// 8192 x 4096 bf16 34.9 us where its bytes take 20.8 at HBM's copy rate, 2000 x 65533 128
-// where they take 80.
+// 8192 x 4096 bf16 34.3 us where its bytes take 20.8 at HBM's copy rate, 2000 x 65533 125
+// where they take 80.  Some 6 us of the 34 are the rows' work in double, which makes do
+// with one division and one logarithm a lane (35.8 with each formed apart).
 #include "mtr_vec.cuh"
 
 namespace mtr {
@@ -262,7 +263,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const Params p) 
   // What needs no sum, by the first warp: the teacher's probabilities, and the terms
   // of S about its largest logit x_s.
   constexpr double NAN_D = 0.0 / 0.0;
-  double pj[SLOTS], ej[SLOTS], mass = 0.0, rest = 0.0, in = 0.0, cross = 0.0;
+  // The teacher's are left divided by `whole` until one division serves the row.
+  double pj[SLOTS], ej[SLOTS], mass = 0.0, rest = 0.0, in = 0.0, cross = 0.0, whole = 1.0;
   float x_s = neg_inf();
   bool empty = false, odd = false, bad_s = false;
   if (warp == 0) {
@@ -297,21 +299,17 @@ __global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const Params p) 
     }
     mass = warp_sum(mass);
     in = warp_sum(in);
-    double log_mass = 0.0;
     if (p.tail) {
       rest = 1.0 - mass;
       if (rest < LEAST_REST) rest = 0.0;
-    } else if (!empty) {
-      log_mass = shift + log(mass);
-      const double over = 1.0 / mass;
-#pragma unroll
-      for (int k = 0; k < SLOTS; ++k) pj[k] *= over;
+    } else if (!empty && !odd) {
+      whole = mass;
       mass = 1.0;
     }
     if (SCAN && p.loss) {
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
-        if (pj[k] > 0.0) cross += pj[k] * (((double)lp[k] - log_mass) - ((double)xs[k] - about) * p.inv_t);
+        if (pj[k] > 0.0) cross += pj[k] * (((double)lp[k] - shift) - ((double)xs[k] - about) * p.inv_t);
       cross = warp_sum(cross);
     }
   }
@@ -364,15 +362,18 @@ __global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const Params p) 
     // both sums about the larger of m_rest and x_s
     const double apart = some && x_s > neg_inf() ? ((double)m_rest - (double)x_s) * p.inv_t : 0.0, shrink = exp(-fabs(apart));
     const double in_part = apart > 0.0 ? in * shrink : in, rest_part = some ? (apart < 0.0 ? sum_rest * shrink : sum_rest) : 0.0;
-    const double all = in_part + rest_part, over_all = 1.0 / all;
+    const double all = in_part + rest_part;
+    // one division for three: all >= 1 or there is nothing, sum_rest >= 1 or there is no rest, whole in [1, n]
+    const double sum_1 = some && !bad ? sum_rest : 1.0, inv = 1.0 / (all * sum_1 * whole), over_all = inv * (sum_1 * whole);
+    const double over_rest = inv * (all * whole), over_whole = p.tail ? 1.0 : inv * (all * sum_1);
     if constexpr (GRAD) {
       const double g = (p.g_loss ? (double)p.g_loss[row] : 1.0) * p.inv_t;
       // e = 2^((x - m_rest) scale): q = e rest_part / (sum_rest all), q / q_t = e / sum_rest
       double c = 0.0;
-      if (!empty && !none && some) c = g * (mass * (rest_part * over_all) - rest * (in_part * over_all)) / sum_rest;
+      if (!empty && !none && some) c = g * (mass * (rest_part * over_all) - rest * (in_part * over_all)) * over_rest;
       if (!empty && (bad || odd)) c = NAN_D;
       q_scale = empty || none ? 0.0 : g * (mass + rest) * over_all * (apart > 0.0 ? shrink : 1.0);
-      own_scale = empty || none ? 0.0 : g;
+      own_scale = empty || none ? 0.0 : g * over_whole;
       if (bad || odd) q_scale = empty ? 0.0 : NAN_D;
       if (lane == 0) {
         sh.row_m = some && !empty && !bad ? m_rest : 0.0f;
@@ -380,13 +381,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const Params p) 
       }
     }
     if constexpr (GRAD && THREADS > 32) sync();  // the others go on with the gradient
-    if (SCAN && p.loss && lane == 0 && rank == 0) {
-      // log sum about x_s: log q_j = (x_j - x_s) / T - log_s
-      const double log_s = none ? 0.0 : log(all) + (apart > 0.0 ? apart : 0.0);
-      double loss = cross + mass * log_s;
+    if (SCAN && p.loss && rank == 0) {
+      // log sum about x_s: log q_j = (x_j - x_s) / T - log_s, and log p_j = l_j - shift - log whole; a lane each
+      // takes the logarithms of all / whole and of what the tail needs
+      const double logs = log(lane == 0 ? all * over_whole : rest * over_rest), log_tail = __shfl_sync(FULL, logs, 1);
+      const double log_s = none ? 0.0 : logs + (apart > 0.0 ? apart : 0.0);
+      double loss = cross * over_whole + mass * log_s;
       if (!(x_s > neg_inf()) && mass > 0.0) loss = (double)pos_inf();
-      if (rest > 0.0) loss += some ? rest * (log(rest) - (log(sum_rest) - log(all) + fmin(apart, 0.0))) : (double)pos_inf();
-      p.loss[row] = empty ? 0.0f : bad || odd ? (float)NAN_D : (float)loss;
+      if (rest > 0.0) loss += some ? rest * (log_tail + logs - fmin(apart, 0.0)) : (double)pos_inf();
+      if (lane == 0) p.loss[row] = empty ? 0.0f : bad || odd ? (float)NAN_D : (float)loss;
     }
     if (SCAN && lane == 0 && rank == 0 && p.stats) p.stats[row] = make_double2((double)m_rest, sum_rest);
     if (SCAN && p.status) {
@@ -499,17 +502,19 @@ static cudaError_t launch(const Params& p, int64_t rows, bool scan, cudaStream_t
 // Threads of a row, by how many rows there are to fill the device's 16 warps an SM
 // and how long they are; CTAs share a row only where they give idle SMs work.
 // Loss and gradient together, with 20 ids (us, 32 / 128 / 256 threads, 148 SMs):
-//   8192 x 1000 bf16    17.3 / 44.8 / 73.3     enough rows: a warp each
-//   8192 x 4096 bf16    35.1
-//   3000 x 4096 fp32    23.8 / 25.4 / 34.0
-//   1000 x 4096 bf16    10.8 /  8.6 / 13.6     few rows: more warps each
-//   2000 x 16384 bf16   44.3 / 33.1 / 39.8     long rows: 128 threads, then 256
-//   300 x 16384 fp32    38.7 / 15.7 / 12.5
-//   2000 x 65533 bf16               / 125.6, 512 threads 123.8
+//   8192 x 1000 bf16    14.9 / 39.5 / 64.2     enough rows: a warp each
+//   8192 x 4096 bf16    34.4 / 47.3 / 75.4
+//   8192 x 8192 bf16    63.0 / 71.7 / 85.0
+//   3000 x 4096 fp32    23.3 / 24.2 / 31.2
+//   1000 x 4096 bf16    10.2 /  7.9 / 12.2     few rows: more warps each
+//   2000 x 16384 bf16   44.3 / 32.5 / 38.0     long rows: 128 threads, then 256
+//   3000 x 32768 bf16    108 / 91.3 / 85.1
+//   300 x 16384 fp32    38.6 / 15.4 / 12.3
+//   2000 x 65533 bf16    181 /  135 /  124, 512 threads 125
 template <typename T>
 static cudaError_t launch(Params p, int64_t rows, bool scan, cudaStream_t s) {
   const int64_t vecs = (int64_t)p.vocab * (int)sizeof(T) / 16, sms = device_sms();
-  int threads = vecs > 4096 ? 256 : vecs > 1024 ? 128 : 32;
+  int threads = vecs > 2560 ? 256 : vecs > 1024 ? 128 : 32;
   while (threads < MOST_THREADS && rows * threads < 16 * 32 * sms && vecs >= 8 * threads) threads *= threads == 32 ? 4 : 2;
   p.cluster = 1;
   while (threads == MOST_THREADS && p.cluster < 8 && scan && vecs >= 2ll * HELD * MOST_THREADS * p.cluster && rows * p.cluster * 2 <= sms)
