@@ -233,7 +233,10 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 constexpr int FEW = 512, MANY = 512;
 constexpr int KEPT = 8;  // ids of a thread whose terms stay in registers
 constexpr int NEAR = 64; // ids of a warp next to the border between p > q and p < q
-constexpr double NOTHING = 0x1p-900;  // a sum of ids without weight stays below it
+// A sum of weights by term() is above this where an id has weight: n ids without any add
+// at most n 2^-1000.  A CTA's share above NOTHING has a warp's piece above LITTLE.
+// Sums by term_or_0 are 0 there.
+constexpr double NOTHING = 0x1p-900, LITTLE = 0x1p-910;
 
 // e^((x - m) / T) in double, x <= m finite or -inf: with c = 64 log2(e) / T,
 // z = (x - m) c = k + r, k whole and |r| <= 1/2, the value is 2^(k / 64) 2^(r / 64): a
@@ -649,16 +652,16 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
       }
       return w;
     };
-    // first piece of n whose running sum passes u (or the last that has any): its index, and the sum before it
-    auto choose = [](auto piece, int n, double u, double& before) {
+    // first piece of n whose running sum passes u (or the last that has any): its index,
+    // and the sum before it.  What has none (w <= none) is passed over: u may be 0.
+    auto choose = [](auto piece, int n, double u, double none, double& before) {
       double run = before, at = before;
       int last = 0;
       for (int k = 0; k < n; ++k) {
         const double w = piece(k);
-        if (w > NOTHING) {
-          last = k;
-          at = run;
-        }
+        if (!(w > none)) continue;
+        last = k;
+        at = run;
         run += w;
         if (run > u) break;
       }
@@ -674,12 +677,12 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
     double before = 0.0;
     int owner = 0;
     if (cs > 1) {
-      owner = choose([&](int k) { return cluster.map_shared_rank(&sh, k)->weight; }, cs, u, before);
+      owner = choose([&](int k) { return cluster.map_shared_rank(&sh, k)->weight; }, cs, u, kept ? 0.0 : NOTHING, before);
       cluster.sync();
       if (rank != owner) return;
     }
     // the piece that decides: a warp's, where terms are kept; else one that is weighed again by runs of a thread
-    int k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
+    int k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, kept ? 0.0 : LITTLE, before);
     double w[MOST], mine = 0.0;
     if constexpr (kept) {
 #pragma unroll
@@ -703,7 +706,7 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
       __syncthreads();
       if (lane == 0) sh.piece[warp] = sum;
       __syncthreads();
-      k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, before);
+      k = choose([&](int k) { return sh.piece[k]; }, PICK_WARPS, u, 0.0, before);
     }
     if (warp == k) {
       double up = mine;  // running sums of the lanes

@@ -452,3 +452,42 @@ def test_same_tokens_on_another_stream_and_in_graphs(cuda_device, batch, vocab):
             t.copy_(new)
         graph.replay()
         assert torch.equal(r.tokens, w.tokens) and torch.equal(r.accepted, w.accepted) and torch.equal(r.logprobs, w.logprobs)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,vocab", [(40, 20001), (2, 131072), (1, 9001), (150, 5000), (64, 4096), (3, 131072), (200, 300)])
+@pytest.mark.parametrize("how", ["behind the drafts", "looked up", "refused", "no draft"])
+def test_uniform_0_behind_masked_ids(cuda_device, dtype, batch, vocab, how):
+    """The smallest id with any weight, although every id of the first half is masked; torch.rand draws 0 too."""
+    target, ids, draft, u = inputs(cuda_device, batch, 1, vocab, dtype, seed=vocab)
+    first = vocab // 2 + 3
+    target[:, :, :first] = -math.inf
+    draft[:, :, :first] = -math.inf
+    gap = draft[:, 0].float() - target[:, 0].float()
+    gap[:, :first] = -math.inf
+    ids[:, 0] = gap.argmax(1)  # an id that the draft gives too much
+    u[:, 0] = 0.0 if how == "behind the drafts" else 1.0 - 2.0 ** -24
+    u[:, 1] = 0.0
+    u[::3, 1] = -1.0
+    if how == "no draft":
+        ids[:] = -1
+    r = check(target, ids, None if how == "looked up" else draft, u, pad=-7)
+    assert bool((r.accepted == (1 if how == "behind the drafts" else 0)).all()) or how == "looked up"
+
+
+@gpu
+@pytest.mark.parametrize("batch,vocab", [(40, 20001), (2, 131072), (64, 4096), (200, 300)])
+@pytest.mark.parametrize("below", [600.0, 630.0, 650.0, 680.0])
+def test_uniform_0_and_weights_next_to_nothing(cuda_device, batch, vocab, below):
+    """Ids of probability e^-600 and less behind masked ones: with a uniform of 0 the border is within double's rounding of
+    many ids, but the token is one that has some weight."""
+    target, ids, _, u = inputs(cuda_device, batch, 1, vocab, torch.float32, seed=vocab)
+    a, z = vocab // 4, vocab // 2
+    target[:, :, :a] = -math.inf
+    target[:, :, a:z] = -below
+    u[:, 1] = 0.0
+    status = torch.full((batch,), -1, dtype=torch.int32, device=cuda_device)
+    r = verify_drafts(target, torch.full_like(ids, -1), None, uniforms=u, pad_token_id=-7, status=status)
+    assert bool((r.tokens[:, 0] >= a).all()) and bool((r.tokens[:, 0] <= z + target[:, 0, z:].isfinite().float().argmax(1)).all())
+    assert bool((status == 0).all())
