@@ -604,9 +604,12 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
     token_s = s.t;
     const double over_t = 1.0 / s.t, over_d = y ? 1.0 / s.d : 0.0;
     bool from_p = false;
-    auto weight = [&](int v, double e, double q) {  // of id v from its two terms
+    // p - q of an id from its two terms, each rounded by itself: 0 where they are equal (a
+    // fused product would leave its rounding, and a token be drawn from that)
+    auto apart = [&](double e, double q) { return __dsub_rn(__dmul_rn(e, over_t), __dmul_rn(q, over_d)); };
+    auto weight = [&](int v, double e, double q) {  // of id v
       if (from_p) return e * over_t;
-      return v == hot ? 0.0 : fmax(fma(e, over_t, -(q * over_d)), 0.0);
+      return v == hot ? 0.0 : fmax(apart(e, q), 0.0);
     };
     // the CTA's weight by pieces of a warp each, in sh.piece; the sum over the cluster
     auto weigh = [&]() {
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
       } else {
         if (y && !from_p) {
           stream(x, y, from, to, [&](int, float xv, float yv) {
-            const double one = fma(term(xv, te, powers), over_t, -(term(yv, de, powers) * over_d));
+            const double one = apart(term(xv, te, powers), term(yv, de, powers));
             if (__double2hiint(one) >= 0) w += one;
           });
         } else {

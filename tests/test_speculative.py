@@ -491,3 +491,16 @@ def test_uniform_0_and_weights_next_to_nothing(cuda_device, batch, vocab, below)
     r = verify_drafts(target, torch.full_like(ids, -1), None, uniforms=u, pad_token_id=-7, status=status)
     assert bool((r.tokens[:, 0] >= a).all()) and bool((r.tokens[:, 0] <= z + target[:, 0, z:].isfinite().float().argmax(1)).all())
     assert bool((status == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,vocab", [(1, 7), (40, 4096), (200, 1000), (8, 4099), (80, 4099), (3, 131072), (80, 20001), (1, 65533)])
+def test_a_draft_that_is_the_target_and_could_not_be_drafted(cuda_device, dtype, batch, vocab):
+    """p - q is 0 everywhere, and the token comes from p."""
+    target, ids, _, u = inputs(cuda_device, batch, 2, vocab, dtype, seed=vocab)
+    ids[:, 0] = torch.arange(batch, device=cuda_device) % vocab
+    target[:, 0].scatter_(1, ids[:, :1], -math.inf)
+    u[:, 2] = (torch.arange(batch, device=cuda_device) + 0.37) / batch
+    r = check(target, ids, target[:, :2].clone(), u)
+    assert bool((r.accepted == 0).all())
