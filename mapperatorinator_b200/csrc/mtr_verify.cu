@@ -726,9 +726,11 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
         bool open = true;
 #pragma unroll
         for (int i = 0; i < MOST; ++i) {
-          run += w[i];
-          if (open && w[i] > 0.0) last = a + i;
-          if (run > u) open = false;
+          run += w[i];  // rounded otherwise than the lanes' sums: it may pass u before an id with weight
+          if (open && w[i] > 0.0) {
+            last = a + i;
+            open = !(run > u);
+          }
         }
         sh.token = last;
       }

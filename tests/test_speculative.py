@@ -504,3 +504,26 @@ def test_a_draft_that_is_the_target_and_could_not_be_drafted(cuda_device, dtype,
     u[:, 2] = (torch.arange(batch, device=cuda_device) + 0.37) / batch
     r = check(target, ids, target[:, :2].clone(), u)
     assert bool((r.accepted == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,batch", [(300, 200), (513, 96), (1000, 96), (4096, 96), (4096, 8), (20001, 80), (131072, 24), (131072, 2)])
+def test_uniforms_on_the_borders_of_equal_ids(cuda_device, dtype, vocab, batch):
+    """n equally probable ids between masked ones and u = j / 16 with u n whole: the border lies on the running sum of
+    u n ids, so rounding decides between two neighbours, and a masked id or none is neither."""
+    g = torch.Generator(device=cuda_device).manual_seed(vocab)
+    keep = torch.rand((batch, vocab), generator=g, device=cuda_device) < 0.3 + 0.4 * torch.rand((batch, 1), generator=g, device=cuda_device)
+    rank = torch.cumsum(keep, 1)
+    keep &= rank <= rank[:, -1:] // 16 * 16
+    n = keep.sum(1)
+    rank = torch.cumsum(keep, 1) - 1  # of an id among those that are left
+    target = torch.where(keep, 0.25, -math.inf)[:, None].to(dtype)
+    none = torch.empty((batch, 0), dtype=torch.int64, device=cuda_device)
+    for j in range(16):
+        u = torch.full((batch, 1), j / 16, device=cuda_device)
+        token = verify_drafts(target, none, uniforms=u, pad_token_id=-7).tokens
+        assert bool((token >= 0).all())
+        assert bool(keep.gather(1, token).all())
+        off = rank.gather(1, token)[:, 0] - n * j // 16
+        assert bool(((off == 0) | (off == -1)).all())
