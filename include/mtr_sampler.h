@@ -586,7 +586,8 @@ int mtr_distill_launch(const MtrDistillArgs* args, void* stream);
  * target row with NaN or +inf (MTR_ROW_NONFINITE) or of -inf alone
  * (MTR_ROW_ALL_MASKED) at the position that decides gives pad_id; such a draft
  * row refuses its token and is drawn from p (same bits).  Positions behind the
- * one that decides are not looked at.
+ * one that decides are not looked at.  Outputs and workspace must not overlap what
+ * is read.
  */
 typedef struct MtrVerifyArgs {
   uint32_t abi_version;         /* = MTR_ABI_VERSION */

@@ -1,5 +1,7 @@
 // mtr_vec.cuh -- rows of fp32, bf16 or fp16 values in 16-byte vectors: what the
-// kernels that stream such rows share (mtr_logprob.cu, mtr_lmhead_i8.cu).
+// kernels that stream such rows share (mtr_logprob.cu, mtr_distill.cu, mtr_verify.cu
+// and, through mtr_quant.cuh, the 8-bit projections), and how the bytes of their
+// arguments are compared.
 #pragma once
 
 #include "mtr_common.cuh"
@@ -32,6 +34,19 @@ inline bool overlap(const Bytes& a, const Bytes& b) {
   if (a.stride != b.stride) return true;
   const int64_t off = (int64_t)(b0 - a0) % a.stride, behind = off < 0 ? off + a.stride : off;  // from a row of a to the next of b
   return behind < a.width || behind + b.width > a.stride;
+}
+// Whether `n` bytes share one with an array of batch x positions rows of `width` bytes (strides in bytes; 0: one for all).
+inline bool meets(const void* at, int64_t n, const void* x, int64_t batch, int64_t batch_stride, int64_t positions, int64_t pos_stride,
+                  int64_t width) {
+  if (!x || width == 0) return false;
+  const int64_t a = (int64_t)(uintptr_t)at, x0 = (int64_t)(uintptr_t)x;
+  if (a + n <= x0 || a >= x0 + (batch - 1) * batch_stride + (positions - 1) * pos_stride + width) return false;
+  for (int64_t j = 0; j < positions; ++j) {
+    const int64_t first = x0 + j * pos_stride, past = a - (first + width);  // >= 0: the first row ends before `at`
+    const int64_t b = past < 0 ? 0 : batch_stride > 0 ? past / batch_stride + 1 : batch;
+    if (b < batch && first + b * batch_stride < a + n) return true;
+  }
+  return false;
 }
 
 // max that gives NaN when an operand is NaN

@@ -871,18 +871,23 @@ int mtr_verify_validate(const MtrVerifyArgs* a) {
       (uintptr_t)a->uniforms % 4 || (uintptr_t)a->out_tokens % 8 || (uintptr_t)a->out_accepted % 4 || (uintptr_t)a->out_logprobs % 4 ||
       (uintptr_t)a->out_status % 4 || (uintptr_t)a->workspace % 16)
     return MTR_ERR_ALIGNMENT;
-  const int64_t more = a->drafts + 1, all = a->batch * more;
-  auto run = [](const void* at, int64_t n) { return mtr::Bytes{at, 1, n, n}; };
-  const mtr::Bytes work = run(a->workspace, need), outs[4] = {run(a->out_tokens, 8 * all), run(a->out_accepted, 4ll * a->batch),
-                                                              run(a->out_logprobs, 4 * all), run(a->out_status, 4ll * a->batch)};
-  for (const mtr::Bytes& o : outs) {
-    if (!o.at) continue;
-    if (need > 0 && overlap(o, work)) return MTR_ERR_BAD_PARAM;
-    if (a->drafts > 0 && overlap(o, mtr::bytes_of(a->draft_ids, a->ids_row_stride ? a->batch : 1, a->ids_row_stride ? a->ids_row_stride : a->drafts,
-                                                  a->drafts, a->ids_dtype == MTR_IDS_I64 ? 8 : 4)))
+  // no sequence's results in what another has yet to read
+  const int64_t more = a->drafts + 1, all = a->batch * more, ids_size = a->ids_dtype == MTR_IDS_I64 ? 8 : 4;
+  struct Run {
+    const void* at;
+    int64_t n;
+  };
+  const Run outs[5] = {{a->workspace, need}, {a->out_tokens, 8 * all}, {a->out_accepted, 4ll * a->batch}, {a->out_logprobs, 4 * all},
+                       {a->out_status, 4ll * a->batch}};
+  for (const Run& o : outs) {
+    if (!o.at || o.n == 0) continue;
+    if (&o != outs && mtr::meets(o.at, o.n, a->workspace, 1, 0, 1, 0, need)) return MTR_ERR_BAD_PARAM;
+    if (mtr::meets(o.at, o.n, a->target_logits, a->batch, a->target_batch_stride * es, more, a->target_pos_stride * es, (int64_t)a->vocab * es) ||
+        mtr::meets(o.at, o.n, a->draft_ids, a->batch, a->ids_row_stride * ids_size, 1, 0, a->drafts * ids_size))
       return MTR_ERR_BAD_PARAM;
-    if (a->do_sample && overlap(o, mtr::bytes_of(a->uniforms, a->uniforms_row_stride ? a->batch : 1,
-                                                 a->uniforms_row_stride ? a->uniforms_row_stride : more, more, 4)))
+    if (a->do_sample &&
+        (mtr::meets(o.at, o.n, a->draft_logits, a->batch, a->draft_batch_stride * es, a->drafts, a->draft_pos_stride * es, (int64_t)a->vocab * es) ||
+         mtr::meets(o.at, o.n, a->uniforms, a->batch, a->uniforms_row_stride * 4, 1, 0, more * 4)))
       return MTR_ERR_BAD_PARAM;
   }
   return MTR_OK;

@@ -177,6 +177,34 @@ def test_arguments_are_checked_on_the_host(kw, code):
         assert lib.mtr_verify_launch(ctypes.byref(a), None) == code
 
 
+@pytest.mark.parametrize("field,need", [("out_tokens", 8 * 149 * 5), ("out_accepted", 4 * 149), ("out_logprobs", 4 * 149 * 5), ("out_status", 4 * 149),
+                                        ("workspace", 16 * 149 * 9)])
+def test_what_is_written_overlaps_nothing_that_is_read(field, need):
+    lib = N.load()
+    ok = dict(batch=149, out_logprobs=0x4200000, out_status=0x4300000)
+
+    def code(at, **kw):
+        return lib.mtr_verify_validate(ctypes.byref(_args(**{**ok, **kw, field: at})))
+
+    # the last byte of each input, and the first behind it
+    target_end = 0x1000000 + 2 * (148 * 500 + 4 * 100 + 100)
+    draft_end = 0x2000000 + 2 * (148 * 400 + 3 * 100 + 100)
+    ids_end, u_end = 0x3000000 + 8 * 149 * 4, 0x3100000 + 4 * 149 * 5
+    up = lambda v: (v + 15) // 16 * 16  # noqa: E731
+    for start, end in ((0x1000000, target_end), (0x2000000, draft_end), (0x3000000, ids_end), (0x3100000, u_end)):
+        inside = (end - 1) // 16 * 16
+        assert code(start) == N.ERR_BAD_PARAM and code(inside) == N.ERR_BAD_PARAM and code(start - up(need) + 16) == N.ERR_BAD_PARAM
+        assert code(up(end)) == N.OK and code(start - up(need)) == N.OK
+    # not read: the draft's logits and the uniforms of a greedy call, no draft's
+    assert code(0x2000000, do_sample=0) == N.OK and code(0x3100000, do_sample=0) == N.OK and code(0x2000000, draft_logits=None) == N.OK
+    # between rows and between positions
+    far = dict(target_logits=0x40000000, target_batch_stride=1 << 20, target_pos_stride=1 << 17)
+    assert code(0x40000000 + 208, **far) == N.OK and code(0x40000000 + (1 << 18) + 208, **far) == N.OK
+    assert code(0x40000000 + (1 << 21) * 3 + (1 << 18) * 2 + 192, **far) == N.ERR_BAD_PARAM
+    # one target for all sequences
+    assert code(0x1000000 + 992, target_batch_stride=0) == N.ERR_BAD_PARAM and code(0x1000000 + 1008, target_batch_stride=0) == N.OK
+
+
 def test_workspace_sizes():
     assert N.verify_workspace(0, 4, 100, 0) == 0 and N.verify_workspace(3, -1, 100, 0) == 0
     assert N.verify_workspace(64, 4, 4096, N.DTYPE_BF16) == 0             # one launch for all
