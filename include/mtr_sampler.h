@@ -538,7 +538,8 @@ int mtr_logprob_grad_launch(const MtrLogprobGradArgs* args, void* stream);
  * is given twice is two entries.  A row with NaN or +inf in the logits or its l
  * (MTR_ROW_NONFINITE) reads NaN; one whose logits are all -inf
  * (MTR_ROW_ALL_MASKED), or without mass where the teacher has some, +inf, the
- * former with gradient 0.
+ * former with gradient 0.  What is written must not overlap what is read, nor
+ * losses, stats and status the gradient.
  */
 typedef struct MtrDistillArgs {
   uint32_t abi_version;         /* = MTR_ABI_VERSION */

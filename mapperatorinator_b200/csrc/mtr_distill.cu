@@ -553,15 +553,31 @@ int mtr_distill_validate(const MtrDistillArgs* a) {
       (uintptr_t)a->teacher_logprobs % 4 || (uintptr_t)a->out_loss % 4 || (uintptr_t)a->stats % 16 ||
       (uintptr_t)a->g_loss % 4 || (uintptr_t)a->grad_logits % es || (uintptr_t)a->out_status % 4)
     return MTR_ERR_ALIGNMENT;
+  const int64_t ids_size = a->ids_dtype == MTR_IDS_I64 ? 8 : 4;
   if (a->grad_logits) {  // a CTA's gradient row must be nothing that another CTA has yet to read
     const mtr::Bytes grad = mtr::bytes_of(a->grad_logits, a->rows, a->grad_row_stride, a->vocab, es);
     auto hits = [&](const void* at, int64_t stride, int64_t cols, int64_t size) {  // stride 0: one row for all
       return at && overlap(grad, mtr::bytes_of(at, stride ? a->rows : 1, stride ? stride : cols, cols, size));
     };
-    if (hits(a->logits, a->logits_row_stride, a->vocab, es) ||
-        hits(a->teacher_ids, a->ids_row_stride, a->n, a->ids_dtype == MTR_IDS_I64 ? 8 : 4) ||
-        hits(a->teacher_logprobs, a->logprobs_row_stride, a->n, 4) || hits(a->g_loss, 1, 1, 4))
+    if (hits(a->logits, a->logits_row_stride, a->vocab, es) || hits(a->teacher_ids, a->ids_row_stride, a->n, ids_size) ||
+        hits(a->teacher_logprobs, a->logprobs_row_stride, a->n, 4) || hits(a->g_loss, 1, 1, 4) ||
+        mtr::meets(a->stats, 16ll * a->rows, a->grad_logits, a->rows, a->grad_row_stride * es, 1, 0, a->vocab * es))
       return MTR_ERR_BAD_PARAM;
+  }
+  if (a->out_loss) {  // and so its loss, statistics and status
+    const struct {
+      const void* at;
+      int64_t size;
+    } outs[3] = {{a->out_loss, 4}, {a->stats, 16}, {a->out_status, 4}};
+    for (const auto& o : outs) {
+      auto hits = [&](const void* at, int64_t stride, int64_t cols, int64_t size) {
+        return mtr::meets(o.at, o.size * a->rows, at, a->rows, stride * size, 1, 0, cols * size);
+      };
+      if (o.at && (hits(a->logits, a->logits_row_stride, a->vocab, es) || hits(a->teacher_ids, a->ids_row_stride, a->n, ids_size) ||
+                   hits(a->teacher_logprobs, a->logprobs_row_stride, a->n, 4) || hits(a->g_loss, 1, 1, 4) ||
+                   hits(a->grad_logits, a->grad_row_stride, a->vocab, es)))
+        return MTR_ERR_BAD_PARAM;
+    }
   }
   return MTR_OK;
 }

@@ -171,6 +171,31 @@ def test_arguments_are_checked_on_the_host(kw, code):
         assert lib.mtr_distill_launch(ctypes.byref(a), None) == code
 
 
+@pytest.mark.parametrize("field,size", [("out_loss", 4), ("stats", 16), ("out_status", 4)])
+def test_what_is_written_overlaps_nothing_that_is_read(field, size):
+    lib = N.load()
+    ok = dict(rows=100, stats=0x7000000, out_status=0x7100000, g_loss=0x6000000)
+
+    def code(at, **kw):
+        return lib.mtr_distill_validate(ctypes.byref(_args(**{**ok, **kw, field: at})))
+
+    # the last byte of logits, ids, log probabilities, gradients of the losses, gradient, and the first behind it
+    up = lambda v: (v + 15) // 16 * 16  # noqa: E731
+    for start, n in ((0x1000000, 100 * 200), (0x2000000, 100 * 64), (0x3000000, 100 * 32), (0x6000000, 400), (0x5000000, 100 * 200)):
+        end = start + n
+        assert code(start) == N.ERR_BAD_PARAM and code((end - 1) // 16 * 16) == N.ERR_BAD_PARAM
+        assert code(start - up(100 * size) + 16) == N.ERR_BAD_PARAM
+        assert code(up(end)) == N.OK and code(start - up(100 * size)) == N.OK
+    assert code(0x1000000 + 9 * 256 + 208, rows=1, logits_row_stride=128) == N.OK
+    assert code(0x2000000 + 64, ids_row_stride=0) == N.OK and code(0x2000000 + 48, ids_row_stride=0) == N.ERR_BAD_PARAM
+    # the gradient alone reads the statistics and writes no loss or status
+    alone = dict(out_loss=None, stats=0x7000000)
+    if field == "stats":
+        assert code(0x5000000 + 19792, **alone) == N.ERR_BAD_PARAM and code(0x1000000, **alone) == N.OK
+    elif field == "out_status":
+        assert code(0x1000000, **alone) == N.OK
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError):
         distillation_loss(torch.zeros((2, 16)), torch.zeros((2, 1), dtype=torch.int64), torch.zeros((2, 1)))
