@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(128, 1)
   bool waited = true;
   if (lane == 0) waited = mbar_wait(&done, 0, WAIT_NS) && !p.give_up;
   waited = __shfl_sync(FULL, waited, 0) != 0;
+  __syncwarp();  // a shuffle orders no memory
   tc_fence_after();
   // tcgen05.ld is warp-collective: the whole warp reads or none of it
   const bool go = __all_sync(FULL, waited && !abort_flag);

@@ -441,6 +441,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
             if (lane == 0) waited = mbar_wait(sc_bar, sc.parity, WAIT_NS) && mbar_wait(done_bar, turn.parity, WAIT_NS) && !hook;
             hook = false;
             waited = __shfl_sync(FULL, waited, 0) != 0;
+            __syncwarp();  // as in both_complete
             if (!waited) break;
           }
           tc_fence_after();

@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(PROJ_THREADS, 1)
       bool waited = true;
       if (lane == 0) waited = mbar_wait(&acc_full[acc], (n >> 1) & 1, WAIT_NS) && !p.give_up;
       waited = __shfl_sync(FULL, waited, 0) != 0;
+      __syncwarp();  // a shuffle orders no memory
       if (!waited) {
         if (lane == 0) gave_up(p.err, 4u);
         // what is not computed reads NaN, which the sampler and the scores report

@@ -81,7 +81,9 @@ __device__ __forceinline__ bool both_complete(bool mine, uint32_t a, uint32_t pa
       : "=r"(ok)
       : "r"((uint32_t)mine), "r"(a), "r"(pa), "r"(b), "r"(pb)
       : "memory");
-  return __any_sync(FULL, ok != 0u);
+  const bool any = __any_sync(FULL, ok != 0u);
+  __syncwarp();  // a vote orders no memory: what the one lane has acquired, the others may read now
+  return any;
 }
 // A value that the compiler keeps in a register: it would form a shared-memory
 // address anew, from the CTA's place in the cluster, wherever it is used.
