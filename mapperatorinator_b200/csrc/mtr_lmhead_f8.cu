@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
     if ((warp - 4) / 4 * PART < BN) {
       const int quad = warp & 3, c0 = (warp - 4) / 4 * PART;
       uint8_t* box = ring + (size_t)S * G::STAGE_BYTES + (size_t)(warp - 4) * G::BOX_BYTES;
-      constexpr int LD = 32, BUFS = 2;
+      constexpr int LD = 32;  // columns of a load; the next one is under way while these are added
       const uint32_t tmem_at = held(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c0);
       const uint32_t done_at = held(smem_u32(done)), empty_at = held(map_to(smem_u32(acc_empty), 0));
       const uint32_t sc_full_at = held(smem_u32(fx.sc_full)), sc_empty_at = held(smem_u32(fx.sc_empty));
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
           }
           tc_fence_after();
           const uint32_t base = tmem_at + (uint32_t)(acc.slot * BN);
-          uint32_t v[BUFS][LD];
+          uint32_t v[2][LD];
           if (live) tmem_ld(base, v[0]);
           const float f = __fmul_rn(load_shared(rows_at + sc.slot * (BM * 4)), load_shared(ids_at + sc.slot * 16));
           auto release = [&]() {  // the warp's part of the accumulator is in registers
@@ -457,13 +457,12 @@ __global__ void __launch_bounds__(Geo<CG, BN>::THREADS, 1)
           if (live) {
 #pragma unroll
             for (int g = 0; g < PART / LD; ++g) {
-              uint32_t(&now)[LD] = v[g % BUFS];
+              uint32_t(&now)[LD] = v[g % 2];
               tmem_wait_ld(now);
               if (g + 1 == PART / LD) release();
-              else if (BUFS > 1) tmem_ld(base + (uint32_t)((g + 1) * LD), v[(g + 1) % BUFS]);
+              else tmem_ld(base + (uint32_t)((g + 1) * LD), v[(g + 1) % 2]);
 #pragma unroll
               for (int i = 0; i < LD; ++i) sum[g * LD + i] = fmaf(__uint_as_float(now[i]), f, sum[g * LD + i]);
-              if (BUFS == 1 && g + 1 < PART / LD) tmem_ld(base + (uint32_t)((g + 1) * LD), v[0]);
             }
           } else {
             release();  // nothing to read here
