@@ -11,18 +11,9 @@ and gradient from one reading of the logits and without an autograd graph.
 from __future__ import annotations
 
 import torch
-import torch.autograd.forward_ad as forward_ad
 
 from . import _native as N
-from .int8_head import DTYPES, launch_on, matrix, same_device
-
-
-def _no_tangent(*tensors: torch.Tensor | None) -> None:
-    if forward_ad._current_level < 0:  # no dual level is open: nothing carries a tangent
-        return
-    for t in tensors:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError("distillation losses have no forward-mode derivative")
+from .int8_head import DTYPES, launch_on, matrix, no_tangent, same_device
 
 
 def _args(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, temperature: float, tail: bool,
@@ -115,7 +106,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     to the logits (once, in reverse mode).  A step that is to be captured in a CUDA
     graph takes :func:`distillation_loss_and_grad`: autograd's backward must not be
     captured while an eager graph of the same leaves is alive."""
-    _no_tangent(logits, teacher_logprobs)
+    no_tangent("distillation losses", logits, teacher_logprobs)
     if torch.is_grad_enabled():
         if teacher_logprobs.requires_grad:
             raise ValueError("teacher_logprobs must not require a gradient: the teacher is a constant")
@@ -137,7 +128,7 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, 
     one reading of the logits.  No autograd graph is needed or made, so a training
     step can be captured in a CUDA graph.  The gradient is ``out`` or a new tensor;
     ``out`` has the logits' shape and dtype and must not overlap them."""
-    _no_tangent(logits, teacher_logprobs, grad_losses)
+    no_tangent("distillation losses", logits, teacher_logprobs, grad_losses)
     a = _args(logits, teacher_ids, teacher_logprobs, temperature, tail, status)
     g = _grad_losses(grad_losses, logits)
     if out is None:

@@ -15,6 +15,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _native as N
 
@@ -46,6 +47,15 @@ def matrix(t: torch.Tensor, what: str, dtypes=DTYPES) -> int:
 def same_device(t: torch.Tensor, device: torch.device, what: str) -> None:
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, not on {device}")
+
+
+def no_tangent(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses tensors that carry a forward-mode tangent, which ``what`` would drop."""
+    if forward_ad._current_level < 0:  # no dual level is open: nothing carries a tangent
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} have no forward-mode derivative")
 
 
 class Int8Weight(NamedTuple):

@@ -15,10 +15,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-import torch.autograd.forward_ad as forward_ad
 
 from . import _native as N
-from .int8_head import DTYPES, same_device, launch_on, matrix
+from .int8_head import DTYPES, launch_on, matrix, no_tangent, same_device
 
 
 class TokenLogprobs(NamedTuple):
@@ -30,14 +29,6 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor          # [R, n] int64, -1 where there are fewer alternatives
     top_logprobs: torch.Tensor     # [R, n] float32
     stats: torch.Tensor            # [R, 4] float32, for token_logprobs_backward
-
-
-def _no_tangent(*tensors: torch.Tensor | None) -> None:
-    if forward_ad._current_level < 0:  # no dual level is open: nothing carries a tangent
-        return
-    for t in tensors:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError("token log probabilities have no forward-mode derivative")
 
 
 def _tokens(tokens: torch.Tensor | None, logits: torch.Tensor) -> torch.Tensor | None:
@@ -103,7 +94,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, r
     graph, so it can be captured in a CUDA graph.  ``logits``, ``tokens`` and
     ``temperature`` are the forward call's; ``out`` has the logits' shape and
     dtype and must not overlap them.  Itself not differentiable."""
-    _no_tangent(logits, grad_logprobs, grad_entropy, grad_lse, grad_top_logprobs)
+    no_tangent("token log probabilities", logits, grad_logprobs, grad_entropy, grad_lse, grad_top_logprobs)
     stride = matrix(logits, "logits")
     rows, vocab = logits.shape
     device = logits.device
@@ -201,7 +192,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     :func:`~mapperatorinator_b200.sampling.row_status_report` reads.  Gradients
     flow from ``logprobs``, ``entropy``, ``lse`` and ``top_logprobs`` to the
     logits (once, in reverse mode; not through ``top_ids``)."""
-    _no_tangent(logits)
+    no_tangent("token log probabilities", logits)
     tokens = _tokens(tokens, logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         hold: list = []

@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
-from .int8_head import DTYPES, launch_on, same_device
+from .int8_head import DTYPES, launch_on, no_tangent, same_device
 
 
 class Verified(NamedTuple):
@@ -80,7 +80,10 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     - A uniform outside [0, 1) is clamped (``bad_uniform``).
 
     Deterministic, without a host sync, capturable in a CUDA graph when ``uniforms``
-    are given."""
+    are given.  Not differentiable: ``logprobs`` carry no graph
+    (:func:`~mapperatorinator_b200.scoring.token_logprobs` of the tokens does), and
+    logits with a forward-mode tangent are refused."""
+    no_tangent("verified tokens", target_logits, draft_logits if do_sample else None)
     t_batch, t_pos = _cube(target_logits, "target_logits")
     batch, more, vocab = target_logits.shape
     device, drafts = target_logits.device, more - 1

@@ -445,6 +445,20 @@ def test_refusals(cuda_device):
 
 
 @gpu
+def test_derivatives(cuda_device):
+    import torch.autograd.forward_ad as fa
+
+    target, ids, draft, u = inputs(cuda_device, 4, 2, 30, torch.float32)
+    with fa.dual_level():
+        for t, d in ((fa.make_dual(target, torch.ones_like(target)), draft), (target, fa.make_dual(draft, torch.ones_like(draft)))):
+            with pytest.raises(NotImplementedError):
+                verify_drafts(t, ids, d, uniforms=u)
+        verify_drafts(target, ids, draft, uniforms=u)
+    r = verify_drafts(target.clone().requires_grad_(True), ids, draft, uniforms=u)
+    assert not r.logprobs.requires_grad
+
+
+@gpu
 def test_no_sequences_and_generated_uniforms(cuda_device):
     target, ids, draft, u = inputs(cuda_device, 4, 2, 30, torch.float32)
     r = verify_drafts(target[:0], ids[:0], draft[:0], uniforms=u[:0])
