@@ -581,7 +581,8 @@ int mtr_distill_launch(const MtrDistillArgs* args, void* stream);
  * w = p.  do_sample = 0: draft j is accepted while it is the largest target logit
  * (the lowest id of equal ones), and the token is that id.
  * The tokens are what real arithmetic decides, but for borders within double's
- * rounding.
+ * rounding and for probabilities of 2^-1000 of the row's largest or less, which
+ * count as 0 (masks of a large negative value forbid, like -inf).
  * A draft id below 0 ends a sequence's drafts (so does one >= vocab, which sets
  * MTR_ROW_BAD_ID).  A uniform outside [0, 1) is clamped (MTR_ROW_BAD_UNIFORM).  A
  * target row with NaN or +inf (MTR_ROW_NONFINITE) or of -inf alone

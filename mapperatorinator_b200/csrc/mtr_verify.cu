@@ -30,6 +30,9 @@ namespace mtr {
 namespace vf {
 
 constexpr double BORDER = 0x1p-14;  // 2 E: two sums
+// (logit - largest) / T of an id that has no probability, 2^-1000 of the largest or less:
+// a mask of the type's lowest value forbids a token whatever the uniform, as -inf does
+constexpr double FAR_LOG = -1000.0 * 0.69314718055994530942;
 
 struct Part {  // of a run of a row
   float m;
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
         } else if (p.greedy) {
           verdict = t.id == (int)id ? 0 : 1;
         } else {
-          const float xt = to_f(t_row(j)[id]);
+          const double z = ((double)to_f(t_row(j)[id]) - (double)t.m) * p.t_inv;
           const double u = uniform(j, st);
           bool q_zero = false, q_bad = false;
           double lq = 0.0;
@@ -468,15 +471,15 @@ __global__ void __launch_bounds__(kept ? FEW : MANY, 1) pick_kernel(const Params
               st |= MTR_ROW_ALL_MASKED;
               q_bad = true;
             } else {
-              const float xd = to_f(d_row(j)[id]);
-              q_zero = xd == neg_inf();
-              lq = ((double)xd - (double)d.m) * p.d_inv - log(d.s);
+              const double z = ((double)to_f(d_row(j)[id]) - (double)d.m) * p.d_inv;
+              q_zero = z <= FAR_LOG;
+              lq = z - log(d.s);
             }
           }
-          if (q_bad || xt == neg_inf()) verdict = 1;
+          if (q_bad || z <= FAR_LOG) verdict = 1;
           else if (q_zero || u == 0.0) verdict = 0;
           else {
-            const double far = log(u) + lq - (((double)xt - (double)t.m) * p.t_inv - log(t.s));
+            const double far = log(u) + lq - (z - log(t.s));
             verdict = far < -BORDER ? 0 : far > BORDER ? 1 : 2;
           }
         }

@@ -71,6 +71,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     maximum, which is also the new token; ``draft_logits`` and ``uniforms`` are not
     read then.
 
+    - A probability of 2^-1000 of the row's largest or less counts as 0: a mask of the
+      type's lowest value forbids a token, as -inf does, whatever the uniform.
     - A draft id below 0 ends a sequence's drafts (uneven lengths); so does one >= V,
       which also sets the ``bad_id`` bit.
     - Where the deciding target row holds a NaN or +inf, or only masked scores, the

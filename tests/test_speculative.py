@@ -569,3 +569,23 @@ def test_uniforms_on_the_borders_of_equal_ids(cuda_device, dtype, vocab, batch):
         assert bool(keep.gather(1, token).all())
         off = rank.gather(1, token)[:, 0] - n * j // 16
         assert bool(((off == 0) | (off == -1)).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [40, 4096, 20001])
+@pytest.mark.parametrize("how", ["with a draft", "a draft that is masked too", "looked up"])
+def test_masks_of_the_lowest_value_forbid(cuda_device, dtype, vocab, how):
+    """A drafted token that the target masks by its type's lowest value is refused whatever the uniform, 0 among them
+    (e^-65504 is not 0, but no token of such a probability is ever wanted), and is not drawn either."""
+    batch = 64
+    target, ids, draft, u = inputs(cuda_device, batch, 1, vocab, dtype, seed=vocab)
+    low = torch.finfo(dtype).min
+    target[:, :, : vocab // 2] = low
+    ids[:, 0] = torch.arange(batch, device=cuda_device) % (vocab // 2)
+    if how == "a draft that is masked too":
+        draft[:, :, : vocab // 2] = low
+    u[: batch // 2, 0] = 0.0
+    u[::4, 1] = 0.0
+    r = check(target, ids, None if how == "looked up" else draft, u, pad=-7)
+    assert bool((r.accepted == 0).all()) and bool((r.tokens[:, 0] >= vocab // 2).all())
