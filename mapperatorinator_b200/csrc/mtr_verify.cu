@@ -20,10 +20,11 @@
 // rows_kernel reads 571 MB (128 x 17 rows of 131072 bf16) in 102 us, 5.6 TB/s; the draw
 // of 128 sequences there takes 62: 69 instructions for an id's two terms, at 0.56 a
 // clock and scheduler, 41 % of the double rate.
-// The bound E: ex2.approx is within 2^-22, its argument within 3 2^-24 |d| of d, and
-// the mean of |d| under the softmax is at most log V < 12; a thread adds at most 16
-// pairs in fp32 before double takes over, and its sum moves to a larger maximum at
-// most 36 times, within 2^-22 each: 2.4e-7 + 2.2e-6 + 1e-6 + 8.6e-6 < 2^-15 = 3.1e-5.
+// The bound E: ex2.approx is within 2^-22, its argument within 3 2^-24 |d| of d (over
+// all moves together, whose distances add up to d), and the mean of |d| under the
+// softmax is at most log V < 12; a thread adds at most 16 pairs in fp32 before double
+// takes over, and its sum moves to a larger maximum at most 40 times (MOVES), within
+// 2^-22 each: 2.4e-7 + 2.2e-6 + 1e-6 + 9.6e-6 < 2^-15 = 3.1e-5.
 #include "mtr_vec.cuh"
 
 namespace mtr {
@@ -87,6 +88,12 @@ __device__ __forceinline__ int64_t draft_id(const Params& p, int64_t b, int j) {
 }
 
 constexpr int HOLD = 4;  // vectors of a thread's tile
+
+// Moves of a sum: an unsplit fp32 row is 32 tiles of 256 threads, 31 of them behind the
+// first; the single logit, the warp's maximum, 7 of the 8 warps in join.  (Rows that are
+// split have 16 runs at most, of two tiles.)
+constexpr int MOVES = MTR_MAX_VOCAB / 4 / (256 * HOLD) - 1 + 1 + 1 + 7;
+static_assert((1 + MOVES) * 0x1p-22 + (3 * 12 + 16) * 0x1p-24 < BORDER / 2, "the fp32 sums' error bound");
 
 // A row's parts joined; every lane the same.
 __device__ __forceinline__ Part join(const Part* parts, int runs, float scale) {

@@ -463,3 +463,24 @@ def test_what_scoring_reports_is_what_is_learned(cuda_device):
     few = token_logprobs(torch.full_like(teacher, -math.inf).scatter_(1, r.top_ids[:, :3], 1.0), top_n=8)
     assert (few.top_ids[:, 3:] == -1).all()
     check(teacher, few.top_ids, few.top_logprobs, True)
+
+
+@gpu
+@pytest.mark.parametrize("order", ["rising", "falling", "as drawn"])
+@pytest.mark.parametrize("tail", [False, True])
+def test_long_rows_whose_maximum_moves(cuda_device, tail, order):
+    """256 threads on rows of 131072 fp32 logits: a thread has 32 tiles of 16, so its sum moves to a larger maximum at most
+    31 times, then to its single logit's, the warp's and the row's: e_R = 35 2^-22 + 16 2^-24 + 3 2^-24 mean |d|, 14 2^-22 more
+    than where rows are shorter or have 512 threads."""
+    rows, vocab, n = 300, 131072, 20
+    logits, ids, lps, w = inputs(cuda_device, rows, vocab, n, torch.float32, seed=1)
+    if order != "as drawn":
+        logits = logits.sort(1, descending=order == "falling").values
+    loss, grad = distillation_loss_and_grad(logits, ids, lps, w, tail=tail)
+    more = 14 * 2.0 ** -22
+    for r in range(0, rows, 60):  # the reference needs some 40 bytes a logit
+        part = slice(r, r + 60)
+        want, tol, want_grad, room = reference(logits[part], ids[part], lps[part], tail, 1.0, w[part])
+        close(loss[part], want, tol + more, "loss")
+        # outside the ids room is at least 2 21 2^-22 of the parts' magnitudes, inside the ids q_t 21 2^-22 of one
+        close(grad[part], want_grad, room * (1 + 14 / 21), "grad")

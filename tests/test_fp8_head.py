@@ -439,3 +439,24 @@ def test_a_draft_model_beside_the_target(cuda_device):
     by_hand = grad.T @ hidden
     # 60 products of fp32 in two orders
     assert float((by_autograd - by_hand).abs().max()) <= 60 * 2.0 ** -23 * float((grad.abs().T @ hidden.abs()).max())
+
+
+@gpu
+@pytest.mark.parametrize("rows", [8, 127])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_sums_keep_24_bits(cuda_device, rows, sign):
+    """Both kernels' instructions add products as fp32 does: 448 * 448 +- 2^-k, k to 6, has at most 24 bits, so a sum that
+    keeps 24 of them is exact wherever in the block the small product stands; one rounding scales it."""
+    h = torch.zeros((127, 128), device=cuda_device)
+    h[:, 0] = 448.0
+    h[torch.arange(127), torch.arange(127) + 1] = sign * 2.0 ** -3
+    powers = torch.tensor([2.0 ** (3 - k) for k in range(-5, 7)], device=cuda_device)  # with 2^-3: 2^5 .. 2^-6
+    w = powers[:, None].repeat(1, 128)
+    w[:, 0] = 448.0
+    q, one = w.to(torch.float8_e4m3fn), torch.ones((1, 1), device=cuda_device)
+    assert torch.equal(q.float(), w)
+    _, scale = quantize_blocks(h)
+    exact = 448.0 * 448.0 + sign * 2.0 ** -3 * powers.double()
+    want = (exact[None] * scale.double()).float()
+    got = torch.cat([lm_head_logits_fp8(h[r:r + rows], q, one, out_dtype=torch.float32) for r in range(0, 127, rows)])
+    assert got.shape == want.shape and torch.equal(got, want), (got != want).nonzero()[:5]
