@@ -610,7 +610,13 @@ static cudaError_t launch_tiles(const MtrLmHeadF8Args& a, const Held& h, cudaStr
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&]() {
-    attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::DYN);
+    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::DYN);
+    if (G::SPLIT && err == cudaSuccess) {  // the epilogue would wait for good for registers that the launch does not have
+      cudaFuncAttributes f;
+      err = cudaFuncGetAttributes(&f, kern);
+      if (err == cudaSuccess && f.numRegs < G::LAUNCH_REGS) err = cudaErrorInvalidKernelImage;
+    }
+    attr_err[dev] = err;
   });
   if (attr_err[dev] != cudaSuccess) return attr_err[dev];
   ProjParams p;
