@@ -416,7 +416,8 @@ int mtr_quantize_blocks_launch(const MtrQuantizeBlocksArgs* args, void* stream);
 /*
  * logits[r, v] = RN(sum_b scale[r, b] * weight_scale[v / 128, b] * sum_{k in block b} q[r, k] * weight[v, k])
  * with q, scale the hidden states quantised by this call (into the workspace where
- * there are more than a few rows); sums in fp32.
+ * there are more than a few rows); sums in fp32, as is the two scales' product, which
+ * has to be in its range.
  */
 typedef struct MtrLmHeadF8Args {
   uint32_t abi_version;         /* = MTR_ABI_VERSION */

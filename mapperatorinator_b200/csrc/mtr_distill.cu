@@ -21,11 +21,17 @@
 // them, owns a row and keeps its first HOLD vectors a thread in registers between the
 // two passes; what a longer row has behind them comes from L2 the second time.  The
 // work of S in double goes on in the first warp while the row is under way.  Losses
-// alone run at 5.9 TB/s (1024 x 131072 fp32, 90.8 us); with gradients of 2-byte rows
-// the instructions bound it (two exponentials, an unpacking and a packing a logit):
-// 8192 x 4096 bf16 34.3 us where its bytes take 20.8 at HBM's copy rate, 2000 x 65533 125
-// where they take 80.  Some 6 us of the 34 are the rows' work in double, which makes do
-// with one division and one logarithm a lane (35.8 with each formed apart).
+// alone run at 6.0 TB/s (1024 x 131072 fp32, 89.3 us).  With gradients of 2-byte rows
+// nothing is full (8192 x 4096 bf16 34.3 us where its bytes take 20.8 at HBM's copy rate:
+// 0.64 instructions a clock and scheduler, exponentials 51 % of their rate, HBM 29 %
+// under the profiler): a row is a chain -- ids, the logits at them, the vectors, sums,
+// the row's work in double, the gradient -- that only the SM's other rows cover, of which
+// 28 fit at 72 registers.  2000 x 65533 takes 125 us, its bytes 80.  Some 6 us of the 34
+// are the rows' work in double, which makes do with one division and one logarithm a
+// lane (35.8 with each formed apart).
+// More than 32 ids (SLOTS 4) spill under these registers, up to 224 bytes a thread: 8192 x
+// 4096 bf16 takes 47 us with 50 ids and 58 with 128, where 20 take 34, 2000 x 65533
+// 153 with 50.
 #include "mtr_vec.cuh"
 
 namespace mtr {
@@ -500,7 +506,9 @@ static cudaError_t launch(const Params& p, int64_t rows, bool scan, cudaStream_t
 }
 
 // Threads of a row, by how many rows there are to fill the device's 16 warps an SM
-// and how long they are; CTAs share a row only where they give idle SMs work.
+// and how long they are; CTAs share a row only where they give idle SMs work, and not
+// where the gradient alone is asked for (4 x 131072 fp32, 32 ids: 16.3 us, the loss before
+// it 6.1, both from one reading in clusters 8.1).
 // Loss and gradient together, with 20 ids (us, 32 / 128 / 256 threads, 148 SMs):
 //   8192 x 1000 bf16    14.9 / 39.5 / 64.2     enough rows: a warp each
 //   8192 x 4096 bf16    34.4 / 47.3 / 75.4

@@ -6,9 +6,10 @@
 // q = e4m3(RN32(x / scale)), so with b the blocks of d
 //   logits[r, v] = sum_b (scale_h[r, b] scale_w[v / 128, b]) sum_{k in b} q_h[r, k] q_w[v, k].
 // The inner sums are the tensor core's, in fp32 (products of two e4m3 are exact);
-// each is scaled in fp32 and added to its logit in a register, so that no sum runs
-// over more than a block and the scales may be any fp32 numbers.  One rounding to
-// the logits' type follows.
+// each is scaled by the two scales' product, rounded to fp32 (so it has to be in
+// fp32's range: beyond 2^128 the logits are not finite, below 2^-126 they lose bits),
+// and added to its logit in a register: no sum runs over more than a block.  One
+// rounding to the logits' type follows.
 #include <type_traits>
 
 #include "mtr_f8.cuh"
@@ -47,8 +48,9 @@ __device__ __forceinline__ void store4(uint8_t* q, int c, int cols, uint32_t w) 
 }
 
 // A row's blocks of 128, a warp for UNITS of them: four values a lane and block.
-// HBM bounds it: 3 bytes a bf16 value.  Fewer units where rows are few, so that there
-// are warps for all SMs.
+// Fewer units where rows are few, so that there are warps for all SMs.  8192 x 4096 fp32
+// 29.7 us, 5.6 TB/s, which HBM bounds; bf16 30.3, 3.3 TB/s: the same 8-byte loads a lane
+// and the same work for half the bytes read.  64 x 768 bf16 1.7 us, a launch.
 template <typename T, bool VEC, int UNITS>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const QuantParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -83,7 +85,9 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const Quan
   }
 }
 
-// 128 rows x 128 values with one scale: a CTA each (weights, once at load time).
+// 128 rows x 128 values with one scale: a CTA each.  Weights pass here once, at load
+// time, and it is not tuned: 16384 x 4096 bf16 170 us, 1.2 TB/s (16 loads and 16 stores of
+// 4 values a thread, a barrier between them); 4096 x 768 13.9 us.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_tiles_kernel(const QuantParams p) {
   __shared__ float tops[QUANT_THREADS / 32];
@@ -188,13 +192,14 @@ __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
 // so that the others' waits give up too; the producer then gives its copies time
 // to land, the epilogue writes NaN for what was not computed, and the CTA returns.
 //
-// What bounds it (8192 x 4096 -> 16384: 530 .. 577 us by the clock that power leaves,
+// What bounds it (8192 x 4096 -> 16384: 521 .. 578 us by the clock that power leaves,
 // quantisation included; clock stamps): a block takes 875 clocks, of which the tensor
 // core is busy 55 %.  The epilogue's own chain of a block -- see it done 140 at least,
 // read, add and hand over 470, the rest of its loop 155 -- takes 730 even where no
 // product is issued, and two accumulators of 256 columns are all that tensor memory
-// holds.  Sums are scalar: packed ones cost a move each (750 -> 605 us with the scales'
-// ring).  Not faster: 16 epilogue warps of 64 columns (700; no registers left), tiles of
+// holds.  That chain is latency: its additions are 256 issue slots a scheduler and its
+// tensor-memory reads 256 clocks, so waits and loop could give way.  Sums are scalar:
+// packed ones cost a move each (750 -> 605 us with the scales' ring).  Not faster: 16 epilogue warps of 64 columns (700; no registers left), tiles of
 // 128 columns and four accumulators (763), halves of a product handed over one by one
 // (685: N = 128 waits for shared memory), one warp that polls for all (757).
 constexpr int RING = 4;  // blocks whose scales are in shared memory
@@ -646,16 +651,17 @@ static cudaError_t launch_tiles(const MtrLmHeadF8Args& a, const Held& h, cudaStr
 
 // The narrowest tiles that still make one round of CTAs; beyond that 128 x 256
 // tiles, or pairs of CTAs on 256 x 256, which take less out of L2.  Measured with the
-// quantisation (us, 148 SMs, weights not in L2; the rule's choice is starred):
+// quantisation (us, 148 SMs, weights not in L2; bf16, the second row fp16 to fp32; the
+// rule's choice is starred):
 //                         64     128    256    pair
-//   128 x 768 -> 4096     6.2*   7.0    8.8    9.5
-//   333 x 1001 -> 4099    11.4   9.7*   14.7   15.2
-//   700 x 1024 -> 4096    14.1   12.8   11.9*  13.0
-//   512 x 768 -> 16384    21.0   16.6   15.6*  16.8
-//   64 x 4096 -> 16384    25.4   18.4*  22.6   24.9
-//   300 x 1024 -> 131072  116    73.1   66.1*  80.6
-//   1024 x 2048 -> 32768  144    89.7   77.1   74.8*
-//   8192 x 768 -> 4096    69.0   47.6   43.3   43.6*
+//   128 x 768 -> 4096     6.4*   7.2    8.9    9.8
+//   333 x 1001 -> 4099    13.2   11.1*  16.5   17.1
+//   700 x 1024 -> 4096    14.2   12.8   11.9*  13.0
+//   512 x 768 -> 16384    21.2   17.0   15.7*  17.2
+//   64 x 4096 -> 16384    25.8   18.9*  22.9   25.3
+//   300 x 1024 -> 131072  117    73.4   65.6*  81.9
+//   1024 x 2048 -> 32768  144    88.3   74.1   73.6*
+//   8192 x 768 -> 4096    68.9   47.7   43.5   43.7*
 template <typename Tout>
 static cudaError_t launch_proj(const MtrLmHeadF8Args& a, const Held& h, cudaStream_t s) {
   const int64_t sms = device_sms(), m = (a.rows + BM - 1) / BM;

@@ -212,10 +212,15 @@ cudaError_t launch_rows(const FewParams& p, cudaStream_t s) {
 
 // Where this kernel is the faster one: every CTA quantises all rows, so their blocks
 // must be few, the fewer the more the vocabulary's own time weighs.  us with weights
-// that are not in L2, here / there (148 SMs): 1 x 768 -> 4096 3.3 / 6.0, 8 x 768 ->
-// 4096 5.5 / 6.2, 8 x 300 -> 65536 12.0 / 12.8, 1 x 1024 -> 65536 16.5 / 16.7; and
-// beyond the bounds 4 x 1024 -> 65536 18.3 / 16.6, 1 x 4096 -> 16384 18.6 / 17.3, 8 x
-// 4096 -> 131072 116 / 93, 16 x 768 -> 4096 (two fragments of rows) 8.0 / 6.2.
+// that are not in L2, here / there (148 SMs): 1 x 768 -> 4096 3.5 / 6.1, 2 x 768 -> 4096
+// 3.7 / 6.2, 8 x 768 -> 4096 5.8 / 6.9; at the bound 8 x 300 -> 65536 12.3 / 11.8 and 1 x
+// 1024 -> 65536 17.6 / 17.1, within 4 % and without a workspace; and beyond it 4 x 1024 ->
+// 65536 18.9 / 17.2, 1 x 4096 -> 16384 18.4 / 17.6, 1 x 4096 -> 131072 101 / 90, 8 x 4096 ->
+// 131072 119 / 91.  Large weights are far from their bytes on either side (1 x 4096 ->
+// 16384 10.2, 1 x 1024 -> 65536 10.2, 8 x 300 -> 65536 3.2): here whole groups are dealt to
+// warps, 4096 to 2368 in the second case, so that some have two and most one, and a step
+// is two blocks where a row may have three; there 120 and more of a tile's 128 rows are
+// empty, behind a launch of its own that quantises.
 bool few_rows(int64_t rows, int64_t d, int64_t vocab) {
   const int64_t blocks = (d + BLOCK - 1) / BLOCK;
   return rows <= ROWS && rows * blocks <= (vocab <= 8192 ? 48 : 24);

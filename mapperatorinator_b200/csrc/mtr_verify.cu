@@ -17,9 +17,13 @@
 //                 once in 10^4 drafts) both sums are formed again in double.  Then it
 //                 draws from the one position that counts, all in double.  It reads
 //                 short rows itself, and one launch does it all.
-// rows_kernel reads 571 MB (128 x 17 rows of 131072 bf16) in 102 us, 5.6 TB/s; the draw
-// of 128 sequences there takes 62: 69 instructions for an id's two terms, at 0.56 a
-// clock and scheduler, 41 % of the double rate.
+// rows_kernel reads 571 MB (128 x 17 rows of 131072 bf16) in 102 us, 5.6 TB/s, and the draw
+// of 128 sequences takes 62 behind it.  Neither its instructions (69 for an id's two
+// terms, 0.56 a clock and scheduler) nor the double rate (41 %) fill that time: one CTA of
+// 16 warps an SM at 126 registers waits for its own chains.  Rows that do not lie alike
+// about 16 bytes (odd vocabularies with a draft's logits) are drawn from a value an
+// access: 182 us at V = 131071 where 131072 takes 167, 59.5 at 64 x 5, V = 65533 fp16 where
+// 65536 takes 54.7.
 // The bound E: ex2.approx is within 2^-22, its argument within 3 2^-24 |d| of d (over
 // all moves together, whose distances add up to d), and the mean of |d| under the
 // softmax is at most log V < 12; a thread adds at most 16 pairs in fp32 before double
@@ -794,11 +798,15 @@ static int64_t rows_of(const MtrVerifyArgs& a) {
 }
 
 // Whether one launch does it all: there is a CTA for each sequence at once, and its
-// rows are short enough for it.  On the GPU that is up to 2 us slower, but a call costs
-// the host 4 us less (a launch, and no workspace), and such calls are bound by it (us
-// on the GPU, one launch / two; a call from Python takes 18.9 / 22.7): 1 x 4 drafts, V =
-// 4096 fp32 11.4 / 10.6, 64 x 8, 4096 bf16 16.3 / 14.2, 1 x 8, 600 bf16 9.3 / 10.3; more
-// rows than that pay there too: 256 x 8, 4096 bf16 32.0 / 29.9.
+// rows are short enough for it.  A call from Python then costs the host 4 to 5 us less
+// (a launch, and no workspace), and is bound by it; on the GPU, which is what a replayed
+// graph pays, it is 2.3 us slower to 0.9 faster (us, one launch / two, GPU and call):
+//   1 x 4 drafts, V = 4096 fp32    12.2 / 11.0   18.9 / 23.5
+//   the same, greedy                6.5 /  5.8   16.5 / 20.8
+//   64 x 8, V = 4096 bf16          16.6 / 14.3   19.9 / 24.1
+//   the same, looked up            10.1 / 11.0   17.9 / 22.1
+//   1 x 8, V = 600 bf16             9.8 / 10.7   19.0 / 23.2
+//   256 x 8, V = 4096 bf16         32.5 / 30.1   26.4 / 26.8   (more sequences than SMs: two)
 static bool in_one(int64_t batch, int64_t rows, int vocab, int es) {
   return batch <= SMS && vocab <= FEW * KEPT && rows * vocab * es <= 160 * 1024;
 }

@@ -4,11 +4,12 @@ and one scale for each block of 128.
 ``Fp8Weight`` holds a weight as checkpoints of this format do: e4m3 values and one
 fp32 scale for each 128 ids x 128 values.  ``lm_head_logits_fp8`` quantises the
 hidden states of a call, one scale for each row's 128 values, and multiplies on
-the tcgen05 tensor cores, each block's sum scaled by both in fp32: the counterpart
-of :func:`~mapperatorinator_b200.sampling.lm_head_logits`
-(modeling_varwhisper.py:1583) and of
-:func:`~mapperatorinator_b200.int8_head.lm_head_logits_int8`, whose one scale a row
-a few large channels coarsen.
+the tcgen05 tensor cores, each block's sum scaled by both in fp32 (their product
+has to be in fp32's range): the counterpart of
+:func:`~mapperatorinator_b200.sampling.lm_head_logits` (modeling_varwhisper.py:1583)
+and of :func:`~mapperatorinator_b200.int8_head.lm_head_logits_int8`, whose one scale
+a row a few large channels coarsen, and which is the faster of the two from a few
+hundred rows on.
 :meth:`~mapperatorinator_b200.sampling.FusedSampler.step_hidden` takes an
 :class:`Fp8Weight` in the weight's place.
 """

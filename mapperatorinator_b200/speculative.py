@@ -23,7 +23,7 @@ class Verified(NamedTuple):
 
     tokens: torch.Tensor    # [B, K + 1] int64: accepted drafts, the new token, pad_token_id
     accepted: torch.Tensor  # [B] int32: how many drafts were accepted
-    logprobs: torch.Tensor  # [B, K + 1] float32: log p of the tokens, 0 for padding
+    logprobs: torch.Tensor  # [B, K + 1] float32: log p of the tokens (sums of fp32 terms), 0 for padding
 
 
 def _cube(t: torch.Tensor, what: str) -> tuple[int, int]:

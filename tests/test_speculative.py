@@ -589,3 +589,41 @@ def test_masks_of_the_lowest_value_forbid(cuda_device, dtype, vocab, how):
     u[::4, 1] = 0.0
     r = check(target, ids, None if how == "looked up" else draft, u, pad=-7)
     assert bool((r.accepted == 0).all()) and bool((r.tokens[:, 0] >= vocab // 2).all())
+
+
+@gpu
+@pytest.mark.parametrize("stateful", [False, True])
+def test_scores_of_the_processor_chain(cuda_device, stateful):
+    """Drafting and verifying through the framework's chain, position by position: every token is one that the chain allows
+    behind what precedes it, and a stateful chain gives the scores of a fresh one."""
+    from mapperatorinator_b200.logit_processors import FusedLogitsProcessor
+
+    batch, drafts, vocab, shifts = 8, 3, 600, (10, 410)
+    make = lambda state: FusedLogitsProcessor(vocab_size=vocab, time_shift_range=shifts, sos_ids=(1,), stateful_monotonic=state,  # noqa: E731
+                                              temperature=0.8, top_k=40, top_p=0.95)
+    target_chain, draft_chain = make(stateful), make(stateful)
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    table = torch.randn((vocab, vocab), generator=g, device=cuda_device) * 2  # a model of the last token
+    other = table + 0.5 * torch.randn((vocab, vocab), generator=g, device=cuda_device)
+    history = torch.randint(10, 100, (batch, 4), generator=g, device=cuda_device)
+    history[:, 0] = 1
+    for _ in range(4):
+        seen, drafted, q = history, [], []
+        for _ in range(drafts):
+            q.append(draft_chain(seen, other[seen[:, -1]].clone()).clone())
+            drafted.append(torch.multinomial(torch.softmax(q[-1], 1), 1, generator=g))
+            seen = torch.cat([seen, drafted[-1]], 1)
+        ids, q = torch.cat(drafted, 1), torch.stack(q, 1)
+        scores, fresh = [], []
+        for j in range(drafts + 1):
+            before = torch.cat([history, ids[:, :j]], 1)
+            scores.append(target_chain(before, table[before[:, -1]].clone()).clone())
+            fresh.append(make(False)(before, table[before[:, -1]].clone()).clone())
+        scores = torch.stack(scores, 1)
+        assert torch.equal(scores, torch.stack(fresh, 1))
+        r = check(scores, ids, q, torch.rand((batch, drafts + 1), generator=g, device=cuda_device))
+        for b in range(batch):
+            for j in range(int(r.accepted[b]) + 1):
+                assert bool(scores[b, j, r.tokens[b, j]] > -math.inf)
+        # the shortest run of new tokens, so that the histories stay one tensor
+        history = torch.cat([history, r.tokens[:, : int(r.accepted.min()) + 1]], 1)
