@@ -94,8 +94,8 @@ __device__ __forceinline__ int64_t draft_id(const Params& p, int64_t b, int j) {
 constexpr int HOLD = 4;  // vectors of a thread's tile
 
 // Moves of a sum: an unsplit fp32 row is 32 tiles of 256 threads, 31 of them behind the
-// first; the single logit, the warp's maximum, 7 of the 8 warps in join.  (Rows that are
-// split have 16 runs at most, of two tiles.)
+// first; the single logit, the warp's maximum, 7 of the 8 warps in join.  (r runs have 32 / r
+// tiles and r - 1 more joins: fewer.)
 constexpr int MOVES = MTR_MAX_VOCAB / 4 / (256 * HOLD) - 1 + 1 + 1 + 7;
 static_assert((1 + MOVES) * 0x1p-22 + (3 * 12 + 16) * 0x1p-24 < BORDER / 2, "the fp32 sums' error bound");
 
